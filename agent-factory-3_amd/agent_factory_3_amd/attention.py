@@ -1,0 +1,194 @@
+"""gpt-oss attention on the MI355X: a sliding window, kept first tokens, learned sinks.
+
+``sink_attention`` is causal attention with one learned logit per query head
+added to the softmax's denominator (``GptOssAttention.sinks``), over every
+earlier token or a sliding window, optionally keeping a sequence's first tokens
+visible; differentiable in q, k, v and the sinks, over a batch, a packed row of
+sequences (the reference's collator packs them, data_collator_with_packing.py:
+5-93) or a few new tokens at the end of a cache.  The HIP kernels are behind
+``af3_sink_attention_fwd`` / ``_bwd``; there is no CPU fallback.
+
+Importing this module registers it with transformers as ``attn_implementation=
+"af3_sink"`` (``register``; ``quantizer_config`` imports it): gpt-oss has no
+sdpa form there, and its flash forms with sinks are CUDA kernels.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _capi
+from .routing import _device_of
+
+HEAD_DIMS = (64, 128)
+MAX_GROUP = 128       # query heads per key/value head
+MAX_LEN = 1 << 29     # tokens of a batch row
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the kernels read it: contiguous head vectors at 16-byte aligned addresses."""
+    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _strides(*ts):
+    """Element strides (batch, head, token) of [B, H, S, D] tensors as a C array (read by the call, never kept)."""
+    v = [s if n > 1 else 0 for t in ts for s, n in zip(t.stride()[:3], t.shape[:3])]
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+class _SinkAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, sinks, scale, window, first, starts, kv_range, need_grad):
+        B, Hq, Sq, D = q.shape
+        Hkv, Sk = k.shape[1], k.shape[2]
+        dev = q.device
+        out = torch.empty(B, Sq, Hq, D, dtype=torch.bfloat16, device=dev)
+        lse = torch.empty(B, Hq, Sq, dtype=torch.float32, device=dev) if need_grad else None
+        ws_n = int(_capi.load().af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first))
+        ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
+        _capi.call("af3_sink_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
+                   _capi.ptr(sinks), int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
+                   _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), _capi.ptr(lse),
+                   _capi.ptr(ws), ws_n, _capi.stream_of(dev))
+        if need_grad:
+            ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, lse)
+            ctx.args = (scale, window, first)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, sinks, starts, kv_range, out, lse = ctx.saved_tensors
+        scale, window, first = ctx.args
+        B, Hq, Sq, D = q.shape
+        Hkv, Sk = k.shape[1], k.shape[2]
+        dev = q.device
+        with _device_of(q):
+            do = _rows(dout.to(torch.bfloat16).transpose(1, 2))
+            dq = torch.empty(B, Sq, Hq, D, dtype=torch.bfloat16, device=dev)
+            dk = torch.empty(B, Sk, Hkv, D, dtype=torch.bfloat16, device=dev)
+            dv = torch.empty_like(dk)
+            dsinks = torch.empty_like(sinks) if sinks is not None else None
+            ws_n = int(_capi.load().af3_sink_attention_bwd_workspace_bytes(B, Hq, Hkv, Sq))
+            ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+            _capi.call("af3_sink_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(),
+                       _strides(q, k, v, do), _capi.ptr(sinks),
+                       int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
+                       _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(),
+                       lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _capi.ptr(dsinks), ws.data_ptr(),
+                       ws_n, _capi.stream_of(dev))
+        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dsinks, *[None] * 6
+
+
+def _check(q, k, v, sinks, scale, window, first):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise RuntimeError(f"sink_attention: {name} must be a GPU tensor (the MI355X path has no CPU implementation)")
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"sink_attention: {name} must be bfloat16 (got {t.dtype})")
+        if t.dim() != 4:
+            raise ValueError(f"sink_attention: {name} must be [batch, heads, tokens, dim], got {tuple(t.shape)}")
+        if t.device != q.device:
+            raise ValueError(f"sink_attention: {name} is on {t.device}, q on {q.device}")
+    B, Hq, Sq, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"sink_attention: shapes do not match: q {tuple(q.shape)}, k {tuple(k.shape)}, "
+                         f"v {tuple(v.shape)}")
+    Hkv = k.shape[1]
+    if Hkv == 0 or Hq == 0 or Hq % Hkv or Hq // Hkv > MAX_GROUP:
+        raise ValueError(f"sink_attention: {Hq} query heads cannot share {Hkv} key/value heads")
+    if D not in HEAD_DIMS:
+        raise ValueError(f"sink_attention: head dimension {D} is not one of {HEAD_DIMS}")
+    if max(Sq, k.shape[2]) >= MAX_LEN:
+        raise ValueError("sink_attention: too many tokens")
+    if sinks is not None:
+        if sinks.shape != (Hq,) or sinks.dtype not in (torch.bfloat16, torch.float32) or sinks.device != q.device:
+            raise ValueError(f"sink_attention: sinks must be [{Hq}] bfloat16 or float32 on {q.device}, got "
+                             f"{tuple(sinks.shape)} {sinks.dtype} on {sinks.device}")
+    if not (0.0 < scale < math.inf):
+        raise ValueError(f"sink_attention: scale must be positive and finite, got {scale}")
+    if window < 0 or first < 0:
+        raise ValueError(f"sink_attention: window and first must not be negative, got {window} and {first}")
+
+
+def _run(q, k, v, sinks, scale, window, first, starts, kv_range):
+    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, sinks))
+    return _SinkAttention.apply(_rows(q), _rows(k), _rows(v), sinks.contiguous() if sinks is not None else None,
+                                scale, window, first, starts, kv_range, need)
+
+
+def sequence_starts(cu_seqlens: torch.Tensor, n_tokens: int) -> torch.Tensor:
+    """[n_tokens] int32: the first token of each token's sequence; t + 1 for a token in none."""
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
+        raise ValueError(f"cu_seqlens must be a [sequences + 1] integer tensor, got {tuple(cu_seqlens.shape)}")
+    cu = cu_seqlens.to(torch.int32).contiguous()
+    starts = torch.empty(n_tokens, dtype=torch.int32, device=cu.device)
+    _capi.call("af3_seq_starts", cu.data_ptr(), cu.numel() - 1, n_tokens, starts.data_ptr(), _capi.stream_of(cu.device))
+    return starts
+
+
+def sequence_starts_of_positions(position_ids: torch.Tensor) -> torch.Tensor:
+    """The same from a packed row's position ids [n_tokens] (a sequence starts where
+    a position is not its predecessor's plus one, as transformers reads them)."""
+    pos = position_ids.reshape(-1).to(torch.int64).contiguous()
+    starts = torch.empty(pos.numel(), dtype=torch.int32, device=pos.device)
+    _capi.call("af3_seq_starts_positions", pos.data_ptr(), pos.numel(), starts.data_ptr(),
+               _capi.stream_of(pos.device))
+    return starts
+
+
+def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: torch.Tensor | None = None, *,
+                   scale: float | None = None, window: int = 0, first: int = 0,
+                   cu_seqlens: torch.Tensor | None = None, kv_range: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention with a sliding window, kept first tokens and learned sinks.
+
+    Query i stands at key position p = i + Sk - Sq (the last query is the last
+    key) and sees the keys j <= p of its sequence with ``j > p - window`` (window
+    0: all of them) or among the sequence's ``first`` tokens.  With z the scaled
+    products, out = sum_j e^z_j v_j / (e^sink + sum_j e^z_j); a row that sees
+    nothing gives 0, and zero gradients.
+
+    Args:
+        q: [B, Hq, Sq, D] bf16, D 64 or 128; any strides (head vectors contiguous
+            and 16-byte aligned are read in place, others copied)
+        k, v: [B, Hkv, Sk, D] bf16; query head h reads head h // (Hq // Hkv)
+        sinks: [Hq] bf16 or fp32 logits, or None
+        scale: 1 / sqrt(D) when None
+        window: keys of the sliding window, the query's own among them; 0 = no window
+        first: tokens at the sequence's start that stay visible with a window
+        cu_seqlens: [sequences + 1] integer cumulative lengths of a packed row (B = 1,
+            Sq = Sk), on the GPU, not decreasing; tokens outside give 0
+        kv_range: [B, 2] integer (begin, end) of each batch row's keys (padding on
+            either side), on the GPU; values are clamped to [0, Sk]
+    Returns:
+        [B, Sq, Hq, D] bf16
+    """
+    scale = q.shape[-1] ** -0.5 if scale is None and q.dim() == 4 and q.shape[-1] else (1.0 if scale is None else float(scale))
+    window, first = int(window), int(first)
+    _check(q, k, v, sinks, scale, window, first)
+    B, _, Sq, _ = q.shape
+    Sk = k.shape[2]
+    window, first = min(window, MAX_LEN), min(first, MAX_LEN)
+    if cu_seqlens is not None and kv_range is not None:
+        raise ValueError("sink_attention: cu_seqlens and kv_range exclude each other")
+    for name, t in (("cu_seqlens", cu_seqlens), ("kv_range", kv_range)):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"sink_attention: {name} is on {t.device}, q on {q.device}")
+    with _device_of(q):
+        starts = None
+        if cu_seqlens is not None:
+            if B != 1 or Sq != Sk:
+                raise ValueError(f"sink_attention: a packed row has batch 1 and as many keys as queries, got q "
+                                 f"{tuple(q.shape)}, k {tuple(k.shape)}")
+            starts = sequence_starts(cu_seqlens, Sk)
+        if kv_range is not None:
+            if kv_range.shape != (B, 2) or kv_range.is_floating_point():
+                raise ValueError(f"sink_attention: kv_range must be a [{B}, 2] integer tensor, got "
+                                 f"{tuple(kv_range.shape)} {kv_range.dtype}")
+            kv_range = kv_range.to(torch.int32).contiguous()
+        return _run(q, k, v, sinks, scale, window, first, starts, kv_range)

@@ -17,8 +17,10 @@ All index work runs in HIP kernels on the caller's stream (no host sync).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
+import math
 from dataclasses import dataclass, field
 
 import torch
@@ -298,6 +300,91 @@ def routing(logits: torch.Tensor, n_expts_act: int, sm_first: bool = False, expt
     if n_rows is not None:
         logits = logits[:n_rows]
     return _run_routing(logits, n_expts_act, expt_indx)
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, n_expts_act, expt_indx, token_mask):
+        T, E = logits.shape
+        dev = logits.device
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        stats = torch.empty(E + 1, dtype=torch.int32, device=dev)
+        ws_n = int(_capi.load().af3_balance_loss_workspace_bytes(T, E))
+        ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+        ld = logits.stride(0) if T > 1 else E
+        _capi.call("af3_balance_loss_fwd", logits.data_ptr(), ld, _capi.ptr(expt_indx), _capi.ptr(token_mask), T, E,
+                   n_expts_act, loss.data_ptr(), counts.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws_n,
+                   _capi.stream_of(dev))
+        ctx.save_for_backward(logits, token_mask, stats)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _):
+        logits, token_mask, stats = ctx.saved_tensors
+        T, E = logits.shape
+        d = torch.empty(T, E, dtype=torch.bfloat16, device=logits.device)
+        g = g.to(device=logits.device, dtype=torch.float32)
+        with _device_of(logits):
+            _capi.call("af3_balance_loss_bwd", logits.data_ptr(), logits.stride(0) if T > 1 else E,
+                       _capi.ptr(token_mask), T, E, stats.data_ptr(), g.data_ptr(), d.data_ptr(),
+                       _capi.stream_of(logits.device))
+        return d, None, None, None
+
+
+def _device_of(t: torch.Tensor):
+    """Context with the tensor's GPU as the current one (nothing done when it already is)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def balance_loss(logits: torch.Tensor, n_expts_act: int, expt_indx: torch.Tensor | None = None,
+                 token_mask: torch.Tensor | None = None):
+    """Load-balancing loss of a router and the tokens per expert.
+
+    With n counted tokens, c_e the number of them routed to expert e and
+    P_e = (1/n) sum_t softmax(logits_t)_e:  loss = E sum_e (c_e / n) P_e, the loss
+    transformers' ``load_balancing_loss_func`` computes for one layer (K when
+    balanced); c is taken as constant, so the gradient flows through P.
+
+    Args:
+        logits: [..., E] router logits (taken in bf16, as the routing does); E <= 1024
+        n_expts_act: K
+        expt_indx: [..., K] expert ids used (routing replay), ids outside [0, E)
+            counting for no expert; None: the top K as ``routing`` picks them
+        token_mask: [...] tokens to count (nonzero); None: all.  A token left out
+            has no influence, whatever its logits, and a zero gradient
+    Returns:
+        (loss fp32 scalar, counts [E] int32); the loss is 0 when no token counts
+    """
+    if not logits.is_cuda:
+        raise RuntimeError("router logits must be a GPU tensor (the MI355X path has no CPU implementation)")
+    if logits.dim() < 1 or not logits.is_floating_point():
+        raise ValueError(f"balance_loss: logits must be a floating-point [..., E] tensor, got {logits.dtype} "
+                         f"{tuple(logits.shape)}")
+    lead, E, K = tuple(logits.shape[:-1]), logits.shape[-1], int(n_expts_act)
+    if not 0 < E <= PLAN_MAX_E:
+        raise ValueError(f"balance_loss: {E} experts (1 to {PLAN_MAX_E} are supported)")
+    if not 0 < K <= E:
+        raise ValueError(f"balance_loss: n_expts_act must be in 1..{E}, got {K}")
+    T = math.prod(lead)
+    with _device_of(logits):
+        lg = _bf16_logits(logits.reshape(T, E))
+        if T > 1 and lg.stride(0) < E:  # a row broadcast over the tokens
+            lg = lg.contiguous()
+        if expt_indx is not None:
+            if tuple(expt_indx.shape) not in (lead + (K,), (T, K)):
+                raise ValueError(f"balance_loss: expt_indx is {tuple(expt_indx.shape)}, expected {lead + (K,)}")
+            expt_indx = expt_indx.to(device=lg.device, dtype=torch.int32).contiguous()
+        if token_mask is not None:
+            if tuple(token_mask.shape) not in (lead, (T,)):
+                raise ValueError(f"balance_loss: token_mask is {tuple(token_mask.shape)}, expected {lead}")
+            token_mask = token_mask.to(lg.device)
+            token_mask = (token_mask if token_mask.dtype == torch.bool else token_mask != 0).contiguous()
+        return _BalanceLoss.apply(lg, K, expt_indx, token_mask)
 
 
 def dense_routing(n_rows: int, device) -> RoutingData:

@@ -1,0 +1,903 @@
+// Causal attention over a sliding window, with a sequence's first tokens kept
+// visible and one learned sink logit per query head (gpt-oss attention), forward
+// and backward.  No kernel of the reference: its models call the attention that
+// transformers selects.
+//
+//   z_ij = scale q_i . k_j over the keys i sees:  lo_i <= j <= min(p_i, hi - 1)
+//          and (no window, or j > p_i - window, or j < lo_i + first)
+//   o_i  = sum_j e^{z_ij} v_j / (e^{sink} + sum_j e^{z_ij})      (0 where the denominator is 0)
+//   delta_i = do_i . o_i,  p_ij = e^{z_ij - lse_i},  dz_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j dz_ij k_j,  dk_j = scale sum_i dz_ij q_i,  dv_j = sum_i p_ij do_i,
+//   dsink = -sum_i e^{sink - lse_i} delta_i
+//
+// with p_i = i + (Sk - Sq) (the last query is the last key), lo / hi the batch
+// row's key range, or lo_i the start of token i's sequence in a packed row.
+//
+// Rows.  The G query heads of a key/value head are rows of one tile: row r of a
+// tile is (token r / G, head r % G), so a K / V tile in LDS serves every head
+// that shares it, a 128-row tile spans only 128 / G tokens (a window of 128
+// costs few keys beyond it), the gradients of a shared K / V row are one sum in
+// registers, and a single token fills G rows.
+//
+// Layouts.  All products run on v_mfma_f32_32x32x16_bf16 with the tile's own
+// row (query in forward and dq, key in dk / dv) in the lane and the other side
+// in the 16 accumulator registers, register r of half h holding entry
+// 8 (r / 4) + 4 h + r % 4.  Row statistics are then one value per lane, and the
+// probabilities (rounded to bf16, as the operand needs) are the next product's
+// B operand where they lie: a contraction may take its 16 entries in any order
+// that both operands share, so the other operand's transposing LDS reads
+// (ds_read_b64_tr_b16) fetch entries 4 h .. 4 h + 3 and 8 + 4 h .. in the
+// accumulators' order.  Sums, statistics and the accumulators are fp32.
+#include "af3_common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxLen = 1 << 29;   // tokens (positions and their sums with a window stay in 32 bits)
+constexpr float kLowest = -1e30f;  // running maximum of a row that has seen nothing (finite: -inf - it is -inf)
+
+struct SaParams {
+  const uint16_t *q, *k, *v;              // [B][H][S][D] by strides, D contiguous
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  const void* sinks;                      // [Hq] or NULL
+  int sinks_f32;
+  const int32_t* starts;                  // [Sk] start of each token's sequence (packed row), or NULL
+  const int32_t* kv_range;                // [B][2] or NULL
+  int B, Hq, Hkv, G, Sq, Sk, window, first;
+  int tok;                                // tokens of a row tile
+  int n_tiles, n_split;
+  float scale, scale2;                    // scale2 = scale log2(e)
+  uint16_t* out;                          // [B][Sq][Hq][D]
+  float* lse;                             // [B][Hkv][Sq][G], log2 units; or NULL
+  float* part;                            // n_split > 1: [n_split][B][Hkv][Sq][G][D] then (m, l) pairs
+  // backward
+  const uint16_t* dout;                   // [B][Sq][Hq][D] by strides
+  int64_t do_sb, do_sh, do_st;
+  float* delta;                           // as lse
+  float* dsink_part;                      // [n_tiles][B][Hq]
+  uint16_t *dq, *dk, *dv;                 // [B][S][H][D]
+};
+
+__device__ __forceinline__ void a_dma16(const void* gptr, uint32_t lds_byte_addr) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "{m0}"(lds_byte_addr) : "memory");
+}
+#define A_WAIT_VM(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
+#define A_BARRIER() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
+
+__device__ __forceinline__ uint32_t a_lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// XOR of a row's 16-byte chunk index: 8 rows' equal chunks (row reads) and 4
+// rows' 2 chunks (transposing reads) fall into distinct bank groups
+__device__ __forceinline__ int a_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+template <int D>
+__device__ __forceinline__ int a_off(int row, int chunk) { return row * (D * 2) + ((chunk ^ a_swz(row)) << 4); }
+
+// entries row0 + 4 h .. + 3 and row0 + 8 + 4 h .. + 3 of column col0 + lane % 32
+template <int D>
+__device__ __forceinline__ af3_bf16x8 a_tr8(const uint8_t* tile, int row0, int col0, int lane) {
+  const int r = row0 + ((lane >> 5) << 2) + ((lane & 15) >> 2);
+  const int c = col0 + (((lane >> 4) & 1) << 4) + ((lane & 3) << 2);
+  const uint8_t* p0 = tile + a_off<D>(r, c >> 3) + ((c & 7) << 1);
+  const uint8_t* p1 = tile + a_off<D>(r + 8, c >> 3) + ((c & 7) << 1);
+  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p0);
+  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p1);
+  return af3_bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+template <int D>
+__device__ __forceinline__ af3_bf16x8 a_row8(const uint8_t* tile, int row, int ks, int h) {
+  return *(const af3_bf16x8*)(tile + a_off<D>(row, 2 * ks + h));
+}
+
+__device__ __forceinline__ af3_f32x16 a_mfma(af3_bf16x8 a, af3_bf16x8 b, af3_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ af3_f32x16 a_zero() {
+  af3_f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// registers 8 t .. 8 t + 7 of an accumulator as a bf16 operand
+__device__ __forceinline__ af3_bf16x8 a_pack8(const af3_f32x16& p, int t) {
+  af3_u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = af3_pack_bf16x2(p[8 * t + 2 * i], p[8 * t + 2 * i + 1]);
+  return __builtin_bit_cast(af3_bf16x8, w);
+}
+
+__device__ __forceinline__ float a_xhalf(float x) { return __shfl_xor(x, 32); }
+
+__device__ __forceinline__ float a_sink2(const SaParams& p, int h) {
+  const float s = p.sinks_f32 ? ((const float*)p.sinks)[h] : af3_bf16_to_f32(((const uint16_t*)p.sinks)[h]);
+  return s * kLog2e;
+}
+
+// key range of a batch row, inside [0, Sk] whatever the tensor holds
+__device__ __forceinline__ void a_kv_range(const SaParams& p, int b, int& lo, int& hi) {
+  lo = 0;
+  hi = p.Sk;
+  if (p.kv_range) {
+    lo = min(max(p.kv_range[2 * b], 0), p.Sk);
+    hi = min(max(p.kv_range[2 * b + 1], lo), p.Sk);
+  }
+}
+
+// What a row sees: j in [lo, hi], and j >= wl or j < fl
+struct Vis {
+  int lo, hi, wl, fl;
+  __device__ __forceinline__ bool operator()(int j) const { return j >= lo && j <= hi && (j >= wl || j < fl); }
+};
+
+__device__ __forceinline__ Vis a_vis(const SaParams& p, int pos, int lo, int hi) {
+  Vis v;
+  v.lo = lo;
+  v.hi = min(pos, hi - 1);
+  v.wl = p.window > 0 ? pos - p.window + 1 : lo;
+  v.fl = lo + p.first;
+  return v;
+}
+
+// The keys a row tile runs over: [a0, a1) are first tokens before the window,
+// [b0, b1) the rest; unions over the tile's rows.
+struct Keys {
+  int a0, a1, b0, b1;
+};
+
+__device__ __forceinline__ Keys a_keys(const SaParams& p, int pos0, int pos1, int lo, int hi) {
+  Keys s;
+  s.b1 = min(hi, pos1 + 1);
+  s.b0 = p.window > 0 ? max(lo, pos0 - p.window + 1) : lo;
+  s.a0 = lo;
+  s.a1 = min(lo + p.first, min(s.b0, s.b1));
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// forward.  Block = 4 waves of 32 rows; 64-key tiles of K and V through a
+// two-stage LDS ring (global->LDS copies one tile ahead).  S^T = K Q^T puts a
+// row's scores into its lane; the running maximum moves only when it grows by
+// more than 8 (log2 units: probabilities stay below 256), so most tiles need
+// no rescaling of the output.
+// ---------------------------------------------------------------------------
+constexpr int kRows = 128;  // rows of a tile
+constexpr int kBN = 64;     // keys of a tile
+
+// one K (or V) tile of 64 rows into LDS by the block's 4 waves; rows past `last` repeat it
+template <int D>
+__device__ __forceinline__ void a_load_tile(const uint16_t* base, int64_t st, int j0, int last, uint32_t lds,
+                                            int wave, int lane) {
+  constexpr int CH = D / 8;               // chunks per row
+  constexpr int RPI = 64 / CH;            // rows per instruction
+  constexpr int N = kBN / RPI / 4;        // instructions per wave
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int row = (wave * N + i) * RPI + lane / CH;
+    const int j = min(j0 + row, last);
+    a_dma16(base + j * st + (((lane % CH) ^ a_swz(row)) << 3), lds + (uint32_t)((wave * N + i) * 1024));
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void sa_fwd_kernel(SaParams p) {
+  constexpr int KS = D / 16, DB = D / 32;
+  constexpr int kTile = kBN * D * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
+  const int bh = blockIdx.x % (p.B * p.Hkv);
+  const int rest = blockIdx.x / (p.B * p.Hkv);
+  const int split = rest % p.n_split;
+  const int tile = p.n_tiles - 1 - rest / p.n_split;  // the longest rows first
+  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, lh = lane >> 5;
+  const int off = p.Sk - p.Sq;
+  const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;  // tokens of the tile
+  const int row = wave * 32 + lr;
+  const int tk = row / p.G, g = row % p.G;
+  const bool valid = t0 + tk <= t1;
+  const int t = valid ? t0 + tk : t0;
+  const int head = hk * p.G + (valid ? g : 0);
+  int lo, hi;
+  a_kv_range(p, b, lo, hi);
+  const int row_lo = p.starts ? p.starts[t] : lo;
+  const int tile_lo = p.starts ? p.starts[t0] : lo;
+  const int tile_hi_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start
+  const Vis vis = a_vis(p, t + off, row_lo, hi);
+  const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
+  const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
+  // the wave's positions, to pass over tiles that none of its rows sees
+  const int wt0 = t0 + (wave * 32) / p.G, wt1 = min(t1, t0 + (wave * 32 + 31) / p.G);
+  int i0 = 0, i1 = na + nb;
+  if (p.n_split > 1) {
+    const int per = (na + nb + p.n_split - 1) / p.n_split;
+    i0 = min(split * per, na + nb);
+    i1 = min(i0 + per, na + nb);
+  }
+
+  af3_bf16x8 qf[KS];
+  {
+    const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
+  }
+  float m = kLowest, l = 0.f;
+  if (p.sinks && split == 0) {
+    const float s2 = a_sink2(p, head);
+    m = fmaxf(s2, kLowest);
+    l = lh == 0 ? __builtin_amdgcn_exp2f(s2 - m) : 0.f;
+  }
+  af3_f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = a_zero();
+
+  const uint16_t* kb = p.k + b * p.k_sb + hk * p.k_sh;
+  const uint16_t* vb = p.v + b * p.v_sb + hk * p.v_sh;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
+  auto first_key = [&](int i) { return i < na ? ks.a0 + i * kBN : ks.b0 + (i - na) * kBN; };
+  auto issue = [&](int i, int stage) {
+    const int j0 = first_key(i), last = (i < na ? ks.a1 : ks.b1) - 1;
+    const uint32_t st = lds0 + (uint32_t)(stage * 2 * kTile);
+    a_load_tile<D>(kb, p.k_st, j0, last, st, wave, lane);
+    a_load_tile<D>(vb, p.v_st, j0, last, st + kTile, wave, lane);
+  };
+  if (i0 < i1) issue(i0, 0);
+  for (int i = i0; i < i1; ++i) {
+    A_WAIT_VM(0);
+    A_BARRIER();
+    if (i + 1 < i1) issue(i + 1, (i + 1 - i0) & 1);
+    const uint8_t* kt = lds + ((i - i0) & 1) * 2 * kTile;
+    const uint8_t* vt = kt + kTile;
+    const int j0 = first_key(i), end = i < na ? ks.a1 : ks.b1;
+    if (wt0 > t1 || j0 > wt1 + off) continue;  // nothing for this wave
+    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wt0 + off - p.window) continue;
+
+    af3_f32x16 s[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      s[c] = a_zero();
+#pragma unroll
+      for (int x = 0; x < KS; ++x) s[c] = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s[c]);
+    }
+    const bool whole = j0 + kBN <= end && j0 + kBN - 1 <= wt0 + off && j0 >= tile_hi_lo &&
+                       (p.window <= 0 || j0 > wt1 + off - p.window);
+    if (!whole) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + c * 32 + 8 * (r / 4) + 4 * lh + r % 4;
+          s[c][r] = j < end && vis(j) ? s[c][r] : -INFINITY;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[c][r]);
+    mx = fmaxf(mx, a_xhalf(mx)) * p.scale2;
+    if (__any(mx > m + 8.f)) {
+      const float nm = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - nm);
+      m = nm;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[c][r] = __builtin_amdgcn_exp2f(fmaf(s[c][r], p.scale2, -m));
+        l += s[c][r];
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const af3_bf16x8 pf = a_pack8(s[c], u);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = a_mfma(a_tr8<D>(vt, c * 32 + u * 16, d * 32, lane), pf, o[d]);
+      }
+    }
+  }
+  l += a_xhalf(l);
+  if (!valid) return;
+  const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + g;
+  if (p.n_split > 1) {
+    const int64_t rows = (int64_t)p.B * p.Hkv * p.Sq * p.G;
+    float* po = p.part + (split * rows + prow) * D;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(float4*)(po + d * 32 + 2 * r + 4 * lh) = float4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+    if (lh == 0) *(float2*)(p.part + p.n_split * rows * D + (split * rows + prow) * 2) = float2{m, l};
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
+  uint16_t* orow = p.out + (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *(u32x2*)(orow + d * 32 + 2 * r + 4 * lh) = u32x2{af3_pack_bf16x2(o[d][r] * inv, o[d][r + 1] * inv),
+                                                        af3_pack_bf16x2(o[d][r + 2] * inv, o[d][r + 3] * inv)};
+  if (p.lse && lh == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// joins the splits of a row: one wave per row, D / 64 columns per lane
+template <int D>
+__global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.Sq * p.G;
+  const int64_t prow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (prow >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const float* ml = p.part + p.n_split * rows * D;
+  float m = kLowest;
+  for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, ml[(s * rows + prow) * 2]);
+  float l = 0.f, o[D / 64] = {};
+  for (int s = 0; s < p.n_split; ++s) {
+    const float2 x = *(const float2*)(ml + (s * rows + prow) * 2);
+    const float w = __builtin_amdgcn_exp2f(x.x - m);
+    l += w * x.y;
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) o[d] += w * p.part[(s * rows + prow) * D + d * 64 + lane];
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int g = (int)(prow % p.G);
+  const int64_t u = prow / p.G;
+  const int t = (int)(u % p.Sq);
+  const int bh = (int)(u / p.Sq), b = bh / p.Hkv, hk = bh % p.Hkv;
+  uint16_t* orow = p.out + (((int64_t)b * p.Sq + t) * p.Hq + hk * p.G + g) * D;
+#pragma unroll
+  for (int d = 0; d < D / 64; ++d) orow[d * 64 + lane] = (uint16_t)af3_f32_to_bf16(o[d] * inv);
+  if (p.lse && lane == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// ---------------------------------------------------------------------------
+// backward, queries: dq, delta and the sinks' partial sums.  The forward's
+// tiles and layouts; p comes back from the saved log-sum.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(256) void sa_dq_kernel(SaParams p) {
+  constexpr int KS = D / 16, DB = D / 32;
+  constexpr int kTile = kBN * D * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
+  __shared__ float ds_row[kRows];
+  const int bh = blockIdx.x % (p.B * p.Hkv);
+  const int tile = p.n_tiles - 1 - blockIdx.x / (p.B * p.Hkv);
+  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, lh = lane >> 5;
+  const int off = p.Sk - p.Sq;
+  const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;
+  const int row = wave * 32 + lr;
+  const int tk = row / p.G, g = row % p.G;
+  const bool valid = t0 + tk <= t1;
+  const int t = valid ? t0 + tk : t0;
+  const int head = hk * p.G + (valid ? g : 0);
+  int lo, hi;
+  a_kv_range(p, b, lo, hi);
+  const int row_lo = p.starts ? p.starts[t] : lo;
+  const int tile_lo = p.starts ? p.starts[t0] : lo;
+  const int tile_hi_lo = p.starts ? p.starts[t1] : lo;
+  const Vis vis = a_vis(p, t + off, row_lo, hi);
+  const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
+  const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
+  const int wt0 = t0 + (wave * 32) / p.G, wt1 = min(t1, t0 + (wave * 32 + 31) / p.G);
+
+  const uint16_t* kb = p.k + b * p.k_sb + hk * p.k_sh;
+  const uint16_t* vb = p.v + b * p.v_sb + hk * p.v_sh;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
+  auto first_key = [&](int i) { return i < na ? ks.a0 + i * kBN : ks.b0 + (i - na) * kBN; };
+  auto issue = [&](int i, int stage) {
+    const int j0 = first_key(i), last = (i < na ? ks.a1 : ks.b1) - 1;
+    const uint32_t st = lds0 + (uint32_t)(stage * 2 * kTile);
+    a_load_tile<D>(kb, p.k_st, j0, last, st, wave, lane);
+    a_load_tile<D>(vb, p.v_st, j0, last, st + kTile, wave, lane);
+  };
+
+  const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + (valid ? g : 0);
+  af3_bf16x8 qf[KS], df[KS];
+  float delta = 0.f;
+  {
+    const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
+    const uint16_t* dr = p.dout + b * p.do_sb + head * p.do_sh + t * p.do_st;
+    const uint16_t* orow = p.out + (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
+      df[s] = *(const af3_bf16x8*)(dr + s * 16 + lh * 8);
+      const af3_bf16x8 of = *(const af3_bf16x8*)(orow + s * 16 + lh * 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[i], delta);
+    }
+    delta += a_xhalf(delta);
+  }
+  const float lse = p.lse[prow];
+  if (valid && lh == 0) p.delta[prow] = delta;
+  if (p.sinks) {
+    if (lh == 0) ds_row[row] = valid ? -__builtin_amdgcn_exp2f(a_sink2(p, head) - lse) * delta : 0.f;
+    __syncthreads();
+    if ((int)threadIdx.x < p.G) {  // the tile's sum for each of the shared heads, in token order
+      float sum = 0.f;
+      for (int x = 0; x < p.tok; ++x) sum += ds_row[x * p.G + threadIdx.x];
+      p.dsink_part[((int64_t)tile * p.B + b) * p.Hq + hk * p.G + threadIdx.x] = sum;
+    }
+  }
+  A_WAIT_VM(0);
+  if (na + nb > 0) issue(0, 0);
+
+  af3_f32x16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) acc[d] = a_zero();
+  for (int i = 0; i < na + nb; ++i) {
+    A_WAIT_VM(0);
+    A_BARRIER();
+    if (i + 1 < na + nb) issue(i + 1, (i + 1) & 1);
+    const uint8_t* kt = lds + (i & 1) * 2 * kTile;
+    const uint8_t* vt = kt + kTile;
+    const int j0 = first_key(i), end = i < na ? ks.a1 : ks.b1;
+    if (wt0 > t1 || j0 > wt1 + off) continue;
+    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wt0 + off - p.window) continue;
+    const bool whole = j0 + kBN <= end && j0 + kBN - 1 <= wt0 + off && j0 >= tile_hi_lo &&
+                       (p.window <= 0 || j0 > wt1 + off - p.window);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      af3_f32x16 s = a_zero(), dp = a_zero();
+#pragma unroll
+      for (int x = 0; x < KS; ++x) s = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s);
+#pragma unroll
+      for (int x = 0; x < KS; ++x) dp = a_mfma(a_row8<D>(vt, c * 32 + lr, x, lh), df[x], dp);
+      if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + c * 32 + 8 * (r / 4) + 4 * lh + r % 4;
+          const bool on = j < end && vis(j);
+          s[r] = on ? s[r] : -INFINITY;
+          dp[r] = on ? dp[r] : delta;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse)) * (dp[r] - delta);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const af3_bf16x8 pf = a_pack8(s, u);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] = a_mfma(a_tr8<D>(kt, c * 32 + u * 16, d * 32, lane), pf, acc[d]);
+      }
+    }
+  }
+  if (!valid) return;
+  uint16_t* qrow = p.dq + (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *(u32x2*)(qrow + d * 32 + 2 * r + 4 * lh) =
+          u32x2{af3_pack_bf16x2(acc[d][r] * p.scale, acc[d][r + 1] * p.scale),
+                af3_pack_bf16x2(acc[d][r + 2] * p.scale, acc[d][r + 3] * p.scale)};
+}
+
+// one block per head: the sinks' gradient from the tiles' sums (a fixed order)
+__global__ __launch_bounds__(256) void sa_dsink_kernel(const float* __restrict__ part, int n, int Hq, int f32,
+                                                       void* __restrict__ out) {
+  __shared__ float sh[256];
+  const int h = blockIdx.x;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) s += part[(int64_t)i * Hq + h];
+  sh[threadIdx.x] = s;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    if (f32)
+      ((float*)out)[h] = sh[0];
+    else
+      ((uint16_t*)out)[h] = (uint16_t)af3_f32_to_bf16(sh[0]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward, keys: dk and dv.  Block = 4 waves of 32 keys of one key/value head,
+// K and V rows in registers; the (token, head) rows that see them go through a
+// two-stage LDS ring, 64 at a time (q, dout, and their lse, delta, position and
+// sequence start).  S = Q K^T puts a key's column into its lane; the sum over
+// the heads that share the key is the sum over rows.
+// ---------------------------------------------------------------------------
+constexpr int kKeys = 128;  // keys of a block
+constexpr int kRT = 64;     // rows of a step
+
+// first token after t0 whose sequence starts later than t0's (starts does not
+// decrease), or n: 64 probes a round, the answer stays in (lo, hi]
+__device__ __forceinline__ int a_sequence_end(const int32_t* starts, int t0, int n, int lane) {
+  const int s0 = starts[t0];
+  int lo = t0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64;
+    const int at = lo + step * (lane + 1);
+    const int same = __popcll(__ballot(at < hi && starts[at] == s0));
+    hi = min(hi, lo + step * (same + 1));
+    lo += step * same;
+  }
+  return hi;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void sa_dkv_kernel(SaParams p) {
+  constexpr int KS = D / 16, DB = D / 32;
+  constexpr int kTile = kRT * D * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
+  __shared__ __attribute__((aligned(16))) float st_lse[2][kRT], st_delta[2][kRT];
+  __shared__ __attribute__((aligned(16))) int st_pos[2][kRT], st_lo[2][kRT];
+  const int bh = blockIdx.x % (p.B * p.Hkv);
+  const int j0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kKeys;  // the longest columns first
+  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, lh = lane >> 5;
+  const int off = p.Sk - p.Sq;
+  int lo, hi;
+  a_kv_range(p, b, lo, hi);
+  const int jl = min(j0 + kKeys, p.Sk) - 1;  // last key of the block
+  const int j = j0 + wave * 32 + lr;
+  const bool kvalid = j <= jl;
+
+  // tokens that may see a key of the block
+  int ta = max(0, max(j0, lo) - off), tb = p.Sq;  // [ta, tb)
+  int s_last = lo;
+  if (p.starts) {
+    s_last = p.starts[jl];
+    tb = a_sequence_end(p.starts, jl, p.Sk, lane);
+  }
+  if (p.window > 0 && s_last + p.first <= max(j0, lo)) tb = min(tb, jl + p.window - off);
+  if (jl < lo || j0 >= hi) tb = ta;
+  const int64_t ra = (int64_t)ta * p.G, rb = (int64_t)max(tb, ta) * p.G;  // their rows
+  const int n_steps = (int)((rb - ra + kRT - 1) / kRT);
+
+  af3_bf16x8 kf[KS], vf[KS];
+  {
+    const int64_t jj = kvalid ? j : jl;
+    const uint16_t* kr = p.k + b * p.k_sb + hk * p.k_sh + jj * p.k_st;
+    const uint16_t* vr = p.v + b * p.v_sb + hk * p.v_sh + jj * p.v_st;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      kf[s] = *(const af3_bf16x8*)(kr + s * 16 + lh * 8);
+      vf[s] = *(const af3_bf16x8*)(vr + s * 16 + lh * 8);
+    }
+  }
+  const bool jin = kvalid && j >= lo && j < hi;
+  const int fl_key = j - p.first;  // the key is a first token of sequences that start after fl_key
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
+  const uint16_t* qb = p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
+  const uint16_t* db = p.dout + b * p.do_sb + (int64_t)hk * p.G * p.do_sh;
+  const int64_t sb = ((int64_t)b * p.Hkv + hk) * p.Sq * p.G;
+  float v_lse = 0.f, v_delta = 0.f;
+  int v_pos = 0, v_lo = 0;
+  auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..63
+    const int64_t r0 = ra + (int64_t)i * kRT;
+    const uint32_t st = lds0 + (uint32_t)((i & 1) * 2 * kTile);
+    constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / 4;
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const int row = (wave * N + x) * RPI + lane / CH;
+      const int64_t r = min(r0 + row, rb - 1);
+      const int64_t t = r / p.G, g = r % p.G;
+      const int col = ((lane % CH) ^ a_swz(row)) << 3;
+      a_dma16(qb + t * p.q_st + g * p.q_sh + col, st + (uint32_t)((wave * N + x) * 1024));
+      a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + (uint32_t)((wave * N + x) * 1024));
+    }
+    if (threadIdx.x < kRT) {
+      const int64_t r = min(r0 + threadIdx.x, rb - 1);
+      const int t = (int)(r / p.G);
+      v_lse = p.lse[sb + r];
+      v_delta = p.delta[sb + r];
+      v_pos = r0 + threadIdx.x < rb ? t + off : -kMaxLen;  // sees nothing
+      v_lo = p.starts ? p.starts[t] : lo;
+    }
+  };
+  auto store_rows = [&](int i) {
+    if (threadIdx.x < kRT) {
+      st_lse[i & 1][threadIdx.x] = v_lse;
+      st_delta[i & 1][threadIdx.x] = v_delta;
+      st_pos[i & 1][threadIdx.x] = v_pos;
+      st_lo[i & 1][threadIdx.x] = v_lo;
+    }
+  };
+
+  af3_f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dk[d] = a_zero(), dv[d] = a_zero();
+  if (n_steps > 0) issue(0);
+  for (int i = 0; i < n_steps; ++i) {
+    A_WAIT_VM(0);
+    store_rows(i);
+    A_BARRIER();
+    if (i + 1 < n_steps) issue(i + 1);
+    const uint8_t* qt = lds + (i & 1) * 2 * kTile;
+    const uint8_t* dt = qt + kTile;
+    const int w = i & 1;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      af3_f32x16 s = a_zero(), dp = a_zero();
+#pragma unroll
+      for (int x = 0; x < KS; ++x) s = a_mfma(a_row8<D>(qt, c * 32 + lr, x, lh), kf[x], s);
+#pragma unroll
+      for (int x = 0; x < KS; ++x) dp = a_mfma(a_row8<D>(dt, c * 32 + lr, x, lh), vf[x], dp);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r4 = c * 32 + 8 * q + 4 * lh;
+        const float4 ls = *(const float4*)&st_lse[w][r4];
+        const float4 de = *(const float4*)&st_delta[w][r4];
+        const int4 po = *(const int4*)&st_pos[w][r4];
+        const int4 rl = *(const int4*)&st_lo[w][r4];
+        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
+        const int pov[4] = {po.x, po.y, po.z, po.w}, rlv[4] = {rl.x, rl.y, rl.z, rl.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int r = 4 * q + y;
+          const bool on = jin && j <= pov[y] && j >= rlv[y] &&
+                          (p.window <= 0 || j > pov[y] - p.window || fl_key < rlv[y]);
+          const float pr = on ? __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lsv[y])) : 0.f;
+          s[r] = pr;
+          dp[r] = on ? pr * (dp[r] - dev[y]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const af3_bf16x8 pf = a_pack8(s, u), sf = a_pack8(dp, u);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          dv[d] = a_mfma(a_tr8<D>(dt, c * 32 + u * 16, d * 32, lane), pf, dv[d]);
+          dk[d] = a_mfma(a_tr8<D>(qt, c * 32 + u * 16, d * 32, lane), sf, dk[d]);
+        }
+      }
+    }
+  }
+  if (!kvalid) return;
+  const int64_t o = (((int64_t)b * p.Sk + j) * p.Hkv + hk) * D;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int64_t c = o + d * 32 + 2 * r + 4 * lh;
+      *(u32x2*)(p.dv + c) = u32x2{af3_pack_bf16x2(dv[d][r], dv[d][r + 1]), af3_pack_bf16x2(dv[d][r + 2], dv[d][r + 3])};
+      *(u32x2*)(p.dk + c) = u32x2{af3_pack_bf16x2(dk[d][r] * p.scale, dk[d][r + 1] * p.scale),
+                                  af3_pack_bf16x2(dk[d][r + 2] * p.scale, dk[d][r + 3] * p.scale)};
+    }
+}
+
+// ---------------------------------------------------------------------------
+// where each token's sequence starts: tokens in no sequence get t + 1 (they see
+// nothing).  Every value lies in [0, t + 1] whatever the input holds.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void sa_starts_kernel(const int32_t* __restrict__ cu, int n, int T,
+                                                        int32_t* __restrict__ starts) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= T) return;
+  int a = 0, b = n;  // the last s with cu[s] <= t lies in [a - 1, b)
+  while (a < b) {
+    const int mid = (a + b) >> 1;
+    if (cu[mid] <= t) a = mid + 1; else b = mid;
+  }
+  starts[t] = a > 0 && t < cu[a] ? max(cu[a - 1], 0) : t + 1;
+}
+
+// one block: a sequence starts where a position is not its predecessor's plus one
+__global__ __launch_bounds__(1024) void sa_starts_pos_kernel(const int64_t* __restrict__ pos, int T,
+                                                             int32_t* __restrict__ starts) {
+  __shared__ int sh[2][1024];
+  const int n = (T + 1023) / 1024;
+  const int t0 = min((int)threadIdx.x * n, T), t1 = min(t0 + n, T);
+  int last = -1;  // the last start in this thread's range
+  for (int t = t0; t < t1; ++t)
+    if (t == 0 || pos[t] != pos[t - 1] + 1) last = t;
+  sh[0][threadIdx.x] = last;
+  __syncthreads();
+  int cur = 0;
+  for (int o = 1; o < 1024; o <<= 1) {  // inclusive maximum over the threads
+    const int x = sh[cur][threadIdx.x];
+    sh[cur ^ 1][threadIdx.x] = (int)threadIdx.x >= o ? max(x, sh[cur][threadIdx.x - o]) : x;
+    cur ^= 1;
+    __syncthreads();
+  }
+  int s = threadIdx.x > 0 ? max(sh[cur][threadIdx.x - 1], 0) : 0;
+  for (int t = t0; t < t1; ++t) {
+    if (t == 0 || pos[t] != pos[t - 1] + 1) s = t;
+    starts[t] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// Splits of a row tile's keys over blocks.  One block per (batch row, key/value
+// head, row tile) leaves most of the 256 CUs idle when there are few rows.
+int sa_splits(int B, int Hkv, int64_t n_tiles, int64_t keys) {
+  const int64_t blocks = (int64_t)B * Hkv * n_tiles;
+  if (blocks == 0 || blocks >= 256) return 1;
+  const int64_t most = (keys + 255) / 256;  // at least four key tiles each
+  int64_t n = (512 + blocks - 1) / blocks;
+  if (n > most) n = most;
+  return n < 1 ? 1 : n > 256 ? 256 : (int)n;
+}
+
+struct SaShape {
+  int tok, n_tiles, n_split, window, first;
+};
+
+SaShape sa_shape(int B, int Hq, int Hkv, int Sq, int Sk, int window, int first) {
+  SaShape s;
+  const int G = Hq / Hkv;
+  s.window = window >= Sk ? 0 : window;  // it covers every key
+  s.first = s.window > 0 ? (first < Sk ? first : Sk) : 0;
+  s.tok = kRows / G;
+  s.n_tiles = (int)af3_cdiv(Sq, s.tok);
+  int64_t keys = s.window > 0 ? (int64_t)s.window + s.tok + s.first : Sk;
+  if (keys > Sk) keys = Sk;
+  s.n_split = sa_splits(B, Hkv, s.n_tiles, keys);
+  return s;
+}
+
+int sa_check(const char* who, int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first, float scale,
+             const int64_t* strides, int n_strides, const int32_t* starts, const int32_t* kv_range) {
+  AF3_REQUIRE(B >= 0 && Sq >= 0 && Sk >= 0 && Sq < kMaxLen && Sk < kMaxLen, "%s: bad batch or length", who);
+  AF3_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "%s: %d query heads do not share %d key/value heads", who, Hq, Hkv);
+  AF3_REQUIRE(Hq / Hkv <= kRows, "%s: more than %d query heads per key/value head", who, kRows);
+  AF3_REQUIRE(D == 64 || D == 128, "%s: head dimension %d is not 64 or 128", who, D);
+  AF3_REQUIRE(window >= 0 && first >= 0, "%s: negative window or first", who);
+  AF3_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", who);
+  AF3_REQUIRE(strides, "%s: null strides", who);
+  for (int i = 0; i < n_strides; ++i) AF3_REQUIRE(strides[i] % 8 == 0, "%s: strides must be multiples of 8", who);
+  AF3_REQUIRE(!starts || (B <= 1 && Sq == Sk && !kv_range), "%s: a packed row has batch 1, Sq == Sk and no kv_range", who);
+  AF3_REQUIRE((int64_t)B * Hkv * (Sq + Sk + 1) < 0x7fffffffLL, "%s: too many rows", who);
+  return 0;
+}
+
+SaParams sa_params(const SaShape& s, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* st,
+                   const void* sinks, int sinks_f32, const int32_t* starts, const int32_t* kv_range, int B, int Hq,
+                   int Hkv, int Sq, int Sk, float scale) {
+  SaParams p = {};
+  p.q = q; p.k = k; p.v = v;
+  p.q_sb = st[0]; p.q_sh = st[1]; p.q_st = st[2];
+  p.k_sb = st[3]; p.k_sh = st[4]; p.k_st = st[5];
+  p.v_sb = st[6]; p.v_sh = st[7]; p.v_st = st[8];
+  p.sinks = sinks; p.sinks_f32 = sinks_f32;
+  p.starts = starts; p.kv_range = kv_range;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.Sq = Sq; p.Sk = Sk;
+  p.window = s.window; p.first = s.first; p.tok = s.tok; p.n_tiles = s.n_tiles; p.n_split = 1;
+  p.scale = scale; p.scale2 = scale * kLog2e;
+  return p;
+}
+
+size_t sa_up(size_t n) { return (n + 255) / 256 * 256; }
+
+bool sa_al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+extern "C" int af3_seq_starts(const int32_t* cu_seqlens, int n_seqs, int n_tokens, int32_t* starts, void* stream_) {
+  AF3_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && n_tokens < kMaxLen, "seq_starts: bad sizes");
+  if (n_tokens == 0) return 0;
+  AF3_REQUIRE(cu_seqlens && starts, "seq_starts: null pointer");
+  hipLaunchKernelGGL(sa_starts_kernel, dim3((n_tokens + 255) / 256), dim3(256), 0, (hipStream_t)stream_, cu_seqlens,
+                     n_seqs, n_tokens, starts);
+  return af3::check_launch("seq_starts");
+}
+
+extern "C" int af3_seq_starts_positions(const int64_t* position_ids, int n_tokens, int32_t* starts, void* stream_) {
+  AF3_REQUIRE(n_tokens >= 0 && n_tokens < kMaxLen, "seq_starts_positions: bad size");
+  if (n_tokens == 0) return 0;
+  AF3_REQUIRE(position_ids && starts, "seq_starts_positions: null pointer");
+  hipLaunchKernelGGL(sa_starts_pos_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream_, position_ids, n_tokens, starts);
+  return af3::check_launch("seq_starts_positions");
+}
+
+extern "C" size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int window,
+                                                     int first) {
+  if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq / Hkv > kRows || Sq <= 0 || Sk < 0) return 0;
+  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
+  return s.n_split > 1 ? (size_t)s.n_split * B * Hq * Sq * (D + 2) * 4 : 0;
+}
+
+extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
+                                      const void* sinks, int sinks_f32, const int32_t* starts, const int32_t* kv_range,
+                                      int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first, float scale,
+                                      uint16_t* out, float* lse, void* workspace, size_t ws_bytes, void* stream_) {
+  const char* who = "sink_attention_fwd";
+  if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 9, starts, kv_range)) return rc;
+  if (B == 0 || Sq == 0) return 0;
+  AF3_REQUIRE(q && out && (Sk == 0 || (k && v)), "%s: null pointer", who);
+  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(out), "%s: rows must be 16-byte aligned", who);
+  hipStream_t stream = (hipStream_t)stream_;
+  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
+  SaParams p = sa_params(s, q, k, v, strides, sinks, sinks_f32, starts, kv_range, B, Hq, Hkv, Sq, Sk, scale);
+  p.out = out;
+  p.lse = lse;
+  p.n_split = s.n_split;
+  const int64_t grid = (int64_t)s.n_tiles * B * Hkv * s.n_split;
+  if (s.n_split > 1) {
+    AF3_REQUIRE(workspace && sa_al16(workspace) &&
+                    ws_bytes >= af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first),
+                "%s: workspace too small", who);
+    p.part = (float*)workspace;
+  }
+  if (D == 64)
+    hipLaunchKernelGGL(sa_fwd_kernel<64>, dim3((unsigned)grid), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL(sa_fwd_kernel<128>, dim3((unsigned)grid), dim3(256), 0, stream, p);
+  if (s.n_split > 1) {
+    const unsigned g = (unsigned)af3_cdiv((int64_t)B * Hq * Sq, 4);
+    if (D == 64)
+      hipLaunchKernelGGL(sa_join_kernel<64>, dim3(g), dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL(sa_join_kernel<128>, dim3(g), dim3(256), 0, stream, p);
+  }
+  return af3::check_launch(who);
+}
+
+extern "C" size_t af3_sink_attention_bwd_workspace_bytes(int B, int Hq, int Hkv, int Sq) {
+  if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq / Hkv > kRows || Sq <= 0) return 0;
+  const int64_t n_tiles = af3_cdiv(Sq, kRows / (Hq / Hkv));
+  return sa_up((size_t)B * Hq * Sq * 4) + (size_t)n_tiles * B * Hq * 4;
+}
+
+extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* dout,
+                                      const int64_t* strides, const void* sinks, int sinks_f32, const int32_t* starts,
+                                      const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk, int D,
+                                      int window, int first, float scale, const uint16_t* out, const float* lse,
+                                      uint16_t* dq, uint16_t* dk, uint16_t* dv, void* dsinks, void* workspace,
+                                      size_t ws_bytes, void* stream_) {
+  const char* who = "sink_attention_bwd";
+  if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 12, starts, kv_range)) return rc;
+  const bool nq = B > 0 && Sq > 0, nk = B > 0 && Sk > 0;
+  AF3_REQUIRE((!nq || (q && dout && out && lse && dq && workspace)) && (!nk || (k && v && dk && dv)) &&
+                  (!sinks || dsinks),
+              "%s: null pointer", who);
+  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(dout) && sa_al16(out) && sa_al16(dq) && sa_al16(dk) &&
+                  sa_al16(dv) && sa_al16(workspace),
+              "%s: rows must be 16-byte aligned", who);
+  AF3_REQUIRE(ws_bytes >= af3_sink_attention_bwd_workspace_bytes(B, Hq, Hkv, Sq), "%s: workspace too small", who);
+  hipStream_t stream = (hipStream_t)stream_;
+  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
+  SaParams p = sa_params(s, q, k, v, strides, sinks, sinks_f32, starts, kv_range, B, Hq, Hkv, Sq, Sk, scale);
+  p.dout = dout;
+  p.do_sb = strides[9]; p.do_sh = strides[10]; p.do_st = strides[11];
+  p.out = (uint16_t*)out;
+  p.lse = (float*)lse;
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  p.delta = (float*)workspace;
+  p.dsink_part = (float*)((uint8_t*)workspace + sa_up((size_t)B * Hq * Sq * 4));
+  const unsigned gq = (unsigned)((int64_t)s.n_tiles * B * Hkv), gk = (unsigned)(af3_cdiv(Sk, kKeys) * B * Hkv);
+  if (gq) {
+    if (D == 64)
+      hipLaunchKernelGGL(sa_dq_kernel<64>, dim3(gq), dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL(sa_dq_kernel<128>, dim3(gq), dim3(256), 0, stream, p);
+  }
+  if (sinks)  // (no query rows: a sum over nothing)
+    hipLaunchKernelGGL(sa_dsink_kernel, dim3(Hq), dim3(256), 0, stream, p.dsink_part, s.n_tiles * B, Hq, sinks_f32,
+                       dsinks);
+  if (gk) {
+    if (D == 64)
+      hipLaunchKernelGGL(sa_dkv_kernel<64>, dim3(gk), dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL(sa_dkv_kernel<128>, dim3(gk), dim3(256), 0, stream, p);
+  }
+  return af3::check_launch(who);
+}

@@ -418,6 +418,64 @@ int af3_lm_head_dz_chunk(const float* logits, int64_t ldl, int M, int v_begin, i
                          int64_t dlp_stride, float dlp_scale, const float* dentropy, uint16_t* dz, int64_t lddz,
                          void* stream);
 
+/* Router load-balancing loss.  No counterpart in the reference (its router
+ * takes no gradient, quantization.py:421).  logits [T][ld] bf16; the K experts
+ * of a token are expt_indx [T][K] (ids outside [0, E) count for no expert) or,
+ * when it is NULL, the top K logits (ties to the lower id); token_mask [T]
+ * bytes or NULL: tokens with 0 are left out.  With n the tokens counted,
+ *   counts[e] = their selections of expert e,
+ *   loss = E sum_e (counts[e] / n) (sum_t softmax(logits_t)[e] / n)   (0 if n = 0)
+ * and the backward's dlogits [T][E] bf16 = dloss[0] d loss / d logits (0 for a
+ * token left out).  stats [E + 1] int32 (the counts, then n) carries the
+ * forward's result to the backward; E <= 1024, K <= E. */
+size_t af3_balance_loss_workspace_bytes(int64_t n_tokens, int n_expts_tot);
+int af3_balance_loss_fwd(const uint16_t* logits, int64_t ld_logits, const int32_t* expt_indx,
+                         const uint8_t* token_mask, int64_t n_tokens, int n_expts_tot, int n_expts_act, float* loss,
+                         int32_t* counts, int32_t* stats, void* workspace, size_t ws_bytes, void* stream);
+int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_t* token_mask, int64_t n_tokens,
+                         int n_expts_tot, const int32_t* stats, const float* dloss, uint16_t* dlogits, void* stream);
+
+/* Causal attention with a sliding window, kept first tokens and learned sink
+ * logits (no counterpart in the reference, whose models call the attention
+ * transformers selects).  bf16; head dimension D = 64 or 128; Hq / Hkv <= 128
+ * query heads share a key/value head (query head h reads head h / (Hq / Hkv)).
+ * strides: host array of the element strides of q, k, v (and, for the backward,
+ * dout): batch, head, token of each; the D elements are contiguous, strides
+ * multiples of 8, addresses 16-byte aligned.  Query i stands at key position
+ * p = i + Sk - Sq and sees the keys j <= p of its range with j > p - window or
+ * j < (range start) + first (window 0: all of them).  The range is
+ * kv_range[b] = (begin, end) (device int32 [B][2], clamped to [0, Sk]; NULL: all
+ * keys), or, for a packed row (B = 1, Sq = Sk), from starts[p] (device int32
+ * [Sk], af3_seq_starts): the start of the token's own sequence.  sinks [Hq]
+ * (bf16, or fp32 with sinks_f32; NULL: none) adds e^sink to the softmax's
+ * denominator.  A row that sees nothing gives 0.
+ *   forward: out [B][Sq][Hq][D]; lse [B][Hkv][Sq][Hq/Hkv] fp32 (log2 units) or
+ *   NULL; workspace of af3_sink_attention_workspace_bytes (0: none needed).
+ *   backward: dq [B][Sq][Hq][D], dk and dv [B][Sk][Hkv][D], dsinks [Hq] in the
+ *   sinks' type, from the forward's out and lse; every sum is in a fixed order.
+ * A key outside every row's range is never read into a product; NaN or infinity
+ * in a key, value or gradient row that some row of the same 128-row or 64-key
+ * tile sees may reach that tile's other rows.
+ * Lengths below 2^29 tokens. */
+int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
+                           const void* sinks, int sinks_f32, const int32_t* starts, const int32_t* kv_range, int B,
+                           int Hq, int Hkv, int Sq, int Sk, int D, int window, int first, float scale, uint16_t* out,
+                           float* lse, void* workspace, size_t ws_bytes, void* stream);
+size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first);
+size_t af3_sink_attention_bwd_workspace_bytes(int B, int Hq, int Hkv, int Sq);
+int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* dout,
+                           const int64_t* strides, const void* sinks, int sinks_f32, const int32_t* starts,
+                           const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk, int D, int window,
+                           int first, float scale, const uint16_t* out, const float* lse, uint16_t* dq, uint16_t* dk,
+                           uint16_t* dv, void* dsinks, void* workspace, size_t ws_bytes, void* stream);
+
+/* starts [n_tokens] of a packed row: from cumulative lengths cu_seqlens
+ * [n_seqs + 1] (device int32; tokens before the first or past the last sequence
+ * get t + 1 and see nothing), or from position ids (device int64): a sequence
+ * starts where a position is not its predecessor's plus one. */
+int af3_seq_starts(const int32_t* cu_seqlens, int n_seqs, int n_tokens, int32_t* starts, void* stream);
+int af3_seq_starts_positions(const int64_t* position_ids, int n_tokens, int32_t* starts, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,268 @@
+"""Sink attention on the GPU against the float64 oracle, with its derived element-wise bounds."""
+import math
+
+import pytest
+import torch
+
+from oracle import attention as oa
+
+pytestmark = pytest.mark.gpu
+
+
+def _make(dev, B, Hq, Hkv, Sq, Sk, D, seed=0, sinks=torch.bfloat16, layout="token"):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s, std=1.0: (torch.randn(*s, generator=g) * std).to(torch.bfloat16).to(dev)  # noqa: E731
+    if layout == "token":   # [B, S, H, D] storage, as a projection leaves it
+        q, k, v = r(B, Sq, Hq, D, std=2.0).transpose(1, 2), r(B, Sk, Hkv, D).transpose(1, 2), r(B, Sk, Hkv, D).transpose(1, 2)
+    elif layout == "head":
+        q, k, v = r(B, Hq, Sq, D, std=2.0), r(B, Hkv, Sk, D), r(B, Hkv, Sk, D)
+    elif layout == "fused":  # views of one fused projection
+        f = r(B, max(Sq, Sk), (Hq + 2 * Hkv) * D)
+        h = f.view(B, max(Sq, Sk), Hq + 2 * Hkv, D).transpose(1, 2)
+        q, k, v = h[:, :Hq, :Sq], h[:, Hq:Hq + Hkv, :Sk], h[:, Hq + Hkv:, :Sk]
+    else:                    # odd address, odd strides: copied
+        f = r(B, Hq + 2 * Hkv, max(Sq, Sk), D + 3)[..., 1:D + 1]
+        q, k, v = f[:, :Hq, :Sq], f[:, Hq:Hq + Hkv, :Sk], f[:, Hq + Hkv:, :Sk]
+    s = (torch.randn(Hq, generator=g) * 1.5).to(sinks).to(dev) if sinks is not None else None
+    return q, k, v, s, r(B, Sq, Hq, D)
+
+
+def _close(got, ref, tol, what):
+    got = got.detach().cpu().double()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    assert torch.isfinite(got).all(), what
+    bad = (got - ref).abs() > tol
+    assert not bad.any(), (what, int(bad.sum()), bad.nonzero()[:3].tolist(),
+                           float(((got - ref).abs() / tol)[bad].max()))
+
+
+def _check(dev, B, Hq, Hkv, Sq, Sk, D, *, train=True, sinks=torch.bfloat16, layout="token", seed=0, **kw):
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, B, Hq, Hkv, Sq, Sk, D, seed, sinks, layout)
+    okw = dict(kw)
+    if kw.get("cu_seqlens") is not None:
+        kw["cu_seqlens"] = torch.tensor(kw["cu_seqlens"], dtype=torch.int32, device=dev)
+    if kw.get("kv_range") is not None:
+        kw["kv_range"] = torch.tensor(kw["kv_range"], dtype=torch.int32, device=dev)
+    ref = oa.attention(q, k, v, s, dout=do if train else None, bounds=True, **okw)
+    if not train:
+        with torch.no_grad():
+            out = sink_attention(q, k, v, s, **kw)
+        _close(out, ref["out"], ref["out_tol"], "out")
+        return
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, s) if t is not None]
+    out = sink_attention(*(leaves if s is not None else leaves + [None]), **kw)
+    _close(out, ref["out"], ref["out_tol"], "out")
+    for n, g in zip(("dq", "dk", "dv", "dsinks"), torch.autograd.grad(out, leaves, do)):
+        _close(g, ref[n], ref[n + "_tol"], n)
+
+
+# one key tile, its edges, several row and key tiles; one token to some hundred
+@pytest.mark.parametrize("S", [1, 2, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 255, 300])
+def test_lengths(dev, S):
+    _check(dev, 1, 8, 1, S, S, 64, seed=S)
+
+
+@pytest.mark.parametrize("window,first", [(1, 0), (2, 0), (31, 0), (64, 0), (65, 3), (128, 0), (128, 64), (128, 65),
+                                          (10, 200), (299, 0), (300, 7), (1000, 1)])
+def test_windows(dev, window, first):
+    _check(dev, 1, 8, 2, 300, 300, 64, window=window, first=first, seed=window)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(1, 1), (3, 3), (2, 1), (10, 2), (7, 1), (16, 2), (64, 8), (64, 1), (128, 1), (100, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_head_layouts(dev, Hq, Hkv, D):
+    _check(dev, 1, Hq, Hkv, 70, 70, D, window=40, seed=Hq)
+
+
+@pytest.mark.parametrize("layout", ["token", "head", "fused", "odd"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_storage(dev, layout, D):
+    _check(dev, 2, 8, 2, 130, 130, D, layout=layout, window=50, first=2)
+
+
+@pytest.mark.parametrize("sinks", [None, torch.float32, torch.bfloat16])
+def test_sinks(dev, sinks):
+    _check(dev, 2, 6, 3, 90, 90, 64, sinks=sinks)
+
+
+@pytest.mark.parametrize("cu", [[0, 200], [0, 1, 2, 3, 200], [0, 0, 77, 77, 200, 200], [0, 64, 128, 192, 200],
+                                [5, 60, 150], [0, 190], [200, 200], [0], [30, 31]])
+@pytest.mark.parametrize("window,first", [(0, 0), (20, 0), (20, 9)])
+def test_packed(dev, cu, window, first):
+    _check(dev, 1, 8, 2, 200, 200, 64, cu_seqlens=cu, window=window, first=first)
+
+
+def test_packed_many_short_sequences(dev):
+    g = torch.Generator().manual_seed(5)
+    cuts = sorted(torch.randint(0, 700, (90,), generator=g).tolist())
+    _check(dev, 1, 4, 2, 700, 700, 64, cu_seqlens=[0] + cuts + [700])
+    _check(dev, 1, 4, 4, 700, 700, 128, cu_seqlens=[0] + cuts + [700], window=30, first=2)
+
+
+@pytest.mark.parametrize("rng", [[(0, 100), (0, 37), (0, 0)], [(0, 100), (63, 100), (100, 100)],
+                                 [(10, 90), (64, 65), (-5, 400)]])
+@pytest.mark.parametrize("window,first", [(0, 0), (24, 0), (24, 5)])
+def test_padded_batches(dev, rng, window, first):
+    _check(dev, 3, 8, 1, 100, 100, 64, kv_range=rng, window=window, first=first)
+
+
+@pytest.mark.parametrize("Sq,Sk", [(1, 1), (1, 50), (1, 257), (3, 1000), (9, 2100), (17, 300), (5, 2), (40, 0), (130, 700)])
+@pytest.mark.parametrize("window,first", [(0, 0), (100, 0), (100, 70)])
+def test_few_queries_over_a_cache(dev, Sq, Sk, window, first):
+    _check(dev, 2, 16, 2, Sq, Sk, 64, train=False, window=window, first=first)
+    if Sk <= 1000:
+        _check(dev, 2, 16, 2, Sq, Sk, 64, window=window, first=first)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_token_over_long_caches(dev, D):
+    _check(dev, 3, 8, 2, 1, 5000, D, train=False, kv_range=[(0, 5000), (4000, 5000), (4999, 5000)])
+    _check(dev, 1, 64, 8, 1, 9001, D, train=False)
+    _check(dev, 1, 64, 8, 2, 3001, D, window=2500, first=4, sinks=None)
+
+
+def test_nothing_visible(dev):
+    from agent_factory_3_amd.attention import sink_attention
+    for sinks in (None, torch.bfloat16):
+        q, k, v, s, do = _make(dev, 2, 4, 2, 20, 20, 64, sinks=sinks)
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        out = sink_attention(q, k, v, s, kv_range=torch.zeros(2, 2, dtype=torch.int64, device=dev))
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        assert all((t == 0).all() for t in (out, *grads))
+    # no tokens at all
+    q, k, v, s, do = _make(dev, 2, 4, 2, 0, 0, 64)
+    q, s = q.detach().requires_grad_(), s.requires_grad_()
+    out = sink_attention(q, k, v, s)
+    dq, ds = torch.autograd.grad(out, (q, s), do)
+    assert out.shape == (2, 0, 4, 64) and dq.shape == q.shape and (ds == 0).all()
+
+
+def test_garbage_outside_the_range_has_no_influence(dev):
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 2, 8, 2, 100, 100, 64)
+    rng = torch.tensor([[0, 61], [30, 100]], dtype=torch.int32, device=dev)
+    res = []
+    for bad in (0.0, math.nan, math.inf, float(torch.finfo(torch.bfloat16).min)):
+        k2, v2 = k.clone(), v.clone()
+        for b, (lo, hi) in enumerate(rng.tolist()):
+            for t in (k2, v2):
+                t[b, :, :lo] = bad
+                t[b, :, hi:] = bad
+        leaves = [t.detach().requires_grad_() for t in (q, k2, v2, s)]
+        out = sink_attention(*leaves, window=20, kv_range=rng)
+        res.append([out.detach(), *torch.autograd.grad(out, leaves, do)])
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, res[0]))
+    assert all(torch.isfinite(t).all() for t in res[0])
+
+
+def test_large_scores_and_lowest_values(dev):
+    """Scores far beyond the exponential's range, and a sink of -inf or a very large one."""
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 1, 4, 2, 150, 150, 64)
+    s = torch.tensor([-math.inf, 200.0, -1e30, 0.0], device=dev)
+    q = (q.float() * 60).to(torch.bfloat16)
+    ref = oa.attention(q, k, v, s, window=64, bounds=True)
+    _close(sink_attention(q, k, v, s, window=64), ref["out"], ref["out_tol"], "out")
+
+
+def test_same_bits_each_time_and_on_another_stream(dev):
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 1, 16, 2, 333, 333, 64)
+
+    def go():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, s)]
+        out = sink_attention(*leaves, window=100, first=3)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    a = go()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = go()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_captured_and_replayed(dev):
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, _ = _make(dev, 2, 16, 2, 1, 3000, 64)
+    rng = torch.tensor([[0, 3000], [7, 3000]], dtype=torch.int32, device=dev)
+    with torch.no_grad():
+        want0 = sink_attention(q, k, v, s, kv_range=rng)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = sink_attention(q, k, v, s, kv_range=rng)
+        for n in range(3):
+            if n:
+                q.copy_(torch.randn(q.shape, device=dev))
+                rng.copy_(torch.tensor([[n, 3000], [100 * n, 3000]], dtype=torch.int32))
+            want = sink_attention(q, k, v, s, kv_range=rng)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            assert n or torch.equal(want, want0)
+
+
+def test_expanded_gradient_and_broadcast_inputs(dev):
+    """The gradient of a sum arrives with stride 0; keys shared by the batch are one tensor, their gradient a sum."""
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, _ = _make(dev, 3, 4, 2, 50, 50, 64)
+    kl = k[:1].detach().requires_grad_()
+    out = sink_attention(q, kl.expand(3, -1, -1, -1), v, s)
+    (g,) = torch.autograd.grad(out.sum(), kl)
+    ref = oa.attention(q, k[:1].expand(3, -1, -1, -1), v, s, dout=torch.ones_like(out), bounds=True)
+    # torch sums the three batch rows' bf16 gradients
+    tol = ref["dk_tol"].sum(0, keepdim=True) + 2 * oa.U * ref["dk"].abs().sum(0, keepdim=True)
+    _close(g, ref["dk"].sum(0, keepdim=True), tol, "dk")
+
+
+def test_refusals(dev):
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, _ = _make(dev, 2, 4, 2, 8, 8, 64)
+    cu = torch.tensor([0, 8], dtype=torch.int32, device=dev)
+    rng = torch.tensor([[0, 8], [0, 8]], dtype=torch.int32, device=dev)
+    for exc, args, kw in [
+            (TypeError, (q.float(), k, v), {}), (TypeError, (q, k.half(), v), {}),
+            (ValueError, (q[0], k, v), {}), (ValueError, (q, k[:1], v[:1]), {}), (ValueError, (q, k, v[:, :, :4]), {}),
+            (ValueError, (q[:, :3], k, v), {}), (ValueError, (q[..., :32], k[..., :32], v[..., :32]), {}),
+            (ValueError, (q, k[:, :0], v[:, :0]), {}),
+            (ValueError, (q, k, v, s[:3]), {}), (ValueError, (q, k, v, s.half()), {}),
+            (ValueError, (q, k, v, s.cpu()), {}), (RuntimeError, (q.cpu(), k, v), {}),
+            (ValueError, (q, k, v), dict(window=-1)), (ValueError, (q, k, v), dict(first=-1)),
+            (ValueError, (q, k, v), dict(scale=0.0)), (ValueError, (q, k, v), dict(scale=math.nan)),
+            (ValueError, (q, k, v), dict(scale=-1.0)), (ValueError, (q, k, v), dict(cu_seqlens=cu)),
+            (ValueError, (q[:1], k[:1], v[:1]), dict(cu_seqlens=cu, kv_range=rng[:1])),
+            (ValueError, (q[:1, :, :3], k[:1], v[:1]), dict(cu_seqlens=cu)),
+            (ValueError, (q[:1], k[:1], v[:1]), dict(cu_seqlens=cu.cpu())),
+            (ValueError, (q[:1], k[:1], v[:1]), dict(cu_seqlens=cu.float())),
+            (ValueError, (q, k, v), dict(kv_range=rng[:1])), (ValueError, (q, k, v), dict(kv_range=rng.float())),
+            (ValueError, (q, k, v), dict(kv_range=rng.cpu()))]:
+        with pytest.raises(exc):
+            sink_attention(*args, **kw)
+
+
+def test_unordered_lengths_stay_in_bounds(dev):
+    """Cumulative lengths that decrease or leave the row give some finite answer and touch nothing else."""
+    from agent_factory_3_amd.attention import sequence_starts, sink_attention
+    q, k, v, s, do = _make(dev, 1, 4, 2, 200, 200, 64)
+    t = torch.arange(200)
+    for cu in ([150, 20, 90], [-40, 500], [0, 1000, -1000, 7]):
+        cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+        st = sequence_starts(cu, 200).cpu()
+        assert (st >= 0).all() and (st <= t + 1).all()
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, s)]
+        out = sink_attention(*leaves, cu_seqlens=cu, window=30, first=4)
+        assert all(torch.isfinite(x).all() for x in (out, *torch.autograd.grad(out, leaves, do)))
+
+
+@pytest.mark.parametrize("lens", [[1], [5, 3], [700, 1, 1, 324], [1500] * 3])
+def test_starts_of_positions(dev, lens):
+    from agent_factory_3_amd.attention import sequence_starts, sequence_starts_of_positions
+    pos = torch.cat([torch.arange(n) for n in lens]).to(dev)
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), device=dev)
+    want = oa.starts_of(cu.tolist(), pos.numel()).to(torch.int32)
+    assert torch.equal(sequence_starts_of_positions(pos[None]).cpu(), want)
+    assert torch.equal(sequence_starts(cu, pos.numel()).cpu(), want)
