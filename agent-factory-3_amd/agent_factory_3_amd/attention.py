@@ -48,22 +48,23 @@ class _SinkAttention(torch.autograd.Function):
         Hkv, Sk = k.shape[1], k.shape[2]
         dev = q.device
         out = torch.empty(B, Sq, Hq, D, dtype=torch.bfloat16, device=dev)
+        out_lo = torch.empty_like(out) if need_grad else None
         lse = torch.empty(B, Hq, Sq, dtype=torch.float32, device=dev) if need_grad else None
         ws_n = int(_capi.load().af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first))
         ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
         _capi.call("af3_sink_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
                    _capi.ptr(sinks), int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
-                   _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), _capi.ptr(lse),
-                   _capi.ptr(ws), ws_n, _capi.stream_of(dev))
+                   _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), _capi.ptr(out_lo),
+                   _capi.ptr(lse), _capi.ptr(ws), ws_n, _capi.stream_of(dev))
         if need_grad:
-            ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, lse)
+            ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, out_lo, lse)
             ctx.args = (scale, window, first)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, sinks, starts, kv_range, out, lse = ctx.saved_tensors
+        q, k, v, sinks, starts, kv_range, out, out_lo, lse = ctx.saved_tensors
         scale, window, first = ctx.args
         B, Hq, Sq, D = q.shape
         Hkv, Sk = k.shape[1], k.shape[2]
@@ -80,7 +81,7 @@ class _SinkAttention(torch.autograd.Function):
                        _strides(q, k, v, do), _capi.ptr(sinks),
                        int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
                        _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(),
-                       lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _capi.ptr(dsinks), ws.data_ptr(),
+                       out_lo.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _capi.ptr(dsinks), ws.data_ptr(),
                        ws_n, _capi.stream_of(dev))
         return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dsinks, *[None] * 6
 

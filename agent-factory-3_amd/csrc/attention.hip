@@ -51,7 +51,7 @@ struct SaParams {
   int tok;                                // tokens of a row tile
   int n_tiles, n_split;
   float scale, scale2;                    // scale2 = scale log2(e)
-  uint16_t* out;                          // [B][Sq][Hq][D]
+  uint16_t *out, *out_lo;                 // [B][Sq][Hq][D]; out_lo: what rounding out left, or NULL
   float* lse;                             // [B][Hkv][Sq][G], log2 units; or NULL
   float* part;                            // n_split > 1: [n_split][B][Hkv][Sq][G][D] then (m, l) pairs
   // backward
@@ -188,7 +188,7 @@ __device__ __forceinline__ void a_load_tile(const uint16_t* base, int64_t st, in
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void sa_fwd_kernel(SaParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kBN * D * 2;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
@@ -325,13 +325,21 @@ __global__ __launch_bounds__(256) void sa_fwd_kernel(SaParams p) {
     return;
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
-  uint16_t* orow = p.out + (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
+  const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *(u32x2*)(orow + d * 32 + 2 * r + 4 * lh) = u32x2{af3_pack_bf16x2(o[d][r] * inv, o[d][r + 1] * inv),
-                                                        af3_pack_bf16x2(o[d][r + 2] * inv, o[d][r + 3] * inv)};
+    for (int r = 0; r < 16; r += 4) {
+      u32x2 w, e;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float y0 = o[d][r + 2 * x] * inv, y1 = o[d][r + 2 * x + 1] * inv;
+        w[x] = af3_pack_bf16x2(y0, y1);
+        e[x] = af3_pack_bf16x2(y0 - af3_bf16_to_f32(w[x] & 0xFFFFu), y1 - af3_bf16_to_f32(w[x] >> 16));
+      }
+      *(u32x2*)(p.out + orow + d * 32 + 2 * r + 4 * lh) = w;
+      if (p.out_lo) *(u32x2*)(p.out_lo + orow + d * 32 + 2 * r + 4 * lh) = e;
+    }
   if (p.lse && lh == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -358,9 +366,14 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
   const int64_t u = prow / p.G;
   const int t = (int)(u % p.Sq);
   const int bh = (int)(u / p.Sq), b = bh / p.Hkv, hk = bh % p.Hkv;
-  uint16_t* orow = p.out + (((int64_t)b * p.Sq + t) * p.Hq + hk * p.G + g) * D;
+  const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + hk * p.G + g) * D;
 #pragma unroll
-  for (int d = 0; d < D / 64; ++d) orow[d * 64 + lane] = (uint16_t)af3_f32_to_bf16(o[d] * inv);
+  for (int d = 0; d < D / 64; ++d) {
+    const float y = o[d] * inv;
+    const uint32_t w = af3_f32_to_bf16(y);
+    p.out[orow + d * 64 + lane] = (uint16_t)w;
+    if (p.out_lo) p.out_lo[orow + d * 64 + lane] = (uint16_t)af3_f32_to_bf16(y - af3_bf16_to_f32(w));
+  }
   if (p.lse && lane == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -369,7 +382,7 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
 // tiles and layouts; p comes back from the saved log-sum.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ __launch_bounds__(256) void sa_dq_kernel(SaParams p) {
+__global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kBN * D * 2;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
@@ -414,14 +427,15 @@ __global__ __launch_bounds__(256) void sa_dq_kernel(SaParams p) {
   {
     const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
     const uint16_t* dr = p.dout + b * p.do_sb + head * p.do_sh + t * p.do_st;
-    const uint16_t* orow = p.out + (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
+    const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
       df[s] = *(const af3_bf16x8*)(dr + s * 16 + lh * 8);
-      const af3_bf16x8 of = *(const af3_bf16x8*)(orow + s * 16 + lh * 8);
+      const af3_bf16x8 of = *(const af3_bf16x8*)(p.out + orow + s * 16 + lh * 8);
+      const af3_bf16x8 oe = *(const af3_bf16x8*)(p.out_lo + orow + s * 16 + lh * 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[i], delta);
+      for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[i] + (float)oe[i], delta);
     }
     delta += a_xhalf(delta);
   }
@@ -455,7 +469,9 @@ __global__ __launch_bounds__(256) void sa_dq_kernel(SaParams p) {
                        (p.window <= 0 || j0 > wt1 + off - p.window);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      af3_f32x16 s = a_zero(), dp = a_zero();
+      af3_f32x16 s = a_zero(), dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = -delta;
 #pragma unroll
       for (int x = 0; x < KS; ++x) s = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s);
 #pragma unroll
@@ -466,12 +482,12 @@ __global__ __launch_bounds__(256) void sa_dq_kernel(SaParams p) {
           const int j = j0 + c * 32 + 8 * (r / 4) + 4 * lh + r % 4;
           const bool on = j < end && vis(j);
           s[r] = on ? s[r] : -INFINITY;
-          dp[r] = on ? dp[r] : delta;
+          dp[r] = on ? dp[r] : 0.f;
         }
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse)) * (dp[r] - delta);
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse)) * dp[r];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const af3_bf16x8 pf = a_pack8(s, u);
@@ -513,14 +529,18 @@ __global__ __launch_bounds__(256) void sa_dsink_kernel(const float* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// backward, keys: dk and dv.  Block = 4 waves of 32 keys of one key/value head,
-// K and V rows in registers; the (token, head) rows that see them go through a
-// two-stage LDS ring, 64 at a time (q, dout, and their lse, delta, position and
-// sequence start).  S = Q K^T puts a key's column into its lane; the sum over
-// the heads that share the key is the sum over rows.
+// backward, keys: dk and dv.  Block = 128 keys of one key/value head, K and V
+// rows in registers; the (token, head) rows that see them go through a
+// two-stage LDS ring, 128 at a time (q, dout, and their lse, delta, position and
+// sequence start).  Waves 0-3 (32 keys each) take the first 64 rows of a step,
+// waves 4-7 the others, and their sums are joined at the end: two waves per
+// SIMD, so that one's exponentials run beside the other's products, and half
+// the steps for the first keys, which every later row sees.  S = Q K^T puts a
+// key's column into its lane; the sum over the heads that share the key is the
+// sum over rows.
 // ---------------------------------------------------------------------------
 constexpr int kKeys = 128;  // keys of a block
-constexpr int kRT = 64;     // rows of a step
+constexpr int kRT = 128;    // rows of a step
 
 // first token after t0 whose sequence starts later than t0's (starts does not
 // decrease), or n: 64 probes a round, the answer stays in (lo, hi]
@@ -538,9 +558,10 @@ __device__ __forceinline__ int a_sequence_end(const int32_t* starts, int t0, int
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void sa_dkv_kernel(SaParams p) {
+__global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kRT * D * 2;
+  constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / 8;  // chunks per row, rows per copy, copies per wave
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
   __shared__ __attribute__((aligned(16))) float st_lse[2][kRT], st_delta[2][kRT];
   __shared__ __attribute__((aligned(16))) int st_pos[2][kRT], st_lo[2][kRT];
@@ -549,25 +570,28 @@ __global__ __launch_bounds__(256) void sa_dkv_kernel(SaParams p) {
   const int b = bh / p.Hkv, hk = bh % p.Hkv;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = wave >> 2;  // rows 64 half .. + 63 of a step
   const int lr = lane & 31, lh = lane >> 5;
   const int off = p.Sk - p.Sq;
   int lo, hi;
   a_kv_range(p, b, lo, hi);
   const int jl = min(j0 + kKeys, p.Sk) - 1;  // last key of the block
-  const int j = j0 + wave * 32 + lr;
+  const int jw = j0 + (wave & 3) * 32;       // first key of the wave
+  const int j = jw + lr;
   const bool kvalid = j <= jl;
 
   // tokens that may see a key of the block
-  int ta = max(0, max(j0, lo) - off), tb = p.Sq;  // [ta, tb)
-  int s_last = lo;
+  const int ta = max(0, max(j0, lo) - off);  // [ta, tb)
+  int tb = p.Sq, s_last = lo;
   if (p.starts) {
     s_last = p.starts[jl];
     tb = a_sequence_end(p.starts, jl, p.Sk, lane);
   }
-  if (p.window > 0 && s_last + p.first <= max(j0, lo)) tb = min(tb, jl + p.window - off);
-  if (jl < lo || j0 >= hi) tb = ta;
-  const int64_t ra = (int64_t)ta * p.G, rb = (int64_t)max(tb, ta) * p.G;  // their rows
-  const int n_steps = (int)((rb - ra + kRT - 1) / kRT);
+  // (the last key's sequence may have first tokens in the block; an earlier one ends in it)
+  if (p.window > 0 && (p.first == 0 || s_last + p.first <= j0)) tb = min(tb, jl + p.window - off);
+  tb = jl < lo || j0 >= hi ? ta : max(ta, min(tb, p.Sq));
+  const int64_t n_rows = (int64_t)(tb - ta) * p.G;
+  const int n_steps = (int)((n_rows + kRT - 1) / kRT);
 
   af3_bf16x8 kf[KS], vf[KS];
   {
@@ -581,39 +605,53 @@ __global__ __launch_bounds__(256) void sa_dkv_kernel(SaParams p) {
     }
   }
   const bool jin = kvalid && j >= lo && j < hi;
-  const int fl_key = j - p.first;  // the key is a first token of sequences that start after fl_key
+  const bool wave_in = jw >= lo && jw + 31 < hi && jw + 31 <= jl;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
   const uint16_t* qb = p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
   const uint16_t* db = p.dout + b * p.do_sb + (int64_t)hk * p.G * p.do_sh;
-  const int64_t sb = ((int64_t)b * p.Hkv + hk) * p.Sq * p.G;
+  const int64_t sb = ((int64_t)b * p.Hkv + hk) * p.Sq * p.G + (int64_t)ta * p.G;
+  // (token, head) of the thread's rows, kept from step to step (no division)
+  const int adv_t = kRT / p.G, adv_g = kRT % p.G;
+  int ct[N], cg[N], rt, rg;
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    const int row = (wave * N + x) * RPI + lane / CH;
+    ct[x] = ta + row / p.G;
+    cg[x] = row % p.G;
+  }
+  rt = ta + (int)threadIdx.x / p.G;
+  rg = (int)threadIdx.x % p.G;
   float v_lse = 0.f, v_delta = 0.f;
   int v_pos = 0, v_lo = 0;
-  auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..63
-    const int64_t r0 = ra + (int64_t)i * kRT;
+  auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..127
     const uint32_t st = lds0 + (uint32_t)((i & 1) * 2 * kTile);
-    constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / 4;
 #pragma unroll
     for (int x = 0; x < N; ++x) {
       const int row = (wave * N + x) * RPI + lane / CH;
-      const int64_t r = min(r0 + row, rb - 1);
-      const int64_t t = r / p.G, g = r % p.G;
+      const int64_t t = min(ct[x], tb - 1), g = cg[x];
       const int col = ((lane % CH) ^ a_swz(row)) << 3;
       a_dma16(qb + t * p.q_st + g * p.q_sh + col, st + (uint32_t)((wave * N + x) * 1024));
       a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + (uint32_t)((wave * N + x) * 1024));
+      ct[x] += adv_t;
+      cg[x] += adv_g;
+      if (cg[x] >= p.G) cg[x] -= p.G, ++ct[x];
     }
     if (threadIdx.x < kRT) {
-      const int64_t r = min(r0 + threadIdx.x, rb - 1);
-      const int t = (int)(r / p.G);
+      const bool in = rt < tb;
+      const int64_t r = min((int64_t)i * kRT + threadIdx.x, n_rows - 1);
       v_lse = p.lse[sb + r];
       v_delta = p.delta[sb + r];
-      v_pos = r0 + threadIdx.x < rb ? t + off : -kMaxLen;  // sees nothing
-      v_lo = p.starts ? p.starts[t] : lo;
+      v_pos = in ? rt + off : -kMaxLen;  // sees nothing
+      v_lo = p.starts ? p.starts[min(rt, tb - 1)] : lo;
+      rt += adv_t;
+      rg += adv_g;
+      if (rg >= p.G) rg -= p.G, ++rt;
     }
   };
   auto store_rows = [&](int i) {
     if (threadIdx.x < kRT) {
       st_lse[i & 1][threadIdx.x] = v_lse;
-      st_delta[i & 1][threadIdx.x] = v_delta;
+      st_delta[i & 1][threadIdx.x] = -v_delta;
       st_pos[i & 1][threadIdx.x] = v_pos;
       st_lo[i & 1][threadIdx.x] = v_lo;
     }
@@ -628,35 +666,54 @@ __global__ __launch_bounds__(256) void sa_dkv_kernel(SaParams p) {
     store_rows(i);
     A_BARRIER();
     if (i + 1 < n_steps) issue(i + 1);
-    const uint8_t* qt = lds + (i & 1) * 2 * kTile;
+    const uint8_t* qt = lds + (i & 1) * 2 * kTile + half * (kTile / 2);
     const uint8_t* dt = qt + kTile;
-    const int w = i & 1;
+    const int w = i & 1, rb = half * 64;
+    // positions and starts do not decrease over the valid rows, which come first
+    const int pos0 = __builtin_amdgcn_readfirstlane(st_pos[w][rb]);
+    const int pos1 = __builtin_amdgcn_readfirstlane(st_pos[w][rb + 63]);
+    const int lo1 = __builtin_amdgcn_readfirstlane(st_lo[w][rb + 63]);
+    const bool full = pos1 >= 0;  // the last row is valid
+    if (pos0 < 0 || (full && jw > pos1)) continue;  // the wave's keys are seen by none of the rows
+    if (p.window > 0 && p.first == 0 && jw + 31 <= pos0 - p.window) continue;
+    const bool whole = full && wave_in && jw + 31 <= pos0 && jw >= lo1 && (p.window <= 0 || jw > pos1 - p.window);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      af3_f32x16 s = a_zero(), dp = a_zero();
+      af3_f32x16 s = a_zero(), dp;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // dp starts at -delta
+        const float4 de = *(const float4*)&st_delta[w][rb + c * 32 + 8 * q + 4 * lh];
+        dp[4 * q] = de.x; dp[4 * q + 1] = de.y; dp[4 * q + 2] = de.z; dp[4 * q + 3] = de.w;
+      }
 #pragma unroll
       for (int x = 0; x < KS; ++x) s = a_mfma(a_row8<D>(qt, c * 32 + lr, x, lh), kf[x], s);
 #pragma unroll
       for (int x = 0; x < KS; ++x) dp = a_mfma(a_row8<D>(dt, c * 32 + lr, x, lh), vf[x], dp);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int r4 = c * 32 + 8 * q + 4 * lh;
-        const float4 ls = *(const float4*)&st_lse[w][r4];
-        const float4 de = *(const float4*)&st_delta[w][r4];
-        const int4 po = *(const int4*)&st_pos[w][r4];
-        const int4 rl = *(const int4*)&st_lo[w][r4];
-        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
-        const int pov[4] = {po.x, po.y, po.z, po.w}, rlv[4] = {rl.x, rl.y, rl.z, rl.w};
+        const float4 ls = *(const float4*)&st_lse[w][rb + c * 32 + 8 * q + 4 * lh];
+        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int r = 4 * q + y;
-          const bool on = jin && j <= pov[y] && j >= rlv[y] &&
-                          (p.window <= 0 || j > pov[y] - p.window || fl_key < rlv[y]);
-          const float pr = on ? __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lsv[y])) : 0.f;
-          s[r] = pr;
-          dp[r] = on ? pr * (dp[r] - dev[y]) : 0.f;
+        for (int y = 0; y < 4; ++y) s[4 * q + y] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + y], p.scale2, -lsv[y]));
+      }
+      if (!whole) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int4 po = *(const int4*)&st_pos[w][rb + c * 32 + 8 * q + 4 * lh];
+          const int4 rl = *(const int4*)&st_lo[w][rb + c * 32 + 8 * q + 4 * lh];
+          const int pov[4] = {po.x, po.y, po.z, po.w}, rlv[4] = {rl.x, rl.y, rl.z, rl.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int r = 4 * q + y;
+            const bool on = jin && j <= pov[y] && j >= rlv[y] &&
+                            (p.window <= 0 || j > pov[y] - p.window || j < rlv[y] + p.first);
+            s[r] = on ? s[r] : 0.f;
+            dp[r] = on ? dp[r] : 0.f;
+          }
         }
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] *= s[r];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const af3_bf16x8 pf = a_pack8(s, u), sf = a_pack8(dp, u);
@@ -668,16 +725,32 @@ __global__ __launch_bounds__(256) void sa_dkv_kernel(SaParams p) {
       }
     }
   }
-  if (!kvalid) return;
+  // waves 4-7 hand their sums to waves 0-3 through the ring's LDS
+  A_BARRIER();
+  float* sum = (float*)lds + ((wave & 3) * 64 + lane) * 4;  // four values of a lane, then the next four 4 KB on
+  if (half) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        *(float4*)(sum + (d * 8 + r / 4) * 1024) = float4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+        *(float4*)(sum + (d * 8 + 4 + r / 4) * 1024) = float4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+      }
+  }
+  A_BARRIER();
+  if (half || !kvalid) return;
   const int64_t o = (((int64_t)b * p.Sk + j) * p.Hkv + hk) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
+      const float4 k4 = *(const float4*)(sum + (d * 8 + r / 4) * 1024);
+      const float4 v4 = *(const float4*)(sum + (d * 8 + 4 + r / 4) * 1024);
       const int64_t c = o + d * 32 + 2 * r + 4 * lh;
-      *(u32x2*)(p.dv + c) = u32x2{af3_pack_bf16x2(dv[d][r], dv[d][r + 1]), af3_pack_bf16x2(dv[d][r + 2], dv[d][r + 3])};
-      *(u32x2*)(p.dk + c) = u32x2{af3_pack_bf16x2(dk[d][r] * p.scale, dk[d][r + 1] * p.scale),
-                                  af3_pack_bf16x2(dk[d][r + 2] * p.scale, dk[d][r + 3] * p.scale)};
+      *(u32x2*)(p.dv + c) = u32x2{af3_pack_bf16x2(dv[d][r] + v4.x, dv[d][r + 1] + v4.y),
+                                  af3_pack_bf16x2(dv[d][r + 2] + v4.z, dv[d][r + 3] + v4.w)};
+      *(u32x2*)(p.dk + c) = u32x2{af3_pack_bf16x2((dk[d][r] + k4.x) * p.scale, (dk[d][r + 1] + k4.y) * p.scale),
+                                  af3_pack_bf16x2((dk[d][r + 2] + k4.z) * p.scale, (dk[d][r + 3] + k4.w) * p.scale)};
     }
 }
 
@@ -818,16 +891,19 @@ extern "C" size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int
 extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
                                       const void* sinks, int sinks_f32, const int32_t* starts, const int32_t* kv_range,
                                       int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first, float scale,
-                                      uint16_t* out, float* lse, void* workspace, size_t ws_bytes, void* stream_) {
+                                      uint16_t* out, uint16_t* out_lo, float* lse, void* workspace, size_t ws_bytes,
+                                      void* stream_) {
   const char* who = "sink_attention_fwd";
   if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 9, starts, kv_range)) return rc;
   if (B == 0 || Sq == 0) return 0;
   AF3_REQUIRE(q && out && (Sk == 0 || (k && v)), "%s: null pointer", who);
-  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(out), "%s: rows must be 16-byte aligned", who);
+  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(out) && sa_al16(out_lo),
+              "%s: rows must be 16-byte aligned", who);
   hipStream_t stream = (hipStream_t)stream_;
   const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
   SaParams p = sa_params(s, q, k, v, strides, sinks, sinks_f32, starts, kv_range, B, Hq, Hkv, Sq, Sk, scale);
   p.out = out;
+  p.out_lo = out_lo;
   p.lse = lse;
   p.n_split = s.n_split;
   const int64_t grid = (int64_t)s.n_tiles * B * Hkv * s.n_split;
@@ -860,16 +936,16 @@ extern "C" size_t af3_sink_attention_bwd_workspace_bytes(int B, int Hq, int Hkv,
 extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* dout,
                                       const int64_t* strides, const void* sinks, int sinks_f32, const int32_t* starts,
                                       const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk, int D,
-                                      int window, int first, float scale, const uint16_t* out, const float* lse,
-                                      uint16_t* dq, uint16_t* dk, uint16_t* dv, void* dsinks, void* workspace,
+                                      int window, int first, float scale, const uint16_t* out, const uint16_t* out_lo,
+                                      const float* lse, uint16_t* dq, uint16_t* dk, uint16_t* dv, void* dsinks, void* workspace,
                                       size_t ws_bytes, void* stream_) {
   const char* who = "sink_attention_bwd";
   if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 12, starts, kv_range)) return rc;
   const bool nq = B > 0 && Sq > 0, nk = B > 0 && Sk > 0;
-  AF3_REQUIRE((!nq || (q && dout && out && lse && dq && workspace)) && (!nk || (k && v && dk && dv)) &&
+  AF3_REQUIRE((!nq || (q && dout && out && out_lo && lse && dq && workspace)) && (!nk || (k && v && dk && dv)) &&
                   (!sinks || dsinks),
               "%s: null pointer", who);
-  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(dout) && sa_al16(out) && sa_al16(dq) && sa_al16(dk) &&
+  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(dout) && sa_al16(out) && sa_al16(out_lo) && sa_al16(dq) && sa_al16(dk) &&
                   sa_al16(dv) && sa_al16(workspace),
               "%s: rows must be 16-byte aligned", who);
   AF3_REQUIRE(ws_bytes >= af3_sink_attention_bwd_workspace_bytes(B, Hq, Hkv, Sq), "%s: workspace too small", who);
@@ -879,6 +955,7 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
   p.dout = dout;
   p.do_sb = strides[9]; p.do_sh = strides[10]; p.do_st = strides[11];
   p.out = (uint16_t*)out;
+  p.out_lo = (uint16_t*)out_lo;
   p.lse = (float*)lse;
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = (float*)workspace;
@@ -895,9 +972,9 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
                        dsinks);
   if (gk) {
     if (D == 64)
-      hipLaunchKernelGGL(sa_dkv_kernel<64>, dim3(gk), dim3(256), 0, stream, p);
+      hipLaunchKernelGGL(sa_dkv_kernel<64>, dim3(gk), dim3(512), 0, stream, p);
     else
-      hipLaunchKernelGGL(sa_dkv_kernel<128>, dim3(gk), dim3(256), 0, stream, p);
+      hipLaunchKernelGGL(sa_dkv_kernel<128>, dim3(gk), dim3(512), 0, stream, p);
   }
   return af3::check_launch(who);
 }
