@@ -91,6 +91,15 @@ __device__ __forceinline__ af3_bf16x8 a_tr8(const uint8_t* tile, int row0, int c
   return af3_bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
+// The loads of these operands end here.  Left to their first use in the loop, the
+// compiler's wait for them would stand there in every step and wait for the
+// step's copies to LDS too, which it does not know of.
+template <int N>
+__device__ __forceinline__ void a_landed(af3_bf16x8 (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 template <int D>
 __device__ __forceinline__ af3_bf16x8 a_row8(const uint8_t* tile, int row, int ks, int h) {
   return *(const af3_bf16x8*)(tile + a_off<D>(row, 2 * ks + h));
@@ -132,19 +141,41 @@ __device__ __forceinline__ void a_kv_range(const SaParams& p, int b, int& lo, in
   }
 }
 
-// What a row sees: j in [lo, hi], and j >= wl or j < fl
+// What a row sees, as two runs of keys: wn keys from w (the window, or all) and
+// fn keys from lo (the kept first tokens)
 struct Vis {
-  int lo, hi, wl, fl;
-  __device__ __forceinline__ bool operator()(int j) const { return j >= lo && j <= hi && (j >= wl || j < fl); }
+  int w, wn, lo, fn;
 };
 
 __device__ __forceinline__ Vis a_vis(const SaParams& p, int pos, int lo, int hi) {
+  const int end = min(pos + 1, hi);
   Vis v;
   v.lo = lo;
-  v.hi = min(pos, hi - 1);
-  v.wl = p.window > 0 ? pos - p.window + 1 : lo;
-  v.fl = lo + p.first;
+  v.w = p.window > 0 ? max(lo, pos - p.window + 1) : lo;
+  v.wn = max(0, end - v.w);
+  v.fn = max(0, min(p.first, end - lo));
   return v;
+}
+
+// scores outside [lo, lo + n) to `off` (register r: key j + 8 (r / 4) + r % 4)
+template <int N>
+__device__ __forceinline__ void a_mask(af3_f32x16 (&s)[N], int j, int lo, int n, float off) {
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      s[c][r] = (uint32_t)(j - lo + c * 32 + 8 * (r / 4) + r % 4) < (uint32_t)n ? s[c][r] : off;
+}
+// ... outside both runs
+template <int N>
+__device__ __forceinline__ void a_mask2(af3_f32x16 (&s)[N], int j, const Vis& v, float off) {
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int x = j + c * 32 + 8 * (r / 4) + r % 4;
+      s[c][r] = (uint32_t)(x - v.w) < (uint32_t)v.wn || (uint32_t)(x - v.lo) < (uint32_t)v.fn ? s[c][r] : off;
+    }
 }
 
 // The keys a row tile runs over: [a0, a1) are first tokens before the window,
@@ -211,12 +242,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p
   a_kv_range(p, b, lo, hi);
   const int row_lo = p.starts ? p.starts[t] : lo;
   const int tile_lo = p.starts ? p.starts[t0] : lo;
-  const int tile_hi_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start
+  const int tile_hi_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start (the latest)
   const Vis vis = a_vis(p, t + off, row_lo, hi);
   const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
   // the wave's positions, to pass over tiles that none of its rows sees
   const int wt0 = t0 + (wave * 32) / p.G, wt1 = min(t1, t0 + (wave * 32 + 31) / p.G);
+  const int wpos0 = wt0 + off, wpos1 = wt1 + off, wlo1 = tile_hi_lo;
   int i0 = 0, i1 = na + nb;
   if (p.n_split > 1) {
     const int per = (na + nb + p.n_split - 1) / p.n_split;
@@ -229,6 +261,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p
     const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
+    a_landed(qf);
   }
   float m = kLowest, l = 0.f;
   if (p.sinks && split == 0) {
@@ -257,9 +290,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p
     if (i + 1 < i1) issue(i + 1, (i + 1 - i0) & 1);
     const uint8_t* kt = lds + ((i - i0) & 1) * 2 * kTile;
     const uint8_t* vt = kt + kTile;
-    const int j0 = first_key(i), end = i < na ? ks.a1 : ks.b1;
-    if (wt0 > t1 || j0 > wt1 + off) continue;  // nothing for this wave
-    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wt0 + off - p.window) continue;
+    const int j0 = first_key(i);
+    if (wt0 > t1 || j0 > wpos1) continue;  // nothing for this wave
+    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wpos0 - p.window) continue;
 
     af3_f32x16 s[2];
 #pragma unroll
@@ -268,17 +301,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p
 #pragma unroll
       for (int x = 0; x < KS; ++x) s[c] = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s[c]);
     }
-    const bool whole = j0 + kBN <= end && j0 + kBN - 1 <= wt0 + off && j0 >= tile_hi_lo &&
-                       (p.window <= 0 || j0 > wt1 + off - p.window);
-    if (!whole) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + c * 32 + 8 * (r / 4) + 4 * lh + r % 4;
-          s[c][r] = j < end && vis(j) ? s[c][r] : -INFINITY;
-        }
-    }
+    // (a row's runs end before `end`, but for the first tokens of tiles before the window)
+    if (i < na)
+      a_mask(s, j0 + 4 * lh, vis.lo, max(0, min(vis.fn, ks.a1 - vis.lo)), -INFINITY);
+    else if (p.first > 0 && j0 < wlo1 + p.first)
+      a_mask2(s, j0 + 4 * lh, vis, -INFINITY);
+    else if (j0 + kBN - 1 > wpos0 || j0 < wlo1 || j0 + kBN > ks.b1 || (p.window > 0 && j0 <= wpos1 - p.window))
+      a_mask(s, j0 + 4 * lh, vis.w, vis.wn, -INFINITY);
     float mx = s[0][0];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -409,6 +438,7 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
   const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
   const int wt0 = t0 + (wave * 32) / p.G, wt1 = min(t1, t0 + (wave * 32 + 31) / p.G);
+  const int wpos0 = wt0 + off, wpos1 = wt1 + off, wlo1 = tile_hi_lo;
 
   const uint16_t* kb = p.k + b * p.k_sb + hk * p.k_sh;
   const uint16_t* vb = p.v + b * p.v_sb + hk * p.v_sh;
@@ -438,8 +468,11 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
       for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[i] + (float)oe[i], delta);
     }
     delta += a_xhalf(delta);
+    a_landed(qf);
+    a_landed(df);
   }
-  const float lse = p.lse[prow];
+  float lse = p.lse[prow];
+  asm volatile("" : "+v"(lse));  // landed, as the operands
   if (valid && lh == 0) p.delta[prow] = delta;
   if (p.sinks) {
     if (lh == 0) ds_row[row] = valid ? -__builtin_amdgcn_exp2f(a_sink2(p, head) - lse) * delta : 0.f;
@@ -462,35 +495,31 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
     if (i + 1 < na + nb) issue(i + 1, (i + 1) & 1);
     const uint8_t* kt = lds + (i & 1) * 2 * kTile;
     const uint8_t* vt = kt + kTile;
-    const int j0 = first_key(i), end = i < na ? ks.a1 : ks.b1;
-    if (wt0 > t1 || j0 > wt1 + off) continue;
-    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wt0 + off - p.window) continue;
-    const bool whole = j0 + kBN <= end && j0 + kBN - 1 <= wt0 + off && j0 >= tile_hi_lo &&
-                       (p.window <= 0 || j0 > wt1 + off - p.window);
+    const int j0 = first_key(i);
+    if (wt0 > t1 || j0 > wpos1) continue;
+    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wpos0 - p.window) continue;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      af3_f32x16 s = a_zero(), dp;
+      af3_f32x16 s[1] = {a_zero()}, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = -delta;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) s = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s);
+      for (int x = 0; x < KS; ++x) s[0] = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s[0]);
 #pragma unroll
       for (int x = 0; x < KS; ++x) dp = a_mfma(a_row8<D>(vt, c * 32 + lr, x, lh), df[x], dp);
-      if (!whole) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + c * 32 + 8 * (r / 4) + 4 * lh + r % 4;
-          const bool on = j < end && vis(j);
-          s[r] = on ? s[r] : -INFINITY;
-          dp[r] = on ? dp[r] : 0.f;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse)) * dp[r];
+      for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -lse)) * dp[r];
+      // (the product is set to zero, not the score: whatever stands at a key that the row does not see)
+      const int jc = j0 + c * 32 + 4 * lh;
+      if (i < na)
+        a_mask(s, jc, vis.lo, max(0, min(vis.fn, ks.a1 - vis.lo)), 0.f);
+      else if (p.first > 0 && j0 < wlo1 + p.first)
+        a_mask2(s, jc, vis, 0.f);
+      else if (j0 + kBN - 1 > wpos0 || j0 < wlo1 || j0 + kBN > ks.b1 || (p.window > 0 && j0 <= wpos1 - p.window))
+        a_mask(s, jc, vis.w, vis.wn, 0.f);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const af3_bf16x8 pf = a_pack8(s, u);
+        const af3_bf16x8 pf = a_pack8(s[0], u);
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = a_mfma(a_tr8<D>(kt, c * 32 + u * 16, d * 32, lane), pf, acc[d]);
       }
@@ -564,7 +593,7 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
   constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / 8;  // chunks per row, rows per copy, copies per wave
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
   __shared__ __attribute__((aligned(16))) float st_lse[2][kRT], st_delta[2][kRT];
-  __shared__ __attribute__((aligned(16))) int st_pos[2][kRT], st_lo[2][kRT];
+  __shared__ __attribute__((aligned(16))) int st_w[2][kRT], st_wn[2][kRT], st_lo[2][kRT], st_fn[2][kRT];
   const int bh = blockIdx.x % (p.B * p.Hkv);
   const int j0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kKeys;  // the longest columns first
   const int b = bh / p.Hkv, hk = bh % p.Hkv;
@@ -603,8 +632,10 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
       kf[s] = *(const af3_bf16x8*)(kr + s * 16 + lh * 8);
       vf[s] = *(const af3_bf16x8*)(vr + s * 16 + lh * 8);
     }
+    a_landed(kf);
+    a_landed(vf);
   }
-  const bool jin = kvalid && j >= lo && j < hi;
+  const int jm = kvalid && j >= lo && j < hi ? j : 2 * kMaxLen;  // beyond every row's run
   const bool wave_in = jw >= lo && jw + 31 < hi && jw + 31 <= jl;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
   const uint16_t* qb = p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
@@ -621,8 +652,10 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
   }
   rt = ta + (int)threadIdx.x / p.G;
   rg = (int)threadIdx.x % p.G;
+  // tokens of the first and the last row of the wave's half of a step
+  int ut[2] = {ta + half * 64 / p.G, ta + (half * 64 + 63) / p.G}, ug[2] = {half * 64 % p.G, (half * 64 + 63) % p.G};
   float v_lse = 0.f, v_delta = 0.f;
-  int v_pos = 0, v_lo = 0;
+  Vis v_vis = {};
   auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..127
     const uint32_t st = lds0 + (uint32_t)((i & 1) * 2 * kTile);
 #pragma unroll
@@ -637,12 +670,12 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
       if (cg[x] >= p.G) cg[x] -= p.G, ++ct[x];
     }
     if (threadIdx.x < kRT) {
-      const bool in = rt < tb;
       const int64_t r = min((int64_t)i * kRT + threadIdx.x, n_rows - 1);
       v_lse = p.lse[sb + r];
       v_delta = p.delta[sb + r];
-      v_pos = in ? rt + off : -kMaxLen;  // sees nothing
-      v_lo = p.starts ? p.starts[min(rt, tb - 1)] : lo;
+      const int t = min(rt, tb - 1);
+      v_vis = a_vis(p, t + off, p.starts ? p.starts[t] : lo, hi);
+      if (rt >= tb) v_vis.wn = v_vis.fn = 0;
       rt += adv_t;
       rg += adv_g;
       if (rg >= p.G) rg -= p.G, ++rt;
@@ -652,8 +685,10 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
     if (threadIdx.x < kRT) {
       st_lse[i & 1][threadIdx.x] = v_lse;
       st_delta[i & 1][threadIdx.x] = -v_delta;
-      st_pos[i & 1][threadIdx.x] = v_pos;
-      st_lo[i & 1][threadIdx.x] = v_lo;
+      st_w[i & 1][threadIdx.x] = v_vis.w;
+      st_wn[i & 1][threadIdx.x] = v_vis.wn;
+      st_lo[i & 1][threadIdx.x] = v_vis.lo;
+      st_fn[i & 1][threadIdx.x] = v_vis.fn;
     }
   };
 
@@ -669,14 +704,21 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
     const uint8_t* qt = lds + (i & 1) * 2 * kTile + half * (kTile / 2);
     const uint8_t* dt = qt + kTile;
     const int w = i & 1, rb = half * 64;
-    // positions and starts do not decrease over the valid rows, which come first
-    const int pos0 = __builtin_amdgcn_readfirstlane(st_pos[w][rb]);
-    const int pos1 = __builtin_amdgcn_readfirstlane(st_pos[w][rb + 63]);
-    const int lo1 = __builtin_amdgcn_readfirstlane(st_lo[w][rb + 63]);
-    const bool full = pos1 >= 0;  // the last row is valid
-    if (pos0 < 0 || (full && jw > pos1)) continue;  // the wave's keys are seen by none of the rows
-    if (p.window > 0 && p.first == 0 && jw + 31 <= pos0 - p.window) continue;
-    const bool whole = full && wave_in && jw + 31 <= pos0 && jw >= lo1 && (p.window <= 0 || jw > pos1 - p.window);
+    // the half's tokens; what rows see does not begin earlier from one to the next
+    const int64_t r0 = (int64_t)i * kRT + rb;
+    const bool full = r0 + 64 <= n_rows;  // rows past the last see nothing
+    const int pos0 = ut[0] + off, pos1 = min(ut[1], tb - 1) + off;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      ut[x] += adv_t;
+      ug[x] += adv_g;
+      if (ug[x] >= p.G) ug[x] -= p.G, ++ut[x];
+    }
+    if (r0 >= n_rows || jw > pos1) continue;  // none of the wave's keys is seen
+    const int w0 = __builtin_amdgcn_readfirstlane(st_w[w][rb]);
+    const int w1 = __builtin_amdgcn_readfirstlane(st_w[w][rb + 63]);
+    if (p.first == 0 && jw + 31 < w0) continue;
+    const bool whole = full && wave_in && jw + 31 <= pos0 && jw >= w1;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       af3_f32x16 s = a_zero(), dp;
@@ -699,16 +741,15 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
       if (!whole) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int4 po = *(const int4*)&st_pos[w][rb + c * 32 + 8 * q + 4 * lh];
-          const int4 rl = *(const int4*)&st_lo[w][rb + c * 32 + 8 * q + 4 * lh];
-          const int pov[4] = {po.x, po.y, po.z, po.w}, rlv[4] = {rl.x, rl.y, rl.z, rl.w};
+          const int at = rb + c * 32 + 8 * q + 4 * lh;
+          const int4 w4 = *(const int4*)&st_w[w][at], n4 = *(const int4*)&st_wn[w][at];
+          const int wv[4] = {w4.x, w4.y, w4.z, w4.w}, nv[4] = {n4.x, n4.y, n4.z, n4.w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const int r = 4 * q + y;
-            const bool on = jin && j <= pov[y] && j >= rlv[y] &&
-                            (p.window <= 0 || j > pov[y] - p.window || j < rlv[y] + p.first);
-            s[r] = on ? s[r] : 0.f;
-            dp[r] = on ? dp[r] : 0.f;
+            bool on = (uint32_t)(jm - wv[y]) < (uint32_t)nv[y];
+            if (p.first > 0) on = on || (uint32_t)(jm - st_lo[w][at + y]) < (uint32_t)st_fn[w][at + y];
+            s[4 * q + y] = on ? s[4 * q + y] : 0.f;
+            dp[4 * q + y] = on ? dp[4 * q + y] : 0.f;
           }
         }
       }
