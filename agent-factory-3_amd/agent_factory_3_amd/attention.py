@@ -25,14 +25,19 @@ from .routing import _device_of
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 128       # query heads per key/value head
 MAX_LEN = 1 << 29     # tokens of a batch row
+MAX_STRIDE = 1 << 23  # elements between two tokens (and heads, of q and dout) read in place
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the kernels read it: contiguous head vectors at 16-byte aligned addresses."""
-    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
+def _rows(t: torch.Tensor, heads: bool = False) -> torch.Tensor:
+    """[B, H, S, D] as the kernels read it: contiguous head vectors at 16-byte aligned
+    addresses, tokens (with ``heads``, heads too) less than MAX_STRIDE apart."""
+    sb, sh, st, sd = t.stride()
+    B, H, S, _ = t.shape
+    if (sd == 1 and t.data_ptr() % 16 == 0 and (B < 2 or sb % 8 == 0)
+            and (H < 2 or (sh % 8 == 0 and (sh < MAX_STRIDE or not heads))) and (S < 2 or (st % 8 == 0 and st < MAX_STRIDE))):
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    c = t.transpose(1, 2).contiguous()   # token-major: small strides whatever the length
+    return (c if c.data_ptr() % 16 == 0 else c.clone()).transpose(1, 2)
 
 
 def _strides(*ts):
@@ -70,7 +75,7 @@ class _SinkAttention(torch.autograd.Function):
         Hkv, Sk = k.shape[1], k.shape[2]
         dev = q.device
         with _device_of(q):
-            do = _rows(dout.to(torch.bfloat16).transpose(1, 2))
+            do = _rows(dout.to(torch.bfloat16).transpose(1, 2), heads=True)
             dq = torch.empty(B, Sq, Hq, D, dtype=torch.bfloat16, device=dev)
             dk = torch.empty(B, Sk, Hkv, D, dtype=torch.bfloat16, device=dev)
             dv = torch.empty_like(dk)
@@ -119,7 +124,7 @@ def _check(q, k, v, sinks, scale, window, first):
 
 def _run(q, k, v, sinks, scale, window, first, starts, kv_range):
     need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, sinks))
-    return _SinkAttention.apply(_rows(q), _rows(k), _rows(v), sinks.contiguous() if sinks is not None else None,
+    return _SinkAttention.apply(_rows(q, heads=True), _rows(k), _rows(v), sinks.contiguous() if sinks is not None else None,
                                 scale, window, first, starts, kv_range, need)
 
 

@@ -38,6 +38,7 @@ typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxLen = 1 << 29;   // tokens (positions and their sums with a window stay in 32 bits)
+constexpr int kMaxStride = 1 << 23; // elements between heads or tokens (128 of them within 32-bit byte offsets)
 constexpr float kLowest = -1e30f;  // running maximum of a row that has seen nothing (finite: -inf - it is -inf)
 
 struct SaParams {
@@ -48,6 +49,7 @@ struct SaParams {
   const int32_t* starts;                  // [Sk] start of each token's sequence (packed row), or NULL
   const int32_t* kv_range;                // [B][2] or NULL
   int B, Hq, Hkv, G, Sq, Sk, window, first;
+  int g_mul;                              // x / G = x g_mul >> 16 for x < 128
   int tok;                                // tokens of a row tile
   int n_tiles, n_split;
   float scale, scale2;                    // scale2 = scale log2(e)
@@ -65,6 +67,10 @@ struct SaParams {
 __device__ __forceinline__ void a_dma16(const void* gptr, uint32_t lds_byte_addr) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "{m0}"(lds_byte_addr) : "memory");
 }
+// the same from a wave-uniform base plus a 32-bit lane offset in bytes
+__device__ __forceinline__ void a_dma16_s(const void* sbase, uint32_t voff, uint32_t lds_byte_addr) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_byte_addr) : "memory");
+}
 #define A_WAIT_VM(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 #define A_BARRIER() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
@@ -79,17 +85,34 @@ __device__ __forceinline__ int a_swz(int row) { return ((row & 3) << 1) | ((row 
 template <int D>
 __device__ __forceinline__ int a_off(int row, int chunk) { return row * (D * 2) + ((chunk ^ a_swz(row)) << 4); }
 
-// entries row0 + 4 h .. + 3 and row0 + 8 + 4 h .. + 3 of column col0 + lane % 32
+// A lane's LDS offsets of the operands it reads from a [rows][D] tile.  The
+// swizzle depends on a row's low three bits alone, so every other row, chunk and
+// column block is a constant away.
 template <int D>
-__device__ __forceinline__ af3_bf16x8 a_tr8(const uint8_t* tile, int row0, int col0, int lane) {
-  const int r = row0 + ((lane >> 5) << 2) + ((lane & 15) >> 2);
-  const int c = col0 + (((lane >> 4) & 1) << 4) + ((lane & 3) << 2);
-  const uint8_t* p0 = tile + a_off<D>(r, c >> 3) + ((c & 7) << 1);
-  const uint8_t* p1 = tile + a_off<D>(r + 8, c >> 3) + ((c & 7) << 1);
-  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p0);
-  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p1);
-  return af3_bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
+struct Frag {
+  uint32_t row[4], tr[2];
+  __device__ __forceinline__ explicit Frag(int lane) {
+    const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) row[x] = a_off<D>(r, 2 * x + h);
+    const int tr_r = (h << 2) + ((lane & 15) >> 2);
+    const int c = (((lane >> 4) & 1) << 4) + ((lane & 3) << 2);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) tr[d] = a_off<D>(tr_r, (d * 32 + c) >> 3) + ((c & 7) << 1);
+  }
+  // chunk 2 x + h of row r0 + lane % 32 of the tile at LDS address `tile` (r0 % 8 == 0)
+  __device__ __forceinline__ af3_bf16x8 row8(uint32_t tile, int r0, int x) const {
+    typedef const __attribute__((address_space(3))) af3_bf16x8 T;
+    return *(T*)(tile + row[x & 3] + (uint32_t)((x >> 2) * 128 + r0 * D * 2));
+  }
+  // rows r0 + 4 h .. + 3 and r0 + 8 + 4 h .. + 3 of column 32 d + lane % 32
+  __device__ __forceinline__ af3_bf16x8 tr8(uint32_t tile, int r0, int d) const {
+    const uint32_t at = tile + tr[d & 1] + (uint32_t)((d >> 1) * 128 + r0 * D * 2);
+    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)at);
+    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at + 8 * D * 2));
+    return af3_bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+};
 
 // The loads of these operands end here.  Left to their first use in the loop, the
 // compiler's wait for them would stand there in every step and wait for the
@@ -98,11 +121,6 @@ template <int N>
 __device__ __forceinline__ void a_landed(af3_bf16x8 (&f)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
-}
-
-template <int D>
-__device__ __forceinline__ af3_bf16x8 a_row8(const uint8_t* tile, int row, int ks, int h) {
-  return *(const af3_bf16x8*)(tile + a_off<D>(row, 2 * ks + h));
 }
 
 __device__ __forceinline__ af3_f32x16 a_mfma(af3_bf16x8 a, af3_bf16x8 b, af3_f32x16 c) {
@@ -124,7 +142,15 @@ __device__ __forceinline__ af3_bf16x8 a_pack8(const af3_f32x16& p, int t) {
   return __builtin_bit_cast(af3_bf16x8, w);
 }
 
-__device__ __forceinline__ float a_xhalf(float x) { return __shfl_xor(x, 32); }
+// over a lane and its partner in the other half (lane ^ 32)
+__device__ __forceinline__ float a_max_halves(float x) {
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float a_sum_halves(float x) {
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 __device__ __forceinline__ float a_sink2(const SaParams& p, int h) {
   const float s = p.sinks_f32 ? ((const float*)p.sinks)[h] : af3_bf16_to_f32(((const uint16_t*)p.sinks)[h]);
@@ -141,40 +167,47 @@ __device__ __forceinline__ void a_kv_range(const SaParams& p, int b, int& lo, in
   }
 }
 
-// What a row sees, as two runs of keys: wn keys from w (the window, or all) and
-// fn keys from lo (the kept first tokens)
+// What a row sees: keys [w, end) (the window, or all) and the fn keys from lo
+// (the kept first tokens)
 struct Vis {
-  int w, wn, lo, fn;
+  int w, end, lo, fn;
 };
 
 __device__ __forceinline__ Vis a_vis(const SaParams& p, int pos, int lo, int hi) {
-  const int end = min(pos + 1, hi);
   Vis v;
   v.lo = lo;
+  v.end = min(pos + 1, hi);
   v.w = p.window > 0 ? max(lo, pos - p.window + 1) : lo;
-  v.wn = max(0, end - v.w);
-  v.fn = max(0, min(p.first, end - lo));
+  v.fn = max(0, min(p.first, v.end - lo));
   return v;
 }
 
-// scores outside [lo, lo + n) to `off` (register r: key j + 8 (r / 4) + r % 4)
+// scores of keys at or past `end` / before `from` to `to`; register r of s[c] is
+// key j + 32 c + 8 (r / 4) + r % 4
 template <int N>
-__device__ __forceinline__ void a_mask(af3_f32x16 (&s)[N], int j, int lo, int n, float off) {
+__device__ __forceinline__ void a_mask_end(af3_f32x16 (&s)[N], int j, int end, float to) {
 #pragma unroll
   for (int c = 0; c < N; ++c)
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      s[c][r] = (uint32_t)(j - lo + c * 32 + 8 * (r / 4) + r % 4) < (uint32_t)n ? s[c][r] : off;
+    for (int r = 0; r < 16; ++r) s[c][r] = c * 32 + 8 * (r / 4) + r % 4 < end - j ? s[c][r] : to;
 }
-// ... outside both runs
 template <int N>
-__device__ __forceinline__ void a_mask2(af3_f32x16 (&s)[N], int j, const Vis& v, float off) {
+__device__ __forceinline__ void a_mask_from(af3_f32x16 (&s)[N], int j, int from, float to) {
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[c][r] = c * 32 + 8 * (r / 4) + r % 4 >= from - j ? s[c][r] : to;
+}
+// keys outside both of a row's runs
+template <int N>
+__device__ __forceinline__ void a_mask_both(af3_f32x16 (&s)[N], int j, const Vis& v, float to) {
+  const uint32_t n = max(0, v.end - v.w);
 #pragma unroll
   for (int c = 0; c < N; ++c)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int x = j + c * 32 + 8 * (r / 4) + r % 4;
-      s[c][r] = (uint32_t)(x - v.w) < (uint32_t)v.wn || (uint32_t)(x - v.lo) < (uint32_t)v.fn ? s[c][r] : off;
+      s[c][r] = (uint32_t)(x - v.w) < n || (uint32_t)(x - v.lo) < (uint32_t)v.fn ? s[c][r] : to;
     }
 }
 
@@ -202,66 +235,95 @@ __device__ __forceinline__ Keys a_keys(const SaParams& p, int pos0, int pos1, in
 // ---------------------------------------------------------------------------
 constexpr int kRows = 128;  // rows of a tile
 constexpr int kBN = 64;     // keys of a tile
+constexpr int kMaxSplit = 256;
 
-// one K (or V) tile of 64 rows into LDS by the block's 4 waves; rows past `last` repeat it
+// K (or V) tiles of 64 rows into LDS by the block's 4 waves.  A whole tile's
+// copies take the tile's address (scalar) and lane offsets that never change; a
+// tile that ends early repeats its last row.
 template <int D>
-__device__ __forceinline__ void a_load_tile(const uint16_t* base, int64_t st, int j0, int last, uint32_t lds,
-                                            int wave, int lane) {
-  constexpr int CH = D / 8;               // chunks per row
-  constexpr int RPI = 64 / CH;            // rows per instruction
-  constexpr int N = kBN / RPI / 4;        // instructions per wave
+struct KvCopy {
+  static constexpr int CH = D / 8;         // chunks per row
+  static constexpr int RPI = 64 / CH;      // rows per copy
+  static constexpr int N = kBN / RPI / 4;  // copies per wave
+  const uint16_t* base;
+  int64_t st;
+  uint32_t off[N];
+  int row0;  // the lane's row of copy x: row0 + x RPI
+  __device__ __forceinline__ KvCopy(const uint16_t* base_, int64_t st_, int wave, int lane) : base(base_), st(st_) {
+    row0 = wave * N * RPI + lane / CH;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int row = (wave * N + i) * RPI + lane / CH;
-    const int j = min(j0 + row, last);
-    a_dma16(base + j * st + (((lane % CH) ^ a_swz(row)) << 3), lds + (uint32_t)((wave * N + i) * 1024));
+    for (int x = 0; x < N; ++x) {
+      const int row = row0 + x * RPI;
+      off[x] = (uint32_t)(row * (int)st + (((lane % CH) ^ a_swz(row)) << 3)) * 2;
+    }
   }
-}
+  __device__ __forceinline__ void operator()(int j0, int last, uint32_t lds, int wave) const {
+    const uint16_t* t = base + j0 * st;
+    const uint32_t at = lds + (uint32_t)(wave * N * 1024);
+    if (j0 + kBN - 1 <= last) {
+#pragma unroll
+      for (int x = 0; x < N; ++x) a_dma16_s(t, off[x], at + x * 1024);
+    } else {
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int over = max(0, row0 + x * RPI - (last - j0));
+        a_dma16_s(t, off[x] - (uint32_t)(over * (int)st) * 2, at + x * 1024);
+      }
+    }
+  }
+};
 
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kBN * D * 2;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[5 * kTile];
   const int bh = blockIdx.x % (p.B * p.Hkv);
   const int rest = blockIdx.x / (p.B * p.Hkv);
-  const int split = rest % p.n_split;
-  const int tile = p.n_tiles - 1 - rest / p.n_split;  // the longest rows first
-  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int split = p.n_split > 1 ? rest % p.n_split : 0;
+  const int tile = p.n_tiles - 1 - (p.n_split > 1 ? rest / p.n_split : rest);  // the longest rows first
+  const int b = p.B > 1 ? bh / p.Hkv : 0, hk = bh - b * p.Hkv;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, lh = lane >> 5;
   const int off = p.Sk - p.Sq;
   const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;  // tokens of the tile
-  const int row = wave * 32 + lr;
-  const int tk = row / p.G, g = row % p.G;
-  const bool valid = t0 + tk <= t1;
-  const int t = valid ? t0 + tk : t0;
-  const int head = hk * p.G + (valid ? g : 0);
   int lo, hi;
   a_kv_range(p, b, lo, hi);
-  const int row_lo = p.starts ? p.starts[t] : lo;
   const int tile_lo = p.starts ? p.starts[t0] : lo;
-  const int tile_hi_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start (the latest)
-  const Vis vis = a_vis(p, t + off, row_lo, hi);
+  const int last_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start (the latest)
   const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
-  // the wave's positions, to pass over tiles that none of its rows sees
-  const int wt0 = t0 + (wave * 32) / p.G, wt1 = min(t1, t0 + (wave * 32 + 31) / p.G);
-  const int wpos0 = wt0 + off, wpos1 = wt1 + off, wlo1 = tile_hi_lo;
   int i0 = 0, i1 = na + nb;
   if (p.n_split > 1) {
     const int per = (na + nb + p.n_split - 1) / p.n_split;
     i0 = min(split * per, na + nb);
     i1 = min(i0 + per, na + nb);
   }
+  const KvCopy<D> kc(p.k + b * p.k_sb + hk * p.k_sh, p.k_st, wave, lane);
+  const KvCopy<D> vc(p.v + b * p.v_sb + hk * p.v_sh, p.v_st, wave, lane);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
+  auto first_key = [&](int i) { return i < na ? ks.a0 + i * kBN : ks.b0 + (i - na) * kBN; };
+  // K and V of tile i; K goes round two stages, V round three
+  auto load = [&](int i, int kst, int vst) {
+    const int j0 = first_key(i), last = (i < na ? ks.a1 : ks.b1) - 1;
+    kc(j0, last, lds0 + (uint32_t)(kst * kTile), wave);
+    vc(j0, last, lds0 + (uint32_t)((2 + vst) * kTile), wave);
+  };
+  if (i0 < i1) load(i0, 0, 0);
+  if (i0 + 1 < i1) load(i0 + 1, 1, 1);
 
+  const int row = wave * 32 + lr;
+  const int tk = row * p.g_mul >> 16, g = row - tk * p.G;
+  const bool valid = t0 + tk <= t1;
+  const int t = valid ? t0 + tk : t0;
+  const int head = hk * p.G + (valid ? g : 0);
+  const Vis vis = a_vis(p, t + off, p.starts ? p.starts[t] : lo, hi);
   af3_bf16x8 qf[KS];
   {
     const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
-    a_landed(qf);
   }
   float m = kLowest, l = 0.f;
   if (p.sinks && split == 0) {
@@ -269,51 +331,44 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p
     m = fmaxf(s2, kLowest);
     l = lh == 0 ? __builtin_amdgcn_exp2f(s2 - m) : 0.f;
   }
+  a_landed(qf);
   af3_f32x16 o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = a_zero();
 
-  const uint16_t* kb = p.k + b * p.k_sb + hk * p.k_sh;
-  const uint16_t* vb = p.v + b * p.v_sb + hk * p.v_sh;
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
-  auto first_key = [&](int i) { return i < na ? ks.a0 + i * kBN : ks.b0 + (i - na) * kBN; };
-  auto issue = [&](int i, int stage) {
-    const int j0 = first_key(i), last = (i < na ? ks.a1 : ks.b1) - 1;
-    const uint32_t st = lds0 + (uint32_t)(stage * 2 * kTile);
-    a_load_tile<D>(kb, p.k_st, j0, last, st, wave, lane);
-    a_load_tile<D>(vb, p.v_st, j0, last, st + kTile, wave, lane);
-  };
-  if (i0 < i1) issue(i0, 0);
-  for (int i = i0; i < i1; ++i) {
-    A_WAIT_VM(0);
-    A_BARRIER();
-    if (i + 1 < i1) issue(i + 1, (i + 1 - i0) & 1);
-    const uint8_t* kt = lds + ((i - i0) & 1) * 2 * kTile;
-    const uint8_t* vt = kt + kTile;
-    const int j0 = first_key(i);
-    if (wt0 > t1 || j0 > wpos1) continue;  // nothing for this wave
-    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wpos0 - p.window) continue;
+  // The wave's positions; its tiles [own0, own1) (the others hold nothing that its
+  // rows see) and among them [free0, free1), of which its rows see every key.
+  const int wt0 = t0 + (wave * 32 * p.g_mul >> 16), wt1 = min(t1, t0 + ((wave * 32 + 31) * p.g_mul >> 16));
+  const int wpos0 = wt0 + off, wpos1 = wt1 + off;
+  const int from = p.window > 0 ? max(last_lo + p.first, wpos1 - p.window + 1) : last_lo;
+  const int own1 = wt0 > t1 ? 0 : min(i1, na + max(0, wpos1 - ks.b0 + kBN) / kBN);
+  const int own0 = p.window > 0 && p.first == 0 ? max(i0, na + max(0, wpos0 - p.window + 1 - ks.b0) / kBN) : i0;
+  const int free0 = na + max(0, from - ks.b0 + kBN - 1) / kBN;
+  const int free1 = na + max(0, min(wpos0 + 1, ks.b1) - ks.b0) / kBN;
+  const Frag<D> fr(lane);
 
-    af3_f32x16 s[2];
+  // the softmax of 32 keys (half c of tile i) and their product with V; beside it the scores of the next 32
+  auto step = [&](int i, int c, uint32_t vt, af3_f32x16 (&s)[1], uint32_t kt, af3_f32x16& next) {
+    // (past the last tile these are what the ring holds, and nothing reads their scores)
+    af3_bf16x8 kf[KS];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      s[c] = a_zero();
-#pragma unroll
-      for (int x = 0; x < KS; ++x) s[c] = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s[c]);
+    for (int x = 0; x < KS; ++x) kf[x] = fr.row8(kt, (c ^ 1) * 32, x);
+    if (i < free0 || i >= free1) {
+      const int j = first_key(i) + c * 32;
+      if (i < na) {  // first tokens before the window
+        a_mask_end(s, j + 4 * lh, min(vis.lo + vis.fn, ks.a1), -INFINITY);
+        a_mask_from(s, j + 4 * lh, vis.lo, -INFINITY);
+      } else if (p.first > 0 && j < last_lo + p.first) {
+        a_mask_both(s, j + 4 * lh, vis, -INFINITY);
+      } else {
+        if (j + 31 > wpos0 || j + 32 > ks.b1) a_mask_end(s, j + 4 * lh, vis.end, -INFINITY);
+        if (j < from) a_mask_from(s, j + 4 * lh, vis.w, -INFINITY);
+      }
     }
-    // (a row's runs end before `end`, but for the first tokens of tiles before the window)
-    if (i < na)
-      a_mask(s, j0 + 4 * lh, vis.lo, max(0, min(vis.fn, ks.a1 - vis.lo)), -INFINITY);
-    else if (p.first > 0 && j0 < wlo1 + p.first)
-      a_mask2(s, j0 + 4 * lh, vis, -INFINITY);
-    else if (j0 + kBN - 1 > wpos0 || j0 < wlo1 || j0 + kBN > ks.b1 || (p.window > 0 && j0 <= wpos1 - p.window))
-      a_mask(s, j0 + 4 * lh, vis.w, vis.wn, -INFINITY);
     float mx = s[0][0];
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[c][r]);
-    mx = fmaxf(mx, a_xhalf(mx)) * p.scale2;
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[0][r]);
+    mx = a_max_halves(mx) * p.scale2;
     if (__any(mx > m + 8.f)) {
       const float nm = fmaxf(m, mx);
       const float alpha = __builtin_amdgcn_exp2f(m - nm);
@@ -324,22 +379,65 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
+    // Written in the order in which it has to issue (the barriers hold it): each
+    // score product of the next keys has exponentials behind it, which run while
+    // the matrix unit is busy, and the first half's product with V stands between
+    // the second half's exponentials.
+    af3_bf16x8 vf[DB], pf;
+    next = a_zero();
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int x = 0; x < KS; ++x) {
+      next = a_mfma(kf[x], qf[x], next);
+      if (x == KS / 2 - 1)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[c][r] = __builtin_amdgcn_exp2f(fmaf(s[c][r], p.scale2, -m));
-        l += s[c][r];
+        for (int d = 0; d < DB; ++d) vf[d] = fr.tr8(vt, c * 32, d);
+      if (x == KS / 2) pf = a_pack8(s[0], 0);
+      if (x >= KS / 2) o[x - KS / 2] = a_mfma(vf[x - KS / 2], pf, o[x - KS / 2]);
+#pragma unroll
+      for (int r = x * (16 / KS); r < (x + 1) * (16 / KS); ++r) {
+        s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -m));
+        l += s[0][r];
       }
+      if (x == KS - 1)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const af3_bf16x8 pf = a_pack8(s[c], u);
+        for (int d = 0; d < DB; ++d) vf[d] = fr.tr8(vt, c * 32 + 16, d);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    pf = a_pack8(s[0], 1);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] = a_mfma(a_tr8<D>(vt, c * 32 + u * 16, d * 32, lane), pf, o[d]);
-      }
+    for (int d = 0; d < DB; ++d) o[d] = a_mfma(vf[d], pf, o[d]);
+  };
+  // K of tile i is done with after the scores of its second half (two stages), V
+  // after its second half's product (three)
+  af3_f32x16 sa[1], sb[1];
+  A_WAIT_VM(0);
+  A_BARRIER();
+  if (own0 == i0 && i0 < own1) {
+    sa[0] = a_zero();
+#pragma unroll
+    for (int x = 0; x < KS; ++x) sa[0] = a_mfma(fr.row8(lds0, 0, x), qf[x], sa[0]);
+  }
+  int kst = 0, vst = 0;
+  for (int i = i0; i < i1; ++i) {
+    const bool mine = i >= own0 && i < own1;
+    const uint32_t vt = lds0 + (uint32_t)((2 + vst) * kTile);
+    if (mine) step(i, 0, vt, sa, lds0 + (uint32_t)(kst * kTile), sb[0]);
+    A_WAIT_VM(0);  // K and V of tile i + 1
+    A_BARRIER();   // and every wave is past K of tile i and V of tile i - 1
+    vst = vst == 2 ? 0 : vst + 1;
+    if (i + 2 < i1) load(i + 2, kst, vst == 2 ? 0 : vst + 1);
+    kst ^= 1;
+    const uint32_t kt = lds0 + (uint32_t)(kst * kTile);
+    if (mine) {
+      step(i, 1, vt, sb, kt, sa[0]);
+    } else if (i + 1 == own0) {
+      sa[0] = a_zero();
+#pragma unroll
+      for (int x = 0; x < KS; ++x) sa[0] = a_mfma(fr.row8(kt, 0, x), qf[x], sa[0]);
     }
   }
-  l += a_xhalf(l);
+  l = a_sum_halves(l);
   if (!valid) return;
   const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + g;
   if (p.n_split > 1) {
@@ -372,38 +470,53 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_fwd_kernel(SaParams p
   if (p.lse && lh == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// joins the splits of a row: one wave per row, D / 64 columns per lane
+// joins the splits of a row: one block per row, each wave a quarter of the splits
 template <int D>
 __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
+  __shared__ float sw[kMaxSplit], so[4][D], sl[4];
   const int64_t rows = (int64_t)p.B * p.Hkv * p.Sq * p.G;
-  const int64_t prow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (prow >= rows) return;
-  const int lane = threadIdx.x & 63;
+  const int64_t prow = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* ml = p.part + p.n_split * rows * D;
-  float m = kLowest;
-  for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, ml[(s * rows + prow) * 2]);
-  float l = 0.f, o[D / 64] = {};
-  for (int s = 0; s < p.n_split; ++s) {
-    const float2 x = *(const float2*)(ml + (s * rows + prow) * 2);
-    const float w = __builtin_amdgcn_exp2f(x.x - m);
-    l += w * x.y;
+  const int s0 = threadIdx.x;
+  const float2 x = s0 < p.n_split ? *(const float2*)(ml + (s0 * rows + prow) * 2) : float2{kLowest, 0.f};
+  float m = x.x;
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) o[d] += w * p.part[(s * rows + prow) * D + d * 64 + lane];
-  }
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (lane == 0) sl[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sl[0], sl[1]), fmaxf(sl[2], sl[3]));
+  const float w = __builtin_amdgcn_exp2f(x.x - m);
+  sw[s0] = w;
+  float l = w * x.y;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  __syncthreads();
+  if (lane == 0) sl[wave] = l;
+  float o[D / 64] = {};
+  const float* po = p.part + prow * D + lane;
+#pragma unroll 8
+  for (int s = wave; s < p.n_split; s += 4)
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) o[d] = fmaf(sw[s], po[s * rows * D + d * 64], o[d]);
+#pragma unroll
+  for (int d = 0; d < D / 64; ++d) so[wave][d * 64 + lane] = o[d];
+  __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const int g = (int)(prow % p.G);
   const int64_t u = prow / p.G;
   const int t = (int)(u % p.Sq);
   const int bh = (int)(u / p.Sq), b = bh / p.Hkv, hk = bh % p.Hkv;
   const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + hk * p.G + g) * D;
-#pragma unroll
-  for (int d = 0; d < D / 64; ++d) {
-    const float y = o[d] * inv;
-    const uint32_t w = af3_f32_to_bf16(y);
-    p.out[orow + d * 64 + lane] = (uint16_t)w;
-    if (p.out_lo) p.out_lo[orow + d * 64 + lane] = (uint16_t)af3_f32_to_bf16(y - af3_bf16_to_f32(w));
+  if ((int)threadIdx.x < D) {
+    const int d = threadIdx.x;
+    const float y = ((so[0][d] + so[1][d]) + (so[2][d] + so[3][d])) * inv;
+    const uint32_t r = af3_f32_to_bf16(y);
+    p.out[orow + d] = (uint16_t)r;
+    if (p.out_lo) p.out_lo[orow + d] = (uint16_t)af3_f32_to_bf16(y - af3_bf16_to_f32(r));
   }
-  if (p.lse && lane == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (p.lse && threadIdx.x == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // ---------------------------------------------------------------------------
@@ -411,7 +524,7 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
 // tiles and layouts; p comes back from the saved log-sum.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kBN * D * 2;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
@@ -425,7 +538,7 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
   const int off = p.Sk - p.Sq;
   const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;
   const int row = wave * 32 + lr;
-  const int tk = row / p.G, g = row % p.G;
+  const int tk = row * p.g_mul >> 16, g = row - tk * p.G;
   const bool valid = t0 + tk <= t1;
   const int t = valid ? t0 + tk : t0;
   const int head = hk * p.G + (valid ? g : 0);
@@ -437,18 +550,18 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
   const Vis vis = a_vis(p, t + off, row_lo, hi);
   const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
-  const int wt0 = t0 + (wave * 32) / p.G, wt1 = min(t1, t0 + (wave * 32 + 31) / p.G);
+  const int wt0 = t0 + (wave * 32 * p.g_mul >> 16), wt1 = min(t1, t0 + ((wave * 32 + 31) * p.g_mul >> 16));
   const int wpos0 = wt0 + off, wpos1 = wt1 + off, wlo1 = tile_hi_lo;
 
-  const uint16_t* kb = p.k + b * p.k_sb + hk * p.k_sh;
-  const uint16_t* vb = p.v + b * p.v_sb + hk * p.v_sh;
+  const KvCopy<D> kc(p.k + b * p.k_sb + hk * p.k_sh, p.k_st, wave, lane);
+  const KvCopy<D> vc(p.v + b * p.v_sb + hk * p.v_sh, p.v_st, wave, lane);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
   auto first_key = [&](int i) { return i < na ? ks.a0 + i * kBN : ks.b0 + (i - na) * kBN; };
   auto issue = [&](int i, int stage) {
     const int j0 = first_key(i), last = (i < na ? ks.a1 : ks.b1) - 1;
     const uint32_t st = lds0 + (uint32_t)(stage * 2 * kTile);
-    a_load_tile<D>(kb, p.k_st, j0, last, st, wave, lane);
-    a_load_tile<D>(vb, p.v_st, j0, last, st + kTile, wave, lane);
+    kc(j0, last, st, wave);
+    vc(j0, last, st + kTile, wave);
   };
 
   const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + (valid ? g : 0);
@@ -467,7 +580,7 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[i] + (float)oe[i], delta);
     }
-    delta += a_xhalf(delta);
+    delta = a_sum_halves(delta);
     a_landed(qf);
     a_landed(df);
   }
@@ -486,6 +599,7 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
   A_WAIT_VM(0);
   if (na + nb > 0) issue(0, 0);
 
+  const Frag<D> fr(lane);
   af3_f32x16 acc[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = a_zero();
@@ -493,8 +607,7 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
     A_WAIT_VM(0);
     A_BARRIER();
     if (i + 1 < na + nb) issue(i + 1, (i + 1) & 1);
-    const uint8_t* kt = lds + (i & 1) * 2 * kTile;
-    const uint8_t* vt = kt + kTile;
+    const uint32_t kt = lds0 + (uint32_t)((i & 1) * 2 * kTile), vt = kt + kTile;
     const int j0 = first_key(i);
     if (wt0 > t1 || j0 > wpos1) continue;
     if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wpos0 - p.window) continue;
@@ -504,24 +617,27 @@ __global__ __launch_bounds__(256, 2) void sa_dq_kernel(SaParams p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = -delta;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) s[0] = a_mfma(a_row8<D>(kt, c * 32 + lr, x, lh), qf[x], s[0]);
+      for (int x = 0; x < KS; ++x) s[0] = a_mfma(fr.row8(kt, c * 32, x), qf[x], s[0]);
 #pragma unroll
-      for (int x = 0; x < KS; ++x) dp = a_mfma(a_row8<D>(vt, c * 32 + lr, x, lh), df[x], dp);
+      for (int x = 0; x < KS; ++x) dp = a_mfma(fr.row8(vt, c * 32, x), df[x], dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -lse)) * dp[r];
       // (the product is set to zero, not the score: whatever stands at a key that the row does not see)
       const int jc = j0 + c * 32 + 4 * lh;
-      if (i < na)
-        a_mask(s, jc, vis.lo, max(0, min(vis.fn, ks.a1 - vis.lo)), 0.f);
-      else if (p.first > 0 && j0 < wlo1 + p.first)
-        a_mask2(s, jc, vis, 0.f);
-      else if (j0 + kBN - 1 > wpos0 || j0 < wlo1 || j0 + kBN > ks.b1 || (p.window > 0 && j0 <= wpos1 - p.window))
-        a_mask(s, jc, vis.w, vis.wn, 0.f);
+      if (i < na) {
+        a_mask_end(s, jc, min(vis.lo + vis.fn, ks.a1), 0.f);
+        a_mask_from(s, jc, vis.lo, 0.f);
+      } else if (p.first > 0 && j0 < wlo1 + p.first) {
+        a_mask_both(s, jc, vis, 0.f);
+      } else {
+        if (j0 + kBN - 1 > wpos0 || j0 + kBN > ks.b1) a_mask_end(s, jc, vis.end, 0.f);
+        if (j0 < wlo1 || (p.window > 0 && j0 <= wpos1 - p.window)) a_mask_from(s, jc, vis.w, 0.f);
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const af3_bf16x8 pf = a_pack8(s[0], u);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) acc[d] = a_mfma(a_tr8<D>(kt, c * 32 + u * 16, d * 32, lane), pf, acc[d]);
+        for (int d = 0; d < DB; ++d) acc[d] = a_mfma(fr.tr8(kt, c * 32 + u * 16, d), pf, acc[d]);
       }
     }
   }
@@ -656,18 +772,41 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
   int ut[2] = {ta + half * 64 / p.G, ta + (half * 64 + 63) / p.G}, ug[2] = {half * 64 % p.G, (half * 64 + 63) % p.G};
   float v_lse = 0.f, v_delta = 0.f;
   Vis v_vis = {};
-  auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..127
-    const uint32_t st = lds0 + (uint32_t)((i & 1) * 2 * kTile);
+  int v_n = 0;
+  // copies: where 128 rows are whole tokens, lane offsets never change and the
+  // scalar base moves on; else, and in the last step, each row is looked up
+  const bool even = adv_g == 0;
+  uint32_t qo[N], od[N];
 #pragma unroll
-    for (int x = 0; x < N; ++x) {
-      const int row = (wave * N + x) * RPI + lane / CH;
-      const int64_t t = min(ct[x], tb - 1), g = cg[x];
-      const int col = ((lane % CH) ^ a_swz(row)) << 3;
-      a_dma16(qb + t * p.q_st + g * p.q_sh + col, st + (uint32_t)((wave * N + x) * 1024));
-      a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + (uint32_t)((wave * N + x) * 1024));
-      ct[x] += adv_t;
-      cg[x] += adv_g;
-      if (cg[x] >= p.G) cg[x] -= p.G, ++ct[x];
+  for (int x = 0; x < N; ++x) {
+    const int row = (wave * N + x) * RPI + lane / CH;
+    const int col = ((lane % CH) ^ a_swz(row)) << 3;
+    qo[x] = (uint32_t)((ct[x] - ta) * (int)p.q_st + cg[x] * (int)p.q_sh + col) * 2;
+    od[x] = (uint32_t)((ct[x] - ta) * (int)p.do_st + cg[x] * (int)p.do_sh + col) * 2;
+  }
+  auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..127
+    const uint32_t st = lds0 + (uint32_t)((i & 1) * 2 * kTile + wave * N * 1024);
+    if (even && (int64_t)(i + 1) * kRT <= n_rows) {
+      const int64_t t = ta + (int64_t)i * adv_t;
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        a_dma16_s(qb + t * p.q_st, qo[x], st + x * 1024);
+        a_dma16_s(db + t * p.do_st, od[x], st + kTile + x * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int row = (wave * N + x) * RPI + lane / CH;
+        const int64_t t = min((even ? i * adv_t : 0) + ct[x], tb - 1), g = cg[x];
+        const int col = ((lane % CH) ^ a_swz(row)) << 3;
+        a_dma16(qb + t * p.q_st + g * p.q_sh + col, st + x * 1024);
+        a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + x * 1024);
+        if (!even) {
+          ct[x] += adv_t;
+          cg[x] += adv_g;
+          if (cg[x] >= p.G) cg[x] -= p.G, ++ct[x];
+        }
+      }
     }
     if (threadIdx.x < kRT) {
       const int64_t r = min((int64_t)i * kRT + threadIdx.x, n_rows - 1);
@@ -675,7 +814,8 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
       v_delta = p.delta[sb + r];
       const int t = min(rt, tb - 1);
       v_vis = a_vis(p, t + off, p.starts ? p.starts[t] : lo, hi);
-      if (rt >= tb) v_vis.wn = v_vis.fn = 0;
+      v_n = rt < tb ? max(0, v_vis.end - v_vis.w) : 0;
+      if (rt >= tb) v_vis.fn = 0;
       rt += adv_t;
       rg += adv_g;
       if (rg >= p.G) rg -= p.G, ++rt;
@@ -686,12 +826,13 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
       st_lse[i & 1][threadIdx.x] = v_lse;
       st_delta[i & 1][threadIdx.x] = -v_delta;
       st_w[i & 1][threadIdx.x] = v_vis.w;
-      st_wn[i & 1][threadIdx.x] = v_vis.wn;
+      st_wn[i & 1][threadIdx.x] = v_n;
       st_lo[i & 1][threadIdx.x] = v_vis.lo;
       st_fn[i & 1][threadIdx.x] = v_vis.fn;
     }
   };
 
+  const Frag<D> fr(lane);
   af3_f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = a_zero(), dv[d] = a_zero();
@@ -701,8 +842,7 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
     store_rows(i);
     A_BARRIER();
     if (i + 1 < n_steps) issue(i + 1);
-    const uint8_t* qt = lds + (i & 1) * 2 * kTile + half * (kTile / 2);
-    const uint8_t* dt = qt + kTile;
+    const uint32_t qt = lds0 + (uint32_t)((i & 1) * 2 * kTile + half * (kTile / 2)), dt = qt + kTile;
     const int w = i & 1, rb = half * 64;
     // the half's tokens; what rows see does not begin earlier from one to the next
     const int64_t r0 = (int64_t)i * kRT + rb;
@@ -728,9 +868,9 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
         dp[4 * q] = de.x; dp[4 * q + 1] = de.y; dp[4 * q + 2] = de.z; dp[4 * q + 3] = de.w;
       }
 #pragma unroll
-      for (int x = 0; x < KS; ++x) s = a_mfma(a_row8<D>(qt, c * 32 + lr, x, lh), kf[x], s);
+      for (int x = 0; x < KS; ++x) s = a_mfma(fr.row8(qt, c * 32, x), kf[x], s);
 #pragma unroll
-      for (int x = 0; x < KS; ++x) dp = a_mfma(a_row8<D>(dt, c * 32 + lr, x, lh), vf[x], dp);
+      for (int x = 0; x < KS; ++x) dp = a_mfma(fr.row8(dt, c * 32, x), vf[x], dp);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float4 ls = *(const float4*)&st_lse[w][rb + c * 32 + 8 * q + 4 * lh];
@@ -760,8 +900,8 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
         const af3_bf16x8 pf = a_pack8(s, u), sf = a_pack8(dp, u);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          dv[d] = a_mfma(a_tr8<D>(dt, c * 32 + u * 16, d * 32, lane), pf, dv[d]);
-          dk[d] = a_mfma(a_tr8<D>(qt, c * 32 + u * 16, d * 32, lane), sf, dk[d]);
+          dv[d] = a_mfma(fr.tr8(dt, c * 32 + u * 16, d), pf, dv[d]);
+          dk[d] = a_mfma(fr.tr8(qt, c * 32 + u * 16, d), sf, dk[d]);
         }
       }
     }
@@ -841,14 +981,18 @@ __global__ __launch_bounds__(1024) void sa_starts_pos_kernel(const int64_t* __re
 // ---------------------------------------------------------------------------
 
 // Splits of a row tile's keys over blocks.  One block per (batch row, key/value
-// head, row tile) leaves most of the 256 CUs idle when there are few rows.
-int sa_splits(int B, int Hkv, int64_t n_tiles, int64_t keys) {
+// head, row tile) leaves most of the 256 CUs idle when there are few of them.  A
+// block whose rows fill one wave at most (a few new tokens) is bound by reading K
+// and V: three such blocks fit a CU, and more come in a second round (131072 keys:
+// 512 blocks 42 us, 768 44, 1024 52).
+int sa_splits(int B, int Hkv, int64_t n_tiles, int64_t rows, int64_t keys) {
   const int64_t blocks = (int64_t)B * Hkv * n_tiles;
-  if (blocks == 0 || blocks >= 256) return 1;
-  const int64_t most = (keys + 255) / 256;  // at least four key tiles each
-  int64_t n = (512 + blocks - 1) / blocks;
+  const bool few = rows <= 32;
+  if (blocks == 0 || blocks > (few ? 384 : 255)) return 1;
+  const int64_t most = keys / 256;  // at least four key tiles each
+  int64_t n = (few ? 768 : 512) / blocks;
   if (n > most) n = most;
-  return n < 1 ? 1 : n > 256 ? 256 : (int)n;
+  return n < 1 ? 1 : n > kMaxSplit ? kMaxSplit : (int)n;
 }
 
 struct SaShape {
@@ -864,7 +1008,7 @@ SaShape sa_shape(int B, int Hq, int Hkv, int Sq, int Sk, int window, int first) 
   s.n_tiles = (int)af3_cdiv(Sq, s.tok);
   int64_t keys = s.window > 0 ? (int64_t)s.window + s.tok + s.first : Sk;
   if (keys > Sk) keys = Sk;
-  s.n_split = sa_splits(B, Hkv, s.n_tiles, keys);
+  s.n_split = sa_splits(B, Hkv, s.n_tiles, (int64_t)Sq * G, keys);
   return s;
 }
 
@@ -877,7 +1021,12 @@ int sa_check(const char* who, int B, int Hq, int Hkv, int Sq, int Sk, int D, int
   AF3_REQUIRE(window >= 0 && first >= 0, "%s: negative window or first", who);
   AF3_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", who);
   AF3_REQUIRE(strides, "%s: null strides", who);
-  for (int i = 0; i < n_strides; ++i) AF3_REQUIRE(strides[i] % 8 == 0, "%s: strides must be multiples of 8", who);
+  for (int i = 0; i < n_strides; ++i) {
+    AF3_REQUIRE(strides[i] % 8 == 0, "%s: strides must be multiples of 8", who);
+    // (a tile's tokens, and a token's heads, are reached by 32-bit offsets from the tile's address)
+    AF3_REQUIRE((i % 3 != 2 && i != 1 && i != 10) || (strides[i] >= 0 && strides[i] < kMaxStride),
+                "%s: token strides, and head strides of q and dout, must be below %d", who, kMaxStride);
+  }
   AF3_REQUIRE(!starts || (B <= 1 && Sq == Sk && !kv_range), "%s: a packed row has batch 1, Sq == Sk and no kv_range", who);
   AF3_REQUIRE((int64_t)B * Hkv * (Sq + Sk + 1) < 0x7fffffffLL, "%s: too many rows", who);
   return 0;
@@ -895,6 +1044,7 @@ SaParams sa_params(const SaShape& s, const uint16_t* q, const uint16_t* k, const
   p.starts = starts; p.kv_range = kv_range;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.Sq = Sq; p.Sk = Sk;
   p.window = s.window; p.first = s.first; p.tok = s.tok; p.n_tiles = s.n_tiles; p.n_split = 1;
+  p.g_mul = (65536 + p.G - 1) / p.G;
   p.scale = scale; p.scale2 = scale * kLog2e;
   return p;
 }
@@ -959,7 +1109,7 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
   else
     hipLaunchKernelGGL(sa_fwd_kernel<128>, dim3((unsigned)grid), dim3(256), 0, stream, p);
   if (s.n_split > 1) {
-    const unsigned g = (unsigned)af3_cdiv((int64_t)B * Hq * Sq, 4);
+    const unsigned g = (unsigned)((int64_t)B * Hq * Sq);
     if (D == 64)
       hipLaunchKernelGGL(sa_join_kernel<64>, dim3(g), dim3(256), 0, stream, p);
     else

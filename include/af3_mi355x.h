@@ -441,7 +441,8 @@ int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_
  * query heads share a key/value head (query head h reads head h / (Hq / Hkv)).
  * strides: host array of the element strides of q, k, v (and, for the backward,
  * dout): batch, head, token of each; the D elements are contiguous, strides
- * multiples of 8, addresses 16-byte aligned.  Query i stands at key position
+ * multiples of 8, addresses 16-byte aligned; token strides, and head strides of q
+ * and dout, below 2^23.  Query i stands at key position
  * p = i + Sk - Sq and sees the keys j <= p of its range with j > p - window or
  * j < (range start) + first (window 0: all of them).  The range is
  * kv_range[b] = (begin, end) (device int32 [B][2], clamped to [0, Sk]; NULL: all
