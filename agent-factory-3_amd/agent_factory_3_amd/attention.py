@@ -15,6 +15,7 @@ sdpa form there, and its flash forms with sinks are CUDA kernels.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -28,67 +29,88 @@ MAX_LEN = 1 << 29     # tokens of a batch row
 MAX_STRIDE = 1 << 23  # elements between two tokens (and heads, of q and dout) read in place
 
 
-def _rows(t: torch.Tensor, heads: bool = False) -> torch.Tensor:
-    """[B, H, S, D] as the kernels read it: contiguous head vectors at 16-byte aligned
-    addresses, tokens (with ``heads``, heads too) less than MAX_STRIDE apart."""
-    sb, sh, st, sd = t.stride()
+def _rows(t: torch.Tensor, heads: bool = False):
+    """[B, H, S, D] as the kernels read it, with its element strides (batch, head,
+    token): contiguous head vectors at 16-byte aligned addresses, tokens (with
+    ``heads``, heads too) less than MAX_STRIDE apart.  Other tensors are copied."""
     B, H, S, _ = t.shape
-    if (sd == 1 and t.data_ptr() % 16 == 0 and (B < 2 or sb % 8 == 0)
-            and (H < 2 or (sh % 8 == 0 and (sh < MAX_STRIDE or not heads))) and (S < 2 or (st % 8 == 0 and st < MAX_STRIDE))):
-        return t
+    sb, sh, st, sd = t.stride()
+    sb, sh, st = sb if B > 1 else 0, sh if H > 1 else 0, st if S > 1 else 0
+    if (sd == 1 and not (sb | sh | st) & 7 and st < MAX_STRIDE and (sh < MAX_STRIDE or not heads)
+            and t.data_ptr() % 16 == 0):
+        return t, (sb, sh, st)
     c = t.transpose(1, 2).contiguous()   # token-major: small strides whatever the length
-    return (c if c.data_ptr() % 16 == 0 else c.clone()).transpose(1, 2)
+    t = (c if c.data_ptr() % 16 == 0 else c.clone()).transpose(1, 2)
+    return t, t.stride()[:3]
 
 
-def _strides(*ts):
-    """Element strides (batch, head, token) of [B, H, S, D] tensors as a C array (read by the call, never kept)."""
-    v = [s if n > 1 else 0 for t in ts for s, n in zip(t.stride()[:3], t.shape[:3])]
-    return (ctypes.c_int64 * len(v))(*v)
+@functools.lru_cache(maxsize=64)
+def _fwd_workspace(B, Hq, Hkv, Sq, Sk, D, window, first) -> int:
+    return int(_capi.load().af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first))
+
+
+@functools.lru_cache(maxsize=64)
+def _bwd_workspace(B, Hq, Hkv, Sq) -> int:
+    return int(_capi.load().af3_sink_attention_bwd_workspace_bytes(B, Hq, Hkv, Sq))
+
+
+@functools.lru_cache(maxsize=64)
+def _c_strides(strides: tuple):
+    """``strides`` as a C array (read by the call it is passed to, never written)."""
+    return (ctypes.c_int64 * len(strides))(*strides)
+
+
+def _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, kv_range, out_lo, lse):
+    B, Hq, Sq, D = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    dev = q.device
+    out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=dev)
+    ws_n = _fwd_workspace(B, Hq, Hkv, Sq, Sk, D, window, first)
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
+    _capi.call("af3_sink_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _c_strides(strides),
+               _capi.ptr(sinks), int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(cu_seqlens),
+               cu_seqlens.numel() - 1 if cu_seqlens is not None else 0, _capi.ptr(starts), _capi.ptr(kv_range), B, Hq,
+               Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), out_lo, lse, _capi.ptr(ws), ws_n,
+               _capi.stream_of(dev))
+    return out
 
 
 class _SinkAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, sinks, scale, window, first, starts, kv_range, need_grad):
+    def forward(ctx, q, k, v, sinks, strides, scale, window, first, cu_seqlens, starts, kv_range):
         B, Hq, Sq, D = q.shape
-        Hkv, Sk = k.shape[1], k.shape[2]
-        dev = q.device
-        out = torch.empty(B, Sq, Hq, D, dtype=torch.bfloat16, device=dev)
-        out_lo = torch.empty_like(out) if need_grad else None
-        lse = torch.empty(B, Hq, Sq, dtype=torch.float32, device=dev) if need_grad else None
-        ws_n = int(_capi.load().af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first))
-        ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
-        _capi.call("af3_sink_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
-                   _capi.ptr(sinks), int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
-                   _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), _capi.ptr(out_lo),
-                   _capi.ptr(lse), _capi.ptr(ws), ws_n, _capi.stream_of(dev))
-        if need_grad:
-            ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, out_lo, lse)
-            ctx.args = (scale, window, first)
+        # kept for the backward in one buffer: what rounding the output left, and the rows' log-sums
+        n = B * Hq * Sq
+        keep = torch.empty(n * (2 * D + 4), dtype=torch.uint8, device=q.device)
+        out = _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, kv_range, keep.data_ptr(),
+                       keep.data_ptr() + 2 * D * n)
+        ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, keep)
+        ctx.args = (strides, scale, window, first)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, sinks, starts, kv_range, out, out_lo, lse = ctx.saved_tensors
-        scale, window, first = ctx.args
+        q, k, v, sinks, starts, kv_range, out, keep = ctx.saved_tensors
+        strides, scale, window, first = ctx.args
         B, Hq, Sq, D = q.shape
         Hkv, Sk = k.shape[1], k.shape[2]
         dev = q.device
         with _device_of(q):
-            do = _rows(dout.to(torch.bfloat16).transpose(1, 2), heads=True)
-            dq = torch.empty(B, Sq, Hq, D, dtype=torch.bfloat16, device=dev)
-            dk = torch.empty(B, Sk, Hkv, D, dtype=torch.bfloat16, device=dev)
-            dv = torch.empty_like(dk)
+            do, st = _rows(dout.transpose(1, 2), heads=True)
+            dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=dev)
+            dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=dev)
+            dv = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=dev)
             dsinks = torch.empty_like(sinks) if sinks is not None else None
-            ws_n = int(_capi.load().af3_sink_attention_bwd_workspace_bytes(B, Hq, Hkv, Sq))
+            ws_n = _bwd_workspace(B, Hq, Hkv, Sq)
             ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
             _capi.call("af3_sink_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(),
-                       _strides(q, k, v, do), _capi.ptr(sinks),
+                       _c_strides(strides + st), _capi.ptr(sinks),
                        int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
                        _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(),
-                       out_lo.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _capi.ptr(dsinks), ws.data_ptr(),
-                       ws_n, _capi.stream_of(dev))
-        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dsinks, *[None] * 6
+                       keep.data_ptr(), keep.data_ptr() + 2 * D * B * Hq * Sq, dq.data_ptr(), dk.data_ptr(),
+                       dv.data_ptr(), _capi.ptr(dsinks), ws.data_ptr(), ws_n, _capi.stream_of(dev))
+        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dsinks, *[None] * 7
 
 
 def _check(q, k, v, sinks, scale, window, first):
@@ -122,19 +144,34 @@ def _check(q, k, v, sinks, scale, window, first):
         raise ValueError(f"sink_attention: window and first must not be negative, got {window} and {first}")
 
 
-def _run(q, k, v, sinks, scale, window, first, starts, kv_range):
-    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, sinks))
-    return _SinkAttention.apply(_rows(q, heads=True), _rows(k), _rows(v), sinks.contiguous() if sinks is not None else None,
-                                scale, window, first, starts, kv_range, need)
+def _run(q, k, v, sinks, scale, window, first, cu_seqlens, starts, kv_range):
+    need = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                        or (sinks is not None and sinks.requires_grad))
+    (q, sq), (k, sk), (v, sv) = _rows(q, heads=True), _rows(k), _rows(v)
+    if sinks is not None and not sinks.is_contiguous():
+        sinks = sinks.contiguous()
+    args = (sq + sk + sv, sinks, scale, window, first, cu_seqlens, starts, kv_range)
+    if not need:
+        return _forward(q, k, v, *args, None, None)
+    return _SinkAttention.apply(q, k, v, sinks, sq + sk + sv, *args[2:])
+
+
+def _cu(cu_seqlens: torch.Tensor) -> torch.Tensor:
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
+        raise ValueError(f"cu_seqlens must be a [sequences + 1] integer tensor, got {tuple(cu_seqlens.shape)} "
+                         f"{cu_seqlens.dtype}")
+    if cu_seqlens.dtype != torch.int32:
+        cu_seqlens = cu_seqlens.clamp(-1, MAX_LEN).to(torch.int32)
+    return cu_seqlens.contiguous()
 
 
 def sequence_starts(cu_seqlens: torch.Tensor, n_tokens: int) -> torch.Tensor:
     """[n_tokens] int32: the first token of each token's sequence; t + 1 for a token in none."""
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
-        raise ValueError(f"cu_seqlens must be a [sequences + 1] integer tensor, got {tuple(cu_seqlens.shape)}")
-    cu = cu_seqlens.to(torch.int32).contiguous()
+    cu = _cu(cu_seqlens)
     starts = torch.empty(n_tokens, dtype=torch.int32, device=cu.device)
-    _capi.call("af3_seq_starts", cu.data_ptr(), cu.numel() - 1, n_tokens, starts.data_ptr(), _capi.stream_of(cu.device))
+    with _device_of(cu):
+        _capi.call("af3_seq_starts", cu.data_ptr(), cu.numel() - 1, n_tokens, starts.data_ptr(),
+                   _capi.stream_of(cu.device))
     return starts
 
 
@@ -143,8 +180,9 @@ def sequence_starts_of_positions(position_ids: torch.Tensor) -> torch.Tensor:
     a position is not its predecessor's plus one, as transformers reads them)."""
     pos = position_ids.reshape(-1).to(torch.int64).contiguous()
     starts = torch.empty(pos.numel(), dtype=torch.int32, device=pos.device)
-    _capi.call("af3_seq_starts_positions", pos.data_ptr(), pos.numel(), starts.data_ptr(),
-               _capi.stream_of(pos.device))
+    with _device_of(pos):
+        _capi.call("af3_seq_starts_positions", pos.data_ptr(), pos.numel(), starts.data_ptr(),
+                   _capi.stream_of(pos.device))
     return starts
 
 
@@ -174,7 +212,8 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
     Returns:
         [B, Sq, Hq, D] bf16
     """
-    scale = q.shape[-1] ** -0.5 if scale is None and q.dim() == 4 and q.shape[-1] else (1.0 if scale is None else float(scale))
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     window, first = int(window), int(first)
     _check(q, k, v, sinks, scale, window, first)
     B, _, Sq, _ = q.shape
@@ -191,10 +230,13 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
             if B != 1 or Sq != Sk:
                 raise ValueError(f"sink_attention: a packed row has batch 1 and as many keys as queries, got q "
                                  f"{tuple(q.shape)}, k {tuple(k.shape)}")
-            starts = sequence_starts(cu_seqlens, Sk)
+            cu_seqlens = _cu(cu_seqlens)
+            starts = torch.empty(Sk, dtype=torch.int32, device=q.device)
         if kv_range is not None:
             if kv_range.shape != (B, 2) or kv_range.is_floating_point():
                 raise ValueError(f"sink_attention: kv_range must be a [{B}, 2] integer tensor, got "
                                  f"{tuple(kv_range.shape)} {kv_range.dtype}")
-            kv_range = kv_range.to(torch.int32).contiguous()
-        return _run(q, k, v, sinks, scale, window, first, starts, kv_range)
+            if kv_range.dtype != torch.int32:
+                kv_range = kv_range.clamp(0, Sk).to(torch.int32)
+            kv_range = kv_range.contiguous()
+        return _run(q, k, v, sinks, scale, window, first, cu_seqlens, starts, kv_range)

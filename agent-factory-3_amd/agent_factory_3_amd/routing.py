@@ -302,20 +302,29 @@ def routing(logits: torch.Tensor, n_expts_act: int, sm_first: bool = False, expt
     return _run_routing(logits, n_expts_act, expt_indx)
 
 
+@functools.lru_cache(maxsize=64)
+def _balance_workspace(T: int, E: int) -> int:
+    return int(_capi.load().af3_balance_loss_workspace_bytes(T, E))
+
+
+def _balance_forward(logits, n_expts_act, expt_indx, token_mask):
+    T, E = logits.shape
+    dev = logits.device
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    stats = torch.empty(E + 1, dtype=torch.int32, device=dev)  # (the counts may be changed in place by their owner)
+    ws_n = _balance_workspace(T, E)
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+    _capi.call("af3_balance_loss_fwd", logits.data_ptr(), logits.stride(0) if T > 1 else E, _capi.ptr(expt_indx),
+               _capi.ptr(token_mask), T, E, n_expts_act, loss.data_ptr(), counts.data_ptr(), stats.data_ptr(),
+               ws.data_ptr(), ws_n, _capi.stream_of(dev))
+    return loss, counts, stats
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, n_expts_act, expt_indx, token_mask):
-        T, E = logits.shape
-        dev = logits.device
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        counts = torch.empty(E, dtype=torch.int32, device=dev)
-        stats = torch.empty(E + 1, dtype=torch.int32, device=dev)
-        ws_n = int(_capi.load().af3_balance_loss_workspace_bytes(T, E))
-        ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
-        ld = logits.stride(0) if T > 1 else E
-        _capi.call("af3_balance_loss_fwd", logits.data_ptr(), ld, _capi.ptr(expt_indx), _capi.ptr(token_mask), T, E,
-                   n_expts_act, loss.data_ptr(), counts.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws_n,
-                   _capi.stream_of(dev))
+        loss, counts, stats = _balance_forward(logits, n_expts_act, expt_indx, token_mask)
         ctx.save_for_backward(logits, token_mask, stats)
         ctx.mark_non_differentiable(counts)
         return loss, counts
@@ -325,12 +334,12 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, g, _):
         logits, token_mask, stats = ctx.saved_tensors
         T, E = logits.shape
-        d = torch.empty(T, E, dtype=torch.bfloat16, device=logits.device)
-        g = g.to(device=logits.device, dtype=torch.float32)
+        dev = logits.device
         with _device_of(logits):
+            d = torch.empty((T, E), dtype=torch.bfloat16, device=dev)
             _capi.call("af3_balance_loss_bwd", logits.data_ptr(), logits.stride(0) if T > 1 else E,
                        _capi.ptr(token_mask), T, E, stats.data_ptr(), g.data_ptr(), d.data_ptr(),
-                       _capi.stream_of(logits.device))
+                       _capi.stream_of(dev))
         return d, None, None, None
 
 
@@ -384,7 +393,9 @@ def balance_loss(logits: torch.Tensor, n_expts_act: int, expt_indx: torch.Tensor
                 raise ValueError(f"balance_loss: token_mask is {tuple(token_mask.shape)}, expected {lead}")
             token_mask = token_mask.to(lg.device)
             token_mask = (token_mask if token_mask.dtype == torch.bool else token_mask != 0).contiguous()
-        return _BalanceLoss.apply(lg, K, expt_indx, token_mask)
+        if torch.is_grad_enabled() and lg.requires_grad:
+            return _BalanceLoss.apply(lg, K, expt_indx, token_mask)
+        return _balance_forward(lg, K, expt_indx, token_mask)[:2]
 
 
 def dense_routing(n_rows: int, device) -> RoutingData:

@@ -1080,9 +1080,9 @@ extern "C" size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int
 }
 
 extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
-                                      const void* sinks, int sinks_f32, const int32_t* starts, const int32_t* kv_range,
-                                      int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first, float scale,
-                                      uint16_t* out, uint16_t* out_lo, float* lse, void* workspace, size_t ws_bytes,
+                                      const void* sinks, int sinks_f32, const int32_t* cu_seqlens, int n_seqs,
+                                      int32_t* starts, const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk,
+                                      int D, int window, int first, float scale, uint16_t* out, uint16_t* out_lo, float* lse, void* workspace, size_t ws_bytes,
                                       void* stream_) {
   const char* who = "sink_attention_fwd";
   if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 9, starts, kv_range)) return rc;
@@ -1091,6 +1091,9 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
   AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(out) && sa_al16(out_lo),
               "%s: rows must be 16-byte aligned", who);
   hipStream_t stream = (hipStream_t)stream_;
+  AF3_REQUIRE(!cu_seqlens || starts, "%s: cu_seqlens without starts", who);
+  if (cu_seqlens)
+    if (int rc = af3_seq_starts(cu_seqlens, n_seqs, Sk, starts, stream_)) return rc;
   const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
   SaParams p = sa_params(s, q, k, v, strides, sinks, sinks_f32, starts, kv_range, B, Hq, Hkv, Sq, Sk, scale);
   p.out = out;

@@ -447,7 +447,8 @@ int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_
  * j < (range start) + first (window 0: all of them).  The range is
  * kv_range[b] = (begin, end) (device int32 [B][2], clamped to [0, Sk]; NULL: all
  * keys), or, for a packed row (B = 1, Sq = Sk), from starts[p] (device int32
- * [Sk], af3_seq_starts): the start of the token's own sequence.  sinks [Hq]
+ * [Sk], af3_seq_starts): the start of the token's own sequence; with cu_seqlens
+ * the forward writes starts first (as af3_seq_starts), else it reads them.  sinks [Hq]
  * (bf16, or fp32 with sinks_f32; NULL: none) adds e^sink to the softmax's
  * denominator.  A row that sees nothing gives 0.
  *   forward: out [B][Sq][Hq][D]; out_lo, as out: bf16 of what rounding out left,
@@ -461,9 +462,9 @@ int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_
  * tile sees may reach that tile's other rows.
  * Lengths below 2^29 tokens. */
 int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
-                           const void* sinks, int sinks_f32, const int32_t* starts, const int32_t* kv_range, int B,
-                           int Hq, int Hkv, int Sq, int Sk, int D, int window, int first, float scale, uint16_t* out,
-                           uint16_t* out_lo, float* lse, void* workspace, size_t ws_bytes, void* stream);
+                           const void* sinks, int sinks_f32, const int32_t* cu_seqlens, int n_seqs, int32_t* starts,
+                           const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk, int D, int window,
+                           int first, float scale, uint16_t* out, uint16_t* out_lo, float* lse, void* workspace, size_t ws_bytes, void* stream);
 size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first);
 size_t af3_sink_attention_bwd_workspace_bytes(int B, int Hq, int Hkv, int Sq);
 int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* dout,
