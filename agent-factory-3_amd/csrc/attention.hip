@@ -49,7 +49,7 @@ struct SaParams {
   const int32_t* starts;                  // [Sk] start of each token's sequence (packed row), or NULL
   const int32_t* kv_range;                // [B][2] or NULL
   int B, Hq, Hkv, G, Sq, Sk, window, first;
-  int g_mul;                              // x / G = x g_mul >> 16 for x < 128
+  int g_mul;                              // x / G = x g_mul >> 16 for x < 512
   int tok;                                // tokens of a row tile
   int n_tiles, n_split;
   float scale, scale2;                    // scale2 = scale log2(e)
@@ -78,38 +78,47 @@ __device__ __forceinline__ uint32_t a_lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
-// XOR of a row's 16-byte chunk index: 8 rows' equal chunks (row reads) and 4
-// rows' 2 chunks (transposing reads) fall into distinct bank groups
-__device__ __forceinline__ int a_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+// XOR of a row's 16-byte chunk index.  A 16-byte read takes 16 rows' equal chunks
+// at a time, a transposing read 4 rows' 4 chunks per half wave; over 64 banks (256
+// bytes: two rows of D = 64, one of 128) both then fall into distinct bank groups.
+template <int D>
+__device__ __forceinline__ int a_swz(int row) {
+  if constexpr (D == 64)
+    return ((row & 2) << 1) | ((row >> 1) & 2) | ((row >> 3) & 1);
+  else
+    return ((row & 3) << 2) | ((row >> 2) & 3);
+}
 
 template <int D>
-__device__ __forceinline__ int a_off(int row, int chunk) { return row * (D * 2) + ((chunk ^ a_swz(row)) << 4); }
+__device__ __forceinline__ int a_off(int row, int chunk) { return row * (D * 2) + ((chunk ^ a_swz<D>(row)) << 4); }
 
 // A lane's LDS offsets of the operands it reads from a [rows][D] tile.  The
-// swizzle depends on a row's low three bits alone, so every other row, chunk and
-// column block is a constant away.
+// swizzle depends on a row's low four bits alone, so the same rows further down
+// are a constant away.
 template <int D>
 struct Frag {
-  uint32_t row[4], tr[2];
+  uint32_t row[D / 16], tr[D / 32], tr8_[D / 32];
   __device__ __forceinline__ explicit Frag(int lane) {
     const int r = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) row[x] = a_off<D>(r, 2 * x + h);
+    for (int x = 0; x < D / 16; ++x) row[x] = a_off<D>(r, 2 * x + h);
     const int tr_r = (h << 2) + ((lane & 15) >> 2);
     const int c = (((lane >> 4) & 1) << 4) + ((lane & 3) << 2);
 #pragma unroll
-    for (int d = 0; d < 2; ++d) tr[d] = a_off<D>(tr_r, (d * 32 + c) >> 3) + ((c & 7) << 1);
+    for (int d = 0; d < D / 32; ++d) {
+      tr[d] = a_off<D>(tr_r, (d * 32 + c) >> 3) + ((c & 7) << 1);
+      tr8_[d] = a_off<D>(tr_r + 8, (d * 32 + c) >> 3) + ((c & 7) << 1);
+    }
   }
-  // chunk 2 x + h of row r0 + lane % 32 of the tile at LDS address `tile` (r0 % 8 == 0)
+  // chunk 2 x + h of row r0 + lane % 32 of the tile at LDS address `tile` (r0 % 32 == 0)
   __device__ __forceinline__ af3_bf16x8 row8(uint32_t tile, int r0, int x) const {
     typedef const __attribute__((address_space(3))) af3_bf16x8 T;
-    return *(T*)(tile + row[x & 3] + (uint32_t)((x >> 2) * 128 + r0 * D * 2));
+    return *(T*)(tile + row[x] + (uint32_t)(r0 * D * 2));
   }
-  // rows r0 + 4 h .. + 3 and r0 + 8 + 4 h .. + 3 of column 32 d + lane % 32
+  // rows r0 + 4 h .. + 3 and r0 + 8 + 4 h .. + 3 of column 32 d + lane % 32 (r0 % 16 == 0)
   __device__ __forceinline__ af3_bf16x8 tr8(uint32_t tile, int r0, int d) const {
-    const uint32_t at = tile + tr[d & 1] + (uint32_t)((d >> 1) * 128 + r0 * D * 2);
-    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)at);
-    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at + 8 * D * 2));
+    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + tr[d] + (uint32_t)(r0 * D * 2)));
+    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + tr8_[d] + (uint32_t)(r0 * D * 2)));
     return af3_bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 };
@@ -254,7 +263,7 @@ struct KvCopy {
 #pragma unroll
     for (int x = 0; x < N; ++x) {
       const int row = row0 + x * RPI;
-      off[x] = (uint32_t)(row * (int)st + (((lane % CH) ^ a_swz(row)) << 3)) * 2;
+      off[x] = (uint32_t)(row * (int)st + (((lane % CH) ^ a_swz<D>(row)) << 3)) * 2;
     }
   }
   __device__ __forceinline__ void operator()(int j0, int last, uint32_t lds, int wave) const {
@@ -546,12 +555,17 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
   a_kv_range(p, b, lo, hi);
   const int row_lo = p.starts ? p.starts[t] : lo;
   const int tile_lo = p.starts ? p.starts[t0] : lo;
-  const int tile_hi_lo = p.starts ? p.starts[t1] : lo;
+  const int last_lo = p.starts ? p.starts[t1] : lo;
   const Vis vis = a_vis(p, t + off, row_lo, hi);
   const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
   const int wt0 = t0 + (wave * 32 * p.g_mul >> 16), wt1 = min(t1, t0 + ((wave * 32 + 31) * p.g_mul >> 16));
-  const int wpos0 = wt0 + off, wpos1 = wt1 + off, wlo1 = tile_hi_lo;
+  const int wpos0 = wt0 + off, wpos1 = wt1 + off;
+  const int from = p.window > 0 ? max(last_lo + p.first, wpos1 - p.window + 1) : last_lo;
+  const int own1 = wt0 > t1 ? 0 : min(na + nb, na + max(0, wpos1 - ks.b0 + kBN) / kBN);
+  const int own0 = p.window > 0 && p.first == 0 ? na + max(0, wpos0 - p.window + 1 - ks.b0) / kBN : 0;
+  const int free0 = na + max(0, from - ks.b0 + kBN - 1) / kBN;
+  const int free1 = na + max(0, min(wpos0 + 1, ks.b1) - ks.b0) / kBN;
 
   const KvCopy<D> kc(p.k + b * p.k_sb + hk * p.k_sh, p.k_st, wave, lane);
   const KvCopy<D> vc(p.v + b * p.v_sb + hk * p.v_sh, p.v_st, wave, lane);
@@ -608,37 +622,52 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
     A_BARRIER();
     if (i + 1 < na + nb) issue(i + 1, (i + 1) & 1);
     const uint32_t kt = lds0 + (uint32_t)((i & 1) * 2 * kTile), vt = kt + kTile;
-    const int j0 = first_key(i);
-    if (wt0 > t1 || j0 > wpos1) continue;
-    if (i >= na && p.window > 0 && p.first == 0 && j0 + kBN - 1 <= wpos0 - p.window) continue;
+    if (i < own0 || i >= own1) continue;
+    // (reads ahead of their use, held by the barriers, as in the dk / dv kernel)
+    af3_bf16x8 kr[KS], vr[KS], tr[DB];
+#pragma unroll
+    for (int x = 0; x < KS; ++x) kr[x] = fr.row8(kt, 0, x);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       af3_f32x16 s[1] = {a_zero()}, dp;
 #pragma unroll
+      for (int x = 0; x < KS; ++x) vr[x] = fr.row8(vt, c * 32, x);
+#pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = -delta;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) s[0] = a_mfma(fr.row8(kt, c * 32, x), qf[x], s[0]);
+      for (int x = 0; x < KS; ++x) s[0] = a_mfma(kr[x], qf[x], s[0]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < KS; ++x) dp = a_mfma(fr.row8(vt, c * 32, x), df[x], dp);
+      for (int d = 0; d < DB; ++d) tr[d] = fr.tr8(kt, c * 32, d);
+#pragma unroll
+      for (int x = 0; x < KS; ++x) dp = a_mfma(vr[x], df[x], dp);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -lse)) * dp[r];
       // (the product is set to zero, not the score: whatever stands at a key that the row does not see)
-      const int jc = j0 + c * 32 + 4 * lh;
-      if (i < na) {
-        a_mask_end(s, jc, min(vis.lo + vis.fn, ks.a1), 0.f);
-        a_mask_from(s, jc, vis.lo, 0.f);
-      } else if (p.first > 0 && j0 < wlo1 + p.first) {
-        a_mask_both(s, jc, vis, 0.f);
-      } else {
-        if (j0 + kBN - 1 > wpos0 || j0 + kBN > ks.b1) a_mask_end(s, jc, vis.end, 0.f);
-        if (j0 < wlo1 || (p.window > 0 && j0 <= wpos1 - p.window)) a_mask_from(s, jc, vis.w, 0.f);
+      if (i < free0 || i >= free1) {
+        const int j = first_key(i) + c * 32;
+        if (i < na) {
+          a_mask_end(s, j + 4 * lh, min(vis.lo + vis.fn, ks.a1), 0.f);
+          a_mask_from(s, j + 4 * lh, vis.lo, 0.f);
+        } else if (p.first > 0 && j < last_lo + p.first) {
+          a_mask_both(s, j + 4 * lh, vis, 0.f);
+        } else {
+          if (j + 31 > wpos0 || j + 32 > ks.b1) a_mask_end(s, j + 4 * lh, vis.end, 0.f);
+          if (j < from) a_mask_from(s, j + 4 * lh, vis.w, 0.f);
+        }
       }
+      const af3_bf16x8 p0 = a_pack8(s[0], 0), p1 = a_pack8(s[0], 1);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const af3_bf16x8 pf = a_pack8(s[0], u);
+      for (int d = 0; d < DB; ++d) acc[d] = a_mfma(tr[d], p0, acc[d]);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) acc[d] = a_mfma(fr.tr8(kt, c * 32 + u * 16, d), pf, acc[d]);
-      }
+      for (int d = 0; d < DB; ++d) tr[d] = fr.tr8(kt, c * 32 + 16, d);
+      if (c == 0)
+#pragma unroll
+        for (int x = 0; x < KS; ++x) kr[x] = fr.row8(kt, 32, x);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] = a_mfma(tr[d], p1, acc[d]);
     }
   }
   if (!valid) return;
@@ -674,19 +703,18 @@ __global__ __launch_bounds__(256) void sa_dsink_kernel(const float* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// backward, keys: dk and dv.  Block = 128 keys of one key/value head, K and V
-// rows in registers; the (token, head) rows that see them go through a
-// two-stage LDS ring, 128 at a time (q, dout, and their lse, delta, position and
-// sequence start).  Waves 0-3 (32 keys each) take the first 64 rows of a step,
-// waves 4-7 the others, and their sums are joined at the end: two waves per
-// SIMD, so that one's exponentials run beside the other's products, and half
-// the steps for the first keys, which every later row sees.  S = Q K^T puts a
-// key's column into its lane; the sum over the heads that share the key is the
-// sum over rows.
+// backward, keys: dk and dv.  Block = 64 keys of one key/value head, K and V rows
+// in registers; the (token, head) rows that see them go through a two-stage LDS
+// ring, 128 at a time (q, dout, and their lse, delta and what they see).  Waves 0
+// and 1 (32 keys each) take the first 64 rows of a step, waves 2 and 3 the others,
+// and their sums are joined at the end.  S = Q K^T puts a key's column into its
+// lane; the sum over the heads that share the key is the sum over rows.  Two
+// blocks fit a CU (D = 64), each at its own point of a step, so that one's
+// exponentials run beside the other's products.  Kernel time, packed 8192 tokens,
+// 64/8 heads, window 128 / full attention: 64 keys x 128 rows 82 / 855 us, 64 x
+// 256 (one block of 8 waves per CU) 103 / 816, 128 x 128 (8 waves) 103 / 917, 128
+// x 64 (4 waves) 89 / 1360.
 // ---------------------------------------------------------------------------
-constexpr int kKeys = 128;  // keys of a block
-constexpr int kRT = 128;    // rows of a step
-
 // first token after t0 whose sequence starts later than t0's (starts does not
 // decrease), or n: 64 probes a round, the answer stays in (lo, hi]
 __device__ __forceinline__ int a_sequence_end(const int32_t* starts, int t0, int n, int lane) {
@@ -702,11 +730,14 @@ __device__ __forceinline__ int a_sequence_end(const int32_t* starts, int t0, int
   return hi;
 }
 
+constexpr int KG = 2, NH = 2;                                      // key groups, row groups (waves: KG NH)
+constexpr int kKeys = 32 * KG, kRT = 64 * NH, kDkvWaves = KG * NH;  // keys of a block, rows of a step
+
 template <int D>
-__global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
+__global__ __launch_bounds__(64 * kDkvWaves, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kRT * D * 2;
-  constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / 8;  // chunks per row, rows per copy, copies per wave
+  constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / kDkvWaves;  // chunks per row, rows per copy, copies per wave
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
   __shared__ __attribute__((aligned(16))) float st_lse[2][kRT], st_delta[2][kRT];
   __shared__ __attribute__((aligned(16))) int st_w[2][kRT], st_wn[2][kRT], st_lo[2][kRT], st_fn[2][kRT];
@@ -715,13 +746,13 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
   const int b = bh / p.Hkv, hk = bh % p.Hkv;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = wave >> 2;  // rows 64 half .. + 63 of a step
+  const int part = wave / KG;  // rows 64 part .. + 63 of a step
   const int lr = lane & 31, lh = lane >> 5;
   const int off = p.Sk - p.Sq;
   int lo, hi;
   a_kv_range(p, b, lo, hi);
   const int jl = min(j0 + kKeys, p.Sk) - 1;  // last key of the block
-  const int jw = j0 + (wave & 3) * 32;       // first key of the wave
+  const int jw = j0 + (wave % KG) * 32;      // first key of the wave
   const int j = jw + lr;
   const bool kvalid = j <= jl;
 
@@ -757,78 +788,67 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
   const uint16_t* qb = p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
   const uint16_t* db = p.dout + b * p.do_sb + (int64_t)hk * p.G * p.do_sh;
   const int64_t sb = ((int64_t)b * p.Hkv + hk) * p.Sq * p.G + (int64_t)ta * p.G;
-  // (token, head) of the thread's rows, kept from step to step (no division)
-  const int adv_t = kRT / p.G, adv_g = kRT % p.G;
-  int ct[N], cg[N], rt, rg;
-#pragma unroll
-  for (int x = 0; x < N; ++x) {
-    const int row = (wave * N + x) * RPI + lane / CH;
-    ct[x] = ta + row / p.G;
-    cg[x] = row % p.G;
-  }
-  rt = ta + (int)threadIdx.x / p.G;
-  rg = (int)threadIdx.x % p.G;
-  // tokens of the first and the last row of the wave's half of a step
-  int ut[2] = {ta + half * 64 / p.G, ta + (half * 64 + 63) / p.G}, ug[2] = {half * 64 % p.G, (half * 64 + 63) % p.G};
-  float v_lse = 0.f, v_delta = 0.f;
-  Vis v_vis = {};
-  int v_n = 0;
-  // copies: where 128 rows are whole tokens, lane offsets never change and the
-  // scalar base moves on; else, and in the last step, each row is looked up
+  // Steps run from the last rows back, so that the blocks of a head, which all end
+  // at the same rows, read them at about the same time (out of the XCD's L2; from
+  // each block's own first row on, every block read other rows: 1194 TODO us).
+  // nt, ng: token and head of the first row of the step to be copied next.
+  const int back = (int)((n_rows - 1) & (kRT - 1)), back_t = (int)((uint32_t)back * p.g_mul >> 16);
+  const int adv_t = kRT / p.G, adv_g = kRT - adv_t * p.G;
+  int nt = tb - 1 - back_t, ng = p.G - 1 - (back - back_t * p.G);
+  // Copies: where 128 rows are whole tokens, lane offsets never change and the
+  // scalar base moves on; else, and in the last rows' step, each row is looked up.
   const bool even = adv_g == 0;
   uint32_t qo[N], od[N];
 #pragma unroll
   for (int x = 0; x < N; ++x) {
-    const int row = (wave * N + x) * RPI + lane / CH;
-    const int col = ((lane % CH) ^ a_swz(row)) << 3;
-    qo[x] = (uint32_t)((ct[x] - ta) * (int)p.q_st + cg[x] * (int)p.q_sh + col) * 2;
-    od[x] = (uint32_t)((ct[x] - ta) * (int)p.do_st + cg[x] * (int)p.do_sh + col) * 2;
+    const int row = (wave * N + x) * RPI + lane / CH, t = row * p.g_mul >> 16, g = row - t * p.G;
+    const int col = ((lane % CH) ^ a_swz<D>(row)) << 3;
+    qo[x] = (uint32_t)(t * (int)p.q_st + g * (int)p.q_sh + col) * 2;
+    od[x] = (uint32_t)(t * (int)p.do_st + g * (int)p.do_sh + col) * 2;
   }
+  float v_lse = 0.f, v_delta = 0.f;
+  int v_t = 0, v_start = lo;
   auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..127
     const uint32_t st = lds0 + (uint32_t)((i & 1) * 2 * kTile + wave * N * 1024);
-    if (even && (int64_t)(i + 1) * kRT <= n_rows) {
-      const int64_t t = ta + (int64_t)i * adv_t;
+    if (even && i < n_steps - 1) {
+      const uint16_t *q0 = qb + nt * p.q_st, *d0 = db + nt * p.do_st;
 #pragma unroll
       for (int x = 0; x < N; ++x) {
-        a_dma16_s(qb + t * p.q_st, qo[x], st + x * 1024);
-        a_dma16_s(db + t * p.do_st, od[x], st + kTile + x * 1024);
+        a_dma16_s(q0, qo[x], st + x * 1024);
+        a_dma16_s(d0, od[x], st + kTile + x * 1024);
       }
     } else {
 #pragma unroll
       for (int x = 0; x < N; ++x) {
-        const int row = (wave * N + x) * RPI + lane / CH;
-        const int64_t t = min((even ? i * adv_t : 0) + ct[x], tb - 1), g = cg[x];
-        const int col = ((lane % CH) ^ a_swz(row)) << 3;
+        const int row = (wave * N + x) * RPI + lane / CH, y = ng + row, yt = y * p.g_mul >> 16;
+        const int64_t t = min(nt + yt, tb - 1), g = y - yt * p.G;
+        const int col = ((lane % CH) ^ a_swz<D>(row)) << 3;
         a_dma16(qb + t * p.q_st + g * p.q_sh + col, st + x * 1024);
         a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + x * 1024);
-        if (!even) {
-          ct[x] += adv_t;
-          cg[x] += adv_g;
-          if (cg[x] >= p.G) cg[x] -= p.G, ++ct[x];
-        }
       }
     }
     if (threadIdx.x < kRT) {
       const int64_t r = min((int64_t)i * kRT + threadIdx.x, n_rows - 1);
       v_lse = p.lse[sb + r];
       v_delta = p.delta[sb + r];
-      const int t = min(rt, tb - 1);
-      v_vis = a_vis(p, t + off, p.starts ? p.starts[t] : lo, hi);
-      v_n = rt < tb ? max(0, v_vis.end - v_vis.w) : 0;
-      if (rt >= tb) v_vis.fn = 0;
-      rt += adv_t;
-      rg += adv_g;
-      if (rg >= p.G) rg -= p.G, ++rt;
+      v_t = nt + ((ng + (int)threadIdx.x) * p.g_mul >> 16);
+      if (p.starts) v_start = p.starts[min(v_t, tb - 1)];  // (used after the next wait: here it would wait for the copies)
     }
+    nt -= adv_t;
+    ng -= adv_g;
+    if (ng < 0) ng += p.G, --nt;
   };
   auto store_rows = [&](int i) {
     if (threadIdx.x < kRT) {
       st_lse[i & 1][threadIdx.x] = v_lse;
       st_delta[i & 1][threadIdx.x] = -v_delta;
-      st_w[i & 1][threadIdx.x] = v_vis.w;
-      st_wn[i & 1][threadIdx.x] = v_n;
-      st_lo[i & 1][threadIdx.x] = v_vis.lo;
-      st_fn[i & 1][threadIdx.x] = v_vis.fn;
+      const Vis v = a_vis(p, min(v_t, tb - 1) + off, v_start, hi);
+      st_w[i & 1][threadIdx.x] = v.w;
+      st_wn[i & 1][threadIdx.x] = v_t < tb ? max(0, v.end - v.w) : 0;
+      if (p.first > 0) {
+        st_lo[i & 1][threadIdx.x] = v.lo;
+        st_fn[i & 1][threadIdx.x] = v_t < tb ? v.fn : 0;
+      }
     }
   };
 
@@ -836,60 +856,78 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
   af3_f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = a_zero(), dv[d] = a_zero();
-  if (n_steps > 0) issue(0);
-  for (int i = 0; i < n_steps; ++i) {
+  if (n_steps > 0) issue(n_steps - 1);
+  for (int i = n_steps - 1; i >= 0; --i) {
     A_WAIT_VM(0);
     store_rows(i);
     A_BARRIER();
-    if (i + 1 < n_steps) issue(i + 1);
-    const uint32_t qt = lds0 + (uint32_t)((i & 1) * 2 * kTile + half * (kTile / 2)), dt = qt + kTile;
-    const int w = i & 1, rb = half * 64;
+    const int ct = nt + adv_t + (ng + adv_g >= p.G), cg = ng + adv_g - (ng + adv_g >= p.G ? p.G : 0);  // this step's first row
+    if (i > 0) issue(i - 1);
+    const uint32_t qt = lds0 + (uint32_t)((i & 1) * 2 * kTile + part * (64 * D * 2)), dt = qt + kTile;
+    const int w = i & 1, rb = part * 64;
     // the half's tokens; what rows see does not begin earlier from one to the next
     const int64_t r0 = (int64_t)i * kRT + rb;
     const bool full = r0 + 64 <= n_rows;  // rows past the last see nothing
-    const int pos0 = ut[0] + off, pos1 = min(ut[1], tb - 1) + off;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      ut[x] += adv_t;
-      ug[x] += adv_g;
-      if (ug[x] >= p.G) ug[x] -= p.G, ++ut[x];
-    }
+    const int pos0 = ct + ((cg + rb) * p.g_mul >> 16) + off;
+    const int pos1 = min(ct + ((cg + rb + 63) * p.g_mul >> 16), tb - 1) + off;
     if (r0 >= n_rows || jw > pos1) continue;  // none of the wave's keys is seen
     const int w0 = __builtin_amdgcn_readfirstlane(st_w[w][rb]);
     const int w1 = __builtin_amdgcn_readfirstlane(st_w[w][rb + 63]);
     if (p.first == 0 && jw + 31 < w0) continue;
     const bool whole = full && wave_in && jw + 31 <= pos0 && jw >= w1;
+    // LDS reads stand well before their use (the barriers hold the order): a read
+    // right at its product costs its whole latency, 16 times a step.
+    af3_bf16x8 qr[KS], dr[KS], td[DB], tq[DB];
+#pragma unroll
+    for (int x = 0; x < KS; ++x) qr[x] = fr.row8(qt, 0, x);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) dr[x] = fr.row8(dt, 0, x);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+      const int at = rb + c * 32 + 4 * lh;  // registers 4 q .. + 3: rows at + 8 q .. + 3
       af3_f32x16 s = a_zero(), dp;
+      float4 ls[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {  // dp starts at -delta
-        const float4 de = *(const float4*)&st_delta[w][rb + c * 32 + 8 * q + 4 * lh];
+        const float4 de = *(const float4*)&st_delta[w][at + 8 * q];
         dp[4 * q] = de.x; dp[4 * q + 1] = de.y; dp[4 * q + 2] = de.z; dp[4 * q + 3] = de.w;
+        ls[q] = *(const float4*)&st_lse[w][at + 8 * q];
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < KS; ++x) s = a_mfma(fr.row8(qt, c * 32, x), kf[x], s);
+      for (int x = 0; x < KS; ++x) s = a_mfma(qr[x], kf[x], s);
 #pragma unroll
-      for (int x = 0; x < KS; ++x) dp = a_mfma(fr.row8(dt, c * 32, x), vf[x], dp);
+      for (int x = 0; x < KS; ++x) dp = a_mfma(dr[x], vf[x], dp);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        td[d] = fr.tr8(dt, c * 32, d);
+        tq[d] = fr.tr8(qt, c * 32, d);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float4 ls = *(const float4*)&st_lse[w][rb + c * 32 + 8 * q + 4 * lh];
-        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w};
+        const float lsv[4] = {ls[q].x, ls[q].y, ls[q].z, ls[q].w};
 #pragma unroll
         for (int y = 0; y < 4; ++y) s[4 * q + y] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + y], p.scale2, -lsv[y]));
       }
       if (!whole) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int at = rb + c * 32 + 8 * q + 4 * lh;
-          const int4 w4 = *(const int4*)&st_w[w][at], n4 = *(const int4*)&st_wn[w][at];
+          const int4 w4 = *(const int4*)&st_w[w][at + 8 * q], n4 = *(const int4*)&st_wn[w][at + 8 * q];
           const int wv[4] = {w4.x, w4.y, w4.z, w4.w}, nv[4] = {n4.x, n4.y, n4.z, n4.w};
+          bool on[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) on[y] = (uint32_t)(jm - wv[y]) < (uint32_t)nv[y];
+          if (p.first > 0) {
+            const int4 l4 = *(const int4*)&st_lo[w][at + 8 * q], f4 = *(const int4*)&st_fn[w][at + 8 * q];
+            const int lv[4] = {l4.x, l4.y, l4.z, l4.w}, fv[4] = {f4.x, f4.y, f4.z, f4.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) on[y] |= (uint32_t)(jm - lv[y]) < (uint32_t)fv[y];
+          }
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            bool on = (uint32_t)(jm - wv[y]) < (uint32_t)nv[y];
-            if (p.first > 0) on = on || (uint32_t)(jm - st_lo[w][at + y]) < (uint32_t)st_fn[w][at + y];
-            s[4 * q + y] = on ? s[4 * q + y] : 0.f;
-            dp[4 * q + y] = on ? dp[4 * q + y] : 0.f;
+            s[4 * q + y] = on[y] ? s[4 * q + y] : 0.f;
+            dp[4 * q + y] = on[y] ? dp[4 * q + y] : 0.f;
           }
         }
       }
@@ -900,38 +938,62 @@ __global__ __launch_bounds__(512, 2) void sa_dkv_kernel(SaParams p) {
         const af3_bf16x8 pf = a_pack8(s, u), sf = a_pack8(dp, u);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          dv[d] = a_mfma(fr.tr8(dt, c * 32 + u * 16, d), pf, dv[d]);
-          dk[d] = a_mfma(fr.tr8(qt, c * 32 + u * 16, d), sf, dk[d]);
+          dv[d] = a_mfma(td[d], pf, dv[d]);
+          dk[d] = a_mfma(tq[d], sf, dk[d]);
         }
+        if (u == 0) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            td[d] = fr.tr8(dt, c * 32 + 16, d);
+            tq[d] = fr.tr8(qt, c * 32 + 16, d);
+          }
+        } else if (c == 0) {
+#pragma unroll
+          for (int x = 0; x < KS; ++x) qr[x] = fr.row8(qt, 32, x);
+#pragma unroll
+          for (int x = 0; x < KS; ++x) dr[x] = fr.row8(dt, 32, x);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
-  // waves 4-7 hand their sums to waves 0-3 through the ring's LDS
-  A_BARRIER();
-  float* sum = (float*)lds + ((wave & 3) * 64 + lane) * 4;  // four values of a lane, then the next four 4 KB on
-  if (half) {
+  // the first waves take the other row groups' sums, one group after another, through the ring's LDS
+  float* sum = (float*)lds + ((wave % KG) * 64 + lane) * 4;  // four values of a lane, then the next four KG KB on
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+  for (int x = 1; x < NH; ++x) {
+    A_BARRIER();
+    if (part == x) {
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        *(float4*)(sum + (d * 8 + r / 4) * 1024) = float4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
-        *(float4*)(sum + (d * 8 + 4 + r / 4) * 1024) = float4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
-      }
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          *(float4*)(sum + (d * 8 + r / 4) * KG * 256) = float4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+          *(float4*)(sum + (d * 8 + 4 + r / 4) * KG * 256) = float4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+        }
+    }
+    A_BARRIER();
+    if (part == 0) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const float4 k4 = *(const float4*)(sum + (d * 8 + r / 4) * KG * 256);
+          const float4 v4 = *(const float4*)(sum + (d * 8 + 4 + r / 4) * KG * 256);
+          dk[d][r] += k4.x; dk[d][r + 1] += k4.y; dk[d][r + 2] += k4.z; dk[d][r + 3] += k4.w;
+          dv[d][r] += v4.x; dv[d][r + 1] += v4.y; dv[d][r + 2] += v4.z; dv[d][r + 3] += v4.w;
+        }
+    }
   }
-  A_BARRIER();
-  if (half || !kvalid) return;
+  if (part || !kvalid) return;
   const int64_t o = (((int64_t)b * p.Sk + j) * p.Hkv + hk) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const float4 k4 = *(const float4*)(sum + (d * 8 + r / 4) * 1024);
-      const float4 v4 = *(const float4*)(sum + (d * 8 + 4 + r / 4) * 1024);
       const int64_t c = o + d * 32 + 2 * r + 4 * lh;
-      *(u32x2*)(p.dv + c) = u32x2{af3_pack_bf16x2(dv[d][r] + v4.x, dv[d][r + 1] + v4.y),
-                                  af3_pack_bf16x2(dv[d][r + 2] + v4.z, dv[d][r + 3] + v4.w)};
-      *(u32x2*)(p.dk + c) = u32x2{af3_pack_bf16x2((dk[d][r] + k4.x) * p.scale, (dk[d][r + 1] + k4.y) * p.scale),
-                                  af3_pack_bf16x2((dk[d][r + 2] + k4.z) * p.scale, (dk[d][r + 3] + k4.w) * p.scale)};
+      *(u32x2*)(p.dv + c) = u32x2{af3_pack_bf16x2(dv[d][r], dv[d][r + 1]), af3_pack_bf16x2(dv[d][r + 2], dv[d][r + 3])};
+      *(u32x2*)(p.dk + c) = u32x2{af3_pack_bf16x2(dk[d][r] * p.scale, dk[d][r + 1] * p.scale),
+                                  af3_pack_bf16x2(dk[d][r + 2] * p.scale, dk[d][r + 3] * p.scale)};
     }
 }
 
@@ -1154,7 +1216,7 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = (float*)workspace;
   p.dsink_part = (float*)((uint8_t*)workspace + sa_up((size_t)B * Hq * Sq * 4));
-  const unsigned gq = (unsigned)((int64_t)s.n_tiles * B * Hkv), gk = (unsigned)(af3_cdiv(Sk, kKeys) * B * Hkv);
+  const unsigned gq = (unsigned)((int64_t)s.n_tiles * B * Hkv);
   if (gq) {
     if (D == 64)
       hipLaunchKernelGGL(sa_dq_kernel<64>, dim3(gq), dim3(256), 0, stream, p);
@@ -1164,11 +1226,12 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
   if (sinks)  // (no query rows: a sum over nothing)
     hipLaunchKernelGGL(sa_dsink_kernel, dim3(Hq), dim3(256), 0, stream, p.dsink_part, s.n_tiles * B, Hq, sinks_f32,
                        dsinks);
-  if (gk) {
+  if (nk) {
+    const dim3 grid((unsigned)(af3_cdiv(Sk, kKeys) * B * Hkv)), block(64 * kDkvWaves);
     if (D == 64)
-      hipLaunchKernelGGL(sa_dkv_kernel<64>, dim3(gk), dim3(512), 0, stream, p);
+      hipLaunchKernelGGL(sa_dkv_kernel<64>, grid, block, 0, stream, p);
     else
-      hipLaunchKernelGGL(sa_dkv_kernel<128>, dim3(gk), dim3(512), 0, stream, p);
+      hipLaunchKernelGGL(sa_dkv_kernel<128>, grid, block, 0, stream, p);
   }
   return af3::check_launch(who);
 }
