@@ -8,9 +8,9 @@ sequences (the reference's collator packs them, data_collator_with_packing.py:
 5-93) or a few new tokens at the end of a cache.  The HIP kernels are behind
 ``af3_sink_attention_fwd`` / ``_bwd``; there is no CPU fallback.
 
-Importing this module registers it with transformers as ``attn_implementation=
-"af3_sink"`` (``register``; ``quantizer_config`` imports it): gpt-oss has no
-sdpa form there, and its flash forms with sinks are CUDA kernels.
+``register`` makes it transformers' ``attn_implementation="af3_sink"`` (importing
+``quantizer_config`` calls it): gpt-oss has no sdpa form there, its flash forms
+with sinks are CUDA kernels, and its eager form holds the [heads, S, S] scores.
 """
 from __future__ import annotations
 
@@ -240,3 +240,77 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
                 kv_range = kv_range.clamp(0, Sk).to(torch.int32)
             kv_range = kv_range.contiguous()
         return _run(q, k, v, sinks, scale, window, first, cu_seqlens, starts, kv_range)
+
+
+# ---------------------------------------------------------------------------
+# transformers: attn_implementation="af3_sink"
+# ---------------------------------------------------------------------------
+
+ATTN_IMPLEMENTATION = "af3_sink"
+
+
+def attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None,
+                   use_vmap=False, **kwargs):
+    """What transformers hands every layer as its mask (causal order and window are
+    the attention's own): None, or [B, 2] int32 key ranges of a batch padded on
+    either side.  Reads the padding mask once per forward (a host synchronisation,
+    as its flash forms do)."""
+    if use_vmap:
+        raise NotImplementedError("af3_sink: custom mask functions are not supported")
+    if isinstance(q_offset, torch.Tensor) or kv_offset + kv_length != q_offset + q_length:
+        raise NotImplementedError("af3_sink: the last key must be the last query's (a cache that grows, "
+                                  "not one of fixed length)")
+    if attention_mask is None:
+        return None
+    m = attention_mask[:, kv_offset:kv_offset + kv_length].to(torch.int32)
+    if m.shape[1] != kv_length:
+        raise ValueError(f"af3_sink: the attention mask covers {attention_mask.shape[1]} tokens, the keys reach "
+                         f"{kv_offset + kv_length}")
+    n = m.sum(1)
+    begin = m.argmax(1)
+    end = kv_length - m.flip(1).argmax(1)
+    end = torch.where(n == 0, begin, end)
+    holes, full = torch.stack([(end - begin != n).any(), (n == kv_length).all()]).tolist()
+    if holes:
+        raise ValueError("af3_sink: a row of the attention mask must be one run of tokens (packed sequences go by "
+                         "position_ids or cu_seq_lens_q)")
+    return None if full else torch.stack([begin, end], 1).to(torch.int32)
+
+
+def attention_forward(module, query, key, value, attention_mask, scaling=None, dropout=0.0, sliding_window=None,
+                      s_aux=None, **kwargs):
+    """transformers' attention interface over ``sink_attention``: query [B, Hq, Sq, D]
+    -> ([B, Sq, Hq, D], None).  A packed row (B = 1) is read from ``cu_seq_lens_q``
+    or, like its flash forms, from position ids that start again."""
+    if dropout:
+        raise NotImplementedError("af3_sink: attention dropout is not supported")
+    causal = kwargs.get("is_causal")
+    if not (getattr(module, "is_causal", True) if causal is None else causal):
+        raise NotImplementedError("af3_sink: only causal attention is supported")
+    if attention_mask is not None and attention_mask.shape != (query.shape[0], 2):
+        raise ValueError("af3_sink: the mask must be the one that its own mask function makes (or None), got "
+                         f"{tuple(attention_mask.shape)}")
+    if s_aux is not None and s_aux.dtype not in (torch.bfloat16, torch.float32):
+        s_aux = s_aux.float()
+    args = dict(scale=scaling, window=sliding_window or 0, kv_range=attention_mask)
+    cu, pos = kwargs.get("cu_seq_lens_q"), kwargs.get("position_ids")
+    if cu is not None:
+        cu_k = kwargs.get("cu_seq_lens_k")
+        if cu_k is not None and cu_k is not cu and cu_k.shape != cu.shape:
+            raise ValueError("af3_sink: cu_seq_lens_q and cu_seq_lens_k differ")
+        return sink_attention(query, key, value, s_aux, cu_seqlens=cu, **args), None
+    if (pos is not None and attention_mask is None and query.shape[0] == 1 and query.shape[2] == key.shape[2] > 1
+            and pos.numel() == query.shape[2]):
+        starts = sequence_starts_of_positions(pos.to(query.device))
+        scale = query.shape[-1] ** -0.5 if scaling is None else scaling
+        _check(query, key, value, s_aux, scale, args["window"], 0)
+        with _device_of(query):
+            return _run(query, key, value, s_aux, scale, min(args["window"], MAX_LEN), 0, None, starts, None), None
+    return sink_attention(query, key, value, s_aux, **args), None
+
+
+def register() -> None:
+    """Register with transformers as attn_implementation="af3_sink" (again is harmless)."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+    AttentionInterface.register(ATTN_IMPLEMENTATION, attention_forward)
+    AttentionMaskInterface.register(ATTN_IMPLEMENTATION, attention_mask)

@@ -52,6 +52,7 @@ from torch import nn
 from . import _capi, kernels
 from .kernels import mxfp4_to_bf16_hip, swiglu_backward_raw, swiglu_forward
 from .routing import (  # noqa: F401  (re-exported names of the routing layer)
+    _COLLECTORS,
     SHORT_TILES, ExptData, GatherIndx, RoutingData, ScatterIndx, compute_expt_data, compute_expt_data_torch,
     dense_routing, gemm_order_for, max_tiles, router_linear, routing, routing_replay,
 )
@@ -1306,7 +1307,10 @@ def mlp_forward(self, hidden_states, router_indices=None):
                                                                          dtype=torch.int32)
             routing_data, gather_idx, scatter_idx = routing_replay(router_logits, expt_indx, self.router.top_k)
         else:
+            expt_indx = None
             routing_data, gather_idx, scatter_idx = route(router_logits, self.router.top_k)
+        if _COLLECTORS:  # collect_balance
+            _COLLECTORS[-1].add(self, router_logits, self.router.top_k, expt_indx)
     routed_out = self.experts(hidden_states, routing_data, gather_idx, scatter_idx=scatter_idx)
     routed_out = routed_out.reshape(batch_size, -1, self.router.hidden_dim)
     return routed_out, router_logits

@@ -12,7 +12,8 @@ reference's ``quantizer_config.py:49-226``:
 
 Differences: the environment check asks for a ROCm GPU with the built HIP
 library instead of Triton / the kernels hub, and nothing is fetched from the
-network.  ``dequant_dtype`` "bf16" and "fp8" are both served by the HIP path.  Importing this module registers the config (once per process).
+network.  ``dequant_dtype`` "bf16" and "fp8" are both served by the HIP path.  Importing this module registers the config (once per process),
+and ``attn_implementation="af3_sink"`` (``attention.register``).
 """
 from __future__ import annotations
 
@@ -129,6 +130,8 @@ def register() -> None:
         auto.register_quantization_config(QUANT_METHOD)(Mxfp4Bf16DequantConfig)
     if QUANT_METHOD not in q_map:
         auto.register_quantizer(QUANT_METHOD)(Mxfp4Bf16DequantQuantizer)
+    from . import attention
+    attention.register()
 
 
 register()

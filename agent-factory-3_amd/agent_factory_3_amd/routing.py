@@ -398,6 +398,68 @@ def balance_loss(logits: torch.Tensor, n_expts_act: int, expt_indx: torch.Tensor
         return _balance_forward(lg, K, expt_indx, token_mask)[:2]
 
 
+class BalanceCollector:
+    """Router logits of the MoE layers that ran inside ``collect_balance``, by layer (of
+    a layer that ran twice, the last run), and the losses made of them."""
+
+    def __init__(self, token_mask=None):
+        self.token_mask = token_mask
+        self._seen = {}
+        self._made = None
+
+    def add(self, layer, logits, n_expts_act, expt_indx=None):
+        # Only kept here: the loss is made outside the layer, so that a layer under
+        # activation checkpointing saves the same tensors when it runs again (in the
+        # backward, which adds nothing).
+        if torch._C._current_graph_task_id() == -1:
+            self._seen[layer] = (logits, n_expts_act, expt_indx)
+            self._made = None
+
+    def _results(self) -> list:
+        if not self._seen:
+            raise RuntimeError("collect_balance: no MoE layer ran")
+        if self._made is None:
+            mask = self.token_mask.reshape(-1) if self.token_mask is not None else None
+            self._made = [balance_loss(lg, k, ids, mask) for lg, k, ids in self._seen.values()]
+        return self._made
+
+    def losses(self) -> torch.Tensor:
+        """[layers] fp32, differentiable in the routers' logits."""
+        return torch.stack([x[0] for x in self._results()])
+
+    def loss(self) -> torch.Tensor:
+        """Mean over the layers (a scalar to scale and add to the training loss)."""
+        return self.losses().mean()
+
+    def counts(self) -> torch.Tensor:
+        """[layers, E] int32: tokens per expert."""
+        return torch.stack([x[1] for x in self._results()])
+
+
+_COLLECTORS: list = []  # the innermost collect_balance gets the layers
+
+
+@contextlib.contextmanager
+def collect_balance(token_mask: torch.Tensor | None = None):
+    """Within it, every MoE layer that ``quantization.mlp_forward`` runs leaves its
+    router logits for a balance loss and counts (replayed experts count as routed):
+
+        with collect_balance(attention_mask) as balance:
+            out = model(input_ids, attention_mask=attention_mask)
+        loss = policy_loss(out) + coef * balance.loss()
+
+    token_mask: [B, S] (or flat) tokens to count, None = all.  Activation
+    checkpointing works in its non-reentrant form (the reentrant one runs the
+    layers without gradients first, so its losses have none).
+    """
+    c = BalanceCollector(token_mask)
+    _COLLECTORS.append(c)
+    try:
+        yield c
+    finally:
+        _COLLECTORS.remove(c)
+
+
 def dense_routing(n_rows: int, device) -> RoutingData:
     """Single-expert routing (matmul_ogs with routing_data=None)."""
     hist = torch.tensor([n_rows], dtype=torch.int32, device=device)
