@@ -45,8 +45,8 @@ def _rows(t: torch.Tensor, heads: bool = False):
 
 
 @functools.lru_cache(maxsize=64)
-def _fwd_workspace(B, Hq, Hkv, Sq, Sk, D, window, first) -> int:
-    return int(_capi.load().af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first))
+def _fwd_workspace(B, Hq, Hkv, Sq, Sk, D, window, first, ranges) -> int:
+    return int(_capi.load().af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first, ranges))
 
 
 @functools.lru_cache(maxsize=64)
@@ -65,7 +65,7 @@ def _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, 
     Hkv, Sk = k.shape[1], k.shape[2]
     dev = q.device
     out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=dev)
-    ws_n = _fwd_workspace(B, Hq, Hkv, Sq, Sk, D, window, first)
+    ws_n = _fwd_workspace(B, Hq, Hkv, Sq, Sk, D, window, first, int(kv_range is not None))
     ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
     _capi.call("af3_sink_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _c_strides(strides),
                _capi.ptr(sinks), int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(cu_seqlens),

@@ -1045,14 +1045,18 @@ __global__ __launch_bounds__(1024) void sa_starts_pos_kernel(const int64_t* __re
 // Splits of a row tile's keys over blocks.  One block per (batch row, key/value
 // head, row tile) leaves most of the 256 CUs idle when there are few of them.  A
 // block whose rows fill one wave at most (a few new tokens) is bound by reading K
-// and V: three such blocks fit a CU, and more come in a second round (131072 keys:
-// 512 blocks 42 us, 768 44, 1024 52).
-int sa_splits(int B, int Hkv, int64_t n_tiles, int64_t rows, int64_t keys) {
+// and V.  Where every batch row has all keys, two such blocks per CU read fastest
+// (one token over 131072 keys, 8 key/value heads: 512 blocks 43 us, 768 45, 1024
+// 46, 2048 47); with ranges of their own the rows end unevenly and smaller pieces
+// level them (32 rows of 90 to 4099 keys: 512 blocks 35 us, 1024 29, 2048 26.5).
+// Fuller tiles are split only below a block per CU (the join reads their rows too).
+int sa_splits(int B, int Hkv, int64_t n_tiles, int64_t rows, int64_t keys, bool ranges) {
   const int64_t blocks = (int64_t)B * Hkv * n_tiles;
   const bool few = rows <= 32;
-  if (blocks == 0 || blocks > (few ? 384 : 255)) return 1;
+  const int64_t target = few && ranges ? 2048 : 512;
+  if (blocks == 0 || blocks > (few ? target / 2 : 255)) return 1;
   const int64_t most = keys / 256;  // at least four key tiles each
-  int64_t n = (few ? 768 : 512) / blocks;
+  int64_t n = target / blocks;
   if (n > most) n = most;
   return n < 1 ? 1 : n > kMaxSplit ? kMaxSplit : (int)n;
 }
@@ -1061,7 +1065,7 @@ struct SaShape {
   int tok, n_tiles, n_split, window, first;
 };
 
-SaShape sa_shape(int B, int Hq, int Hkv, int Sq, int Sk, int window, int first) {
+SaShape sa_shape(int B, int Hq, int Hkv, int Sq, int Sk, int window, int first, bool ranges) {
   SaShape s;
   const int G = Hq / Hkv;
   s.window = window >= Sk ? 0 : window;  // it covers every key
@@ -1070,7 +1074,7 @@ SaShape sa_shape(int B, int Hq, int Hkv, int Sq, int Sk, int window, int first) 
   s.n_tiles = (int)af3_cdiv(Sq, s.tok);
   int64_t keys = s.window > 0 ? (int64_t)s.window + s.tok + s.first : Sk;
   if (keys > Sk) keys = Sk;
-  s.n_split = sa_splits(B, Hkv, s.n_tiles, (int64_t)Sq * G, keys);
+  s.n_split = sa_splits(B, Hkv, s.n_tiles, (int64_t)Sq * G, keys, ranges);
   return s;
 }
 
@@ -1135,9 +1139,9 @@ extern "C" int af3_seq_starts_positions(const int64_t* position_ids, int n_token
 }
 
 extern "C" size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int window,
-                                                     int first) {
+                                                     int first, int ranges) {
   if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq / Hkv > kRows || Sq <= 0 || Sk < 0) return 0;
-  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
+  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first, ranges != 0);
   return s.n_split > 1 ? (size_t)s.n_split * B * Hq * Sq * (D + 2) * 4 : 0;
 }
 
@@ -1156,7 +1160,7 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
   AF3_REQUIRE(!cu_seqlens || starts, "%s: cu_seqlens without starts", who);
   if (cu_seqlens)
     if (int rc = af3_seq_starts(cu_seqlens, n_seqs, Sk, starts, stream_)) return rc;
-  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
+  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first, kv_range != nullptr);
   SaParams p = sa_params(s, q, k, v, strides, sinks, sinks_f32, starts, kv_range, B, Hq, Hkv, Sq, Sk, scale);
   p.out = out;
   p.out_lo = out_lo;
@@ -1165,7 +1169,7 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
   const int64_t grid = (int64_t)s.n_tiles * B * Hkv * s.n_split;
   if (s.n_split > 1) {
     AF3_REQUIRE(workspace && sa_al16(workspace) &&
-                    ws_bytes >= af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first),
+                    ws_bytes >= af3_sink_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, first, kv_range != nullptr),
                 "%s: workspace too small", who);
     p.part = (float*)workspace;
   }
@@ -1206,7 +1210,7 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
               "%s: rows must be 16-byte aligned", who);
   AF3_REQUIRE(ws_bytes >= af3_sink_attention_bwd_workspace_bytes(B, Hq, Hkv, Sq), "%s: workspace too small", who);
   hipStream_t stream = (hipStream_t)stream_;
-  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first);
+  const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first, kv_range != nullptr);
   SaParams p = sa_params(s, q, k, v, strides, sinks, sinks_f32, starts, kv_range, B, Hq, Hkv, Sq, Sk, scale);
   p.dout = dout;
   p.do_sb = strides[9]; p.do_sh = strides[10]; p.do_st = strides[11];

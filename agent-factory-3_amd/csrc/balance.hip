@@ -23,6 +23,7 @@ namespace {
 constexpr int kBalThreads = 512;
 constexpr int kBalMaxBlocks = 512;
 constexpr int kBalMaxE = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // bf16 bits -> 16-bit key in float order (-0 as +0; NaN lowest)
 __device__ __forceinline__ uint32_t b_key16(uint32_t b) {
@@ -85,24 +86,23 @@ __device__ __forceinline__ void b_load(const uint16_t* row, int E, int l, uint32
   }
 }
 
+// exp(z - max) of the lane's logits, and their sum over the row
 template <int LPR, int C>
-__device__ __forceinline__ void b_softmax(const uint32_t (&w)[4 * C], float (&p)[8 * C]) {
+__device__ __forceinline__ float b_exps(const uint32_t (&w)[4 * C], float (&e)[8 * C]) {
   float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 8 * C; ++i) {
-    p[i] = af3_bf16_to_f32((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu);
-    mx = fmaxf(mx, p[i]);
+    e[i] = __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    mx = fmaxf(mx, e[i]);
   }
-  mx = b_max<LPR>(mx);
+  mx = b_max<LPR>(mx) * kLog2e;
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 8 * C; ++i) {
-    p[i] = __builtin_amdgcn_exp2f((p[i] - mx) * 1.4426950408889634f);
-    s += p[i];
+    e[i] = __builtin_amdgcn_exp2f(fmaf(e[i], kLog2e, -mx));
+    s += e[i];
   }
-  const float inv = 1.f / b_sum<LPR>(s);
-#pragma unroll
-  for (int i = 0; i < 8 * C; ++i) p[i] *= inv;
+  return b_sum<LPR>(s);
 }
 
 struct BalParams {
@@ -149,17 +149,28 @@ __global__ __launch_bounds__(kBalThreads) void balance_sums_kernel(BalParams p) 
   for (int i = 0; i < 8 * C; ++i) sum[i] = 0.f, cnt[i] = 0;
   int32_t n = 0;
   const int64_t step = (int64_t)p.n_blocks * NW * RPW;
-  for (int64_t t0 = ((int64_t)blockIdx.x * NW + wave) * RPW; t0 < p.T; t0 += step) {
+  const int64_t first = ((int64_t)blockIdx.x * NW + wave) * RPW;
+  uint32_t nw[4 * C];  // the next rows, loaded a pass ahead (a pass alone costs a load's latency)
+  uint8_t nm = 1;
+  auto fetch = [&](int64_t t0) {
+    const int64_t t = min(t0 + sub, p.T - 1);
+    b_load<LPR, C, VEC>(p.logits + t * p.ld, p.E, l, nw);
+    if (p.mask) nm = p.mask[t];
+  };
+  if (first < p.T) fetch(first);
+  for (int64_t t0 = first; t0 < p.T; t0 += step) {
     const int64_t t = t0 + sub;
-    const bool on = t < p.T && (!p.mask || p.mask[t]);
+    const bool on = t < p.T && nm;
     uint32_t w[4 * C];
-    b_load<LPR, C, VEC>(p.logits + (t < p.T ? t : t0) * p.ld, p.E, l, w);
-    float pr[8 * C];
-    b_softmax<LPR, C>(w, pr);
+#pragma unroll
+    for (int i = 0; i < 4 * C; ++i) w[i] = nw[i];
+    if (t0 + step < p.T) fetch(t0 + step);
+    float e[8 * C];
+    const float inv = 1.f / b_exps<LPR, C>(w, e);
     if (on) {
       n += l == 0;
 #pragma unroll
-      for (int i = 0; i < 8 * C; ++i) sum[i] += pr[i];
+      for (int i = 0; i < 8 * C; ++i) sum[i] = fmaf(e[i], inv, sum[i]);
     }
     if constexpr (TOPK) {
       uint32_t key[8 * C];
@@ -226,42 +237,49 @@ __global__ __launch_bounds__(kBalThreads) void balance_sums_kernel(BalParams p) 
   }
 }
 
-// column sums and counts over the blocks' partials: 16 experts per block, 16
-// threads each; the block that ends last makes the loss
-__global__ __launch_bounds__(256) void balance_join_kernel(BalParams p) {
-  __shared__ float cs[16][17];
-  __shared__ int32_t cn[16][17];
-  __shared__ bool last;
+// column sums and counts over the blocks' partials: 16 experts per block, 64
+// threads each with all their loads in flight; the block that ends last makes the loss
+__global__ __launch_bounds__(1024) void balance_join_kernel(BalParams p) {
+  constexpr int Y = 64, PER = kBalMaxBlocks / Y;
+  __shared__ float cs[Y][17];
+  __shared__ int32_t cn[Y][17];
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
   const int e = blockIdx.x * 16 + x;  // column E: the number of tokens
+  float v[PER];
+  int32_t n[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int b = y + i * Y;
+    v[i] = b < p.n_blocks && e < p.E ? p.part[(int64_t)b * p.E + e] : 0.f;
+    n[i] = b < p.n_blocks && e <= p.E ? p.part_n[(int64_t)b * (p.E + 1) + e] : 0;
+  }
   float s = 0.f;
   int32_t c = 0;
-  if (e <= p.E)
-    for (int b = y; b < p.n_blocks; b += 16) {
-      if (e < p.E) s += p.part[(int64_t)b * p.E + e];
-      c += p.part_n[(int64_t)b * (p.E + 1) + e];
-    }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) s += v[i], c += n[i];
   cs[y][x] = s;
   cn[y][x] = c;
-  __syncthreads();
-  if (y == 0 && e <= p.E) {
-    s = 0.f;
-    c = 0;
-    for (int i = 0; i < 16; ++i) s += cs[i][x], c += cn[i][x];
-    if (e < p.E) {
-      __hip_atomic_store(&p.colsum[e], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      p.counts[e] = c;
+  for (int o = Y / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (y < o) {
+      cs[y][x] += cs[y + o][x];
+      cn[y][x] += cn[y + o][x];
     }
-    __hip_atomic_store(&p.stats[e], c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0)
-    last = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  if (threadIdx.x < 64) b_finish(p.colsum, p.stats, p.E, p.loss, threadIdx.x);
+  if (threadIdx.x >= 64) return;
+  // the first wave alone writes, takes the ticket (which releases what it wrote)
+  // and, if it is the last, makes the loss
+  if (y == 0 && e <= p.E) {
+    if (e < p.E) {
+      p.colsum[e] = cs[0][x];
+      p.counts[e] = cn[0][x];
+    }
+    p.stats[e] = cn[0][x];
+  }
+  uint32_t t = 0;
+  if (threadIdx.x == 0) t = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+  if (__builtin_amdgcn_readfirstlane(t) != gridDim.x - 1) return;
+  b_finish(p.colsum, p.stats, p.E, p.loss, threadIdx.x);
 }
 
 template <int LPR, int C, bool VEC>
@@ -272,6 +290,15 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(const uint16_t* __res
   constexpr int RPW = 64 / LPR;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane % LPR, sub = lane / LPR;
+  uint32_t nw[4 * C];  // the next rows, loaded a pass ahead (the first before the counts)
+  uint8_t nm = 1;
+  auto fetch = [&](int64_t t0) {
+    const int64_t t = min(t0 + sub, T - 1);
+    b_load<LPR, C, VEC>(logits + t * ld, E, l, nw);
+    if (mask) nm = mask[t];
+  };
+  const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * RPW;
+  if (first < T) fetch(first);
   const float n = (float)stats[E];
   const float inv_n = n > 0.f ? 1.f / n : 0.f;
   const float scale = g[0] * (float)E * inv_n;
@@ -282,33 +309,39 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(const uint16_t* __res
     f[i] = x < E ? (float)stats[x] * inv_n : 0.f;
   }
   const int64_t step = (int64_t)gridDim.x * 4 * RPW;
-  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * RPW; t0 < T; t0 += step) {
+  for (int64_t t0 = first; t0 < T; t0 += step) {
     const int64_t t = t0 + sub;
-    const bool in = t < T, on = in && (!mask || mask[t]);
+    const bool in = t < T, on = in && nm;
     uint32_t w[4 * C];
-    b_load<LPR, C, VEC>(logits + (in ? t : t0) * ld, E, l, w);
-    float p[8 * C];
-    b_softmax<LPR, C>(w, p);
-    float dot = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8 * C; ++i) dot = fmaf(p[i], f[i], dot);
-    dot = b_sum<LPR>(dot);
+    for (int i = 0; i < 4 * C; ++i) w[i] = nw[i];
+    if (t0 + step < T) fetch(t0 + step);
+    // with e = exp(z - max): p = e / sum, p (f - p.f) scale = e (f k - d k), k = scale / sum, d = e.f / sum
+    float e[8 * C];
+    const float inv = 1.f / b_exps<LPR, C>(w, e);
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8 * C; ++i) d = fmaf(e[i], f[i], d);
+    const float k = inv * scale;
+    d = b_sum<LPR>(d) * inv * k;
     if (!in) continue;
     uint16_t* row = out + t * E;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int x0 = (c * LPR + l) * 8;
-      float v[8];
+      af3_u32x4 v;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = on ? p[8 * c + i] * (f[8 * c + i] - dot) * scale : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const int j = 8 * c + 2 * i;
+        const uint32_t y = af3_pack_bf16x2(e[j] * fmaf(f[j], k, -d), e[j + 1] * fmaf(f[j + 1], k, -d));
+        v[i] = on ? y : 0u;  // (whatever the logits of a token left out are)
+      }
       if constexpr (VEC) {
-        if (x0 < E)
-          *(af3_u32x4*)(row + x0) = af3_u32x4{af3_pack_bf16x2(v[0], v[1]), af3_pack_bf16x2(v[2], v[3]),
-                                              af3_pack_bf16x2(v[4], v[5]), af3_pack_bf16x2(v[6], v[7])};
+        if (x0 < E) *(af3_u32x4*)(row + x0) = v;
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (x0 + i < E) row[x0 + i] = (uint16_t)af3_f32_to_bf16(v[i]);
+          if (x0 + i < E) row[x0 + i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
       }
     }
   }
@@ -393,7 +426,7 @@ extern "C" int af3_balance_loss_fwd(const uint16_t* logits, int64_t ld_logits, c
   const bool vec = E % 8 == 0 && ld_logits % 8 == 0 && ((uintptr_t)logits & 15) == 0;
   B_BY_LANES(E, b_launch_sums, p, vec, stream);
   if (p.n_blocks > 1)
-    hipLaunchKernelGGL(balance_join_kernel, dim3(E / 16 + 1), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(balance_join_kernel, dim3(E / 16 + 1), dim3(1024), 0, stream, p);
   return af3::check_launch("balance_loss_fwd");
 }
 

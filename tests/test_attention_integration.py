@@ -123,9 +123,9 @@ def test_c_entries_refuse_bad_arguments():
         with pytest.raises(RuntimeError, match=match):
             fwd(**kw)
     lib = _capi.load()
-    assert lib.af3_sink_attention_workspace_bytes(1, 8, 1, 1, 4096, 64, 0, 0) > 0
-    assert lib.af3_sink_attention_workspace_bytes(1, 8, 1, 0, 4096, 64, 0, 0) == 0
-    assert lib.af3_sink_attention_workspace_bytes(64, 64, 8, 128, 128, 64, 0, 0) == 0
+    assert lib.af3_sink_attention_workspace_bytes(1, 8, 1, 1, 4096, 64, 0, 0, 0) > 0
+    assert lib.af3_sink_attention_workspace_bytes(1, 8, 1, 0, 4096, 64, 0, 0, 1) == 0
+    assert lib.af3_sink_attention_workspace_bytes(64, 64, 8, 128, 128, 64, 0, 0, 0) == 0
     bal = lambda *a: _capi.call("af3_balance_loss_fwd", *a)  # noqa: E731
     for a in ((64, 8, None, None, 4, 0, 1, 64, 64, 64, 64, 1 << 20, None), (64, 8, None, None, 4, 8, 9, 64, 64, 64, 64, 1 << 20, None),
               (64, 8, None, None, 4, 2000, 9, 64, 64, 64, 64, 1 << 20, None), (64, 4, None, None, 4, 8, 2, 64, 64, 64, 64, 1 << 20, None),
