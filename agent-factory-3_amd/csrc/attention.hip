@@ -35,6 +35,7 @@ namespace {
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxLen = 1 << 29;   // tokens (positions and their sums with a window stay in 32 bits)
@@ -49,7 +50,7 @@ struct SaParams {
   const int32_t* starts;                  // [Sk] start of each token's sequence (packed row), or NULL
   const int32_t* kv_range;                // [B][2] or NULL
   int B, Hq, Hkv, G, Sq, Sk, window, first;
-  int g_mul;                              // x / G = x g_mul >> 16 for x < 512
+  int g_mul;                              // x / G = x g_mul >> 16 for x < 256
   int tok;                                // tokens of a row tile
   int n_tiles, n_split;
   float scale, scale2;                    // scale2 = scale log2(e)
@@ -59,7 +60,7 @@ struct SaParams {
   // backward
   const uint16_t* dout;                   // [B][Sq][Hq][D] by strides
   int64_t do_sb, do_sh, do_st;
-  float* delta;                           // as lse
+  float* delta;                           // -delta, as lse
   float* dsink_part;                      // [n_tiles][B][Hq]
   uint16_t *dq, *dk, *dv;                 // [B][S][H][D]
 };
@@ -70,6 +71,13 @@ __device__ __forceinline__ void a_dma16(const void* gptr, uint32_t lds_byte_addr
 // the same from a wave-uniform base plus a 32-bit lane offset in bytes
 __device__ __forceinline__ void a_dma16_s(const void* sbase, uint32_t voff, uint32_t lds_byte_addr) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_byte_addr) : "memory");
+}
+// four bytes per lane
+__device__ __forceinline__ void a_dma4(const void* gptr, uint32_t lds_byte_addr) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(gptr), "{m0}"(lds_byte_addr) : "memory");
+}
+__device__ __forceinline__ void a_dma4_s(const void* sbase, uint32_t voff, uint32_t lds_byte_addr) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_byte_addr) : "memory");
 }
 #define A_WAIT_VM(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 #define A_BARRIER() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
@@ -113,12 +121,12 @@ struct Frag {
   // chunk 2 x + h of row r0 + lane % 32 of the tile at LDS address `tile` (r0 % 32 == 0)
   __device__ __forceinline__ af3_bf16x8 row8(uint32_t tile, int r0, int x) const {
     typedef const __attribute__((address_space(3))) af3_bf16x8 T;
-    return *(T*)(tile + row[x] + (uint32_t)(r0 * D * 2));
+    return *(T*)(uintptr_t)(tile + row[x] + (uint32_t)(r0 * D * 2));
   }
   // rows r0 + 4 h .. + 3 and r0 + 8 + 4 h .. + 3 of column 32 d + lane % 32 (r0 % 16 == 0)
   __device__ __forceinline__ af3_bf16x8 tr8(uint32_t tile, int r0, int d) const {
-    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + tr[d] + (uint32_t)(r0 * D * 2)));
-    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + tr8_[d] + (uint32_t)(r0 * D * 2)));
+    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)(tile + tr[d] + (uint32_t)(r0 * D * 2)));
+    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)(tile + tr8_[d] + (uint32_t)(r0 * D * 2)));
     return af3_bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 };
@@ -160,6 +168,9 @@ __device__ __forceinline__ float a_sum_halves(float x) {
   const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// a row number's distance, kept where 32 bits hold it (a step has 64 rows)
+__device__ __forceinline__ int a_clamp64(int64_t x) { return (int)min(max(x, (int64_t)-1024), (int64_t)1024); }
 
 __device__ __forceinline__ float a_sink2(const SaParams& p, int h) {
   const float s = p.sinks_f32 ? ((const float*)p.sinks)[h] : af3_bf16_to_f32(((const uint16_t*)p.sinks)[h]);
@@ -600,7 +611,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
   }
   float lse = p.lse[prow];
   asm volatile("" : "+v"(lse));  // landed, as the operands
-  if (valid && lh == 0) p.delta[prow] = delta;
+  if (valid && lh == 0) p.delta[prow] = -delta;
   if (p.sinks) {
     if (lh == 0) ds_row[row] = valid ? -__builtin_amdgcn_exp2f(a_sink2(p, head) - lse) * delta : 0.f;
     __syncthreads();
@@ -704,16 +715,14 @@ __global__ __launch_bounds__(256) void sa_dsink_kernel(const float* __restrict__
 
 // ---------------------------------------------------------------------------
 // backward, keys: dk and dv.  Block = 64 keys of one key/value head, K and V rows
-// in registers; the (token, head) rows that see them go through a two-stage LDS
-// ring, 128 at a time (q, dout, and their lse, delta and what they see).  Waves 0
-// and 1 (32 keys each) take the first 64 rows of a step, waves 2 and 3 the others,
-// and their sums are joined at the end.  S = Q K^T puts a key's column into its
-// lane; the sum over the heads that share the key is the sum over rows.  Two
-// blocks fit a CU (D = 64), each at its own point of a step, so that one's
-// exponentials run beside the other's products.  Kernel time, packed 8192 tokens,
-// 64/8 heads, window 128 / full attention: 64 keys x 128 rows 82 / 855 us, 64 x
-// 256 (one block of 8 waves per CU) 103 / 816, 128 x 128 (8 waves) 103 / 917, 128
-// x 64 (4 waves) 89 / 1360.
+// in registers; the (token, head) rows that see them go through a four-stage LDS
+// ring, 64 at a time (q, dout, and their lse and -delta), from the last rows back.
+// Waves 0 and 1 (32 keys each) take the first 32 rows of a step, waves 2 and 3 the
+// others, and their sums are joined at the end.  S = Q K^T puts a key's column
+// into its lane; the sum over the heads that share the key is the sum over rows,
+// and the rows that see a key are one run of row numbers per lane.  A step's
+// exponentials stand between the products of the next step's scores and of its
+// own first half, held in that order, so that the matrix unit works beside them.
 // ---------------------------------------------------------------------------
 // first token after t0 whose sequence starts later than t0's (starts does not
 // decrease), or n: 64 probes a round, the answer stays in (lo, hi]
@@ -730,35 +739,37 @@ __device__ __forceinline__ int a_sequence_end(const int32_t* starts, int t0, int
   return hi;
 }
 
-constexpr int KG = 2, NH = 2;                                      // key groups, row groups (waves: KG NH)
-constexpr int kKeys = 32 * KG, kRT = 64 * NH, kDkvWaves = KG * NH;  // keys of a block, rows of a step
+constexpr int kKeys = 64;  // keys of a block
+constexpr int kRT = 64;    // rows of a step
+constexpr int kStages = 4;
 
 template <int D>
-__global__ __launch_bounds__(64 * kDkvWaves, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kRT * D * 2;
-  constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / kDkvWaves;  // chunks per row, rows per copy, copies per wave
-  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
-  __shared__ __attribute__((aligned(16))) float st_lse[2][kRT], st_delta[2][kRT];
-  __shared__ __attribute__((aligned(16))) int st_w[2][kRT], st_wn[2][kRT], st_lo[2][kRT], st_fn[2][kRT];
+  constexpr int CH = D / 8, RPI = 64 / CH, N = kRT / RPI / 4;  // chunks per row, rows per copy, copies per wave
+  constexpr int EPS = 16 / (2 * KS);                           // exponentials per product slot
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kStages * 2 * kTile];
+  // rows' lse, -delta and (where the block holds a sequence's first key) sequence start
+  __shared__ __attribute__((aligned(16))) float rowv[kStages][4][kRT];
   const int bh = blockIdx.x % (p.B * p.Hkv);
   const int j0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kKeys;  // the longest columns first
-  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int b = p.B > 1 ? bh / p.Hkv : 0, hk = bh - b * p.Hkv;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = wave / KG;  // rows 64 part .. + 63 of a step
+  const int part = wave >> 1;  // rows 32 part .. + 31 of a step
   const int lr = lane & 31, lh = lane >> 5;
   const int off = p.Sk - p.Sq;
   int lo, hi;
   a_kv_range(p, b, lo, hi);
   const int jl = min(j0 + kKeys, p.Sk) - 1;  // last key of the block
-  const int jw = j0 + (wave % KG) * 32;      // first key of the wave
+  const int jw = j0 + (wave & 1) * 32;       // first key of the wave
   const int j = jw + lr;
   const bool kvalid = j <= jl;
 
   // tokens that may see a key of the block
   const int ta = max(0, max(j0, lo) - off);  // [ta, tb)
-  int tb = p.Sq, s_last = lo;
+  int tb = p.Sq, s_last = lo;                // s_last: the latest start among their sequences
   if (p.starts) {
     s_last = p.starts[jl];
     tb = a_sequence_end(p.starts, jl, p.Sk, lane);
@@ -768,6 +779,76 @@ __global__ __launch_bounds__(64 * kDkvWaves, D == 64 ? 2 : 1) void sa_dkv_kernel
   tb = jl < lo || j0 >= hi ? ta : max(ta, min(tb, p.Sq));
   const int64_t n_rows = (int64_t)(tb - ta) * p.G;
   const int n_steps = (int)((n_rows + kRT - 1) / kRT);
+  // Where a sequence starts inside the block (its last at s_last), steps [0, mixed)
+  // hold rows of earlier ones, which ask each row for its own start.  The steps
+  // before them (they run from the last back) are s_last's alone: keys before it
+  // gather anything there, and start again from zero at step mixed - 1.
+  const int mixed = p.starts && s_last > j0 ? ((min(s_last, tb) - ta) * p.G + kRT - 1) / kRT : 0;
+
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
+  const uint32_t rowv0 = __builtin_amdgcn_readfirstlane(a_lds_addr(rowv));
+  const uint16_t* qb = p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
+  const uint16_t* db = p.dout + b * p.do_sb + (int64_t)hk * p.G * p.do_sh;
+  const int64_t sb = ((int64_t)b * p.Hkv + hk) * p.Sq * p.G + (int64_t)ta * p.G;
+  // Steps run from the last rows back, so that the blocks of a head, which end at
+  // the same rows, read them at about the same time.  Copies: where a step's rows
+  // are whole tokens, lane offsets never change and the scalar bases move on; else,
+  // and in the last rows' step, each row is looked up.  ns: the step to be copied
+  // next; nt, ng: token and head of its first row.
+  const int back = (int)((n_rows - 1) & (kRT - 1)), back_t = back * p.g_mul >> 16;
+  const int adv_t = kRT / p.G, adv_g = kRT - adv_t * p.G;
+  const bool even = adv_g == 0;
+  int nt = tb - 1 - back_t, ng = p.G - 1 - (back - back_t * p.G), ns = n_steps - 1;
+  uint32_t qo[N], od[N];
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    const int row = (wave * N + x) * RPI + lane / CH, t = row * p.g_mul >> 16, g = row - t * p.G;
+    const int col = ((lane % CH) ^ a_swz<D>(row)) << 3;
+    qo[x] = (uint32_t)(t * (int)p.q_st + g * (int)p.q_sh + col) * 2;
+    od[x] = (uint32_t)(t * (int)p.do_st + g * (int)p.do_sh + col) * 2;
+  }
+  const uint16_t *qp = qb + (int64_t)nt * p.q_st, *dp_ = db + (int64_t)nt * p.do_st;  // (even: ng is 0)
+  const float* rp = (wave == 1 ? p.delta : p.lse) + sb + (int64_t)ns * kRT;
+  // 2 N + 1 copies per wave and step, always: past the first rows' step that one again,
+  // into a stage nobody reads, so that every wait is a constant
+  auto issue = [&](int stage) {
+    const uint32_t st = lds0 + (uint32_t)(stage * 2 * kTile + wave * N * 1024);
+    const uint32_t rv = rowv0 + (uint32_t)((stage * 4 + wave) * kRT * 4);
+    if (even && ns < n_steps - 1 && ns >= mixed) {
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        a_dma16_s(qp, qo[x], st + x * 1024);
+        a_dma16_s(dp_, od[x], st + kTile + x * 1024);
+      }
+      a_dma4_s(rp, (uint32_t)lane * 4, rv);
+    } else {
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int row = (wave * N + x) * RPI + lane / CH, y = ng + row, yt = y * p.g_mul >> 16;
+        const int64_t t = min(nt + yt, tb - 1), g = y - yt * p.G;
+        const int col = ((lane % CH) ^ a_swz<D>(row)) << 3;
+        a_dma16(qb + t * p.q_st + g * p.q_sh + col, st + x * 1024);
+        a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + x * 1024);
+      }
+      const void* src = rp + (ns == n_steps - 1 ? min(lane, back) : lane);
+      if (wave == 2 && ns < mixed) src = p.starts + min(nt + ((ng + lane) * p.g_mul >> 16), tb - 1);
+      a_dma4(src, rv);
+    }
+    if (ns > 0) {
+      --ns;
+      nt -= adv_t;
+      ng -= adv_g;
+      if (ng < 0) ng += p.G, --nt;
+      qp -= adv_t * p.q_st;
+      dp_ -= adv_t * p.do_st;
+      rp -= kRT;
+    }
+  };
+  if (n_steps > 0) {
+    issue(0);
+    issue(1);
+    issue(2);
+  }
 
   af3_bf16x8 kf[KS], vf[KS];
   {
@@ -782,218 +863,207 @@ __global__ __launch_bounds__(64 * kDkvWaves, D == 64 ? 2 : 1) void sa_dkv_kernel
     a_landed(kf);
     a_landed(vf);
   }
-  const int jm = kvalid && j >= lo && j < hi ? j : 2 * kMaxLen;  // beyond every row's run
+  const bool jin = kvalid && j >= lo && j < hi;
   const bool wave_in = jw >= lo && jw + 31 < hi && jw + 31 <= jl;
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
-  const uint16_t* qb = p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
-  const uint16_t* db = p.dout + b * p.do_sb + (int64_t)hk * p.G * p.do_sh;
-  const int64_t sb = ((int64_t)b * p.Hkv + hk) * p.Sq * p.G + (int64_t)ta * p.G;
-  // Steps run from the last rows back, so that the blocks of a head, which all end
-  // at the same rows, read them at about the same time (out of the XCD's L2; from
-  // each block's own first row on, every block read other rows: 1194 TODO us).
-  // nt, ng: token and head of the first row of the step to be copied next.
-  const int back = (int)((n_rows - 1) & (kRT - 1)), back_t = (int)((uint32_t)back * p.g_mul >> 16);
-  const int adv_t = kRT / p.G, adv_g = kRT - adv_t * p.G;
-  int nt = tb - 1 - back_t, ng = p.G - 1 - (back - back_t * p.G);
-  // Copies: where 128 rows are whole tokens, lane offsets never change and the
-  // scalar base moves on; else, and in the last rows' step, each row is looked up.
-  const bool even = adv_g == 0;
-  uint32_t qo[N], od[N];
-#pragma unroll
-  for (int x = 0; x < N; ++x) {
-    const int row = (wave * N + x) * RPI + lane / CH, t = row * p.g_mul >> 16, g = row - t * p.G;
-    const int col = ((lane % CH) ^ a_swz<D>(row)) << 3;
-    qo[x] = (uint32_t)(t * (int)p.q_st + g * (int)p.q_sh + col) * 2;
-    od[x] = (uint32_t)(t * (int)p.do_st + g * (int)p.do_sh + col) * 2;
+  const bool kept = j < s_last + p.first;  // a first token: its rows end with the sequence
+  const Frag<D> fr(lane);
+
+  // The wave's steps [own0, own1), whose rows see some of its keys, and among them
+  // [free0, free1), whose rows see all of them.  In rows of the block: those that
+  // see key x are (x - off - ta) G up to (x - off - ta + window) G.
+  int own0, own1, free0, free1;
+  {
+    const int64_t k0 = jw - off - ta, k1 = k0 + 31, r0 = part * 32;
+    const int64_t nk = max(k0, (int64_t)s_last + p.first - off - ta);  // the first key that a window ends for
+    const int64_t e1 = p.window > 0 && nk <= k1 ? min(n_rows, (k1 + p.window) * p.G) : n_rows;
+    const int64_t e0 = p.window > 0 && nk <= k1 ? min(n_rows, (nk + p.window) * p.G) : n_rows;
+    const bool some_kept = p.first > 0 && s_last + p.first > jw;
+    own0 = (int)max((int64_t)0, (k0 * p.G - r0 + 32) >> 6);
+    own1 = (int)(((some_kept ? n_rows : e1) - r0 + 63) >> 6);
+    free0 = max((int)max((int64_t)0, (k1 * p.G - r0 + 63) >> 6), mixed);
+    free1 = wave_in ? (int)((e0 - r0 + 32) >> 6) : 0;
   }
-  float v_lse = 0.f, v_delta = 0.f;
-  int v_t = 0, v_start = lo;
-  auto issue = [&](int i) {  // q and dout rows to LDS, the rows' values to registers of threads 0..127
-    const uint32_t st = lds0 + (uint32_t)((i & 1) * 2 * kTile + wave * N * 1024);
-    if (even && i < n_steps - 1) {
-      const uint16_t *q0 = qb + nt * p.q_st, *d0 = db + nt * p.do_st;
-#pragma unroll
-      for (int x = 0; x < N; ++x) {
-        a_dma16_s(q0, qo[x], st + x * 1024);
-        a_dma16_s(d0, od[x], st + kTile + x * 1024);
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < N; ++x) {
-        const int row = (wave * N + x) * RPI + lane / CH, y = ng + row, yt = y * p.g_mul >> 16;
-        const int64_t t = min(nt + yt, tb - 1), g = y - yt * p.G;
-        const int col = ((lane % CH) ^ a_swz<D>(row)) << 3;
-        a_dma16(qb + t * p.q_st + g * p.q_sh + col, st + x * 1024);
-        a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + x * 1024);
-      }
-    }
-    if (threadIdx.x < kRT) {
-      const int64_t r = min((int64_t)i * kRT + threadIdx.x, n_rows - 1);
-      v_lse = p.lse[sb + r];
-      v_delta = p.delta[sb + r];
-      v_t = nt + ((ng + (int)threadIdx.x) * p.g_mul >> 16);
-      if (p.starts) v_start = p.starts[min(v_t, tb - 1)];  // (used after the next wait: here it would wait for the copies)
-    }
-    nt -= adv_t;
-    ng -= adv_g;
-    if (ng < 0) ng += p.G, --nt;
-  };
-  auto store_rows = [&](int i) {
-    if (threadIdx.x < kRT) {
-      st_lse[i & 1][threadIdx.x] = v_lse;
-      st_delta[i & 1][threadIdx.x] = -v_delta;
-      const Vis v = a_vis(p, min(v_t, tb - 1) + off, v_start, hi);
-      st_w[i & 1][threadIdx.x] = v.w;
-      st_wn[i & 1][threadIdx.x] = v_t < tb ? max(0, v.end - v.w) : 0;
-      if (p.first > 0) {
-        st_lo[i & 1][threadIdx.x] = v.lo;
-        st_fn[i & 1][threadIdx.x] = v_t < tb ? v.fn : 0;
-      }
-    }
+  typedef const __attribute__((address_space(3))) f32x4 lds_f4;
+  auto row4 = [&](int stage, int which, int q) {
+    return *(lds_f4*)(uintptr_t)(rowv0 + (uint32_t)(((stage * 4 + which) * kRT + part * 32 + 8 * q) * 4) + (uint32_t)(lh * 16));
   };
 
-  const Frag<D> fr(lane);
   af3_f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = a_zero(), dv[d] = a_zero();
-  if (n_steps > 0) issue(n_steps - 1);
-  for (int i = n_steps - 1; i >= 0; --i) {
-    A_WAIT_VM(0);
-    store_rows(i);
-    A_BARRIER();
-    const int ct = nt + adv_t + (ng + adv_g >= p.G), cg = ng + adv_g - (ng + adv_g >= p.G ? p.G : 0);  // this step's first row
-    if (i > 0) issue(i - 1);
-    const uint32_t qt = lds0 + (uint32_t)((i & 1) * 2 * kTile + part * (64 * D * 2)), dt = qt + kTile;
-    const int w = i & 1, rb = part * 64;
-    // the half's tokens; what rows see does not begin earlier from one to the next
-    const int64_t r0 = (int64_t)i * kRT + rb;
-    const bool full = r0 + 64 <= n_rows;  // rows past the last see nothing
-    const int pos0 = ct + ((cg + rb) * p.g_mul >> 16) + off;
-    const int pos1 = min(ct + ((cg + rb + 63) * p.g_mul >> 16), tb - 1) + off;
-    if (r0 >= n_rows || jw > pos1) continue;  // none of the wave's keys is seen
-    const int w0 = __builtin_amdgcn_readfirstlane(st_w[w][rb]);
-    const int w1 = __builtin_amdgcn_readfirstlane(st_w[w][rb + 63]);
-    if (p.first == 0 && jw + 31 < w0) continue;
-    const bool whole = full && wave_in && jw + 31 <= pos0 && jw >= w1;
-    // LDS reads stand well before their use (the barriers hold the order): a read
-    // right at its product costs its whole latency, 16 times a step.
-    af3_bf16x8 qr[KS], dr[KS], td[DB], tq[DB];
+
+  // scores and dp - delta of the wave's rows of a step, by themselves
+  auto scores = [&](int stage, af3_f32x16& s, af3_f32x16& dp) {
+    const uint32_t qt = lds0 + (uint32_t)(stage * 2 * kTile), dt = qt + kTile;
+    s = a_zero();
 #pragma unroll
-    for (int x = 0; x < KS; ++x) qr[x] = fr.row8(qt, 0, x);
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 de = row4(stage, 1, q);
+      dp[4 * q] = de.x; dp[4 * q + 1] = de.y; dp[4 * q + 2] = de.z; dp[4 * q + 3] = de.w;
+    }
 #pragma unroll
-    for (int x = 0; x < KS; ++x) dr[x] = fr.row8(dt, 0, x);
+    for (int x = 0; x < KS; ++x) s = a_mfma(fr.row8(qt, part * 32, x), kf[x], s);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int at = rb + c * 32 + 4 * lh;  // registers 4 q .. + 3: rows at + 8 q .. + 3
-      af3_f32x16 s = a_zero(), dp;
-      float4 ls[4];
+    for (int x = 0; x < KS; ++x) dp = a_mfma(fr.row8(dt, part * 32, x), vf[x], dp);
+  };
+  // a step's probabilities, dz and products, beside the next step's scores
+  auto run = [&](int i, int stage, int nstage, af3_f32x16& s, af3_f32x16& dp, af3_f32x16& s1, af3_f32x16& dp1) {
+    const uint32_t qt = lds0 + (uint32_t)(stage * 2 * kTile), dt = qt + kTile;
+    const uint32_t qn = lds0 + (uint32_t)(nstage * 2 * kTile), dn = qn + kTile;
+    f32x4 ls[4];
+    af3_bf16x8 qr[KS], dr[KS], td[DB], tq[DB], pf, sf;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {  // dp starts at -delta
-        const float4 de = *(const float4*)&st_delta[w][at + 8 * q];
-        dp[4 * q] = de.x; dp[4 * q + 1] = de.y; dp[4 * q + 2] = de.z; dp[4 * q + 3] = de.w;
-        ls[q] = *(const float4*)&st_lse[w][at + 8 * q];
+    for (int q = 0; q < 4; ++q) ls[q] = row4(stage, 0, q);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) qr[x] = fr.row8(qn, part * 32, x);
+    if (i < free0 || i >= free1) {
+      const int64_t row = (int64_t)i * kRT + part * 32 + 4 * lh;  // register r: row + 8 (r / 4) + r % 4
+      const int64_t d = j - off - ta;
+      const int rlo = jin ? a_clamp64(d * p.G - row) : kRT;
+      const int rw = p.window > 0 ? a_clamp64((d + p.window) * p.G - row) : kRT;
+      const int rhi = min(kept || i < mixed ? kRT : rw, a_clamp64(n_rows - row));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int x = 8 * (r / 4) + r % 4;
+        const bool on = x >= rlo && x < rhi;
+        s[r] = on ? s[r] : -INFINITY;
+        dp[r] = on ? dp[r] : 0.f;
       }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int x = 0; x < KS; ++x) s = a_mfma(qr[x], kf[x], s);
-#pragma unroll
-      for (int x = 0; x < KS; ++x) dp = a_mfma(dr[x], vf[x], dp);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        td[d] = fr.tr8(dt, c * 32, d);
-        tq[d] = fr.tr8(qt, c * 32, d);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float lsv[4] = {ls[q].x, ls[q].y, ls[q].z, ls[q].w};
-#pragma unroll
-        for (int y = 0; y < 4; ++y) s[4 * q + y] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + y], p.scale2, -lsv[y]));
-      }
-      if (!whole) {
+      if (i < mixed) {  // each row's own sequence
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int4 w4 = *(const int4*)&st_w[w][at + 8 * q], n4 = *(const int4*)&st_wn[w][at + 8 * q];
-          const int wv[4] = {w4.x, w4.y, w4.z, w4.w}, nv[4] = {n4.x, n4.y, n4.z, n4.w};
-          bool on[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) on[y] = (uint32_t)(jm - wv[y]) < (uint32_t)nv[y];
-          if (p.first > 0) {
-            const int4 l4 = *(const int4*)&st_lo[w][at + 8 * q], f4 = *(const int4*)&st_fn[w][at + 8 * q];
-            const int lv[4] = {l4.x, l4.y, l4.z, l4.w}, fv[4] = {f4.x, f4.y, f4.z, f4.w};
-#pragma unroll
-            for (int y = 0; y < 4; ++y) on[y] |= (uint32_t)(jm - lv[y]) < (uint32_t)fv[y];
-          }
+          const f32x4 s4 = row4(stage, 2, q);
+          const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            s[4 * q + y] = on[y] ? s[4 * q + y] : 0.f;
-            dp[4 * q + y] = on[y] ? dp[4 * q + y] : 0.f;
+            const int st = __float_as_int(sv[y]);
+            const bool on = j >= st && (8 * q + y < rw || j < st + p.first);
+            s[4 * q + y] = on ? s[4 * q + y] : -INFINITY;
+            dp[4 * q + y] = on ? dp[4 * q + y] : 0.f;
           }
         }
       }
+    }
+    s1 = a_zero();
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+    for (int x = 0; x < 2 * KS; ++x) {
+      if (x < KS)
+        s1 = a_mfma(qr[x], kf[x], s1);
+      else
+        dp1 = a_mfma(dr[x - KS], vf[x - KS], dp1);
+      if (x < KS) dr[x] = fr.row8(dn, part * 32, x);
+      if (x == 0) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const af3_bf16x8 pf = a_pack8(s, u), sf = a_pack8(dp, u);
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 de = row4(nstage, 1, q);
+          dp1[4 * q] = de.x; dp1[4 * q + 1] = de.y; dp1[4 * q + 2] = de.z; dp1[4 * q + 3] = de.w;
+        }
+      }
+      if (x == KS / 2) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          dv[d] = a_mfma(td[d], pf, dv[d]);
-          dk[d] = a_mfma(tq[d], sf, dk[d]);
+          td[d] = fr.tr8(dt, part * 32, d);
+          tq[d] = fr.tr8(qt, part * 32, d);
         }
-        if (u == 0) {
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            td[d] = fr.tr8(dt, c * 32 + 16, d);
-            tq[d] = fr.tr8(qt, c * 32 + 16, d);
-          }
-        } else if (c == 0) {
-#pragma unroll
-          for (int x = 0; x < KS; ++x) qr[x] = fr.row8(qt, 32, x);
-#pragma unroll
-          for (int x = 0; x < KS; ++x) dr[x] = fr.row8(dt, 32, x);
-        }
-        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-  }
-  // the first waves take the other row groups' sums, one group after another, through the ring's LDS
-  float* sum = (float*)lds + ((wave % KG) * 64 + lane) * 4;  // four values of a lane, then the next four KG KB on
+      if (x == KS) {
+        pf = a_pack8(s, 0);
+        sf = a_pack8(dp, 0);
+      }
+      if (x >= KS) {  // the first half's products, one after each of the next step's
+        const int y = x - KS, d = y / 2;
+        if (y & 1)
+          dk[d] = a_mfma(tq[d], sf, dk[d]);
+        else
+          dv[d] = a_mfma(td[d], pf, dv[d]);
+      }
 #pragma unroll
-  for (int x = 1; x < NH; ++x) {
+      for (int r = x * EPS; r < (x + 1) * EPS; ++r) {
+        const f32x4 l4 = ls[r / 4];
+        const float lv = r % 4 == 0 ? l4.x : r % 4 == 1 ? l4.y : r % 4 == 2 ? l4.z : l4.w;
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lv));
+        dp[r] *= s[r];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      td[d] = fr.tr8(dt, part * 32 + 16, d);
+      tq[d] = fr.tr8(qt, part * 32 + 16, d);
+    }
+    pf = a_pack8(s, 1);
+    sf = a_pack8(dp, 1);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      dv[d] = a_mfma(td[d], pf, dv[d]);
+      dk[d] = a_mfma(tq[d], sf, dk[d]);
+    }
+  };
+  static_assert(N == 2 || N == 4, "wait counts");
+  // (2 N + 1 copies a step: the step after next may be under way)
+  auto wait_next = [&]() {
+    if constexpr (N == 2) A_WAIT_VM(5); else A_WAIT_VM(9);
+  };
+  af3_f32x16 s0, dp0, s1, dp1;
+  if (n_steps > 0) {
+    if constexpr (N == 2) A_WAIT_VM(10); else A_WAIT_VM(18);
     A_BARRIER();
-    if (part == x) {
+    if (n_steps <= own1) scores(0, s0, dp0);
+  }
+  int stage = 0;
+  // one step: (s, dp) hold its scores; (sn, dpn) get the next one's
+  auto turn = [&](int i, af3_f32x16& s, af3_f32x16& dp, af3_f32x16& sn, af3_f32x16& dpn) {
+    wait_next();  // the next step's copies
+    A_BARRIER();  // and every wave is past the step before this one
+    issue((stage + 3) & 3);
+    const int nstage = (stage + 1) & 3;
+    if (i == mixed - 1) {
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          *(float4*)(sum + (d * 8 + r / 4) * KG * 256) = float4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
-          *(float4*)(sum + (d * 8 + 4 + r / 4) * KG * 256) = float4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+        for (int r = 0; r < 16; ++r) {
+          dk[d][r] = j < s_last ? 0.f : dk[d][r];
+          dv[d][r] = j < s_last ? 0.f : dv[d][r];
         }
     }
-    A_BARRIER();
-    if (part == 0) {
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const float4 k4 = *(const float4*)(sum + (d * 8 + r / 4) * KG * 256);
-          const float4 v4 = *(const float4*)(sum + (d * 8 + 4 + r / 4) * KG * 256);
-          dk[d][r] += k4.x; dk[d][r + 1] += k4.y; dk[d][r + 2] += k4.z; dk[d][r + 3] += k4.w;
-          dv[d][r] += v4.x; dv[d][r + 1] += v4.y; dv[d][r + 2] += v4.z; dv[d][r + 3] += v4.w;
-        }
-    }
+    if (i >= own0 && i < own1)
+      run(i, stage, nstage, s, dp, sn, dpn);
+    else if (i == own1)
+      scores(nstage, sn, dpn);
+    stage = nstage;
+  };
+  for (int i = n_steps - 1; i >= 0; i -= 2) {
+    turn(i, s0, dp0, s1, dp1);
+    if (i > 0) turn(i - 1, s1, dp1, s0, dp0);
   }
-  if (part || !kvalid) return;
+  A_WAIT_VM(0);  // the repeated copies
+  // waves 2 and 3 hand their sums to waves 0 and 1 through the ring's LDS
+  A_BARRIER();
+  float* sum = (float*)lds + ((wave & 1) * 64 + lane) * 4;  // four values of a lane, then the next four 2 KB on
+  if (part == 1) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        *(float4*)(sum + (d * 8 + r / 4) * 512) = float4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+        *(float4*)(sum + (d * 8 + 4 + r / 4) * 512) = float4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+      }
+  }
+  A_BARRIER();
+  if (part == 1 || !kvalid) return;
   const int64_t o = (((int64_t)b * p.Sk + j) * p.Hkv + hk) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
+      const float4 k4 = *(const float4*)(sum + (d * 8 + r / 4) * 512);
+      const float4 v4 = *(const float4*)(sum + (d * 8 + 4 + r / 4) * 512);
       const int64_t c = o + d * 32 + 2 * r + 4 * lh;
-      *(u32x2*)(p.dv + c) = u32x2{af3_pack_bf16x2(dv[d][r], dv[d][r + 1]), af3_pack_bf16x2(dv[d][r + 2], dv[d][r + 3])};
-      *(u32x2*)(p.dk + c) = u32x2{af3_pack_bf16x2(dk[d][r] * p.scale, dk[d][r + 1] * p.scale),
-                                  af3_pack_bf16x2(dk[d][r + 2] * p.scale, dk[d][r + 3] * p.scale)};
+      *(u32x2*)(p.dv + c) = u32x2{af3_pack_bf16x2(dv[d][r] + v4.x, dv[d][r + 1] + v4.y),
+                                  af3_pack_bf16x2(dv[d][r + 2] + v4.z, dv[d][r + 3] + v4.w)};
+      *(u32x2*)(p.dk + c) = u32x2{af3_pack_bf16x2((dk[d][r] + k4.x) * p.scale, (dk[d][r + 1] + k4.y) * p.scale),
+                                  af3_pack_bf16x2((dk[d][r + 2] + k4.z) * p.scale, (dk[d][r + 3] + k4.w) * p.scale)};
     }
 }
 
@@ -1231,7 +1301,7 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
     hipLaunchKernelGGL(sa_dsink_kernel, dim3(Hq), dim3(256), 0, stream, p.dsink_part, s.n_tiles * B, Hq, sinks_f32,
                        dsinks);
   if (nk) {
-    const dim3 grid((unsigned)(af3_cdiv(Sk, kKeys) * B * Hkv)), block(64 * kDkvWaves);
+    const dim3 grid((unsigned)(af3_cdiv(Sk, kKeys) * B * Hkv)), block(256);
     if (D == 64)
       hipLaunchKernelGGL(sa_dkv_kernel<64>, grid, block, 0, stream, p);
     else

@@ -266,3 +266,24 @@ def test_starts_of_positions(dev, lens):
     want = oa.starts_of(cu.tolist(), pos.numel()).to(torch.int32)
     assert torch.equal(sequence_starts_of_positions(pos[None]).cpu(), want)
     assert torch.equal(sequence_starts(cu, pos.numel()).cpu(), want)
+
+
+@pytest.mark.parametrize("G", [1, 3, 8, 64])
+@pytest.mark.parametrize("start", [1, 31, 32, 33, 40, 63, 64, 65])
+def test_a_sequence_starts_inside_a_key_block(dev, G, start):
+    """Keys of two sequences in one block of the key gradient, at every place of its waves; garbage in
+    the later sequence's gradients must not reach the earlier one's keys."""
+    _check(dev, 1, G, 1, 150, 150, 64, cu_seqlens=[0, start, 150], seed=start)
+    _check(dev, 1, G, 1, 150, 150, 64, cu_seqlens=[0, start, start + 3, 150], window=20, first=2, seed=start)
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 1, G, 1, 150, 150, 64)
+    cu = torch.tensor([0, start, 150], dtype=torch.int32, device=dev)
+    res = []
+    for bad in (0.0, math.nan):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        d2 = do.clone()
+        d2[:, start:] += bad
+        out = sink_attention(*leaves, s, cu_seqlens=cu)
+        res.append([g[:, :, :start] for g in torch.autograd.grad(out, leaves, d2)])
+    if start * G % 64 == 0:   # (else a tile of rows holds both sequences: the documented limit)
+        assert all(torch.equal(a, b) for a, b in zip(*res))
