@@ -63,6 +63,8 @@ struct SaParams {
   float* delta;                           // -delta, as lse
   float* dsink_part;                      // [n_tiles][B][Hq]
   uint16_t *dq, *dk, *dv;                 // [B][S][H][D]
+  void* dsinks;                           // [Hq], in the sinks' type
+  int n_key_blocks;
 };
 
 __device__ __forceinline__ void a_dma16(const void* gptr, uint32_t lds_byte_addr) {
@@ -551,33 +553,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
   __shared__ float ds_row[kRows];
   const int bh = blockIdx.x % (p.B * p.Hkv);
   const int tile = p.n_tiles - 1 - blockIdx.x / (p.B * p.Hkv);
-  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int b = p.B > 1 ? bh / p.Hkv : 0, hk = bh - b * p.Hkv;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, lh = lane >> 5;
   const int off = p.Sk - p.Sq;
   const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;
-  const int row = wave * 32 + lr;
-  const int tk = row * p.g_mul >> 16, g = row - tk * p.G;
-  const bool valid = t0 + tk <= t1;
-  const int t = valid ? t0 + tk : t0;
-  const int head = hk * p.G + (valid ? g : 0);
   int lo, hi;
   a_kv_range(p, b, lo, hi);
-  const int row_lo = p.starts ? p.starts[t] : lo;
   const int tile_lo = p.starts ? p.starts[t0] : lo;
   const int last_lo = p.starts ? p.starts[t1] : lo;
-  const Vis vis = a_vis(p, t + off, row_lo, hi);
   const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
-  const int wt0 = t0 + (wave * 32 * p.g_mul >> 16), wt1 = min(t1, t0 + ((wave * 32 + 31) * p.g_mul >> 16));
-  const int wpos0 = wt0 + off, wpos1 = wt1 + off;
-  const int from = p.window > 0 ? max(last_lo + p.first, wpos1 - p.window + 1) : last_lo;
-  const int own1 = wt0 > t1 ? 0 : min(na + nb, na + max(0, wpos1 - ks.b0 + kBN) / kBN);
-  const int own0 = p.window > 0 && p.first == 0 ? na + max(0, wpos0 - p.window + 1 - ks.b0) / kBN : 0;
-  const int free0 = na + max(0, from - ks.b0 + kBN - 1) / kBN;
-  const int free1 = na + max(0, min(wpos0 + 1, ks.b1) - ks.b0) / kBN;
-
   const KvCopy<D> kc(p.k + b * p.k_sb + hk * p.k_sh, p.k_st, wave, lane);
   const KvCopy<D> vc(p.v + b * p.v_sb + hk * p.v_sh, p.v_st, wave, lane);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
@@ -588,28 +575,38 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
     kc(j0, last, st, wave);
     vc(j0, last, st + kTile, wave);
   };
+  if (na + nb > 0) issue(0, 0);  // (under way while the rows are read)
 
+  const int row = wave * 32 + lr;
+  const int tk = row * p.g_mul >> 16, g = row - tk * p.G;
+  const bool valid = t0 + tk <= t1;
+  const int t = valid ? t0 + tk : t0;
+  const int head = hk * p.G + (valid ? g : 0);
   const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + (valid ? g : 0);
+  const Vis vis = a_vis(p, t + off, p.starts ? p.starts[t] : lo, hi);
+  float lse = p.lse[prow];
   af3_bf16x8 qf[KS], df[KS];
   float delta = 0.f;
   {
     const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
     const uint16_t* dr = p.dout + b * p.do_sb + head * p.do_sh + t * p.do_st;
     const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
+    af3_bf16x8 of[KS], oe[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
       df[s] = *(const af3_bf16x8*)(dr + s * 16 + lh * 8);
-      const af3_bf16x8 of = *(const af3_bf16x8*)(p.out + orow + s * 16 + lh * 8);
-      const af3_bf16x8 oe = *(const af3_bf16x8*)(p.out_lo + orow + s * 16 + lh * 8);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[i] + (float)oe[i], delta);
+      of[s] = *(const af3_bf16x8*)(p.out + orow + s * 16 + lh * 8);
+      oe[s] = *(const af3_bf16x8*)(p.out_lo + orow + s * 16 + lh * 8);
     }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[s][i] + (float)oe[s][i], delta);
     delta = a_sum_halves(delta);
     a_landed(qf);
     a_landed(df);
   }
-  float lse = p.lse[prow];
   asm volatile("" : "+v"(lse));  // landed, as the operands
   if (valid && lh == 0) p.delta[prow] = -delta;
   if (p.sinks) {
@@ -621,9 +618,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
       p.dsink_part[((int64_t)tile * p.B + b) * p.Hq + hk * p.G + threadIdx.x] = sum;
     }
   }
-  A_WAIT_VM(0);
-  if (na + nb > 0) issue(0, 0);
 
+  // the wave's own tiles and those of which its rows see every key, as in the forward
+  const int wt0 = t0 + (wave * 32 * p.g_mul >> 16), wt1 = min(t1, t0 + ((wave * 32 + 31) * p.g_mul >> 16));
+  const int wpos0 = wt0 + off, wpos1 = wt1 + off;
+  const int from = p.window > 0 ? max(last_lo + p.first, wpos1 - p.window + 1) : last_lo;
+  const int own1 = wt0 > t1 ? 0 : min(na + nb, na + max(0, wpos1 - ks.b0 + kBN) / kBN);
+  const int own0 = p.window > 0 && p.first == 0 ? na + max(0, wpos0 - p.window + 1 - ks.b0) / kBN : 0;
+  const int free0 = na + max(0, from - ks.b0 + kBN - 1) / kBN;
+  const int free1 = na + max(0, min(wpos0 + 1, ks.b1) - ks.b0) / kBN;
   const Frag<D> fr(lane);
   af3_f32x16 acc[DB];
 #pragma unroll
@@ -692,13 +695,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
                 af3_pack_bf16x2(acc[d][r + 2] * p.scale, acc[d][r + 3] * p.scale)};
 }
 
-// one block per head: the sinks' gradient from the tiles' sums (a fixed order)
-__global__ __launch_bounds__(256) void sa_dsink_kernel(const float* __restrict__ part, int n, int Hq, int f32,
-                                                       void* __restrict__ out) {
-  __shared__ float sh[256];
-  const int h = blockIdx.x;
+// the sinks' gradient of head h from the tiles' sums, in a fixed order (256 threads)
+__device__ __forceinline__ void a_dsink(const SaParams& p, int h, float* sh) {
+  const int n = p.n_tiles * p.B;
   float s = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) s += part[(int64_t)i * Hq + h];
+  for (int i = threadIdx.x; i < n; i += 256) s += p.dsink_part[(int64_t)i * p.Hq + h];
   sh[threadIdx.x] = s;
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
@@ -706,10 +707,10 @@ __global__ __launch_bounds__(256) void sa_dsink_kernel(const float* __restrict__
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    if (f32)
-      ((float*)out)[h] = sh[0];
+    if (p.sinks_f32)
+      ((float*)p.dsinks)[h] = sh[0];
     else
-      ((uint16_t*)out)[h] = (uint16_t)af3_f32_to_bf16(sh[0]);
+      ((uint16_t*)p.dsinks)[h] = (uint16_t)af3_f32_to_bf16(sh[0]);
   }
 }
 
@@ -724,10 +725,9 @@ __global__ __launch_bounds__(256) void sa_dsink_kernel(const float* __restrict__
 // exponentials stand between the products of the next step's scores and of its
 // own first half, held in that order, so that the matrix unit works beside them.
 // ---------------------------------------------------------------------------
-// first token after t0 whose sequence starts later than t0's (starts does not
-// decrease), or n: 64 probes a round, the answer stays in (lo, hi]
-__device__ __forceinline__ int a_sequence_end(const int32_t* starts, int t0, int n, int lane) {
-  const int s0 = starts[t0];
+// first token after t0, whose sequence starts at s0, of a later sequence (starts does
+// not decrease), or n > t0: 64 probes a round, the answer stays in (lo, hi]
+__device__ __forceinline__ int a_sequence_end(const int32_t* starts, int s0, int t0, int n, int lane) {
   int lo = t0, hi = n;
   while (hi - lo > 1) {
     const int step = (hi - lo + 63) / 64;
@@ -752,6 +752,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   __shared__ __attribute__((aligned(16))) uint8_t lds[kStages * 2 * kTile];
   // rows' lse, -delta and (where the block holds a sequence's first key) sequence start
   __shared__ __attribute__((aligned(16))) float rowv[kStages][4][kRT];
+  if ((int)blockIdx.x >= p.n_key_blocks) {  // the last blocks: the sinks
+    a_dsink(p, blockIdx.x - p.n_key_blocks, (float*)lds);
+    return;
+  }
   const int bh = blockIdx.x % (p.B * p.Hkv);
   const int j0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kKeys;  // the longest columns first
   const int b = p.B > 1 ? bh / p.Hkv : 0, hk = bh - b * p.Hkv;
@@ -770,12 +774,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   // tokens that may see a key of the block
   const int ta = max(0, max(j0, lo) - off);  // [ta, tb)
   int tb = p.Sq, s_last = lo;                // s_last: the latest start among their sequences
-  if (p.starts) {
-    s_last = p.starts[jl];
-    tb = a_sequence_end(p.starts, jl, p.Sk, lane);
-  }
+  if (p.starts) s_last = p.starts[jl];
   // (the last key's sequence may have first tokens in the block; an earlier one ends in it)
   if (p.window > 0 && (p.first == 0 || s_last + p.first <= j0)) tb = min(tb, jl + p.window - off);
+  if (p.starts) tb = a_sequence_end(p.starts, s_last, jl, tb, lane);
   tb = jl < lo || j0 >= hi ? ta : max(ta, min(tb, p.Sq));
   const int64_t n_rows = (int64_t)(tb - ta) * p.G;
   const int n_steps = (int)((n_rows + kRT - 1) / kRT);
@@ -922,12 +924,21 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
       const int rlo = jin ? a_clamp64(d * p.G - row) : kRT;
       const int rw = p.window > 0 ? a_clamp64((d + p.window) * p.G - row) : kRT;
       const int rhi = min(kept || i < mixed ? kRT : rw, a_clamp64(n_rows - row));
+      if (i < free0 || !wave_in) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int x = 8 * (r / 4) + r % 4;
-        const bool on = x >= rlo && x < rhi;
-        s[r] = on ? s[r] : -INFINITY;
-        dp[r] = on ? dp[r] : 0.f;
+        for (int r = 0; r < 16; ++r) {
+          const bool on = 8 * (r / 4) + r % 4 >= rlo;
+          s[r] = on ? s[r] : -INFINITY;
+          dp[r] = on ? dp[r] : 0.f;
+        }
+      }
+      if (i >= free1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool on = 8 * (r / 4) + r % 4 < rhi;
+          s[r] = on ? s[r] : -INFINITY;
+          dp[r] = on ? dp[r] : 0.f;
+        }
       }
       if (i < mixed) {  // each row's own sequence
 #pragma unroll
@@ -1297,11 +1308,11 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
     else
       hipLaunchKernelGGL(sa_dq_kernel<128>, dim3(gq), dim3(256), 0, stream, p);
   }
-  if (sinks)  // (no query rows: a sum over nothing)
-    hipLaunchKernelGGL(sa_dsink_kernel, dim3(Hq), dim3(256), 0, stream, p.dsink_part, s.n_tiles * B, Hq, sinks_f32,
-                       dsinks);
-  if (nk) {
-    const dim3 grid((unsigned)(af3_cdiv(Sk, kKeys) * B * Hkv)), block(256);
+  // (dk, dv, and the sinks' sums over the tiles: over nothing where there are no query rows)
+  p.dsinks = dsinks;
+  p.n_key_blocks = nk ? (int)(af3_cdiv(Sk, kKeys) * B * Hkv) : 0;
+  const dim3 grid((unsigned)(p.n_key_blocks + (sinks ? Hq : 0))), block(256);
+  if (grid.x) {
     if (D == 64)
       hipLaunchKernelGGL(sa_dkv_kernel<64>, grid, block, 0, stream, p);
     else
