@@ -108,16 +108,18 @@ __device__ __forceinline__ int a_off(int row, int chunk) { return row * (D * 2) 
 template <int D>
 struct Frag {
   uint32_t row[D / 16], tr[D / 32], tr8_[D / 32];
-  __device__ __forceinline__ explicit Frag(int lane) {
+  // base: added to every address (the tile's own, where `tile` is then a constant
+  // that fits the reads' offset field)
+  __device__ __forceinline__ explicit Frag(int lane, uint32_t base = 0) {
     const int r = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int x = 0; x < D / 16; ++x) row[x] = a_off<D>(r, 2 * x + h);
+    for (int x = 0; x < D / 16; ++x) row[x] = base + a_off<D>(r, 2 * x + h);
     const int tr_r = (h << 2) + ((lane & 15) >> 2);
     const int c = (((lane >> 4) & 1) << 4) + ((lane & 3) << 2);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
-      tr[d] = a_off<D>(tr_r, (d * 32 + c) >> 3) + ((c & 7) << 1);
-      tr8_[d] = a_off<D>(tr_r + 8, (d * 32 + c) >> 3) + ((c & 7) << 1);
+      tr[d] = base + a_off<D>(tr_r, (d * 32 + c) >> 3) + ((c & 7) << 1);
+      tr8_[d] = base + a_off<D>(tr_r + 8, (d * 32 + c) >> 3) + ((c & 7) << 1);
     }
   }
   // chunk 2 x + h of row r0 + lane % 32 of the tile at LDS address `tile` (r0 % 32 == 0)
@@ -131,6 +133,11 @@ struct Frag {
     const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)(tile + tr8_[d] + (uint32_t)(r0 * D * 2)));
     return af3_bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
+};
+
+template <int V>
+struct Int {
+  static constexpr int value = V;
 };
 
 // The loads of these operands end here.  Left to their first use in the loop, the
@@ -627,16 +634,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
   const int own0 = p.window > 0 && p.first == 0 ? na + max(0, wpos0 - p.window + 1 - ks.b0) / kBN : 0;
   const int free0 = na + max(0, from - ks.b0 + kBN - 1) / kBN;
   const int free1 = na + max(0, min(wpos0 + 1, ks.b1) - ks.b0) / kBN;
-  const Frag<D> fr(lane);
+  const Frag<D> fr(lane, lds0);
   af3_f32x16 acc[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = a_zero();
-  for (int i = 0; i < na + nb; ++i) {
+  auto turn = [&](int i, auto stage) {  // (the stage a constant: its addresses need no arithmetic)
     A_WAIT_VM(0);
     A_BARRIER();
-    if (i + 1 < na + nb) issue(i + 1, (i + 1) & 1);
-    const uint32_t kt = lds0 + (uint32_t)((i & 1) * 2 * kTile), vt = kt + kTile;
-    if (i < own0 || i >= own1) continue;
+    if (i + 1 < na + nb) issue(i + 1, 1 - stage.value);
+    constexpr uint32_t kt = stage.value * 2 * kTile, vt = kt + kTile;
+    if (i < own0 || i >= own1) return;
     // (reads ahead of their use, held by the barriers, as in the dk / dv kernel)
     af3_bf16x8 kr[KS], vr[KS], tr[DB];
 #pragma unroll
@@ -683,6 +690,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
 #pragma unroll
       for (int d = 0; d < DB; ++d) acc[d] = a_mfma(tr[d], p1, acc[d]);
     }
+  };
+  for (int i = 0; i < na + nb; i += 2) {
+    turn(i, Int<0>{});
+    if (i + 1 < na + nb) turn(i + 1, Int<1>{});
   }
   if (!valid) return;
   uint16_t* qrow = p.dq + (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
@@ -868,7 +879,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   const bool jin = kvalid && j >= lo && j < hi;
   const bool wave_in = jw >= lo && jw + 31 < hi && jw + 31 <= jl;
   const bool kept = j < s_last + p.first;  // a first token: its rows end with the sequence
-  const Frag<D> fr(lane);
+  const Frag<D> fr(lane, lds0 + (uint32_t)(part * 32 * D * 2));
+  const uint32_t rv0 = rowv0 + (uint32_t)(part * 128 + lh * 16);
 
   // The wave's steps [own0, own1), whose rows see some of its keys, and among them
   // [free0, free1), whose rows see all of them.  In rows of the block: those that
@@ -887,7 +899,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   }
   typedef const __attribute__((address_space(3))) f32x4 lds_f4;
   auto row4 = [&](int stage, int which, int q) {
-    return *(lds_f4*)(uintptr_t)(rowv0 + (uint32_t)(((stage * 4 + which) * kRT + part * 32 + 8 * q) * 4) + (uint32_t)(lh * 16));
+    return *(lds_f4*)(uintptr_t)(rv0 + (uint32_t)(((stage * 4 + which) * kRT + 8 * q) * 4));
   };
 
   af3_f32x16 dk[DB], dv[DB];
@@ -895,8 +907,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   for (int d = 0; d < DB; ++d) dk[d] = a_zero(), dv[d] = a_zero();
 
   // scores and dp - delta of the wave's rows of a step, by themselves
-  auto scores = [&](int stage, af3_f32x16& s, af3_f32x16& dp) {
-    const uint32_t qt = lds0 + (uint32_t)(stage * 2 * kTile), dt = qt + kTile;
+  auto scores = [&](auto st, af3_f32x16& s, af3_f32x16& dp) {
+    constexpr int stage = st.value;
+    constexpr uint32_t qt = stage * 2 * kTile, dt = qt + kTile;
     s = a_zero();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -904,20 +917,20 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
       dp[4 * q] = de.x; dp[4 * q + 1] = de.y; dp[4 * q + 2] = de.z; dp[4 * q + 3] = de.w;
     }
 #pragma unroll
-    for (int x = 0; x < KS; ++x) s = a_mfma(fr.row8(qt, part * 32, x), kf[x], s);
+    for (int x = 0; x < KS; ++x) s = a_mfma(fr.row8(qt, 0, x), kf[x], s);
 #pragma unroll
-    for (int x = 0; x < KS; ++x) dp = a_mfma(fr.row8(dt, part * 32, x), vf[x], dp);
+    for (int x = 0; x < KS; ++x) dp = a_mfma(fr.row8(dt, 0, x), vf[x], dp);
   };
   // a step's probabilities, dz and products, beside the next step's scores
-  auto run = [&](int i, int stage, int nstage, af3_f32x16& s, af3_f32x16& dp, af3_f32x16& s1, af3_f32x16& dp1) {
-    const uint32_t qt = lds0 + (uint32_t)(stage * 2 * kTile), dt = qt + kTile;
-    const uint32_t qn = lds0 + (uint32_t)(nstage * 2 * kTile), dn = qn + kTile;
+  auto run = [&](int i, auto st, af3_f32x16& s, af3_f32x16& dp, af3_f32x16& s1, af3_f32x16& dp1) {
+    constexpr int stage = st.value, nstage = (stage + 1) & 3;
+    constexpr uint32_t qt = stage * 2 * kTile, dt = qt + kTile, qn = nstage * 2 * kTile, dn = qn + kTile;
     f32x4 ls[4];
     af3_bf16x8 qr[KS], dr[KS], td[DB], tq[DB], pf, sf;
 #pragma unroll
     for (int q = 0; q < 4; ++q) ls[q] = row4(stage, 0, q);
 #pragma unroll
-    for (int x = 0; x < KS; ++x) qr[x] = fr.row8(qn, part * 32, x);
+    for (int x = 0; x < KS; ++x) qr[x] = fr.row8(qn, 0, x);
     if (i < free0 || i >= free1) {
       const int64_t row = (int64_t)i * kRT + part * 32 + 4 * lh;  // register r: row + 8 (r / 4) + r % 4
       const int64_t d = j - off - ta;
@@ -963,7 +976,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
         s1 = a_mfma(qr[x], kf[x], s1);
       else
         dp1 = a_mfma(dr[x - KS], vf[x - KS], dp1);
-      if (x < KS) dr[x] = fr.row8(dn, part * 32, x);
+      if (x < KS) dr[x] = fr.row8(dn, 0, x);
       if (x == 0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -974,8 +987,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
       if (x == KS / 2) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          td[d] = fr.tr8(dt, part * 32, d);
-          tq[d] = fr.tr8(qt, part * 32, d);
+          td[d] = fr.tr8(dt, 0, d);
+          tq[d] = fr.tr8(qt, 0, d);
         }
       }
       if (x == KS) {
@@ -1000,8 +1013,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
     }
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
-      td[d] = fr.tr8(dt, part * 32 + 16, d);
-      tq[d] = fr.tr8(qt, part * 32 + 16, d);
+      td[d] = fr.tr8(dt, 16, d);
+      tq[d] = fr.tr8(qt, 16, d);
     }
     pf = a_pack8(s, 1);
     sf = a_pack8(dp, 1);
@@ -1020,15 +1033,14 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   if (n_steps > 0) {
     if constexpr (N == 2) A_WAIT_VM(10); else A_WAIT_VM(18);
     A_BARRIER();
-    if (n_steps <= own1) scores(0, s0, dp0);
+    if (n_steps <= own1) scores(Int<0>{}, s0, dp0);
   }
-  int stage = 0;
-  // one step: (s, dp) hold its scores; (sn, dpn) get the next one's
-  auto turn = [&](int i, af3_f32x16& s, af3_f32x16& dp, af3_f32x16& sn, af3_f32x16& dpn) {
+  // one step: (s, dp) hold its scores; (sn, dpn) get the next one's.  (The stage is a
+  // constant of each of four turns: its LDS addresses need no arithmetic.)
+  auto turn = [&](int i, auto st, af3_f32x16& s, af3_f32x16& dp, af3_f32x16& sn, af3_f32x16& dpn) {
     wait_next();  // the next step's copies
     A_BARRIER();  // and every wave is past the step before this one
-    issue((stage + 3) & 3);
-    const int nstage = (stage + 1) & 3;
+    issue((st.value + 3) & 3);
     if (i == mixed - 1) {
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -1039,14 +1051,15 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
         }
     }
     if (i >= own0 && i < own1)
-      run(i, stage, nstage, s, dp, sn, dpn);
+      run(i, st, s, dp, sn, dpn);
     else if (i == own1)
-      scores(nstage, sn, dpn);
-    stage = nstage;
+      scores(Int<(st.value + 1) & 3>{}, sn, dpn);
   };
-  for (int i = n_steps - 1; i >= 0; i -= 2) {
-    turn(i, s0, dp0, s1, dp1);
-    if (i > 0) turn(i - 1, s1, dp1, s0, dp0);
+  for (int i = n_steps - 1; i >= 0; i -= 4) {
+    turn(i, Int<0>{}, s0, dp0, s1, dp1);
+    if (i > 0) turn(i - 1, Int<1>{}, s1, dp1, s0, dp0);
+    if (i > 1) turn(i - 2, Int<2>{}, s0, dp0, s1, dp1);
+    if (i > 2) turn(i - 3, Int<3>{}, s1, dp1, s0, dp0);
   }
   A_WAIT_VM(0);  // the repeated copies
   // waves 2 and 3 hand their sums to waves 0 and 1 through the ring's LDS
