@@ -182,8 +182,8 @@ __device__ __forceinline__ float a_sum_halves(float x) {
 __device__ __forceinline__ int a_clamp64(int64_t x) { return (int)min(max(x, (int64_t)-1024), (int64_t)1024); }
 
 __device__ __forceinline__ float a_sink2(const SaParams& p, int h) {
-  const float s = p.sinks_f32 ? ((const float*)p.sinks)[h] : af3_bf16_to_f32(((const uint16_t*)p.sinks)[h]);
-  return s * kLog2e;
+  const float s = (p.sinks_f32 ? ((const float*)p.sinks)[h] : af3_bf16_to_f32(((const uint16_t*)p.sinks)[h])) * kLog2e;
+  return s > 3e38f ? 3e38f : s;  // (finite: nothing is left of any key either way; a NaN stays one)
 }
 
 // key range of a batch row, inside [0, Sk] whatever the tensor holds
@@ -1179,7 +1179,7 @@ int sa_check(const char* who, int B, int Hq, int Hkv, int Sq, int Sk, int D, int
   AF3_REQUIRE(Hq / Hkv <= kRows, "%s: more than %d query heads per key/value head", who, kRows);
   AF3_REQUIRE(D == 64 || D == 128, "%s: head dimension %d is not 64 or 128", who, D);
   AF3_REQUIRE(window >= 0 && first >= 0, "%s: negative window or first", who);
-  AF3_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", who);
+  AF3_REQUIRE(scale > 0.f && scale * kLog2e < INFINITY, "%s: scale must be positive and finite", who);
   AF3_REQUIRE(strides, "%s: null strides", who);
   for (int i = 0; i < n_strides; ++i) {
     AF3_REQUIRE(strides[i] % 8 == 0, "%s: strides must be multiples of 8", who);
@@ -1188,7 +1188,11 @@ int sa_check(const char* who, int B, int Hq, int Hkv, int Sq, int Sk, int D, int
                 "%s: token strides, and head strides of q and dout, must be below %d", who, kMaxStride);
   }
   AF3_REQUIRE(!starts || (B <= 1 && Sq == Sk && !kv_range), "%s: a packed row has batch 1, Sq == Sk and no kv_range", who);
-  AF3_REQUIRE((int64_t)B * Hkv * (Sq + Sk + 1) < 0x7fffffffLL, "%s: too many rows", who);
+  // (a launch holds less than 2^32 threads; row numbers of dk / dv stay in 32 bits)
+  const int64_t tiles = af3_cdiv(Sq, kRows / (Hq / Hkv)), key_blocks = af3_cdiv(Sk, kKeys);
+  AF3_REQUIRE((int64_t)B * Hkv * (Sq + Sk + 1) < 0x7fffffffLL &&
+                  (int64_t)B * Hkv * (tiles > key_blocks ? tiles : key_blocks) + Hq < (1LL << 24),
+              "%s: too many rows", who);
   return 0;
 }
 

@@ -178,3 +178,20 @@ def test_collect_balance_takes_each_layer_once(monkeypatch):
         pass
     with pytest.raises(RuntimeError, match="no MoE layer"):
         b.loss()
+
+
+def test_c_entries_refuse_what_a_launch_or_32_bits_cannot_hold():
+    import ctypes
+
+    from agent_factory_3_amd import _capi
+    if not _capi.lib_path().exists():
+        pytest.skip("library not built")
+    strides = (ctypes.c_int64 * 12)(*[64] * 12)
+    for match, B, Sq, Sk, scale in (("rows", 1 << 21, 1, 1, 0.1), ("rows", 1 << 17, 1, 1 << 20, 0.1),
+                                    ("scale", 1, 4, 4, 3e38)):
+        with pytest.raises(RuntimeError, match=match):
+            _capi.call("af3_sink_attention_fwd", 64, 64, 64, strides, None, 0, None, 0, None, None, B, 8, 8, Sq, Sk, 64,
+                       0, 0, scale, 64, None, None, None, 0, None)
+        with pytest.raises(RuntimeError, match=match):
+            _capi.call("af3_sink_attention_bwd", 64, 64, 64, 64, strides, None, 0, None, None, B, 8, 8, Sq, Sk, 64, 0, 0,
+                       scale, 64, 64, 64, 64, 64, 64, None, 64, 0, None)
