@@ -85,18 +85,22 @@ class _SinkAttention(torch.autograd.Function):
         out = _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, kv_range, keep.data_ptr(),
                        keep.data_ptr() + 2 * D * n)
         ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, keep)
-        ctx.args = (strides, scale, window, first)
+        ctx.args = (scale, window, first)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, sinks, starts, kv_range, out, keep = ctx.saved_tensors
-        strides, scale, window, first = ctx.args
+        scale, window, first = ctx.args
         B, Hq, Sq, D = q.shape
         Hkv, Sk = k.shape[1], k.shape[2]
         dev = q.device
         with _device_of(q):
+            # (saved-tensor hooks, as those that keep them on the host, may give them other strides)
+            (q, sq), (k, sk), (v, sv) = _rows(q, heads=True), _rows(k), _rows(v)
+            sinks, starts, kv_range, out, keep = (t if t is None else t.contiguous()
+                                                  for t in (sinks, starts, kv_range, out, keep))
             do, st = _rows(dout.transpose(1, 2), heads=True)
             dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=dev)
             dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=dev)
@@ -105,7 +109,7 @@ class _SinkAttention(torch.autograd.Function):
             ws_n = _bwd_workspace(B, Hq, Hkv, Sq)
             ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
             _capi.call("af3_sink_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(),
-                       _c_strides(strides + st), _capi.ptr(sinks),
+                       _c_strides(sq + sk + sv + st), _capi.ptr(sinks),
                        int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
                        _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(),
                        keep.data_ptr(), keep.data_ptr() + 2 * D * B * Hq * Sq, dq.data_ptr(), dk.data_ptr(),

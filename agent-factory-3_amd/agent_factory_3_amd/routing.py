@@ -336,6 +336,9 @@ class _BalanceLoss(torch.autograd.Function):
         T, E = logits.shape
         dev = logits.device
         with _device_of(logits):
+            if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):  # (as a saved-tensor hook gave it)
+                logits = logits.contiguous()
+            token_mask, stats = token_mask if token_mask is None else token_mask.contiguous(), stats.contiguous()
             d = torch.empty((T, E), dtype=torch.bfloat16, device=dev)
             _capi.call("af3_balance_loss_bwd", logits.data_ptr(), logits.stride(0) if T > 1 else E,
                        _capi.ptr(token_mask), T, E, stats.data_ptr(), g.data_ptr(), d.data_ptr(),
@@ -406,6 +409,7 @@ class BalanceCollector:
         self.token_mask = token_mask
         self._seen = {}
         self._made = None
+        self._made_with_grad = False
 
     def add(self, layer, logits, n_expts_act, expt_indx=None):
         # Only kept here: the loss is made outside the layer, so that a layer under
@@ -418,7 +422,9 @@ class BalanceCollector:
     def _results(self) -> list:
         if not self._seen:
             raise RuntimeError("collect_balance: no MoE layer ran")
-        if self._made is None:
+        # (losses made without gradients, as counts read under no_grad make them, are made again where gradients are wanted)
+        if self._made is None or (torch.is_grad_enabled() and not self._made_with_grad):
+            self._made_with_grad = torch.is_grad_enabled()
             mask = self.token_mask.reshape(-1) if self.token_mask is not None else None
             self._made = [balance_loss(lg, k, ids, mask) for lg, k, ids in self._seen.values()]
         return self._made

@@ -385,3 +385,41 @@ def test_the_longest_packed_row(dev):
             _close(out[:, a:a + n], r["out"], r["out_tol"], "out")
             for name, t in zip(("dq", "dk", "dv"), grads):
                 _close(t[:, :, a:a + n], r[name], r[name + "_tol"], name)
+
+
+def test_saved_tensors_that_come_back_with_other_strides(dev):
+    """Saved-tensor hooks may hand the backward equal tensors laid out differently (those that keep
+    them on the host give dense ones for views with gaps): the same gradients."""
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 2, 8, 2, 90, 90, 64, layout="fused")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, s)]
+
+    def grads():
+        return torch.autograd.grad(sink_attention(*leaves, window=40, first=2), leaves, do)
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    def spread(t):    # every dimension's stride changed, gaps between all of them
+        return torch.empty([2 * n for n in t.shape[::-1]], dtype=t.dtype, device=t.device).permute(
+            *range(t.dim())[::-1])[tuple(slice(None, None, 2) for _ in t.shape)].copy_(t) if t.dtype == torch.bfloat16 else t
+    with torch.autograd.graph.saved_tensors_hooks(spread, lambda t: t):
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_largest_sinks(dev):
+    """A sink of the type's largest value leaves nothing of any key; of its lowest value, it is no sink."""
+    from agent_factory_3_amd.attention import sink_attention
+    for dtype in (torch.bfloat16, torch.float32):
+        q, k, v, s, do = _make(dev, 1, 4, 2, 90, 90, 64, sinks=dtype)
+        s[0], s[1] = torch.finfo(dtype).max, torch.finfo(dtype).min
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, s)]
+        out = sink_attention(*leaves, window=30)
+        grads = torch.autograd.grad(out, leaves, do)
+        assert not out[:, :, 0].any() and not grads[0][:, 0].any() and not grads[3][:2].any()
+        assert all(torch.isfinite(t).all() for t in (out, *grads))
+        # (the bits of a row go with its tile, whose rows move their running maximum together: the oracle's bounds)
+        none = oa.attention(q[:, 1:2], k[:, :1], v[:, :1], window=30, bounds=True)
+        _close(out[:, :, 1:2], none["out"], none["out_tol"], "out")

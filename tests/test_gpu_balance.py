@@ -169,3 +169,34 @@ def test_refusals(dev):
                           (ValueError, (z, 4), dict(token_mask=torch.ones(9, device=dev)))]:
         with pytest.raises(exc):
             routing.balance_loss(*args, **kw)
+
+
+def test_saved_tensors_that_come_back_with_other_strides(dev):
+    from agent_factory_3_amd import routing
+    wide, _ = _logits(300, 80, 0, dev)
+    z = wide[:, 8:40].detach().requires_grad_()
+    mask = torch.arange(300, device=dev) % 3 != 0
+
+    def grad():
+        return torch.autograd.grad(routing.balance_loss(z, 4, token_mask=mask)[0], z)[0]
+    want = grad()
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.equal(grad(), want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.t().contiguous().t() if t.dim() == 2 else t, lambda t: t):
+        assert torch.equal(grad(), want)
+
+
+def test_losses_read_without_gradients_first(dev):
+    """Counts logged under no_grad before the loss is used must not cost it its gradient."""
+    from agent_factory_3_amd import routing
+    z = _logits(100, 32, 0, dev)[0].requires_grad_()
+    with routing.collect_balance() as balance:
+        routing._COLLECTORS[-1].add("layer", z, 4)
+    with torch.no_grad():
+        counts = balance.counts()
+        value = balance.loss()
+    loss = balance.loss()
+    assert torch.equal(loss.detach(), value) and int(counts.sum()) == 400
+    (d,) = torch.autograd.grad(loss, z)
+    (want,) = torch.autograd.grad(routing.balance_loss(z, 4)[0], z)
+    assert torch.equal(d, want)
