@@ -56,7 +56,7 @@ struct SaParams {
   float scale, scale2;                    // scale2 = scale log2(e)
   uint16_t *out, *out_lo;                 // [B][Sq][Hq][D]; out_lo: what rounding out left, or NULL
   float* lse;                             // [B][Hkv][Sq][G], log2 units; or NULL
-  float* part;                            // n_split > 1: [n_split][B][Hkv][Sq][G][D] then (m, l) pairs
+  float* part;                            // n_split > 1: [n_split][B][Hkv][Sq][G][D] then {m, l, ln, -}
   // backward
   const uint16_t* dout;                   // [B][Sq][Hq][D] by strides
   int64_t do_sb, do_sh, do_st;
@@ -167,6 +167,18 @@ __device__ __forceinline__ af3_bf16x8 a_pack8(const af3_f32x16& p, int t) {
   for (int i = 0; i < 4; ++i) w[i] = af3_pack_bf16x2(p[8 * t + 2 * i], p[8 * t + 2 * i + 1]);
   return __builtin_bit_cast(af3_bf16x8, w);
 }
+
+// sum of a bf16 operand's entries, on x
+__device__ __forceinline__ float a_sum8(af3_bf16x8 p, float x) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[2 * i], p[2 * i + 1]}, one, x, false);
+  return x;
+}
+
+// 1 / x, 0 where a row has seen nothing (a NaN stays one)
+__device__ __forceinline__ float a_inverse(float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : x); }
 
 // over a lane and its partner in the other half (lane ^ 32)
 __device__ __forceinline__ float a_max_halves(float x) {
@@ -302,7 +314,7 @@ struct KvCopy {
   }
 };
 
-template <int D>
+template <int D, bool LSE>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kBN * D * 2;
@@ -354,11 +366,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
   }
-  float m = kLowest, l = 0.f;
+  float m = kLowest, l = 0.f, ln = 0.f;  // ln: the sum of the probabilities as they are rounded
   if (p.sinks && split == 0) {
     const float s2 = a_sink2(p, head);
     m = fmaxf(s2, kLowest);
-    l = lh == 0 ? __builtin_amdgcn_exp2f(s2 - m) : 0.f;
+    ln = lh == 0 ? __builtin_amdgcn_exp2f(s2 - m) : 0.f;
+    l = ln;
   }
   a_landed(qf);
   af3_f32x16 o[DB];
@@ -402,7 +415,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       const float nm = fmaxf(m, mx);
       const float alpha = __builtin_amdgcn_exp2f(m - nm);
       m = nm;
-      l *= alpha;
+      ln *= alpha;
+      if constexpr (LSE) l *= alpha;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -421,12 +435,15 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       if (x == KS / 2 - 1)
 #pragma unroll
         for (int d = 0; d < DB; ++d) vf[d] = fr.tr8(vt, c * 32, d);
-      if (x == KS / 2) pf = a_pack8(s[0], 0);
+      if (x == KS / 2) {
+        pf = a_pack8(s[0], 0);
+        ln = a_sum8(pf, ln);
+      }
       if (x >= KS / 2) o[x - KS / 2] = a_mfma(vf[x - KS / 2], pf, o[x - KS / 2]);
 #pragma unroll
       for (int r = x * (16 / KS); r < (x + 1) * (16 / KS); ++r) {
         s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -m));
-        l += s[0][r];
+        if constexpr (LSE) l += s[0][r];
       }
       if (x == KS - 1)
 #pragma unroll
@@ -434,6 +451,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       __builtin_amdgcn_sched_barrier(0);
     }
     pf = a_pack8(s[0], 1);
+    ln = a_sum8(pf, ln);
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = a_mfma(vf[d], pf, o[d]);
   };
@@ -466,7 +484,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       for (int x = 0; x < KS; ++x) sa[0] = a_mfma(fr.row8(kt, 0, x), qf[x], sa[0]);
     }
   }
-  l = a_sum_halves(l);
+  ln = a_sum_halves(ln);
+  l = LSE ? a_sum_halves(l) : ln;
   if (!valid) return;
   const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + g;
   if (p.n_split > 1) {
@@ -477,10 +496,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
         *(float4*)(po + d * 32 + 2 * r + 4 * lh) = float4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-    if (lh == 0) *(float2*)(p.part + p.n_split * rows * D + (split * rows + prow) * 2) = float2{m, l};
+    if (lh == 0) *(float4*)(p.part + p.n_split * rows * D + (split * rows + prow) * 4) = float4{m, l, ln, 0.f};
     return;
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
+  const float inv = a_inverse(ln);
   const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
@@ -496,19 +515,19 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       *(u32x2*)(p.out + orow + d * 32 + 2 * r + 4 * lh) = w;
       if (p.out_lo) *(u32x2*)(p.out_lo + orow + d * 32 + 2 * r + 4 * lh) = e;
     }
-  if (p.lse && lh == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (LSE && lh == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // joins the splits of a row: one block per row, each wave a quarter of the splits
 template <int D>
 __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
-  __shared__ float sw[kMaxSplit], so[4][D], sl[4];
+  __shared__ float sw[kMaxSplit], so[4][D], sl[4], sn[4];
   const int64_t rows = (int64_t)p.B * p.Hkv * p.Sq * p.G;
   const int64_t prow = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* ml = p.part + p.n_split * rows * D;
   const int s0 = threadIdx.x;
-  const float2 x = s0 < p.n_split ? *(const float2*)(ml + (s0 * rows + prow) * 2) : float2{kLowest, 0.f};
+  const float4 x = s0 < p.n_split ? *(const float4*)(ml + (s0 * rows + prow) * 4) : float4{kLowest, 0.f, 0.f, 0.f};
   float m = x.x;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -517,11 +536,11 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
   m = fmaxf(fmaxf(sl[0], sl[1]), fmaxf(sl[2], sl[3]));
   const float w = __builtin_amdgcn_exp2f(x.x - m);
   sw[s0] = w;
-  float l = w * x.y;
+  float l = w * x.y, ln = w * x.z;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o), ln += __shfl_xor(ln, o);
   __syncthreads();
-  if (lane == 0) sl[wave] = l;
+  if (lane == 0) sl[wave] = l, sn[wave] = ln;
   float o[D / 64] = {};
   const float* po = p.part + prow * D + lane;
 #pragma unroll 8
@@ -532,7 +551,7 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
   for (int d = 0; d < D / 64; ++d) so[wave][d * 64 + lane] = o[d];
   __syncthreads();
   l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const float inv = a_inverse((sn[0] + sn[1]) + (sn[2] + sn[3]));
   const int g = (int)(prow % p.G);
   const int64_t u = prow / p.G;
   const int t = (int)(u % p.Sq);
@@ -1240,7 +1259,7 @@ extern "C" size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int
                                                      int first, int ranges) {
   if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq / Hkv > kRows || Sq <= 0 || Sk < 0) return 0;
   const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first, ranges != 0);
-  return s.n_split > 1 ? (size_t)s.n_split * B * Hq * Sq * (D + 2) * 4 : 0;
+  return s.n_split > 1 ? (size_t)s.n_split * B * Hq * Sq * (D + 4) * 4 : 0;
 }
 
 extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
@@ -1271,16 +1290,20 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
                 "%s: workspace too small", who);
     p.part = (float*)workspace;
   }
-  if (D == 64)
-    hipLaunchKernelGGL(sa_fwd_kernel<64>, dim3((unsigned)grid), dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL(sa_fwd_kernel<128>, dim3((unsigned)grid), dim3(256), 0, stream, p);
+  const dim3 g((unsigned)grid), block(256);
+  if (D == 64) {
+    if (lse) hipLaunchKernelGGL((sa_fwd_kernel<64, true>), g, block, 0, stream, p);
+    else hipLaunchKernelGGL((sa_fwd_kernel<64, false>), g, block, 0, stream, p);
+  } else {
+    if (lse) hipLaunchKernelGGL((sa_fwd_kernel<128, true>), g, block, 0, stream, p);
+    else hipLaunchKernelGGL((sa_fwd_kernel<128, false>), g, block, 0, stream, p);
+  }
   if (s.n_split > 1) {
-    const unsigned g = (unsigned)((int64_t)B * Hq * Sq);
+    const dim3 rows((unsigned)((int64_t)B * Hq * Sq));
     if (D == 64)
-      hipLaunchKernelGGL(sa_join_kernel<64>, dim3(g), dim3(256), 0, stream, p);
+      hipLaunchKernelGGL(sa_join_kernel<64>, rows, block, 0, stream, p);
     else
-      hipLaunchKernelGGL(sa_join_kernel<128>, dim3(g), dim3(256), 0, stream, p);
+      hipLaunchKernelGGL(sa_join_kernel<128>, rows, block, 0, stream, p);
   }
   return af3::check_launch(who);
 }
