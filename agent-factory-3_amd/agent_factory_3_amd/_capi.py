@@ -79,10 +79,10 @@ _SIGNATURES = {
     "af3_seq_starts_positions": (_i32, [_p, _i32, _p, _p]),
     "af3_sink_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "af3_sink_attention_fwd": (_i32, [_p, _p, _p, _p, _p, _i32, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
-                                      _i32, _f32, _p, _p, _p, _p, _sz, _p]),
+                                      _i32, _f32, _p, _p, _p, _sz, _p]),
     "af3_sink_attention_bwd_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "af3_sink_attention_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
-                                      _i32, _f32, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+                                      _i32, _f32, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "af3_balance_loss_workspace_bytes": (_sz, [_i64, _i32]),
     "af3_balance_loss_fwd": (_i32, [_p, _i64, _p, _p, _i64, _i32, _i32, _p, _p, _p, _p, _sz, _p]),
     "af3_balance_loss_bwd": (_i32, [_p, _i64, _p, _i64, _i32, _p, _p, _p, _p]),

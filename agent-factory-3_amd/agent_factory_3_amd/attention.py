@@ -60,7 +60,7 @@ def _c_strides(strides: tuple):
     return (ctypes.c_int64 * len(strides))(*strides)
 
 
-def _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, kv_range, out_lo, lse):
+def _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, kv_range, lse):
     B, Hq, Sq, D = q.shape
     Hkv, Sk = k.shape[1], k.shape[2]
     dev = q.device
@@ -70,7 +70,7 @@ def _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, 
     _capi.call("af3_sink_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _c_strides(strides),
                _capi.ptr(sinks), int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(cu_seqlens),
                cu_seqlens.numel() - 1 if cu_seqlens is not None else 0, _capi.ptr(starts), _capi.ptr(kv_range), B, Hq,
-               Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), out_lo, lse, _capi.ptr(ws), ws_n,
+               Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), _capi.ptr(lse), _capi.ptr(ws), ws_n,
                _capi.stream_of(dev))
     return out
 
@@ -79,19 +79,16 @@ class _SinkAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, sinks, strides, scale, window, first, cu_seqlens, starts, kv_range):
         B, Hq, Sq, D = q.shape
-        # kept for the backward in one buffer: what rounding the output left, and the rows' log-sums
-        n = B * Hq * Sq
-        keep = torch.empty(n * (2 * D + 4), dtype=torch.uint8, device=q.device)
-        out = _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, kv_range, keep.data_ptr(),
-                       keep.data_ptr() + 2 * D * n)
-        ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, keep)
+        lse = torch.empty(B * Hq * Sq, dtype=torch.float32, device=q.device)
+        out = _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, kv_range, lse)
+        ctx.save_for_backward(q, k, v, sinks, starts, kv_range, out, lse)
         ctx.args = (scale, window, first)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, sinks, starts, kv_range, out, keep = ctx.saved_tensors
+        q, k, v, sinks, starts, kv_range, out, lse = ctx.saved_tensors
         scale, window, first = ctx.args
         B, Hq, Sq, D = q.shape
         Hkv, Sk = k.shape[1], k.shape[2]
@@ -99,8 +96,8 @@ class _SinkAttention(torch.autograd.Function):
         with _device_of(q):
             # (saved-tensor hooks, as those that keep them on the host, may give them other strides)
             (q, sq), (k, sk), (v, sv) = _rows(q, heads=True), _rows(k), _rows(v)
-            sinks, starts, kv_range, out, keep = (t if t is None else t.contiguous()
-                                                  for t in (sinks, starts, kv_range, out, keep))
+            sinks, starts, kv_range, out, lse = (t if t is None else t.contiguous()
+                                                 for t in (sinks, starts, kv_range, out, lse))
             do, st = _rows(dout.transpose(1, 2), heads=True)
             dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=dev)
             dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=dev)
@@ -112,8 +109,8 @@ class _SinkAttention(torch.autograd.Function):
                        _c_strides(sq + sk + sv + st), _capi.ptr(sinks),
                        int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(starts),
                        _capi.ptr(kv_range), B, Hq, Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(),
-                       keep.data_ptr(), keep.data_ptr() + 2 * D * B * Hq * Sq, dq.data_ptr(), dk.data_ptr(),
-                       dv.data_ptr(), _capi.ptr(dsinks), ws.data_ptr(), ws_n, _capi.stream_of(dev))
+                       lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _capi.ptr(dsinks), ws.data_ptr(),
+                       ws_n, _capi.stream_of(dev))
         return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dsinks, *[None] * 7
 
 
@@ -156,7 +153,7 @@ def _run(q, k, v, sinks, scale, window, first, cu_seqlens, starts, kv_range):
         sinks = sinks.contiguous()
     args = (sq + sk + sv, sinks, scale, window, first, cu_seqlens, starts, kv_range)
     if not need:
-        return _forward(q, k, v, *args, None, None)
+        return _forward(q, k, v, *args, None)
     return _SinkAttention.apply(q, k, v, sinks, sq + sk + sv, *args[2:])
 
 

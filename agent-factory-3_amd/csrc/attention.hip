@@ -54,9 +54,9 @@ struct SaParams {
   int tok;                                // tokens of a row tile
   int n_tiles, n_split;
   float scale, scale2;                    // scale2 = scale log2(e)
-  uint16_t *out, *out_lo;                 // [B][Sq][Hq][D]; out_lo: what rounding out left, or NULL
+  uint16_t* out;                          // [B][Sq][Hq][D]
   float* lse;                             // [B][Hkv][Sq][G], log2 units; or NULL
-  float* part;                            // n_split > 1: [n_split][B][Hkv][Sq][G][D] then {m, l, ln, -}
+  float* part;                            // n_split > 1: [n_split][B][Hkv][Sq][G][D] then (m, l) pairs
   // backward
   const uint16_t* dout;                   // [B][Sq][Hq][D] by strides
   int64_t do_sb, do_sh, do_st;
@@ -168,18 +168,6 @@ __device__ __forceinline__ af3_bf16x8 a_pack8(const af3_f32x16& p, int t) {
   return __builtin_bit_cast(af3_bf16x8, w);
 }
 
-// sum of a bf16 operand's entries, on x
-__device__ __forceinline__ float a_sum8(af3_bf16x8 p, float x) {
-  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-  const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[2 * i], p[2 * i + 1]}, one, x, false);
-  return x;
-}
-
-// 1 / x, 0 where a row has seen nothing (a NaN stays one)
-__device__ __forceinline__ float a_inverse(float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : x); }
-
 // over a lane and its partner in the other half (lane ^ 32)
 __device__ __forceinline__ float a_max_halves(float x) {
   const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -268,11 +256,25 @@ __device__ __forceinline__ Keys a_keys(const SaParams& p, int pos0, int pos1, in
 }
 
 // ---------------------------------------------------------------------------
-// forward.  Block = 4 waves of 32 rows; 64-key tiles of K and V through a
-// two-stage LDS ring (global->LDS copies one tile ahead).  S^T = K Q^T puts a
-// row's scores into its lane; the running maximum moves only when it grows by
-// more than 8 (log2 units: probabilities stay below 256), so most tiles need
-// no rescaling of the output.
+// forward.  Block = 4 waves of 32 rows; 64-key tiles through LDS, K round two
+// stages and V round three (global->LDS copies a tile ahead, one barrier per
+// tile; 40 KB at D = 64, so four blocks share a CU).  S^T = K Q^T puts a row's
+// scores into its lane; the running maximum moves only when it grows by more
+// than 8 (log2 units: probabilities stay below 256), so most tiles need no
+// rescaling of the output.  Probabilities are rounded to bf16 for the product
+// with V, their sum is not: the output is 1.3 times one bf16 rounding off.
+//
+// Bound by the vector unit, not the matrix unit: an exponential issues over 16
+// cycles, so 32 keys of 32 rows cost 256 cycles of them next to 256 of the two
+// products; the counters give 84% of the cycles to the vector unit and 46% to
+// the matrix unit.  8192 packed rows of 2144 keys on average, 64 heads over 8,
+// D 64: 342 us (840 TFLOP/s); a window of 128: 54 us; 2 x 4096 rows: 319 us (862
+// TFLOP/s).  Where a wave's rows are few the tiles are read at memory speed: one
+// token over 131072 keys 43 us (6.2 TB/s), 32 tokens over 4099: 26.7 us (5.1).
+// A window's block runs three to four tiles, so its start (first copies, q rows)
+// is a third of it.  Stages as constants of six unrolled turns gain 3% on the
+// long rows and lose 10% on the window (code fetched once per block), so the
+// stages stay variables here.
 // ---------------------------------------------------------------------------
 constexpr int kRows = 128;  // rows of a tile
 constexpr int kBN = 64;     // keys of a tile
@@ -314,7 +316,7 @@ struct KvCopy {
   }
 };
 
-template <int D, bool LSE>
+template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kBN * D * 2;
@@ -366,12 +368,11 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
   }
-  float m = kLowest, l = 0.f, ln = 0.f;  // ln: the sum of the probabilities as they are rounded
+  float m = kLowest, l = 0.f;
   if (p.sinks && split == 0) {
     const float s2 = a_sink2(p, head);
     m = fmaxf(s2, kLowest);
-    ln = lh == 0 ? __builtin_amdgcn_exp2f(s2 - m) : 0.f;
-    l = ln;
+    l = lh == 0 ? __builtin_amdgcn_exp2f(s2 - m) : 0.f;
   }
   a_landed(qf);
   af3_f32x16 o[DB];
@@ -415,8 +416,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       const float nm = fmaxf(m, mx);
       const float alpha = __builtin_amdgcn_exp2f(m - nm);
       m = nm;
-      ln *= alpha;
-      if constexpr (LSE) l *= alpha;
+      l *= alpha;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -435,15 +435,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       if (x == KS / 2 - 1)
 #pragma unroll
         for (int d = 0; d < DB; ++d) vf[d] = fr.tr8(vt, c * 32, d);
-      if (x == KS / 2) {
-        pf = a_pack8(s[0], 0);
-        ln = a_sum8(pf, ln);
-      }
+      if (x == KS / 2) pf = a_pack8(s[0], 0);
       if (x >= KS / 2) o[x - KS / 2] = a_mfma(vf[x - KS / 2], pf, o[x - KS / 2]);
 #pragma unroll
       for (int r = x * (16 / KS); r < (x + 1) * (16 / KS); ++r) {
         s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -m));
-        if constexpr (LSE) l += s[0][r];
+        l += s[0][r];
       }
       if (x == KS - 1)
 #pragma unroll
@@ -451,7 +448,6 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       __builtin_amdgcn_sched_barrier(0);
     }
     pf = a_pack8(s[0], 1);
-    ln = a_sum8(pf, ln);
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = a_mfma(vf[d], pf, o[d]);
   };
@@ -484,8 +480,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
       for (int x = 0; x < KS; ++x) sa[0] = a_mfma(fr.row8(kt, 0, x), qf[x], sa[0]);
     }
   }
-  ln = a_sum_halves(ln);
-  l = LSE ? a_sum_halves(l) : ln;
+  l = a_sum_halves(l);
   if (!valid) return;
   const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + g;
   if (p.n_split > 1) {
@@ -496,38 +491,34 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
         *(float4*)(po + d * 32 + 2 * r + 4 * lh) = float4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-    if (lh == 0) *(float4*)(p.part + p.n_split * rows * D + (split * rows + prow) * 4) = float4{m, l, ln, 0.f};
+    if (lh == 0) *(float2*)(p.part + p.n_split * rows * D + (split * rows + prow) * 2) = float2{m, l};
     return;
   }
-  const float inv = a_inverse(ln);
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
   const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      u32x2 w, e;
+      u32x2 w;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float y0 = o[d][r + 2 * x] * inv, y1 = o[d][r + 2 * x + 1] * inv;
-        w[x] = af3_pack_bf16x2(y0, y1);
-        e[x] = af3_pack_bf16x2(y0 - af3_bf16_to_f32(w[x] & 0xFFFFu), y1 - af3_bf16_to_f32(w[x] >> 16));
-      }
+      for (int x = 0; x < 2; ++x) w[x] = af3_pack_bf16x2(o[d][r + 2 * x] * inv, o[d][r + 2 * x + 1] * inv);
       *(u32x2*)(p.out + orow + d * 32 + 2 * r + 4 * lh) = w;
-      if (p.out_lo) *(u32x2*)(p.out_lo + orow + d * 32 + 2 * r + 4 * lh) = e;
     }
-  if (LSE && lh == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (p.lse && lh == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // joins the splits of a row: one block per row, each wave a quarter of the splits
+// (64 rows of 64 splits: 4.0 us, a launch's latency and two dependent loads)
 template <int D>
 __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
-  __shared__ float sw[kMaxSplit], so[4][D], sl[4], sn[4];
+  __shared__ float sw[kMaxSplit], so[4][D], sl[4];
   const int64_t rows = (int64_t)p.B * p.Hkv * p.Sq * p.G;
   const int64_t prow = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* ml = p.part + p.n_split * rows * D;
   const int s0 = threadIdx.x;
-  const float4 x = s0 < p.n_split ? *(const float4*)(ml + (s0 * rows + prow) * 4) : float4{kLowest, 0.f, 0.f, 0.f};
+  const float2 x = s0 < p.n_split ? *(const float2*)(ml + (s0 * rows + prow) * 2) : float2{kLowest, 0.f};
   float m = x.x;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -536,11 +527,11 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
   m = fmaxf(fmaxf(sl[0], sl[1]), fmaxf(sl[2], sl[3]));
   const float w = __builtin_amdgcn_exp2f(x.x - m);
   sw[s0] = w;
-  float l = w * x.y, ln = w * x.z;
+  float l = w * x.y;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o), ln += __shfl_xor(ln, o);
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
   __syncthreads();
-  if (lane == 0) sl[wave] = l, sn[wave] = ln;
+  if (lane == 0) sl[wave] = l;
   float o[D / 64] = {};
   const float* po = p.part + prow * D + lane;
 #pragma unroll 8
@@ -551,7 +542,7 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
   for (int d = 0; d < D / 64; ++d) so[wave][d * 64 + lane] = o[d];
   __syncthreads();
   l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float inv = a_inverse((sn[0] + sn[1]) + (sn[2] + sn[3]));
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const int g = (int)(prow % p.G);
   const int64_t u = prow / p.G;
   const int t = (int)(u % p.Sq);
@@ -559,10 +550,7 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
   const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + hk * p.G + g) * D;
   if ((int)threadIdx.x < D) {
     const int d = threadIdx.x;
-    const float y = ((so[0][d] + so[1][d]) + (so[2][d] + so[3][d])) * inv;
-    const uint32_t r = af3_f32_to_bf16(y);
-    p.out[orow + d] = (uint16_t)r;
-    if (p.out_lo) p.out_lo[orow + d] = (uint16_t)af3_f32_to_bf16(y - af3_bf16_to_f32(r));
+    p.out[orow + d] = (uint16_t)af3_f32_to_bf16(((so[0][d] + so[1][d]) + (so[2][d] + so[3][d])) * inv);
   }
   if (p.lse && threadIdx.x == 0) p.lse[prow] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
@@ -570,9 +558,25 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
 // ---------------------------------------------------------------------------
 // backward, queries: dq, delta and the sinks' partial sums.  The forward's
 // tiles and layouts; p comes back from the saved log-sum.
+//
+// delta.  do . out of the rounded output is off by 2^-9 |do| |out|, which would
+// be the largest error of the whole backward (the error of out is that of every
+// key's probability and of its own rounding): dq 1.66, dk 1.58 times one bf16
+// rounding.  So a tile uses that delta0, and the sums of dz and p k beside dz k
+// give the true one at the end: sum dz = delta - delta0 sum p, sum p = 1 - p_sink,
+// and dq = scale (sum dz k - (delta - delta0) sum p k).  dk, dv and the sinks take
+// the true delta: dq 1.44, dk 1.41 times one rounding (of dz, and the result's),
+// dsinks none.  The bf16 remainder of out kept by the forward costs more (its
+// writing alone 15 us of 70 with a window of 128) and corrects less (dq 1.53).
+//
+// Four products per step on the matrix unit; the second accumulator takes the
+// registers of a third block per CU.  8192 packed rows, 64 heads over 8, D 64:
+// 548 us (of 2144 keys on average; 4 products: 1050 TFLOP/s counting all of them),
+// 102 us with a window of 128, where half is a block's start: q, dout and out rows
+// and the first tiles, 5 us for each of the two blocks a CU holds.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p) {
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kTile = kBN * D * 2;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
@@ -617,34 +621,22 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
     const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
     const uint16_t* dr = p.dout + b * p.do_sb + head * p.do_sh + t * p.do_st;
     const int64_t orow = (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
-    af3_bf16x8 of[KS], oe[KS];
+    af3_bf16x8 of[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qf[s] = *(const af3_bf16x8*)(qr + s * 16 + lh * 8);
       df[s] = *(const af3_bf16x8*)(dr + s * 16 + lh * 8);
       of[s] = *(const af3_bf16x8*)(p.out + orow + s * 16 + lh * 8);
-      oe[s] = *(const af3_bf16x8*)(p.out_lo + orow + s * 16 + lh * 8);
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[s][i] + (float)oe[s][i], delta);
+      for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[s][i], delta);
     delta = a_sum_halves(delta);
     a_landed(qf);
     a_landed(df);
   }
   asm volatile("" : "+v"(lse));  // landed, as the operands
-  if (valid && lh == 0) p.delta[prow] = -delta;
-  if (p.sinks) {
-    if (lh == 0) ds_row[row] = valid ? -__builtin_amdgcn_exp2f(a_sink2(p, head) - lse) * delta : 0.f;
-    __syncthreads();
-    if ((int)threadIdx.x < p.G) {  // the tile's sum for each of the shared heads, in token order
-      float sum = 0.f;
-      for (int x = 0; x < p.tok; ++x) sum += ds_row[x * p.G + threadIdx.x];
-      p.dsink_part[((int64_t)tile * p.B + b) * p.Hq + hk * p.G + threadIdx.x] = sum;
-    }
-  }
-
   // the wave's own tiles and those of which its rows see every key, as in the forward
   const int wt0 = t0 + (wave * 32 * p.g_mul >> 16), wt1 = min(t1, t0 + ((wave * 32 + 31) * p.g_mul >> 16));
   const int wpos0 = wt0 + off, wpos1 = wt1 + off;
@@ -654,75 +646,147 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void sa_dq_kernel(SaParams p)
   const int free0 = na + max(0, from - ks.b0 + kBN - 1) / kBN;
   const int free1 = na + max(0, min(wpos0 + 1, ks.b1) - ks.b0) / kBN;
   const Frag<D> fr(lane, lds0);
-  af3_f32x16 acc[DB];
+  af3_f32x16 acc[DB], pk[DB];  // sum dz k and sum p k
+  float dsum = 0.f;            // sum dz
 #pragma unroll
-  for (int d = 0; d < DB; ++d) acc[d] = a_zero();
+  for (int d = 0; d < DB; ++d) acc[d] = a_zero(), pk[d] = a_zero();
   auto turn = [&](int i, auto stage) {  // (the stage a constant: its addresses need no arithmetic)
     A_WAIT_VM(0);
     A_BARRIER();
     if (i + 1 < na + nb) issue(i + 1, 1 - stage.value);
     constexpr uint32_t kt = stage.value * 2 * kTile, vt = kt + kTile;
     if (i < own0 || i >= own1) return;
-    // (reads ahead of their use, held by the barriers, as in the dk / dv kernel)
-    af3_bf16x8 kr[KS], vr[KS], tr[DB];
-#pragma unroll
-    for (int x = 0; x < KS; ++x) kr[x] = fr.row8(kt, 0, x);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      af3_f32x16 s[1] = {a_zero()}, dp;
-#pragma unroll
-      for (int x = 0; x < KS; ++x) vr[x] = fr.row8(vt, c * 32, x);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = -delta;
-#pragma unroll
-      for (int x = 0; x < KS; ++x) s[0] = a_mfma(kr[x], qf[x], s[0]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) tr[d] = fr.tr8(kt, c * 32, d);
-#pragma unroll
-      for (int x = 0; x < KS; ++x) dp = a_mfma(vr[x], df[x], dp);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -lse)) * dp[r];
-      // (the product is set to zero, not the score: whatever stands at a key that the row does not see)
-      if (i < free0 || i >= free1) {
-        const int j = first_key(i) + c * 32;
-        if (i < na) {
-          a_mask_end(s, j + 4 * lh, min(vis.lo + vis.fn, ks.a1), 0.f);
-          a_mask_from(s, j + 4 * lh, vis.lo, 0.f);
-        } else if (p.first > 0 && j < last_lo + p.first) {
-          a_mask_both(s, j + 4 * lh, vis, 0.f);
-        } else {
-          if (j + 31 > wpos0 || j + 32 > ks.b1) a_mask_end(s, j + 4 * lh, vis.end, 0.f);
-          if (j < from) a_mask_from(s, j + 4 * lh, vis.w, 0.f);
-        }
+    // Written in the order in which it has to issue (the barriers hold it): reads ahead
+    // of their use, the first half's exponentials beside the second's scores, its
+    // products beside the second's exponentials (without: 572 us, with 548).
+    af3_bf16x8 ka[KS], va[KS], kb[KS], vb[KS], tr[DB], ts[DB];
+    af3_f32x16 s0[1] = {a_zero()}, s1[1] = {a_zero()}, d0[1], d1[1];
+    const bool whole = i >= free0 && i < free1;
+    // (dz is set to zero too, not p alone: whatever stands at a key that the row does not see)
+    auto mask = [&](int j, af3_f32x16 (&x)[1]) {
+      if (i < na) {
+        a_mask_end(x, j + 4 * lh, min(vis.lo + vis.fn, ks.a1), 0.f);
+        a_mask_from(x, j + 4 * lh, vis.lo, 0.f);
+      } else if (p.first > 0 && j < last_lo + p.first) {
+        a_mask_both(x, j + 4 * lh, vis, 0.f);
+      } else {
+        if (j + 31 > wpos0 || j + 32 > ks.b1) a_mask_end(x, j + 4 * lh, vis.end, 0.f);
+        if (j < from) a_mask_from(x, j + 4 * lh, vis.w, 0.f);
       }
-      const af3_bf16x8 p0 = a_pack8(s[0], 0), p1 = a_pack8(s[0], 1);
+    };
+    auto exps = [&](af3_f32x16& x, int r0, int n) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d) acc[d] = a_mfma(tr[d], p0, acc[d]);
+      for (int r = r0; r < r0 + n; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], p.scale2, -lse));
+    };
 #pragma unroll
-      for (int d = 0; d < DB; ++d) tr[d] = fr.tr8(kt, c * 32 + 16, d);
-      if (c == 0)
+    for (int x = 0; x < KS; ++x) ka[x] = fr.row8(kt, 0, x);
 #pragma unroll
-        for (int x = 0; x < KS; ++x) kr[x] = fr.row8(kt, 32, x);
+    for (int x = 0; x < KS; ++x) va[x] = fr.row8(vt, 0, x);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) d0[0][r] = d1[0][r] = -delta;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) s0[0] = a_mfma(ka[x], qf[x], s0[0]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) kb[x] = fr.row8(kt, 32, x);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) d0[0] = a_mfma(va[x], df[x], d0[0]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      s1[0] = a_mfma(kb[x], qf[x], s1[0]);
+      vb[x] = fr.row8(vt, 32, x);
+      exps(s0[0], x * (16 / KS), 16 / KS);
       __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-      for (int d = 0; d < DB; ++d) acc[d] = a_mfma(tr[d], p1, acc[d]);
+    for (int d = 0; d < DB; ++d) tr[d] = fr.tr8(kt, 0, d);
+    if (!whole) mask(first_key(i), s0);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      d1[0] = a_mfma(vb[x], df[x], d1[0]);
+#pragma unroll
+      for (int r = x * (16 / KS); r < (x + 1) * (16 / KS); ++r) d0[0][r] *= s0[0][r];
+      if (x >= KS / 2) {
+        const int d = x - KS / 2;
+        ts[d] = fr.tr8(kt, 16, d);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!whole) mask(first_key(i), d0);
+    {
+      const af3_bf16x8 z0 = a_pack8(d0[0], 0), p0 = a_pack8(s0[0], 0), z1 = a_pack8(d0[0], 1), p1 = a_pack8(s0[0], 1);
+      constexpr int E = 16 / (2 * DB);  // exponentials beside a pair of products
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        acc[d] = a_mfma(tr[d], z0, acc[d]);
+        pk[d] = a_mfma(tr[d], p0, pk[d]);
+        exps(s1[0], d * E, E);
+        tr[d] = fr.tr8(kt, 32, d);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        acc[d] = a_mfma(ts[d], z1, acc[d]);
+        pk[d] = a_mfma(ts[d], p1, pk[d]);
+        exps(s1[0], (DB + d) * E, E);
+        ts[d] = fr.tr8(kt, 48, d);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (!whole) mask(first_key(i) + 32, s1);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dsum += d0[0][r];
+      d1[0][r] *= s1[0][r];
+    }
+    if (!whole) mask(first_key(i) + 32, d1);
+    const af3_bf16x8 z0 = a_pack8(d1[0], 0), p0 = a_pack8(s1[0], 0), z1 = a_pack8(d1[0], 1), p1 = a_pack8(s1[0], 1);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      acc[d] = a_mfma(tr[d], z0, acc[d]);
+      pk[d] = a_mfma(tr[d], p0, pk[d]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dsum += d1[0][r];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      acc[d] = a_mfma(ts[d], z1, acc[d]);
+      pk[d] = a_mfma(ts[d], p1, pk[d]);
     }
   };
   for (int i = 0; i < na + nb; i += 2) {
     turn(i, Int<0>{});
     if (i + 1 < na + nb) turn(i + 1, Int<1>{});
   }
+  // The row's true delta, sum p dp = sum dz + delta sum p with sum p = 1 - p_sink, and
+  // what dq lacks for it: -(true delta - delta) sum p k.
+  const float p_sink = p.sinks ? __builtin_amdgcn_exp2f(a_sink2(p, head) - lse) : 0.f;
+  const float c = a_sum_halves(dsum) - delta * p_sink;
+  delta += c;
+  if (valid && lh == 0) p.delta[prow] = -delta;
+  if (p.sinks) {
+    if (lh == 0) ds_row[row] = valid ? -p_sink * delta : 0.f;
+    __syncthreads();
+    if ((int)threadIdx.x < p.G) {  // the tile's sum for each of the shared heads, in token order
+      float sum = 0.f;
+      for (int x = 0; x < p.tok; ++x) sum += ds_row[x * p.G + threadIdx.x];
+      p.dsink_part[((int64_t)tile * p.B + b) * p.Hq + hk * p.G + threadIdx.x] = sum;
+    }
+  }
   if (!valid) return;
   uint16_t* qrow = p.dq + (((int64_t)b * p.Sq + t) * p.Hq + head) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *(u32x2*)(qrow + d * 32 + 2 * r + 4 * lh) =
-          u32x2{af3_pack_bf16x2(acc[d][r] * p.scale, acc[d][r + 1] * p.scale),
-                af3_pack_bf16x2(acc[d][r + 2] * p.scale, acc[d][r + 3] * p.scale)};
+    for (int r = 0; r < 16; r += 4) {
+      u32x2 w;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        w[x] = af3_pack_bf16x2(fmaf(-c, pk[d][r + 2 * x], acc[d][r + 2 * x]) * p.scale,
+                               fmaf(-c, pk[d][r + 2 * x + 1], acc[d][r + 2 * x + 1]) * p.scale);
+      *(u32x2*)(qrow + d * 32 + 2 * r + 4 * lh) = w;
+    }
 }
 
 // the sinks' gradient of head h from the tiles' sums, in a fixed order (256 threads)
@@ -754,6 +818,13 @@ __device__ __forceinline__ void a_dsink(const SaParams& p, int h, float* sh) {
 // and the rows that see a key are one run of row numbers per lane.  A step's
 // exponentials stand between the products of the next step's scores and of its
 // own first half, held in that order, so that the matrix unit works beside them.
+//
+// Two passes over the scores (this and dq's) instead of one with atomic sums of
+// dq: seven products become nine, but every sum has a fixed order and no fp32
+// copy of dq is written and read.  8192 packed rows, 64 heads over 8, D 64: 681 us
+// (of 2144 keys on average; 5 products: 1055 TFLOP/s), matrix unit busy 45%, the
+// rest LDS reads and the exponentials that do not fit beside products; 82 us with
+// a window of 128, where a block's start and its partly visible steps count.
 // ---------------------------------------------------------------------------
 // first token after t0, whose sequence starts at s0, of a later sequence (starts does
 // not decrease), or n > t0: 64 probes a round, the answer stays in (lo, hi]
@@ -1259,19 +1330,19 @@ extern "C" size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int
                                                      int first, int ranges) {
   if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq / Hkv > kRows || Sq <= 0 || Sk < 0) return 0;
   const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first, ranges != 0);
-  return s.n_split > 1 ? (size_t)s.n_split * B * Hq * Sq * (D + 4) * 4 : 0;
+  return s.n_split > 1 ? (size_t)s.n_split * B * Hq * Sq * (D + 2) * 4 : 0;
 }
 
 extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
                                       const void* sinks, int sinks_f32, const int32_t* cu_seqlens, int n_seqs,
                                       int32_t* starts, const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk,
-                                      int D, int window, int first, float scale, uint16_t* out, uint16_t* out_lo, float* lse, void* workspace, size_t ws_bytes,
-                                      void* stream_) {
+                                      int D, int window, int first, float scale, uint16_t* out, float* lse, void* workspace,
+                                      size_t ws_bytes, void* stream_) {
   const char* who = "sink_attention_fwd";
   if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 9, starts, kv_range)) return rc;
   if (B == 0 || Sq == 0) return 0;
   AF3_REQUIRE(q && out && (Sk == 0 || (k && v)), "%s: null pointer", who);
-  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(out) && sa_al16(out_lo),
+  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(out),
               "%s: rows must be 16-byte aligned", who);
   hipStream_t stream = (hipStream_t)stream_;
   AF3_REQUIRE(!cu_seqlens || starts, "%s: cu_seqlens without starts", who);
@@ -1280,7 +1351,6 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
   const SaShape s = sa_shape(B, Hq, Hkv, Sq, Sk, window, first, kv_range != nullptr);
   SaParams p = sa_params(s, q, k, v, strides, sinks, sinks_f32, starts, kv_range, B, Hq, Hkv, Sq, Sk, scale);
   p.out = out;
-  p.out_lo = out_lo;
   p.lse = lse;
   p.n_split = s.n_split;
   const int64_t grid = (int64_t)s.n_tiles * B * Hkv * s.n_split;
@@ -1290,20 +1360,16 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
                 "%s: workspace too small", who);
     p.part = (float*)workspace;
   }
-  const dim3 g((unsigned)grid), block(256);
-  if (D == 64) {
-    if (lse) hipLaunchKernelGGL((sa_fwd_kernel<64, true>), g, block, 0, stream, p);
-    else hipLaunchKernelGGL((sa_fwd_kernel<64, false>), g, block, 0, stream, p);
-  } else {
-    if (lse) hipLaunchKernelGGL((sa_fwd_kernel<128, true>), g, block, 0, stream, p);
-    else hipLaunchKernelGGL((sa_fwd_kernel<128, false>), g, block, 0, stream, p);
-  }
+  if (D == 64)
+    hipLaunchKernelGGL(sa_fwd_kernel<64>, dim3((unsigned)grid), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL(sa_fwd_kernel<128>, dim3((unsigned)grid), dim3(256), 0, stream, p);
   if (s.n_split > 1) {
-    const dim3 rows((unsigned)((int64_t)B * Hq * Sq));
+    const unsigned g = (unsigned)((int64_t)B * Hq * Sq);
     if (D == 64)
-      hipLaunchKernelGGL(sa_join_kernel<64>, rows, block, 0, stream, p);
+      hipLaunchKernelGGL(sa_join_kernel<64>, dim3(g), dim3(256), 0, stream, p);
     else
-      hipLaunchKernelGGL(sa_join_kernel<128>, rows, block, 0, stream, p);
+      hipLaunchKernelGGL(sa_join_kernel<128>, dim3(g), dim3(256), 0, stream, p);
   }
   return af3::check_launch(who);
 }
@@ -1317,16 +1383,16 @@ extern "C" size_t af3_sink_attention_bwd_workspace_bytes(int B, int Hq, int Hkv,
 extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* dout,
                                       const int64_t* strides, const void* sinks, int sinks_f32, const int32_t* starts,
                                       const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk, int D,
-                                      int window, int first, float scale, const uint16_t* out, const uint16_t* out_lo,
-                                      const float* lse, uint16_t* dq, uint16_t* dk, uint16_t* dv, void* dsinks, void* workspace,
+                                      int window, int first, float scale, const uint16_t* out, const float* lse,
+                                      uint16_t* dq, uint16_t* dk, uint16_t* dv, void* dsinks, void* workspace,
                                       size_t ws_bytes, void* stream_) {
   const char* who = "sink_attention_bwd";
   if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 12, starts, kv_range)) return rc;
   const bool nq = B > 0 && Sq > 0, nk = B > 0 && Sk > 0;
-  AF3_REQUIRE((!nq || (q && dout && out && out_lo && lse && dq && workspace)) && (!nk || (k && v && dk && dv)) &&
+  AF3_REQUIRE((!nq || (q && dout && out && lse && dq && workspace)) && (!nk || (k && v && dk && dv)) &&
                   (!sinks || dsinks),
               "%s: null pointer", who);
-  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(dout) && sa_al16(out) && sa_al16(out_lo) && sa_al16(dq) && sa_al16(dk) &&
+  AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(dout) && sa_al16(out) && sa_al16(dq) && sa_al16(dk) &&
                   sa_al16(dv) && sa_al16(workspace),
               "%s: rows must be 16-byte aligned", who);
   AF3_REQUIRE(ws_bytes >= af3_sink_attention_bwd_workspace_bytes(B, Hq, Hkv, Sq), "%s: workspace too small", who);
@@ -1336,7 +1402,6 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
   p.dout = dout;
   p.do_sb = strides[9]; p.do_sh = strides[10]; p.do_st = strides[11];
   p.out = (uint16_t*)out;
-  p.out_lo = (uint16_t*)out_lo;
   p.lse = (float*)lse;
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = (float*)workspace;

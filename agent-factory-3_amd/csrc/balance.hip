@@ -16,6 +16,12 @@
 // (order-preserving logit bits, inverted id) keys, and a lane's column sums and
 // counts stay in its registers over all its rows.  Column sums are fp32 over at
 // most a few hundred rows per lane, then joined in a fixed order.
+//
+// 128000 tokens of 128 experts, ids given: sums 12.1 us (35 MB: 2.9 TB/s), join
+// 4.9, gradient 19.2 (66 MB: 3.4 TB/s); 16384 tokens, top 4: 9.5, 4.1 and 7.3.  A
+// row's exponentials, its reductions and, for the top K, K rounds of maxima are
+// most of the first kernel; the gradient is near what reads and writes mixed reach
+// at this size.  A call of 77 tokens is one launch of 5.2 us and one of 3.0.
 #include "af3_common.h"
 
 namespace {

@@ -451,13 +451,11 @@ int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_
  * the forward writes starts first (as af3_seq_starts), else it reads them.  sinks [Hq]
  * (bf16, or fp32 with sinks_f32; NULL: none) adds e^sink to the softmax's
  * denominator.  A row that sees nothing gives 0.
- *   forward: out [B][Sq][Hq][D]; out_lo, as out: bf16 of what rounding out left,
- *   and lse [B][Hkv][Sq][Hq/Hkv] fp32 (log2 units), both for the backward or
- *   NULL; workspace of af3_sink_attention_workspace_bytes (ranges: whether kv_range is
+ *   forward: out [B][Sq][Hq][D]; lse [B][Hkv][Sq][Hq/Hkv] fp32 (log2 units), for
+ *   the backward, or NULL; workspace of af3_sink_attention_workspace_bytes (ranges: whether kv_range is
  *   given; 0: none needed).
  *   backward: dq [B][Sq][Hq][D], dk and dv [B][Sk][Hkv][D], dsinks [Hq] in the
- *   sinks' type, from the forward's out, out_lo and lse (out + out_lo gives dout . out
- *   to 16 bits: from out alone its error exceeds that of every other rounding); every sum is in a fixed order.
+ *   sinks' type, from the forward's out and lse; every sum is in a fixed order.
  * A key outside every row's range is never read into a product; NaN or infinity
  * in a key, value or gradient row that some row of the same 128-row or 64-key
  * tile sees may reach that tile's other rows.
@@ -465,14 +463,15 @@ int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_
 int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
                            const void* sinks, int sinks_f32, const int32_t* cu_seqlens, int n_seqs, int32_t* starts,
                            const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk, int D, int window,
-                           int first, float scale, uint16_t* out, uint16_t* out_lo, float* lse, void* workspace, size_t ws_bytes, void* stream);
+                           int first, float scale, uint16_t* out, float* lse, void* workspace, size_t ws_bytes,
+                           void* stream);
 size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first,
                                           int ranges);
 size_t af3_sink_attention_bwd_workspace_bytes(int B, int Hq, int Hkv, int Sq);
 int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* dout,
                            const int64_t* strides, const void* sinks, int sinks_f32, const int32_t* starts,
                            const int32_t* kv_range, int B, int Hq, int Hkv, int Sq, int Sk, int D, int window,
-                           int first, float scale, const uint16_t* out, const uint16_t* out_lo, const float* lse,
+                           int first, float scale, const uint16_t* out, const float* lse,
                            uint16_t* dq, uint16_t* dk, uint16_t* dv, void* dsinks, void* workspace, size_t ws_bytes, void* stream);
 
 /* starts [n_tokens] of a packed row: from cumulative lengths cu_seqlens

@@ -111,7 +111,7 @@ def test_c_entries_refuse_bad_arguments():
     def fwd(strides=ok, starts=None, kv=None, B=1, Hq=2, Hkv=1, Sq=4, Sk=4, D=64, window=0, first=0, scale=0.1, q=64,
             cu=None, out=64, ws=None, n=0):
         _capi.call("af3_sink_attention_fwd", q, 64, 64, strides, None, 0, cu, 1 if cu else 0, starts, kv, B, Hq, Hkv,
-                   Sq, Sk, D, window, first, scale, out, None, None, ws, n, None)
+                   Sq, Sk, D, window, first, scale, out, None, ws, n, None)
     for match, kw in (("share", dict(Hq=3, Hkv=2)), ("more than", dict(Hq=256)), ("dimension", dict(D=80)),
                       ("negative", dict(window=-1)), ("scale", dict(scale=0.0)), ("scale", dict(scale=float("nan"))),
                       ("length", dict(Sq=1 << 29)), ("multiples", dict(strides=st(*[64] * 8, 7))),
@@ -191,7 +191,7 @@ def test_c_entries_refuse_what_a_launch_or_32_bits_cannot_hold():
                                     ("scale", 1, 4, 4, 3e38)):
         with pytest.raises(RuntimeError, match=match):
             _capi.call("af3_sink_attention_fwd", 64, 64, 64, strides, None, 0, None, 0, None, None, B, 8, 8, Sq, Sk, 64,
-                       0, 0, scale, 64, None, None, None, 0, None)
+                       0, 0, scale, 64, None, None, 0, None)
         with pytest.raises(RuntimeError, match=match):
             _capi.call("af3_sink_attention_bwd", 64, 64, 64, 64, strides, None, 0, None, None, B, 8, 8, Sq, Sk, 64, 0, 0,
-                       scale, 64, 64, 64, 64, 64, 64, None, 64, 0, None)
+                       scale, 64, 64, 64, 64, 64, None, 64, 0, None)
