@@ -198,6 +198,12 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
     products, out = sum_j e^z_j v_j / (e^sink + sum_j e^z_j); a row that sees
     nothing gives 0, and zero gradients.
 
+    Probabilities and their gradients are rounded to bf16 once, as operands of the
+    next product; every sum is fp32 and in a fixed order.  What stands outside a
+    row's ``kv_range`` has no influence; a NaN or infinity inside it can reach rows
+    of the same tile (128 rows, 64 keys) that do not see it, as 0 times NaN does in
+    any masked product.
+
     Args:
         q: [B, Hq, Sq, D] bf16, D 64 or 128; any strides (head vectors contiguous
             and 16-byte aligned are read in place, others copied)

@@ -266,7 +266,7 @@ __device__ __forceinline__ Keys a_keys(const SaParams& p, int pos0, int pos1, in
 //
 // Bound by the vector unit, not the matrix unit: an exponential issues over 16
 // cycles, so 32 keys of 32 rows cost 256 cycles of them next to 256 of the two
-// products; the counters give 84% of the cycles to the vector unit and 46% to
+// products; the counters give 87% of the cycles to the vector unit and 48% to
 // the matrix unit.  8192 packed rows of 2144 keys on average, 64 heads over 8,
 // D 64: 342 us (840 TFLOP/s); a window of 128: 54 us; 2 x 4096 rows: 319 us (862
 // TFLOP/s).  Where a wave's rows are few the tiles are read at memory speed: one
@@ -571,8 +571,8 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
 //
 // Four products per step on the matrix unit; the second accumulator takes the
 // registers of a third block per CU.  8192 packed rows, 64 heads over 8, D 64:
-// 548 us (of 2144 keys on average; 4 products: 1050 TFLOP/s counting all of them),
-// 102 us with a window of 128, where half is a block's start: q, dout and out rows
+// 548 us (of 2144 keys on average; 4 products: 1050 TFLOP/s), matrix unit busy 56%,
+// vector unit 54%; 102 us with a window of 128, where half is a block's start: q, dout and out rows
 // and the first tiles, 5 us for each of the two blocks a CU holds.
 // ---------------------------------------------------------------------------
 template <int D>
@@ -820,9 +820,9 @@ __device__ __forceinline__ void a_dsink(const SaParams& p, int h, float* sh) {
 // own first half, held in that order, so that the matrix unit works beside them.
 //
 // Two passes over the scores (this and dq's) instead of one with atomic sums of
-// dq: seven products become nine, but every sum has a fixed order and no fp32
+// dq: five products become seven, but every sum has a fixed order and no fp32
 // copy of dq is written and read.  8192 packed rows, 64 heads over 8, D 64: 681 us
-// (of 2144 keys on average; 5 products: 1055 TFLOP/s), matrix unit busy 45%, the
+// (of 2144 keys on average; 4 products: 845 TFLOP/s), matrix unit busy 50%, the
 // rest LDS reads and the exponentials that do not fit beside products; 82 us with
 // a window of 128, where a block's start and its partly visible steps count.
 // ---------------------------------------------------------------------------
