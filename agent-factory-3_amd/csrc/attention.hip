@@ -632,7 +632,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p)
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta = fmaf((float)df[s][i], (float)of[s][i], delta);
+    // (a row that sees nothing has no gradient, whatever its dout holds)
     delta = a_sum_halves(delta);
+    delta = vis.w < vis.end || vis.fn > 0 ? delta : 0.f;
     a_landed(qf);
     a_landed(df);
   }
@@ -877,7 +879,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   int tb = p.Sq, s_last = lo;                // s_last: the latest start among their sequences
   if (p.starts) s_last = p.starts[jl];
   // (the last key's sequence may have first tokens in the block; an earlier one ends in it)
-  if (p.window > 0 && (p.first == 0 || s_last + p.first <= j0)) tb = min(tb, jl + p.window - off);
+  if (p.window > 0 && (p.first == 0 || s_last + p.first <= j0)) tb = min(tb, min(jl, hi - 1) + p.window - off);
   if (p.starts) tb = a_sequence_end(p.starts, s_last, jl, tb, lane);
   tb = jl < lo || j0 >= hi ? ta : max(ta, min(tb, p.Sq));
   const int64_t n_rows = (int64_t)(tb - ta) * p.G;

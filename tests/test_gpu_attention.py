@@ -423,3 +423,23 @@ def test_the_largest_sinks(dev):
         # (the bits of a row go with its tile, whose rows move their running maximum together: the oracle's bounds)
         none = oa.attention(q[:, 1:2], k[:, :1], v[:, :1], window=30, bounds=True)
         _close(out[:, :, 1:2], none["out"], none["out_tol"], "out")
+
+
+@pytest.mark.parametrize("window", [0, 20])
+def test_gradients_of_rows_that_see_nothing_have_no_influence(dev, window):
+    """Rows before a left-padded batch row's first key, and those whose window lies behind a
+    right-padded one's last key, with garbage in their gradients."""
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 2, 8, 2, 150, 150, 64)
+    rng = torch.tensor([[70, 150], [0, 61]], dtype=torch.int32, device=dev)
+    none = 61 + window - 1 if window else 150
+    res = []
+    for bad in (0.0, math.nan, math.inf):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, s)]
+        d = do.clone()
+        d[0, :70] = bad
+        d[1, none:] = bad
+        res.append(torch.autograd.grad(sink_attention(*leaves, window=window, kv_range=rng), leaves, d))
+        assert not res[-1][0][0, :, :70].any() and not res[-1][0][1, :, none:].any()
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, res[0]))
