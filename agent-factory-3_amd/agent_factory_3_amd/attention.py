@@ -161,6 +161,8 @@ def _cu(cu_seqlens: torch.Tensor) -> torch.Tensor:
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
         raise ValueError(f"cu_seqlens must be a [sequences + 1] integer tensor, got {tuple(cu_seqlens.shape)} "
                          f"{cu_seqlens.dtype}")
+    if not cu_seqlens.is_cuda:
+        raise RuntimeError("cu_seqlens must be a GPU tensor (the MI355X path has no CPU implementation)")
     if cu_seqlens.dtype != torch.int32:
         cu_seqlens = cu_seqlens.clamp(-1, MAX_LEN).to(torch.int32)
     return cu_seqlens.contiguous()
@@ -179,6 +181,8 @@ def sequence_starts(cu_seqlens: torch.Tensor, n_tokens: int) -> torch.Tensor:
 def sequence_starts_of_positions(position_ids: torch.Tensor) -> torch.Tensor:
     """The same from a packed row's position ids [n_tokens] (a sequence starts where
     a position is not its predecessor's plus one, as transformers reads them)."""
+    if not position_ids.is_cuda:
+        raise RuntimeError("position_ids must be a GPU tensor (the MI355X path has no CPU implementation)")
     pos = position_ids.reshape(-1).to(torch.int64).contiguous()
     starts = torch.empty(pos.numel(), dtype=torch.int32, device=pos.device)
     with _device_of(pos):

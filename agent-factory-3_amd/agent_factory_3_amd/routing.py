@@ -390,7 +390,10 @@ def balance_loss(logits: torch.Tensor, n_expts_act: int, expt_indx: torch.Tensor
         if expt_indx is not None:
             if tuple(expt_indx.shape) not in (lead + (K,), (T, K)):
                 raise ValueError(f"balance_loss: expt_indx is {tuple(expt_indx.shape)}, expected {lead + (K,)}")
-            expt_indx = expt_indx.to(device=lg.device, dtype=torch.int32).contiguous()
+            expt_indx = expt_indx.to(lg.device)
+            if expt_indx.dtype == torch.int64:   # (ids past 32 bits stay outside)
+                expt_indx = expt_indx.clamp(-1, E)
+            expt_indx = expt_indx.to(torch.int32).contiguous()
         if token_mask is not None:
             if tuple(token_mask.shape) not in (lead, (T,)):
                 raise ValueError(f"balance_loss: token_mask is {tuple(token_mask.shape)}, expected {lead}")

@@ -195,3 +195,12 @@ def test_c_entries_refuse_what_a_launch_or_32_bits_cannot_hold():
         with pytest.raises(RuntimeError, match=match):
             _capi.call("af3_sink_attention_bwd", 64, 64, 64, 64, strides, None, 0, None, None, B, 8, 8, Sq, Sk, 64, 0, 0,
                        scale, 64, 64, 64, 64, 64, None, 64, 0, None)
+
+
+def test_sequence_starts_refuse_host_tensors():
+    with pytest.raises(RuntimeError, match="GPU"):
+        attention.sequence_starts(torch.tensor([0, 4]), 4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        attention.sequence_starts_of_positions(torch.arange(4))
+    with pytest.raises(ValueError):
+        attention.sequence_starts(torch.tensor([0.0, 4.0]), 4)

@@ -200,3 +200,10 @@ def test_losses_read_without_gradients_first(dev):
     (d,) = torch.autograd.grad(loss, z)
     (want,) = torch.autograd.grad(routing.balance_loss(z, 4)[0], z)
     assert torch.equal(d, want)
+
+
+def test_ids_past_32_bits_count_for_no_expert(dev):
+    z, g = _logits(200, 32, 0, dev)
+    ids = torch.stack([torch.randperm(32, generator=g)[:4] for _ in range(200)])
+    ids[::3, 0], ids[1::3, 1], ids[2::3, 2] = 2 ** 32 + 5, -2 ** 40 + 7, 2 ** 31 + 1
+    _check(z, 4, ids.to(dev))
