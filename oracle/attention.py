@@ -4,17 +4,21 @@
 learned sink logits, packed rows or key ranges); with ``dout`` also its
 gradients.  ``bounds=True`` adds how far an implementation may be off that takes
 its operands in bf16, sums in fp32, and rounds to bf16 four things: p (as an
-operand), dz (as an operand), the output (from which it takes delta) and the
-results.  A rounding to bf16 is off by at most u = 2^-8 of the value.  With
+operand), dz (as an operand), the output and the results.  A first delta0 = do .
+out gives dz0 = p (g - delta0), g = do . v; the fp32 sums of dz0 and of p k then
+give delta = delta0 (1 - p_sink) + sum dz0 and dq = scale (sum dz0 k - (delta -
+delta0) sum p k).  A rounding to bf16 is off by at most u = 2^-8 of the value.  With
 e_z the error of z (fp32 sum of D products, relative to the sum of magnitudes,
 and the scaling before the exponential) p has the relative error r = e_z + 2^-21:
 
     |out|     u |out| + (u + r) p |v|
-    |delta|   |do| . |out error|                      (+ its own fp32 sum)
-    |dz|      (u + r) |dz| + p |delta error| + r p (|do| |v| + |delta|)
+    |delta0|  d0 = |do| . |out error|                 (+ its own fp32 sum)
+    |delta|   d1 = r sum p (|do| |v| + |delta| + d0)  (p_sink among the p, + the fp32 sums)
+    |dz|      (u + r) |dz| + p d1 + r p (|do| |v| + |delta|)
     |dv|      u |dv| + (u + r) p^T |do|
-    |dq|      u |dq| + scale (dz error) |k|,    |dk| alike with |q|
-    |dsink|   sum p_sink (|delta error| + r |delta|) (+ u |dsink| in bf16)
+    |dk|      u |dk| + scale (dz error)^T |q|
+    |dq|      u |dq| + scale ((u + r) (|dz| + 2 p d0) + p d1 + r p (|do| |v| + |delta| + d0)) |k|  (+ fp32 sums)
+    |dsink|   sum p_sink (d1 + r |delta|) (+ u |dsink| in bf16)
 """
 from __future__ import annotations
 
@@ -117,12 +121,18 @@ def attention(q, k, v, sinks=None, *, scale=None, window=0, first=0, cu_seqlens=
             if not bounds:
                 continue
             d_tol = (do.abs() * o_tol).sum(1, keepdim=True) + 2 * math.sqrt(D) * U32 * (do * o).abs().sum(1, keepdim=True)
-            z_tol = (U + r) * dz.abs() + p * d_tol + (r + 2 * math.sqrt(D) * U32) * p * (do.abs() @ vh.abs().T + delta.abs())
+            g_mag = do.abs() @ vh.abs().T + delta.abs()
+            rd, n32 = r + 2 * math.sqrt(D) * U32, 2 * math.sqrt(max(Sk, 1)) * U32
+            d1 = (rd * p * (g_mag + d_tol) + n32 * (dz.abs() + p * d_tol)).sum(1, keepdim=True) + 8 * U32 * (delta.abs() + d_tol)
+            if sinks is not None:
+                d1 = d1 + (r.amax(1, keepdim=True) if Sk else 2.0 ** -21) * ps * (delta.abs() + d_tol)
+            z_tol = (U + r) * dz.abs() + p * d1 + rd * p * g_mag
+            q_tol = (U + r + n32) * (dz.abs() + 2 * p * d_tol) + p * d1 + rd * p * (g_mag + d_tol)
             res["dv_tol"][b, h // G] += 1.01 * ((U + r) * p).T @ do.abs()
-            res["dq_tol"][b, h] = 1.01 * c * (z_tol @ kh.abs()) + 1e-30
+            res["dq_tol"][b, h] = 1.01 * c * (q_tol @ kh.abs()) + 1e-30
             res["dk_tol"][b, h // G] += 1.01 * c * (z_tol.T @ qh.abs())
             if sinks is not None:
-                res["dsinks_tol"][h] += 1.01 * (ps * (d_tol + (r.max() if Sk else 2.0 ** -21) * delta.abs())).sum() + \
+                res["dsinks_tol"][h] += 1.01 * (ps * (d1 + (r.max() if Sk else 2.0 ** -21) * delta.abs())).sum() + \
                     2 * math.sqrt(B * Sq) * U32 * (ps * delta.abs()).sum() + 1e-30
     if bounds and dout is not None:
         for n in ("dq", "dk", "dv"):
