@@ -204,8 +204,8 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
 
     Probabilities and their gradients are rounded to bf16 once, as operands of the
     next product; every sum is fp32 and in a fixed order.  What stands outside a
-    row's ``kv_range`` has no influence; a NaN or infinity inside it can reach rows
-    of the same tile (128 rows, 64 keys) that do not see it, as 0 times NaN does in
+    row's ``kv_range``, or in a packed row's tokens of no sequence, has no influence;
+    a NaN or infinity inside can reach rows of the same tile (128 rows, 64 keys) that do not see it, as 0 times NaN does in
     any masked product.
 
     Args:

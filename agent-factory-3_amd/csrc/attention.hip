@@ -211,6 +211,21 @@ __device__ __forceinline__ Vis a_vis(const SaParams& p, int pos, int lo, int hi)
   return v;
 }
 
+// The first and the last of tokens t0 .. t1 that lie in a sequence (k0 > k1 where none
+// does): of a packed row, tokens before the first sequence or past the last have
+// starts[t] = t + 1.  Their keys and rows are left out of every product, whatever they
+// hold, as those outside a key range are; only a tile at an end of the row looks.
+__device__ __forceinline__ void a_live(const int32_t* starts, int t0, int t1, int lane, int& k0, int& k1) {
+  k0 = t1 + 1;
+  k1 = t0 - 1;
+  for (int t = t0; t <= t1; t += 64) {
+    const uint64_t in = __ballot(t + lane <= t1 && starts[t + lane] <= t + lane);
+    if (in == 0) continue;
+    if (k0 > t1) k0 = t + __builtin_ctzll(in);
+    k1 = t + 63 - __builtin_clzll(in);
+  }
+}
+
 // scores of keys at or past `end` / before `from` to `to`; register r of s[c] is
 // key j + 32 c + 8 (r / 4) + r % 4
 template <int N>
@@ -333,9 +348,13 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
   const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;  // tokens of the tile
   int lo, hi;
   a_kv_range(p, b, lo, hi);
-  const int tile_lo = p.starts ? p.starts[t0] : lo;
+  int k0 = t0, k1 = t1, tile_lo = p.starts ? p.starts[t0] : lo;
   const int last_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start (the latest)
-  const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
+  if (p.starts && (tile_lo > t0 || last_lo > t1)) {
+    a_live(p.starts, t0, t1, lane, k0, k1);
+    tile_lo = k0 <= k1 ? p.starts[k0] : k0;
+  }
+  const Keys ks = a_keys(p, k0 + off, k1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
   int i0 = 0, i1 = na + nb;
   if (p.n_split > 1) {
@@ -591,9 +610,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p)
   const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;
   int lo, hi;
   a_kv_range(p, b, lo, hi);
-  const int tile_lo = p.starts ? p.starts[t0] : lo;
-  const int last_lo = p.starts ? p.starts[t1] : lo;
-  const Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
+  int k0 = t0, k1 = t1, tile_lo = p.starts ? p.starts[t0] : lo;
+  const int last_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start (the latest)
+  if (p.starts && (tile_lo > t0 || last_lo > t1)) {
+    a_live(p.starts, t0, t1, lane, k0, k1);
+    tile_lo = k0 <= k1 ? p.starts[k0] : k0;
+  }
+  const Keys ks = a_keys(p, k0 + off, k1 + off, tile_lo, hi);
   const int na = max(0, (ks.a1 - ks.a0 + kBN - 1) / kBN), nb = max(0, (ks.b1 - ks.b0 + kBN - 1) / kBN);
   const KvCopy<D> kc(p.k + b * p.k_sb + hk * p.k_sh, p.k_st, wave, lane);
   const KvCopy<D> vc(p.v + b * p.v_sb + hk * p.v_sh, p.v_st, wave, lane);
@@ -875,12 +898,20 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   const bool kvalid = j <= jl;
 
   // tokens that may see a key of the block
-  const int ta = max(0, max(j0, lo) - off);  // [ta, tb)
-  int tb = p.Sq, s_last = lo;                // s_last: the latest start among their sequences
-  if (p.starts) s_last = p.starts[jl];
+  int tb = p.Sq, s_last = lo;  // [ta, tb); s_last: the latest start among their sequences
+  int j_last = jl;
+  if (p.starts) {
+    s_last = p.starts[jl];
+    if (s_last > jl || p.starts[j0] > j0) {  // keys in no sequence
+      a_live(p.starts, j0, jl, lane, lo, j_last);
+      hi = j_last + 1;
+      s_last = lo <= j_last ? p.starts[j_last] : lo;
+    }
+  }
+  const int ta = max(0, max(j0, lo) - off);
   // (the last key's sequence may have first tokens in the block; an earlier one ends in it)
   if (p.window > 0 && (p.first == 0 || s_last + p.first <= j0)) tb = min(tb, min(jl, hi - 1) + p.window - off);
-  if (p.starts) tb = a_sequence_end(p.starts, s_last, jl, tb, lane);
+  if (p.starts) tb = a_sequence_end(p.starts, s_last, j_last, tb, lane);
   tb = jl < lo || j0 >= hi ? ta : max(ta, min(tb, p.Sq));
   const int64_t n_rows = (int64_t)(tb - ta) * p.G;
   const int n_steps = (int)((n_rows + kRT - 1) / kRT);

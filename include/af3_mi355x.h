@@ -456,7 +456,8 @@ int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_
  *   given; 0: none needed).
  *   backward: dq [B][Sq][Hq][D], dk and dv [B][Sk][Hkv][D], dsinks [Hq] in the
  *   sinks' type, from the forward's out and lse; every sum is in a fixed order.
- * A key outside every row's range is never read into a product; NaN or infinity
+ * A key outside every row's range, and a token of a packed row in no sequence
+ * (starts[t] = t + 1, at the row's ends), is never read into a product; NaN or infinity
  * in a key, value or gradient row that some row of the same 128-row or 64-key
  * tile sees may reach that tile's other rows.
  * Lengths below 2^29 tokens. */

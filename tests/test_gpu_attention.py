@@ -443,3 +443,35 @@ def test_gradients_of_rows_that_see_nothing_have_no_influence(dev, window):
         assert not res[-1][0][0, :, :70].any() and not res[-1][0][1, :, none:].any()
     for r in res[1:]:
         assert all(torch.equal(a, b) for a, b in zip(r, res[0]))
+
+
+@pytest.mark.parametrize("cu", [[0, 190], [5, 200], [70, 75, 130], [3, 3, 64, 128], [64, 192], [199, 200], [0, 1], [200, 200]])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 1), (4, 4), (96, 2)])
+@pytest.mark.parametrize("window,first", [(0, 0), (20, 0), (20, 9)])
+def test_tokens_in_no_sequence_have_no_influence(dev, cu, Hq, Hkv, window, first):
+    """Garbage in q, k, v and dout before a packed row's first sequence and behind its last: the same bits."""
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 1, Hq, Hkv, 200, 200, 64)
+    dead = torch.ones(200, dtype=torch.bool, device=dev)
+    dead[cu[0]:cu[-1]] = False
+    c = torch.tensor(cu, dtype=torch.int32, device=dev)
+    res = []
+    for bad in (0.0, math.nan, math.inf):
+        t = [x.clone() for x in (q, k, v)]
+        for x in t:
+            x[:, :, dead] = bad
+        d = do.clone()
+        d[:, dead] = bad
+        leaves = [x.requires_grad_() for x in (*t, s.detach().clone())]
+        out = sink_attention(*leaves, window=window, first=first, cu_seqlens=c)
+        res.append([out.detach(), *torch.autograd.grad(out, leaves, d)])
+        assert not out[:, dead].any() and not any(g[:, :, dead].any() for g in res[-1][1:4])
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, res[0]))
+    assert all(torch.isfinite(t).all() for t in res[0])
+
+
+def test_tokens_in_no_sequence_d128(dev):
+    for cu, window, first in (([37, 100, 171], 0, 0), ([37, 100, 171], 50, 3)):
+        _check(dev, 1, 6, 2, 200, 200, 128, cu_seqlens=cu, window=window, first=first)
+        test_tokens_in_no_sequence_have_no_influence(dev, cu, 6, 2, window, first)
