@@ -77,6 +77,7 @@ _SIGNATURES = {
                                 _p, _p, _i32, _i32, _p, _sz, _p, _p, _p]),
     "af3_seq_starts": (_i32, [_p, _i32, _i32, _p, _p]),
     "af3_seq_starts_positions": (_i32, [_p, _i32, _p, _p]),
+    "af3_seq_starts_rows": (_i32, [_p, _i64, _i32, _i32, _p, _p, _p]),
     "af3_sink_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "af3_sink_attention_fwd": (_i32, [_p, _p, _p, _p, _p, _i32, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                       _i32, _f32, _p, _p, _p, _sz, _p]),

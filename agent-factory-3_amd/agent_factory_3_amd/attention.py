@@ -69,7 +69,7 @@ def _forward(q, k, v, strides, sinks, scale, window, first, cu_seqlens, starts, 
     ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
     _capi.call("af3_sink_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _c_strides(strides),
                _capi.ptr(sinks), int(sinks is not None and sinks.dtype == torch.float32), _capi.ptr(cu_seqlens),
-               cu_seqlens.numel() - 1 if cu_seqlens is not None else 0, _capi.ptr(starts), _capi.ptr(kv_range), B, Hq,
+               B if cu_seqlens is None else cu_seqlens.numel() - 1, _capi.ptr(starts), _capi.ptr(kv_range), B, Hq,
                Hkv, Sq, Sk, D, window, first, scale, out.data_ptr(), _capi.ptr(lse), _capi.ptr(ws), ws_n,
                _capi.stream_of(dev))
     return out
@@ -191,6 +191,37 @@ def sequence_starts_of_positions(position_ids: torch.Tensor) -> torch.Tensor:
     return starts
 
 
+def sequence_starts_of_rows(position_ids: torch.Tensor, kv_range: torch.Tensor | None = None) -> torch.Tensor:
+    """The same of a batch of packed rows: [B, S] int32, each counted in its own row, from
+    position ids [B, S].  ``kv_range`` [B, 2] (begin, end) where the rows are padded: a
+    sequence starts at begin too, and a token outside lies in no sequence."""
+    if not position_ids.is_cuda:
+        raise RuntimeError("position_ids must be a GPU tensor (the MI355X path has no CPU implementation)")
+    if position_ids.dim() != 2 or position_ids.is_floating_point():
+        raise ValueError(f"position_ids must be a [rows, tokens] integer tensor, got {tuple(position_ids.shape)} "
+                         f"{position_ids.dtype}")
+    B, S = position_ids.shape
+    if kv_range is not None:
+        kv_range = _ranges(kv_range, B, S, position_ids.device)
+    with _device_of(position_ids):
+        pos = position_ids.to(torch.int64).contiguous()
+        starts = torch.empty((B, S), dtype=torch.int32, device=pos.device)
+        _capi.call("af3_seq_starts_rows", pos.data_ptr(), S, B, S, _capi.ptr(kv_range), starts.data_ptr(),
+                   _capi.stream_of(pos.device))
+    return starts
+
+
+def _ranges(kv_range, B, Sk, device):
+    if kv_range.device != device:
+        raise ValueError(f"kv_range is on {kv_range.device}, the rows on {device}")
+    if kv_range.shape != (B, 2) or kv_range.is_floating_point():
+        raise ValueError(f"kv_range must be a [{B}, 2] integer tensor, got {tuple(kv_range.shape)} {kv_range.dtype}")
+    with _device_of(kv_range):
+        if kv_range.dtype != torch.int32:
+            kv_range = kv_range.clamp(0, Sk).to(torch.int32)
+        return kv_range.contiguous()
+
+
 def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: torch.Tensor | None = None, *,
                    scale: float | None = None, window: int = 0, first: int = 0,
                    cu_seqlens: torch.Tensor | None = None, kv_range: torch.Tensor | None = None) -> torch.Tensor:
@@ -244,12 +275,7 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
             cu_seqlens = _cu(cu_seqlens)
             starts = torch.empty(Sk, dtype=torch.int32, device=q.device)
         if kv_range is not None:
-            if kv_range.shape != (B, 2) or kv_range.is_floating_point():
-                raise ValueError(f"sink_attention: kv_range must be a [{B}, 2] integer tensor, got "
-                                 f"{tuple(kv_range.shape)} {kv_range.dtype}")
-            if kv_range.dtype != torch.int32:
-                kv_range = kv_range.clamp(0, Sk).to(torch.int32)
-            kv_range = kv_range.contiguous()
+            kv_range = _ranges(kv_range, B, Sk, q.device)
         return _run(q, k, v, sinks, scale, window, first, cu_seqlens, starts, kv_range)
 
 
@@ -260,17 +286,60 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
 ATTN_IMPLEMENTATION = "af3_sink"
 
 
+@functools.lru_cache(maxsize=1)
+def _mask_codes():
+    """Code objects of what transformers builds its mask functions from: joined by and,
+    sliding window and causal order (honoured by the attention itself), packing, chunks."""
+    from transformers import masking_utils as mu
+    both = mu.sliding_window_causal_mask_function(1)
+    return (both.__code__, {f.__code__ for f in _cells(both)["mask_functions"]},
+            mu.packed_sequence_mask_function(None).__code__,
+            {f.__code__ for f in _cells(mu.chunked_causal_mask_function(1, None))["mask_functions"]})
+
+
+def _cells(f) -> dict:
+    return dict(zip(f.__code__.co_freevars, (c.cell_contents for c in f.__closure__ or ())))
+
+
+def _packing(f, kv_end: int):
+    """The sequence numbers [rows, S] that a mask function keeps apart, or None.  What the
+    attention cannot honour is refused."""
+    joined, own, packed, chunks = _mask_codes()
+    code = getattr(f, "__code__", None)
+    if code is joined:
+        parts = [p for p in (_packing(x, kv_end) for x in _cells(f)["mask_functions"]) if p is not None]
+        if len(parts) < 2:
+            return parts[0] if parts else None
+    elif code is packed:
+        return _cells(f)["packed_sequence_mask"]
+    elif code in own or (code in chunks and kv_end <= _cells(f)["chunk_size"]):
+        return None
+    raise NotImplementedError(f"af3_sink: the mask function {getattr(f, '__qualname__', f)} is not supported (causal "
+                              "order, a sliding window and packed sequences are)")
+
+
 def attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None,
                    use_vmap=False, **kwargs):
     """What transformers hands every layer as its mask (causal order and window are
-    the attention's own): None, or [B, 2] int32 key ranges of a batch padded on
-    either side.  Reads the padding mask once per forward (a host synchronisation,
-    as its flash forms do)."""
+    the attention's own): None; [B, 2] int32 key ranges of a batch padded on either
+    side; or [B, S, 1] int32, where transformers found packed sequences (position ids
+    that start again, which most of its models look for where neither padding nor a
+    cache is given): the start of each token's own.  Other mask functions are refused.
+    Reads the padding mask once per call (a host synchronisation, as its flash forms
+    do)."""
     if use_vmap:
         raise NotImplementedError("af3_sink: custom mask functions are not supported")
     if isinstance(q_offset, torch.Tensor) or kv_offset + kv_length != q_offset + q_length:
         raise NotImplementedError("af3_sink: the last key must be the last query's (a cache that grows, "
                                   "not one of fixed length)")
+    seq = _packing(mask_function, kv_offset + kv_length) if mask_function is not None else None
+    if seq is not None:
+        if attention_mask is not None or q_length != kv_length or seq.shape[-1] != kv_length:
+            raise NotImplementedError("af3_sink: packed sequences with a padding mask or a cache are not supported")
+        at = torch.arange(kv_length, device=seq.device).expand(batch_size, kv_length)
+        new = torch.ones_like(at, dtype=torch.bool)
+        new[:, 1:] = seq[:, 1:] != seq[:, :-1]
+        return torch.where(new, at, 0).cummax(1).values.to(torch.int32)[..., None]
     if attention_mask is None:
         return None
     m = attention_mask[:, kv_offset:kv_offset + kv_length].to(torch.int32)
@@ -291,16 +360,22 @@ def attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mas
 def attention_forward(module, query, key, value, attention_mask, scaling=None, dropout=0.0, sliding_window=None,
                       s_aux=None, **kwargs):
     """transformers' attention interface over ``sink_attention``: query [B, Hq, Sq, D]
-    -> ([B, Sq, Hq, D], None).  A packed row (B = 1) is read from ``cu_seq_lens_q``
-    or, like its flash forms, from position ids that start again."""
+    -> ([B, Sq, Hq, D], None).  A packed row (B = 1) is read from ``cu_seq_lens_q``;
+    one or a batch of them from position ids [B, S] that start again, or from what
+    ``attention_mask`` made of the packing that transformers found."""
     if dropout:
         raise NotImplementedError("af3_sink: attention dropout is not supported")
     causal = kwargs.get("is_causal")
     if not (getattr(module, "is_causal", True) if causal is None else causal):
         raise NotImplementedError("af3_sink: only causal attention is supported")
-    if attention_mask is not None and attention_mask.shape != (query.shape[0], 2):
-        raise ValueError("af3_sink: the mask must be the one that its own mask function makes (or None), got "
-                         f"{tuple(attention_mask.shape)}")
+    B, S, Sk = query.shape[0], query.shape[2], key.shape[2]
+    starts = None
+    if attention_mask is not None:
+        if S == Sk and attention_mask.shape == (B, S, 1):
+            starts, attention_mask = attention_mask[..., 0], None
+        elif attention_mask.shape != (B, 2):
+            raise ValueError("af3_sink: the mask must be the one that its own mask function makes (or None), got "
+                             f"{tuple(attention_mask.shape)}")
     if s_aux is not None and s_aux.dtype not in (torch.bfloat16, torch.float32):
         s_aux = s_aux.float()
     args = dict(scale=scaling, window=sliding_window or 0, kv_range=attention_mask)
@@ -310,13 +385,14 @@ def attention_forward(module, query, key, value, attention_mask, scaling=None, d
         if cu_k is not None and cu_k is not cu and cu_k.shape != cu.shape:
             raise ValueError("af3_sink: cu_seq_lens_q and cu_seq_lens_k differ")
         return sink_attention(query, key, value, s_aux, cu_seqlens=cu, **args), None
-    if (pos is not None and attention_mask is None and query.shape[0] == 1 and query.shape[2] == key.shape[2] > 1
-            and pos.numel() == query.shape[2]):
-        starts = sequence_starts_of_positions(pos.to(query.device))
+    if starts is None and pos is not None and attention_mask is None and S == Sk > 1 and pos.numel() == B * S:
+        starts = sequence_starts_of_rows(pos.to(query.device, torch.int64).reshape(B, S))
+    if starts is not None:
         scale = query.shape[-1] ** -0.5 if scaling is None else scaling
         _check(query, key, value, s_aux, scale, args["window"], 0)
         with _device_of(query):
-            return _run(query, key, value, s_aux, scale, min(args["window"], MAX_LEN), 0, None, starts, None), None
+            return _run(query, key, value, s_aux, scale, min(args["window"], MAX_LEN), 0, None,
+                        starts.to(query.device).contiguous(), None), None
     return sink_attention(query, key, value, s_aux, **args), None
 
 

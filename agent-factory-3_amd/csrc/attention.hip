@@ -47,7 +47,7 @@ struct SaParams {
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
   const void* sinks;                      // [Hq] or NULL
   int sinks_f32;
-  const int32_t* starts;                  // [Sk] start of each token's sequence (packed row), or NULL
+  const int32_t* starts;                  // [B][Sk] start of each token's sequence (packed rows), or NULL
   const int32_t* kv_range;                // [B][2] or NULL
   int B, Hq, Hkv, G, Sq, Sk, window, first;
   int g_mul;                              // x / G = x g_mul >> 16 for x < 256
@@ -194,6 +194,11 @@ __device__ __forceinline__ void a_kv_range(const SaParams& p, int b, int& lo, in
     lo = min(max(p.kv_range[2 * b], 0), p.Sk);
     hi = min(max(p.kv_range[2 * b + 1], lo), p.Sk);
   }
+}
+
+// the sequence starts of a batch row's tokens, or NULL
+__device__ __forceinline__ const int32_t* a_starts(const SaParams& p, int b) {
+  return p.starts ? p.starts + (int64_t)b * p.Sk : nullptr;
 }
 
 // What a row sees: keys [w, end) (the window, or all) and the fn keys from lo
@@ -348,8 +353,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
   const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;  // tokens of the tile
   int lo, hi;
   a_kv_range(p, b, lo, hi);
-  const int tile_lo = p.starts ? p.starts[t0] : lo;
-  const int last_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start (the latest)
+  const int32_t* starts = a_starts(p, b);
+  const int tile_lo = starts ? starts[t0] : lo;
+  const int last_lo = starts ? starts[t1] : lo;  // the last sequence's start (the latest)
   Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   int na, nb, i0, i1;  // tiles of first tokens, of the rest, and the block's own
   auto tiles = [&]() {
@@ -376,10 +382,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
   if (i0 + 1 < i1) load(i0 + 1, 1, 1);
   // Tokens in no sequence: the copies again, without them.  (Looked for before the
   // first copies, they cost a window's forward 3%: 56.0 us instead of 54.3.)
-  if (__builtin_expect(p.starts && (tile_lo > t0 || last_lo > t1), 0)) {
+  if (__builtin_expect(starts && (tile_lo > t0 || last_lo > t1), 0)) {
     int k0, k1;
-    a_live(p.starts, t0, t1, lane, k0, k1);
-    ks = a_keys(p, k0 + off, k1 + off, k0 <= k1 ? p.starts[k0] : k0, hi);
+    a_live(starts, t0, t1, lane, k0, k1);
+    ks = a_keys(p, k0 + off, k1 + off, k0 <= k1 ? starts[k0] : k0, hi);
     tiles();
     A_WAIT_VM(0);
     if (i0 < i1) load(i0, 0, 0);
@@ -391,7 +397,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void sa_fwd_kernel(SaParams p
   const bool valid = t0 + tk <= t1;
   const int t = valid ? t0 + tk : t0;
   const int head = hk * p.G + (valid ? g : 0);
-  const Vis vis = a_vis(p, t + off, p.starts ? p.starts[t] : lo, hi);
+  const Vis vis = a_vis(p, t + off, starts ? starts[t] : lo, hi);
   af3_bf16x8 qf[KS];
   {
     const uint16_t* qr = p.q + b * p.q_sb + head * p.q_sh + t * p.q_st;
@@ -621,8 +627,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p)
   const int t0 = tile * p.tok, t1 = min(t0 + p.tok, p.Sq) - 1;
   int lo, hi;
   a_kv_range(p, b, lo, hi);
-  const int tile_lo = p.starts ? p.starts[t0] : lo;
-  const int last_lo = p.starts ? p.starts[t1] : lo;  // the last sequence's start (the latest)
+  const int32_t* starts = a_starts(p, b);
+  const int tile_lo = starts ? starts[t0] : lo;
+  const int last_lo = starts ? starts[t1] : lo;  // the last sequence's start (the latest)
   Keys ks = a_keys(p, t0 + off, t1 + off, tile_lo, hi);
   int na, nb;
   auto tiles = [&]() {
@@ -640,10 +647,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p)
     vc(j0, last, st + kTile, wave);
   };
   if (na + nb > 0) issue(0, 0);  // (under way while the rows are read)
-  if (__builtin_expect(p.starts && (tile_lo > t0 || last_lo > t1), 0)) {  // as in the forward
+  if (__builtin_expect(starts && (tile_lo > t0 || last_lo > t1), 0)) {  // as in the forward
     int k0, k1;
-    a_live(p.starts, t0, t1, lane, k0, k1);
-    ks = a_keys(p, k0 + off, k1 + off, k0 <= k1 ? p.starts[k0] : k0, hi);
+    a_live(starts, t0, t1, lane, k0, k1);
+    ks = a_keys(p, k0 + off, k1 + off, k0 <= k1 ? starts[k0] : k0, hi);
     tiles();
     A_WAIT_VM(0);
     if (na + nb > 0) issue(0, 0);
@@ -655,7 +662,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p)
   const int t = valid ? t0 + tk : t0;
   const int head = hk * p.G + (valid ? g : 0);
   const int64_t prow = (((int64_t)b * p.Hkv + hk) * p.Sq + t) * p.G + (valid ? g : 0);
-  const Vis vis = a_vis(p, t + off, p.starts ? p.starts[t] : lo, hi);
+  const Vis vis = a_vis(p, t + off, starts ? starts[t] : lo, hi);
   float lse = p.lse[prow];
   af3_bf16x8 qf[KS], df[KS];
   float delta = 0.f;
@@ -911,6 +918,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   const int off = p.Sk - p.Sq;
   int lo, hi;
   a_kv_range(p, b, lo, hi);
+  const int32_t* starts = a_starts(p, b);
   const int jl = min(j0 + kKeys, p.Sk) - 1;  // last key of the block
   const int jw = j0 + (wave & 1) * 32;       // first key of the wave
   const int j = jw + lr;
@@ -919,18 +927,19 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   // tokens that may see a key of the block
   int tb = p.Sq, s_last = lo;  // [ta, tb); s_last: the latest start among their sequences
   int j_last = jl;
-  if (p.starts) {
-    s_last = p.starts[jl];
-    if (__builtin_expect(s_last > jl || p.starts[j0] > j0, 0)) {  // keys in no sequence
-      a_live(p.starts, j0, jl, lane, lo, j_last);
+  if (starts) {
+    const int s_first = starts[j0];
+    s_last = starts[jl];
+    if (__builtin_expect((s_last > jl) | (s_first > j0), 0)) {  // keys in no sequence
+      a_live(starts, j0, jl, lane, lo, j_last);
       hi = j_last + 1;
-      s_last = lo <= j_last ? p.starts[j_last] : lo;
+      s_last = lo <= j_last ? starts[j_last] : lo;
     }
   }
   const int ta = max(0, max(j0, lo) - off);
   // (the last key's sequence may have first tokens in the block; an earlier one ends in it)
   if (p.window > 0 && (p.first == 0 || s_last + p.first <= j0)) tb = min(tb, min(jl, hi - 1) + p.window - off);
-  if (p.starts) tb = a_sequence_end(p.starts, s_last, j_last, tb, lane);
+  if (starts) tb = a_sequence_end(starts, s_last, j_last, tb, lane);
   tb = jl < lo || j0 >= hi ? ta : max(ta, min(tb, p.Sq));
   const int64_t n_rows = (int64_t)(tb - ta) * p.G;
   const int n_steps = (int)((n_rows + kRT - 1) / kRT);
@@ -938,7 +947,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
   // hold rows of earlier ones, which ask each row for its own start.  The steps
   // before them (they run from the last back) are s_last's alone: keys before it
   // gather anything there, and start again from zero at step mixed - 1.
-  const int mixed = p.starts && s_last > j0 ? ((min(s_last, tb) - ta) * p.G + kRT - 1) / kRT : 0;
+  const int mixed = starts && s_last > j0 ? ((min(s_last, tb) - ta) * p.G + kRT - 1) / kRT : 0;
 
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(a_lds_addr(lds));
   const uint32_t rowv0 = __builtin_amdgcn_readfirstlane(a_lds_addr(rowv));
@@ -986,7 +995,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dkv_kernel(SaParams p
         a_dma16(db + t * p.do_st + g * p.do_sh + col, st + kTile + x * 1024);
       }
       const void* src = rp + (ns == n_steps - 1 ? min(lane, back) : lane);
-      if (wave == 2 && ns < mixed) src = p.starts + min(nt + ((ng + lane) * p.g_mul >> 16), tb - 1);
+      if (wave == 2 && ns < mixed) src = starts + min(nt + ((ng + lane) * p.g_mul >> 16), tb - 1);
       a_dma4(src, rv);
     }
     if (ns > 0) {
@@ -1249,13 +1258,23 @@ __global__ __launch_bounds__(256) void sa_starts_kernel(const int32_t* __restric
   starts[t] = a > 0 && t < cu[a] ? max(cu[a - 1], 0) : t + 1;
 }
 
-// one block: a sequence starts where a position is not its predecessor's plus one
-__global__ __launch_bounds__(1024) void sa_starts_pos_kernel(const int64_t* __restrict__ pos, int T,
+// One block per batch row: a sequence starts where a position is not its
+// predecessor's plus one, and at the first token of the row's range; tokens outside
+// the range get t + 1, as those in no sequence above.
+__global__ __launch_bounds__(1024) void sa_starts_pos_kernel(const int64_t* __restrict__ pos, int64_t ld, int T,
+                                                             const int32_t* __restrict__ range,
                                                              int32_t* __restrict__ starts) {
   __shared__ int sh[2][1024];
+  pos += blockIdx.x * ld;
+  starts += (int64_t)blockIdx.x * T;
+  int lo = 0, hi = T;
+  if (range) {
+    lo = min(max(range[2 * blockIdx.x], 0), T);
+    hi = min(max(range[2 * blockIdx.x + 1], lo), T);
+  }
   const int n = (T + 1023) / 1024;
   const int t0 = min((int)threadIdx.x * n, T), t1 = min(t0 + n, T);
-  int last = -1;  // the last start in this thread's range
+  int last = -1;  // the last start in this thread's tokens
   for (int t = t0; t < t1; ++t)
     if (t == 0 || pos[t] != pos[t - 1] + 1) last = t;
   sh[0][threadIdx.x] = last;
@@ -1270,7 +1289,7 @@ __global__ __launch_bounds__(1024) void sa_starts_pos_kernel(const int64_t* __re
   int s = threadIdx.x > 0 ? max(sh[cur][threadIdx.x - 1], 0) : 0;
   for (int t = t0; t < t1; ++t) {
     if (t == 0 || pos[t] != pos[t - 1] + 1) s = t;
-    starts[t] = s;
+    starts[t] = t >= lo && t < hi ? max(s, lo) : t + 1;
   }
 }
 
@@ -1315,7 +1334,7 @@ SaShape sa_shape(int B, int Hq, int Hkv, int Sq, int Sk, int window, int first, 
 }
 
 int sa_check(const char* who, int B, int Hq, int Hkv, int Sq, int Sk, int D, int window, int first, float scale,
-             const int64_t* strides, int n_strides, const int32_t* starts, const int32_t* kv_range) {
+             const int64_t* strides, int n_strides, const int32_t* starts, int n_starts, const int32_t* kv_range) {
   AF3_REQUIRE(B >= 0 && Sq >= 0 && Sk >= 0 && Sq < kMaxLen && Sk < kMaxLen, "%s: bad batch or length", who);
   AF3_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "%s: %d query heads do not share %d key/value heads", who, Hq, Hkv);
   AF3_REQUIRE(Hq / Hkv <= kRows, "%s: more than %d query heads per key/value head", who, kRows);
@@ -1329,7 +1348,8 @@ int sa_check(const char* who, int B, int Hq, int Hkv, int Sq, int Sk, int D, int
     AF3_REQUIRE((i % 3 != 2 && i != 1 && i != 10) || (strides[i] >= 0 && strides[i] < kMaxStride),
                 "%s: token strides, and head strides of q and dout, must be below %d", who, kMaxStride);
   }
-  AF3_REQUIRE(!starts || (B <= 1 && Sq == Sk && !kv_range), "%s: a packed row has batch 1, Sq == Sk and no kv_range", who);
+  AF3_REQUIRE(!starts || ((B <= 1 || B == n_starts) && Sq == Sk && !kv_range),
+              "%s: packed rows have starts of their own, Sq == Sk and no kv_range", who);
   // (a launch holds less than 2^32 threads; row numbers of dk / dv stay in 32 bits)
   const int64_t tiles = af3_cdiv(Sq, kRows / (Hq / Hkv)), key_blocks = af3_cdiv(Sk, kKeys);
   AF3_REQUIRE((int64_t)B * Hkv * (Sq + Sk + 1) < 0x7fffffffLL &&
@@ -1370,12 +1390,20 @@ extern "C" int af3_seq_starts(const int32_t* cu_seqlens, int n_seqs, int n_token
   return af3::check_launch("seq_starts");
 }
 
+extern "C" int af3_seq_starts_rows(const int64_t* position_ids, int64_t ld, int n_rows, int n_tokens,
+                                   const int32_t* kv_range, int32_t* starts, void* stream_) {
+  AF3_REQUIRE(n_rows >= 0 && n_rows < (1 << 22) && n_tokens >= 0 && n_tokens < kMaxLen && (ld == 0 || ld >= n_tokens),
+              "seq_starts_rows: bad sizes");
+  if (n_rows == 0 || n_tokens == 0) return 0;
+  AF3_REQUIRE(position_ids && starts, "seq_starts_rows: null pointer");
+  hipLaunchKernelGGL(sa_starts_pos_kernel, dim3(n_rows), dim3(1024), 0, (hipStream_t)stream_, position_ids, ld,
+                     n_tokens, kv_range, starts);
+  return af3::check_launch("seq_starts_rows");
+}
+
 extern "C" int af3_seq_starts_positions(const int64_t* position_ids, int n_tokens, int32_t* starts, void* stream_) {
   AF3_REQUIRE(n_tokens >= 0 && n_tokens < kMaxLen, "seq_starts_positions: bad size");
-  if (n_tokens == 0) return 0;
-  AF3_REQUIRE(position_ids && starts, "seq_starts_positions: null pointer");
-  hipLaunchKernelGGL(sa_starts_pos_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream_, position_ids, n_tokens, starts);
-  return af3::check_launch("seq_starts_positions");
+  return af3_seq_starts_rows(position_ids, n_tokens, 1, n_tokens, nullptr, starts, stream_);
 }
 
 extern "C" size_t af3_sink_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int window,
@@ -1391,7 +1419,9 @@ extern "C" int af3_sink_attention_fwd(const uint16_t* q, const uint16_t* k, cons
                                       int D, int window, int first, float scale, uint16_t* out, float* lse, void* workspace,
                                       size_t ws_bytes, void* stream_) {
   const char* who = "sink_attention_fwd";
-  if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 9, starts, kv_range)) return rc;
+  if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 9, starts,
+                        cu_seqlens || n_seqs < 1 ? 1 : n_seqs, kv_range))
+    return rc;
   if (B == 0 || Sq == 0) return 0;
   AF3_REQUIRE(q && out && (Sk == 0 || (k && v)), "%s: null pointer", who);
   AF3_REQUIRE(sa_al16(q) && sa_al16(k) && sa_al16(v) && sa_al16(out),
@@ -1439,7 +1469,8 @@ extern "C" int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, cons
                                       uint16_t* dq, uint16_t* dk, uint16_t* dv, void* dsinks, void* workspace,
                                       size_t ws_bytes, void* stream_) {
   const char* who = "sink_attention_bwd";
-  if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 12, starts, kv_range)) return rc;
+  if (int rc = sa_check(who, B, Hq, Hkv, Sq, Sk, D, window, first, scale, strides, 12, starts, B, kv_range))
+    return rc;
   const bool nq = B > 0 && Sq > 0, nk = B > 0 && Sk > 0;
   AF3_REQUIRE((!nq || (q && dout && out && lse && dq && workspace)) && (!nk || (k && v && dk && dv)) &&
                   (!sinks || dsinks),

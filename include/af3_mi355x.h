@@ -448,7 +448,9 @@ int af3_balance_loss_bwd(const uint16_t* logits, int64_t ld_logits, const uint8_
  * kv_range[b] = (begin, end) (device int32 [B][2], clamped to [0, Sk]; NULL: all
  * keys), or, for a packed row (B = 1, Sq = Sk), from starts[p] (device int32
  * [Sk], af3_seq_starts): the start of the token's own sequence; with cu_seqlens
- * the forward writes starts first (as af3_seq_starts), else it reads them.  sinks [Hq]
+ * the forward writes starts first (as af3_seq_starts), else it reads them.  A batch
+ * of packed rows (B > 1) has starts [B][Sk] of its own, each counted in its row
+ * (af3_seq_starts_rows), no cu_seqlens, and n_seqs = B in the forward.  sinks [Hq]
  * (bf16, or fp32 with sinks_f32; NULL: none) adds e^sink to the softmax's
  * denominator.  A row that sees nothing gives 0.
  *   forward: out [B][Sq][Hq][D]; lse [B][Hkv][Sq][Hq/Hkv] fp32 (log2 units), for
@@ -478,9 +480,15 @@ int af3_sink_attention_bwd(const uint16_t* q, const uint16_t* k, const uint16_t*
 /* starts [n_tokens] of a packed row: from cumulative lengths cu_seqlens
  * [n_seqs + 1] (device int32; tokens before the first or past the last sequence
  * get t + 1 and see nothing), or from position ids (device int64): a sequence
- * starts where a position is not its predecessor's plus one. */
+ * starts where a position is not its predecessor's plus one.  Of a batch of
+ * packed rows: starts [n_rows][n_tokens] from position ids [n_rows][ld] (ld 0: one
+ * row of ids for all) and, where the rows are padded, kv_range (device int32
+ * [n_rows][2]: begin, end; NULL: none; clamped to the row): a sequence starts at
+ * begin too, and tokens outside get t + 1. */
 int af3_seq_starts(const int32_t* cu_seqlens, int n_seqs, int n_tokens, int32_t* starts, void* stream);
 int af3_seq_starts_positions(const int64_t* position_ids, int n_tokens, int32_t* starts, void* stream);
+int af3_seq_starts_rows(const int64_t* position_ids, int64_t ld, int n_rows, int n_tokens, const int32_t* kv_range,
+                        int32_t* starts, void* stream);
 
 #ifdef __cplusplus
 }

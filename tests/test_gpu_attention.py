@@ -475,3 +475,40 @@ def test_tokens_in_no_sequence_d128(dev):
     for cu, window, first in (([37, 100, 171], 0, 0), ([37, 100, 171], 50, 3)):
         _check(dev, 1, 6, 2, 200, 200, 128, cu_seqlens=cu, window=window, first=first)
         test_tokens_in_no_sequence_have_no_influence(dev, cu, 6, 2, window, first)
+
+
+@pytest.mark.parametrize("G,D", [(1, 64), (8, 64), (3, 128)])
+@pytest.mark.parametrize("window,first", [(0, 0), (20, 0), (20, 3)])
+def test_a_batch_of_packed_rows(dev, G, D, window, first):
+    """Starts of each batch row's own, forward and backward: every row as by itself, with the same bits."""
+    from agent_factory_3_amd import attention
+    S, cuts = 300, [[0, 70, 71, 300], [0, 150, 300], [0, 300], [0, 64, 128, 299, 300]]
+    q, k, v, s, do = _make(dev, 4, 2 * G, 2, S, S, D)
+    pos = torch.stack([torch.cat([torch.arange(b - a) for a, b in zip(c, c[1:])]) for c in cuts]).to(dev)
+    starts = attention.sequence_starts_of_rows(pos)
+    assert torch.equal(starts.cpu(), torch.stack([oa.starts_of(c, S) for c in cuts]).to(torch.int32))
+    assert torch.equal(attention.sequence_starts_of_rows(pos[:1]), attention.sequence_starts_of_positions(pos[0])[None])
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, s)]
+    out = attention._run(*leaves, D ** -0.5, window, first, None, starts, None)
+    grads = torch.autograd.grad(out, leaves, do)
+    if not first:
+        import types
+        for mask, ids in ((None, pos), (starts[..., None], None)):   # the layers' call, by either
+            one, _ = attention.attention_forward(types.SimpleNamespace(is_causal=True), q, k, v, mask, position_ids=ids,
+                                                 sliding_window=window, s_aux=s)
+            assert torch.equal(one, out)
+    dsinks = torch.zeros(2 * G, dtype=torch.float64)
+    tol = torch.zeros(2 * G, dtype=torch.float64)
+    for b, c in enumerate(cuts):
+        one = [t[b:b + 1].detach().requires_grad_() for t in (q, k, v)]
+        cu = torch.tensor(c, dtype=torch.int32, device=dev)
+        o = attention.sink_attention(*one, s, window=window, first=first, cu_seqlens=cu)
+        assert torch.equal(o, out[b:b + 1])
+        for g, w in zip(torch.autograd.grad(o, one, do[b:b + 1]), grads):
+            assert torch.equal(g, w[b:b + 1])
+        ref = oa.attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], s, window=window, first=first, cu_seqlens=c,
+                           dout=do[b:b + 1], bounds=True)
+        dsinks += ref["dsinks"]
+        tol += ref["dsinks_tol"]
+    # (each row's bound holds a rounding of its own sum to bf16, together no less than the whole's one)
+    _close(grads[3], dsinks, tol, "dsinks")

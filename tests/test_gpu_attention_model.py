@@ -201,3 +201,23 @@ def test_rejects_what_it_cannot_do(dev):
     mask[0, 4] = 0
     with pytest.raises(ValueError, match="one run"):
         model(input_ids=_ids(1, 10).to(dev), attention_mask=mask)
+
+
+def test_a_batch_of_packed_rows_in_the_model(dev):
+    """Rows of a batch that hold several sequences each (by their position ids): every sequence as by itself,
+    also with the cache that a forward makes by default."""
+    routing_replay.enable_routing_replay()
+    lens = [[13, 1, 40], [30, 20, 4]]
+    ids, ri = _ids(2, 54).to(dev), _replay(2, 54).to(dev)
+    pos = torch.stack([torch.cat([torch.arange(n) for n in row]) for row in lens]).to(dev)
+    model = _model(dev, "af3_sink")
+    with torch.no_grad():
+        got = model(input_ids=ids, position_ids=pos, routing_indices=ri, use_cache=False).last_hidden_state
+        assert torch.equal(got, model(input_ids=ids, position_ids=pos, routing_indices=ri).last_hidden_state)
+        for b, row in enumerate(lens):
+            at = 0
+            for n in row:
+                one = model(input_ids=ids[b:b + 1, at:at + n], routing_indices=ri[b:b + 1, at:at + n],
+                            use_cache=False).last_hidden_state
+                assert _rel(got[b:b + 1, at:at + n], one) < 2e-2   # (as for one packed row)
+                at += n
