@@ -361,8 +361,8 @@ def attention_forward(module, query, key, value, attention_mask, scaling=None, d
                       s_aux=None, **kwargs):
     """transformers' attention interface over ``sink_attention``: query [B, Hq, Sq, D]
     -> ([B, Sq, Hq, D], None).  A packed row (B = 1) is read from ``cu_seq_lens_q``;
-    one or a batch of them from position ids [B, S] that start again, or from what
-    ``attention_mask`` made of the packing that transformers found."""
+    one or a batch of them, padded or not, from position ids [B, S] that start again,
+    or from what ``attention_mask`` made of the packing that transformers found."""
     if dropout:
         raise NotImplementedError("af3_sink: attention dropout is not supported")
     causal = kwargs.get("is_causal")
@@ -385,8 +385,8 @@ def attention_forward(module, query, key, value, attention_mask, scaling=None, d
         if cu_k is not None and cu_k is not cu and cu_k.shape != cu.shape:
             raise ValueError("af3_sink: cu_seq_lens_q and cu_seq_lens_k differ")
         return sink_attention(query, key, value, s_aux, cu_seqlens=cu, **args), None
-    if starts is None and pos is not None and attention_mask is None and S == Sk > 1 and pos.numel() == B * S:
-        starts = sequence_starts_of_rows(pos.to(query.device, torch.int64).reshape(B, S))
+    if starts is None and pos is not None and S == Sk > 1 and pos.numel() == B * S:
+        starts = sequence_starts_of_rows(pos.to(query.device, torch.int64).reshape(B, S), attention_mask)
     if starts is not None:
         scale = query.shape[-1] ** -0.5 if scaling is None else scaling
         _check(query, key, value, s_aux, scale, args["window"], 0)

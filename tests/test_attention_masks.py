@@ -40,10 +40,10 @@ def test_layers_read_a_batch_of_packed_rows_from_its_position_ids(monkeypatch):
     """gpt-oss gives its mask functions no position ids: its layers read them, of every row."""
     seen, asked = _stand_in(monkeypatch), []
     monkeypatch.setattr(attention, "sequence_starts_of_rows",
-                        lambda pos, *a: asked.append((pos.tolist(), *a)) or torch.tensor(STARTS, dtype=torch.int32))
+                        lambda pos, rng=None: asked.append((pos.tolist(), rng)) or torch.tensor(STARTS, dtype=torch.int32))
     with torch.no_grad():
         _model()(input_ids=torch.randint(0, 128, (2, 6)), position_ids=torch.tensor(POS))
-    assert asked == [(POS,)] * 2 and [s[1] for s in seen] == [8, 0]
+    assert asked == [(POS, None)] * 2 and [s[1] for s in seen] == [8, 0]
     assert all(s[0] == (2, 2, 6, 64) and s[2].tolist() == STARTS for s in seen)
 
 

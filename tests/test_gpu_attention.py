@@ -512,3 +512,53 @@ def test_a_batch_of_packed_rows(dev, G, D, window, first):
         tol += ref["dsinks_tol"]
     # (each row's bound holds a rounding of its own sum to bf16, together no less than the whole's one)
     _close(grads[3], dsinks, tol, "dsinks")
+
+
+def _by_positions(q, k, v, s, pos, kv_range=None, window=0):
+    """The layers' call: transformers' interface with position ids."""
+    import types
+
+    from agent_factory_3_amd import attention
+    out, _ = attention.attention_forward(types.SimpleNamespace(is_causal=True), q, k, v, kv_range, position_ids=pos,
+                                         sliding_window=window, s_aux=s)
+    return out
+
+
+@pytest.mark.parametrize("pad", [(0, 30), (30, 0), (7, 1), (64, 64), (0, 0)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_padded_packed_row_keeps_its_sequences(dev, pad, window):
+    """One row of sequences by position ids, with padding before or behind: each sequence sees itself alone."""
+    lens = [50, 1, 40, 61]
+    n, S = sum(lens), sum(lens) + sum(pad)
+    q, k, v, s, do = _make(dev, 1, 8, 2, S, S, 64)
+    pos = torch.cat([torch.ones(pad[0], dtype=torch.int64)] + [torch.arange(x) for x in lens] +
+                    [torch.zeros(pad[1], dtype=torch.int64)])[None].to(dev)
+    rng = torch.tensor([[pad[0], pad[0] + n]], dtype=torch.int32, device=dev)
+    cu = [pad[0] + x for x in (0, 50, 51, 91, 152)]
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, s)]
+    out = _by_positions(*leaves, pos, rng, window)
+    ref = oa.attention(q, k, v, s, window=window, cu_seqlens=cu, dout=do, bounds=True)
+    _close(out, ref["out"], ref["out_tol"], "out")
+    for name, g in zip(("dq", "dk", "dv", "dsinks"), torch.autograd.grad(out, leaves, do)):
+        _close(g, ref[name], ref[name + "_tol"], name)
+
+
+def test_starts_of_rows_within_ranges(dev):
+    from agent_factory_3_amd.attention import sequence_starts_of_rows
+    pos = torch.tensor([[1, 1, 0, 1, 2, 0, 1, 0, 0], [0, 1, 2, 3, 4, 5, 0, 1, 0]], device=dev)
+    for dtype in (torch.int32, torch.int64):
+        rng = torch.tensor([[2, 7], [0, 8]], dtype=dtype, device=dev)
+        assert sequence_starts_of_rows(pos, rng).tolist() == [[1, 2, 2, 2, 2, 5, 5, 8, 9], [0] * 6 + [6, 6, 9]]
+    # a range inside a sequence starts it there; outside the row it is clamped
+    t = torch.arange(2000)
+    ends = [(-5, 3000), (700, 1500), (5, 5), (1500, 700), (2000, 2000)]
+    got = sequence_starts_of_rows(t.to(dev).expand(5, -1), torch.tensor(ends, device=dev)).cpu()
+    for row, (a, b) in zip(got, ends):
+        assert torch.equal(row, torch.where((t >= a) & (t < b), max(a, 0), t + 1).to(torch.int32))
+    for bad in (torch.zeros(3, 2, dtype=torch.int32, device=dev), torch.zeros(2, 2, device=dev),
+                torch.zeros(2, 2, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            sequence_starts_of_rows(pos, bad)
+    for bad, exc in ((pos[0], ValueError), (pos.float(), ValueError), (pos.cpu(), RuntimeError)):
+        with pytest.raises(exc):
+            sequence_starts_of_rows(bad)

@@ -221,3 +221,30 @@ def test_a_batch_of_packed_rows_in_the_model(dev):
                             use_cache=False).last_hidden_state
                 assert _rel(got[b:b + 1, at:at + n], one) < 2e-2   # (as for one packed row)
                 at += n
+
+
+@pytest.mark.parametrize("side", ["left", "right"])
+def test_padded_rows_of_sequences(dev, side):
+    """A packed row beside a padded one in a batch, and a padded packed row alone: each sequence as by itself."""
+    routing_replay.enable_routing_replay()
+    lens, S = [[13, 1, 40], [30, 7]], 54
+    ids, ri = _ids(2, S).to(dev), _replay(2, S).to(dev)
+    pos, mask, at0 = torch.zeros(2, S, dtype=torch.long), torch.zeros(2, S, dtype=torch.long), []
+    for b, row in enumerate(lens):
+        n = sum(row)
+        a = S - n if side == "left" else 0
+        pos[b, a:a + n], mask[b, a:a + n] = torch.cat([torch.arange(x) for x in row]), 1
+        at0.append(a)
+    pos, mask = pos.to(dev), mask.to(dev)
+    model = _model(dev, "af3_sink")
+    with torch.no_grad():
+        both = model(input_ids=ids, attention_mask=mask, position_ids=pos, routing_indices=ri).last_hidden_state
+        alone = model(input_ids=ids[1:], attention_mask=mask[1:], position_ids=pos[1:], routing_indices=ri[1:]).last_hidden_state
+        for b, row in enumerate(lens):
+            at = at0[b]
+            for n in row:
+                one = model(input_ids=ids[b:b + 1, at:at + n], routing_indices=ri[b:b + 1, at:at + n],
+                            use_cache=False).last_hidden_state
+                for got in (both[b:b + 1], alone) if b else (both[b:b + 1],):
+                    assert _rel(got[:, at:at + n], one) < 2e-2   # (as for one packed row)
+                at += n
