@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import _capi
-from .routing import _device_of
+from .routing import _device_of, _no_forward_mode
 
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 128       # query heads per key/value head
@@ -88,6 +88,7 @@ class _SinkAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _no_forward_mode("sink_attention backward", dout)
         q, k, v, sinks, starts, kv_range, out, lse = ctx.saved_tensors
         scale, window, first = ctx.args
         B, Hq, Sq, D = q.shape
@@ -115,6 +116,7 @@ class _SinkAttention(torch.autograd.Function):
 
 
 def _check(q, k, v, sinks, scale, window, first):
+    _no_forward_mode("sink_attention", q, k, v, sinks)
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
             raise RuntimeError(f"sink_attention: {name} must be a GPU tensor (the MI355X path has no CPU implementation)")

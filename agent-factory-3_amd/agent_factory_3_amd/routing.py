@@ -24,6 +24,7 @@ import math
 from dataclasses import dataclass, field
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 
@@ -332,6 +333,7 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
+        _no_forward_mode("balance_loss backward", g)
         logits, token_mask, stats = ctx.saved_tensors
         T, E = logits.shape
         dev = logits.device
@@ -344,6 +346,14 @@ class _BalanceLoss(torch.autograd.Function):
                        _capi.ptr(token_mask), T, E, stats.data_ptr(), g.data_ptr(), d.data_ptr(),
                        _capi.stream_of(dev))
         return d, None, None, None
+
+
+def _no_forward_mode(who: str, *tensors):
+    """Refuse dual tensors: the kernels make no forward-mode derivatives, and a call
+    that records no graph would drop the tangents silently."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{who}: forward-mode derivatives are not supported")
 
 
 def _device_of(t: torch.Tensor):
@@ -372,6 +382,7 @@ def balance_loss(logits: torch.Tensor, n_expts_act: int, expt_indx: torch.Tensor
     Returns:
         (loss fp32 scalar, counts [E] int32); the loss is 0 when no token counts
     """
+    _no_forward_mode("balance_loss", logits)
     if not logits.is_cuda:
         raise RuntimeError("router logits must be a GPU tensor (the MI355X path has no CPU implementation)")
     if logits.dim() < 1 or not logits.is_floating_point():

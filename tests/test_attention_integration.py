@@ -204,3 +204,21 @@ def test_sequence_starts_refuse_host_tensors():
         attention.sequence_starts_of_positions(torch.arange(4))
     with pytest.raises(ValueError):
         attention.sequence_starts(torch.tensor([0.0, 4.0]), 4)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor's tangent must not be dropped silently (checked before anything else of the tensors)."""
+    import torch.autograd.forward_ad as fwd
+    q, z = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16), torch.zeros(4, 8)
+    with fwd.dual_level():
+        for i in range(3):
+            t = [q, q, q]
+            t[i] = fwd.make_dual(q, torch.ones_like(q))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                attention.sink_attention(*t)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            attention.sink_attention(q, q, q, fwd.make_dual(torch.zeros(2), torch.ones(2)))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            routing.balance_loss(fwd.make_dual(z, torch.ones_like(z)), 2)
+        with pytest.raises(RuntimeError, match="GPU"):   # no tangent: as outside
+            attention.sink_attention(q, q, q)

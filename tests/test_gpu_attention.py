@@ -562,3 +562,26 @@ def test_starts_of_rows_within_ranges(dev):
     for bad, exc in ((pos[0], ValueError), (pos.float(), ValueError), (pos.cpu(), RuntimeError)):
         with pytest.raises(exc):
             sequence_starts_of_rows(bad)
+
+
+def test_forward_mode_derivatives_are_refused(dev):
+    import torch.autograd.forward_ad as fwd
+
+    from agent_factory_3_amd import routing
+    from agent_factory_3_amd.attention import sink_attention
+    q, k, v, s, do = _make(dev, 1, 4, 2, 20, 20, 64)
+    z = torch.randn(20, 8, device=dev).to(torch.bfloat16)
+    kl, zl = k.detach().requires_grad_(), z.detach().requires_grad_()
+    with fwd.dual_level():
+        out, (loss, _) = sink_attention(q, kl, v, s), routing.balance_loss(zl, 2)
+        dual = lambda t: fwd.make_dual(t.detach(), torch.ones_like(t))  # noqa: E731
+        for keys in (k, kl):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                sink_attention(dual(q), keys, v, s)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            routing.balance_loss(dual(z), 2)
+        # a tangent of the gradient that arrives
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, kl, dual(do))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(loss, zl, dual(torch.ones((), device=dev)))
