@@ -21,6 +21,7 @@ import contextlib
 import ctypes
 import functools
 import math
+import threading
 from dataclasses import dataclass, field
 
 import torch
@@ -456,7 +457,21 @@ class BalanceCollector:
         return torch.stack([x[1] for x in self._results()])
 
 
-_COLLECTORS: list = []  # the innermost collect_balance gets the layers
+class _ThreadStack(threading.local):
+    """Each thread's open collectors (a forward in another thread, as one that scores
+    beside training, leaves its logits to its own)."""
+
+    def __init__(self):
+        self.open = []
+
+    def __bool__(self):
+        return bool(self.open)
+
+    def __getitem__(self, i):
+        return self.open[i]
+
+
+_COLLECTORS = _ThreadStack()  # the innermost collect_balance gets the layers
 
 
 @contextlib.contextmanager
@@ -468,16 +483,17 @@ def collect_balance(token_mask: torch.Tensor | None = None):
             out = model(input_ids, attention_mask=attention_mask)
         loss = policy_loss(out) + coef * balance.loss()
 
-    token_mask: [B, S] (or flat) tokens to count, None = all.  Activation
-    checkpointing works in its non-reentrant form (the reentrant one runs the
-    layers without gradients first, so its losses have none).
+    token_mask: [B, S] (or flat) tokens to count, None = all.  Layers that run in
+    another thread are not collected.  Activation checkpointing works in its
+    non-reentrant form (the reentrant one runs the layers without gradients first,
+    so its losses have none).
     """
     c = BalanceCollector(token_mask)
-    _COLLECTORS.append(c)
+    _COLLECTORS.open.append(c)
     try:
         yield c
     finally:
-        _COLLECTORS.remove(c)
+        _COLLECTORS.open.remove(c)
 
 
 def dense_routing(n_rows: int, device) -> RoutingData:

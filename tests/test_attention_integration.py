@@ -222,3 +222,39 @@ def test_forward_mode_derivatives_are_refused():
             routing.balance_loss(fwd.make_dual(z, torch.ones_like(z)), 2)
         with pytest.raises(RuntimeError, match="GPU"):   # no tangent: as outside
             attention.sink_attention(q, q, q)
+
+
+def test_another_threads_forward_is_not_collected():
+    """Scoring in another thread beside training leaves the collecting thread's logits alone."""
+    import threading
+    logits = {n: torch.full((3, 4), float(i)) for i, n in enumerate(("here", "there"))}
+    seen, other = [], threading.Barrier(2, timeout=20)
+
+    def scoring():
+        other.wait()
+        seen.append(bool(routing._COLLECTORS))
+        if routing._COLLECTORS:
+            routing._COLLECTORS[-1].add("layer", logits["there"], 2)
+        with routing.collect_balance() as mine:
+            routing._COLLECTORS[-1].add("layer", logits["there"], 2)
+            other.wait()
+            other.wait()
+        seen.append(mine)
+    t = threading.Thread(target=scoring)
+    t.start()
+    with routing.collect_balance() as b:
+        routing._COLLECTORS[-1].add("layer", logits["here"], 2)
+        other.wait()
+        other.wait()      # (the other thread's own collector is open)
+        assert routing._COLLECTORS[-1] is b
+        other.wait()
+        t.join(20)
+    assert not routing._COLLECTORS
+    assert seen[0] is False and b._seen["layer"][0] is logits["here"]
+    assert seen[1]._seen["layer"][0] is logits["there"]
+    # nested: the innermost gets the layers
+    with routing.collect_balance() as b:
+        with routing.collect_balance() as inner:
+            assert routing._COLLECTORS[-1] is inner
+        assert routing._COLLECTORS[-1] is b
+    assert not routing._COLLECTORS
