@@ -367,6 +367,8 @@ def attention_forward(module, query, key, value, attention_mask, scaling=None, d
     or from what ``attention_mask`` made of the packing that transformers found."""
     if dropout:
         raise NotImplementedError("af3_sink: attention dropout is not supported")
+    if kwargs.get("softcap") is not None:
+        raise NotImplementedError("af3_sink: capped scores (softcap) are not supported")
     causal = kwargs.get("is_causal")
     if not (getattr(module, "is_causal", True) if causal is None else causal):
         raise NotImplementedError("af3_sink: only causal attention is supported")

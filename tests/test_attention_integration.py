@@ -258,3 +258,13 @@ def test_another_threads_forward_is_not_collected():
             assert routing._COLLECTORS[-1] is inner
         assert routing._COLLECTORS[-1] is b
     assert not routing._COLLECTORS
+
+
+def test_score_capping_is_refused():
+    """Models with capped scores pass softcap: it must not be ignored."""
+    q = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16)
+    m = types.SimpleNamespace(is_causal=True)
+    with pytest.raises(NotImplementedError, match="softcap"):
+        attention.attention_forward(m, q, q, q, None, softcap=30.0)
+    with pytest.raises(RuntimeError, match="GPU"):
+        attention.attention_forward(m, q, q, q, None, softcap=None)
