@@ -166,7 +166,7 @@ def _cu(cu_seqlens: torch.Tensor) -> torch.Tensor:
     if not cu_seqlens.is_cuda:
         raise RuntimeError("cu_seqlens must be a GPU tensor (the MI355X path has no CPU implementation)")
     if cu_seqlens.dtype != torch.int32:
-        cu_seqlens = cu_seqlens.clamp(-1, MAX_LEN).to(torch.int32)
+        cu_seqlens = cu_seqlens.to(torch.int64).clamp(-1, MAX_LEN).to(torch.int32)
     return cu_seqlens.contiguous()
 
 
@@ -220,7 +220,7 @@ def _ranges(kv_range, B, Sk, device):
         raise ValueError(f"kv_range must be a [{B}, 2] integer tensor, got {tuple(kv_range.shape)} {kv_range.dtype}")
     with _device_of(kv_range):
         if kv_range.dtype != torch.int32:
-            kv_range = kv_range.clamp(0, Sk).to(torch.int32)
+            kv_range = kv_range.to(torch.int64).clamp(0, Sk).to(torch.int32)
         return kv_range.contiguous()
 
 

@@ -585,3 +585,13 @@ def test_forward_mode_derivatives_are_refused(dev):
             torch.autograd.grad(out, kl, dual(do))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(loss, zl, dual(torch.ones((), device=dev)))
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int64])
+def test_integer_types_of_lengths_and_ranges(dev, dtype):
+    from agent_factory_3_amd.attention import sequence_starts, sink_attention
+    q, k, v, s, _ = _make(dev, 1, 4, 2, 300, 300, 64)
+    cu, rng = torch.tensor([0, 20, 100], device=dev), torch.tensor([[10, 120]], device=dev)
+    for n, t in (("cu_seqlens", cu), ("kv_range", rng)):
+        assert torch.equal(sink_attention(q, k, v, s, **{n: t.to(dtype)}), sink_attention(q, k, v, s, **{n: t.int()}))
+    assert torch.equal(sequence_starts(cu.to(dtype), 300), sequence_starts(cu.int(), 300))
