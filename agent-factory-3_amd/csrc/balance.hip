@@ -101,7 +101,17 @@ __device__ __forceinline__ float b_exps(const uint32_t (&w)[4 * C], float (&e)[8
     e[i] = __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
     mx = fmaxf(mx, e[i]);
   }
-  mx = b_max<LPR>(mx) * kLog2e;
+  mx = b_max<LPR>(mx);
+  // The rounding of mx log2(e) is a factor common to the row, which its sum takes out
+  // again, while it is small: past 2^20 (experts all masked by the type's lowest value,
+  // say) the row's differences come first.  (Taken first for every row, they cost the
+  // sums of 128000 rows 4%: 13.0 us instead of 12.5.)
+  if (__builtin_expect(fabsf(mx) > 1048576.f, 0)) {
+#pragma unroll
+    for (int i = 0; i < 8 * C; ++i) e[i] -= mx;
+    mx = 0.f;
+  }
+  mx *= kLog2e;
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 8 * C; ++i) {

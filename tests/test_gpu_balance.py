@@ -207,3 +207,19 @@ def test_ids_past_32_bits_count_for_no_expert(dev):
     ids = torch.stack([torch.randperm(32, generator=g)[:4] for _ in range(200)])
     ids[::3, 0], ids[1::3, 1], ids[2::3, 2] = 2 ** 32 + 5, -2 ** 40 + 7, 2 ** 31 + 1
     _check(z, 4, ids.to(dev))
+
+
+@pytest.mark.parametrize("E", [8, 100, 128, 1024])
+def test_logits_at_the_types_limits(dev, E):
+    """Rows of the lowest value (every expert masked), of the largest, one expert's logit alone far above
+    or below: a softmax of differences, never NaN."""
+    big = float(torch.finfo(torch.bfloat16).max)
+    z, _ = _logits(600, E, 1, dev)
+    z[0], z[1], z[2, 1:], z[3, 1:], z[4, 0], z[5, 0] = -big, big, -big, big, -big, big
+    z[6, ::2], z[6, 1::2], z[7], z[7, 3] = big, -big, -big, -3e38
+    z[8], z[9], z[10] = 2.4e38, -2.4e38, 1e30
+    loss, _, d = _check(z, 2)
+    assert torch.isfinite(loss) and torch.isfinite(d).all()
+    mask = torch.ones(600, dtype=torch.bool, device=dev)
+    mask[:11] = False
+    _check(z, 2, None, mask)
