@@ -595,3 +595,24 @@ def test_integer_types_of_lengths_and_ranges(dev, dtype):
     for n, t in (("cu_seqlens", cu), ("kv_range", rng)):
         assert torch.equal(sink_attention(q, k, v, s, **{n: t.to(dtype)}), sink_attention(q, k, v, s, **{n: t.int()}))
     assert torch.equal(sequence_starts(cu.to(dtype), 300), sequence_starts(cu.int(), 300))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (6, 6, 128)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_position_ids_are_the_cumulative_lengths(dev, Hq, Hkv, D, window):
+    """transformers' interface with position ids that start again, forward and backward: the bits of
+    the call with cumulative lengths, and the oracle's bounds."""
+    from agent_factory_3_amd.attention import sink_attention
+    lens = [50, 1, 40, 61]
+    q, k, v, s, do = _make(dev, 1, Hq, Hkv, 152, 152, D)
+    pos = torch.cat([torch.arange(x) for x in lens])[None].to(dev)
+    cu = torch.tensor([0, 50, 51, 91, 152], dtype=torch.int32, device=dev)
+    res = []
+    for call in (lambda *t: _by_positions(*t, pos, None, window), lambda *t: sink_attention(*t, window=window, cu_seqlens=cu)):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, s)]
+        out = call(*leaves)
+        res.append([out.detach(), *torch.autograd.grad(out, leaves, do)])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+    ref = oa.attention(q, k, v, s, window=window, cu_seqlens=cu.tolist(), dout=do, bounds=True)
+    for name, t in zip(("out", "dq", "dk", "dv", "dsinks"), res[0]):
+        _close(t, ref[name], ref[name + "_tol"], name)

@@ -223,3 +223,16 @@ def test_logits_at_the_types_limits(dev, E):
     mask = torch.ones(600, dtype=torch.bool, device=dev)
     mask[:11] = False
     _check(z, 2, None, mask)
+
+
+@pytest.mark.parametrize("T,E,K,replay", [(128000, 128, 4, True), (70000, 1024, 3, False)])
+def test_many_rows_per_lane(dev, T, E, K, replay):
+    """The longest packed row with replayed choices, and 18 rows to a lane's sums."""
+    z, g = _logits(T, E, T, dev)
+    ids = mask = None
+    if replay:
+        ids = torch.stack([torch.randperm(E, generator=g)[:K] for _ in range(1000)]).repeat(T // 1000, 1).to(dev)
+        mask = (torch.rand(T, generator=g) < 0.9).to(dev)
+    # (the sums of _check's bound: 18 additions in a lane, 3 over lanes, 8 waves and 9 levels of the join are
+    # at most 38 roundings of 2^-24 of positive terms, random in sign; its 2^-19 is 32)
+    _check(z, K, ids, mask)
