@@ -616,3 +616,22 @@ def test_position_ids_are_the_cumulative_lengths(dev, Hq, Hkv, D, window):
     ref = oa.attention(q, k, v, s, window=window, cu_seqlens=cu.tolist(), dout=do, bounds=True)
     for name, t in zip(("out", "dq", "dk", "dv", "dsinks"), res[0]):
         _close(t, ref[name], ref[name + "_tol"], name)
+
+
+@pytest.mark.parametrize("S", [1, 4095, 4096, 4097, 12288, 40001])
+def test_starts_of_long_rows(dev, S):
+    """Sequences that cross many blocks' tokens, one that fills its row, and starts at the blocks' edges."""
+    from agent_factory_3_amd.attention import sequence_starts_of_positions, sequence_starts_of_rows
+    g = torch.Generator().manual_seed(S)
+    t = torch.arange(S)
+    rows = [torch.zeros(S, dtype=torch.bool), torch.rand(S, generator=g) < 1e-3, torch.rand(S, generator=g) < 0.5,
+            t % 4096 == 0, t % 4096 == 4095, t % 1024 == 1023, t % 64 == 63, t == 1, t == S - 1]
+    want = torch.stack([torch.where(r, t, 0).cummax(0).values for r in rows])
+    pos = (t - want + torch.randint(0, 1 << 40, (len(rows), 1), generator=g)).to(dev)
+    assert torch.equal(sequence_starts_of_rows(pos).cpu(), want.to(torch.int32))
+    for p, w in zip(pos, want):
+        assert torch.equal(sequence_starts_of_positions(p).cpu(), w.to(torch.int32))
+    a, b = S // 3, S - S // 4
+    rng = torch.tensor([[a, b]] * len(rows), device=dev)
+    inside = torch.where((t >= a) & (t < b), want.clamp(min=a), t + 1)
+    assert torch.equal(sequence_starts_of_rows(pos, rng).cpu(), inside.to(torch.int32))
