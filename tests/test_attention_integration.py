@@ -268,3 +268,24 @@ def test_score_capping_is_refused():
         attention.attention_forward(m, q, q, q, None, softcap=30.0)
     with pytest.raises(RuntimeError, match="GPU"):
         attention.attention_forward(m, q, q, q, None, softcap=None)
+
+
+def test_c_entries_of_starts_refuse_bad_arguments():
+    import ctypes
+
+    from agent_factory_3_amd import _capi
+    if not _capi.lib_path().exists():
+        pytest.skip("library not built")
+    for a in ((64, 8, -1, 8, None, 64, None), (64, 8, 1, -8, None, 64, None), (64, 7, 1, 8, None, 64, None),
+              (64, 1 << 29, 1, 1 << 29, None, 64, None), (64, 8, 1 << 22, 8, None, 64, None),
+              (64, 8192, 1 << 21, 8192, None, 64, None), (None, 8, 1, 8, None, 64, None), (64, 8, 1, 8, None, None, None)):
+        with pytest.raises(RuntimeError, match="seq_starts_rows"):
+            _capi.call("af3_seq_starts_rows", *a)
+    _capi.call("af3_seq_starts_rows", None, 0, 0, 8, None, None, None)   # nothing to do
+    _capi.call("af3_seq_starts_rows", None, 0, 8, 0, None, None, None)
+    # a batch of packed rows says how many rows of starts there are
+    st = (ctypes.c_int64 * 9)(*[64] * 9)
+    for n_seqs, cu in ((0, None), (1, None), (3, None), (2, 64)):
+        with pytest.raises(RuntimeError, match="packed"):
+            _capi.call("af3_sink_attention_fwd", 64, 64, 64, st, None, 0, cu, n_seqs, 64, None, 2, 2, 1, 4, 4, 64, 0, 0,
+                       0.1, 64, None, None, 0, None)

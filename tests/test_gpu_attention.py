@@ -635,3 +635,39 @@ def test_starts_of_long_rows(dev, S):
     rng = torch.tensor([[a, b]] * len(rows), device=dev)
     inside = torch.where((t >= a) & (t < b), want.clamp(min=a), t + 1)
     assert torch.equal(sequence_starts_of_rows(pos, rng).cpu(), inside.to(torch.int32))
+
+
+@pytest.mark.parametrize("window,first", [(0, 0), (600, 0), (600, 70)])
+def test_packed_rows_whose_keys_are_split(dev, window, first):
+    """Few enough tiles that each row's keys go over several blocks: sequences, tokens in none of them
+    at both ends (garbage there too), and a batch of such rows."""
+    from agent_factory_3_amd import attention
+    S, cuts = 1100, [[30, 700, 1050], [0, 1, 1100], [0, 1040]]
+    q, k, v, s, do = _make(dev, 3, 8, 1, S, S, 64)
+    dead = torch.ones(3, S, dtype=torch.bool, device=dev)
+    pos, rng = torch.zeros(3, S, dtype=torch.long), []
+    for b, c in enumerate(cuts):
+        dead[b, c[0]:c[-1]] = False
+        pos[b, c[0]:c[-1]] = torch.cat([torch.arange(y - x) for x, y in zip(c, c[1:])])
+        rng.append((c[0], c[-1]))
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        t.transpose(1, 2)[dead] = math.nan
+    do[dead] = math.inf
+    starts = attention.sequence_starts_of_rows(pos.to(dev), torch.tensor(rng, device=dev))
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention._run(*leaves, s, 0.125, window, first, None, starts, None)
+    grads = torch.autograd.grad(out, leaves, do)
+    for b, c in enumerate(cuts):
+        one = [t[b:b + 1].detach().requires_grad_() for t in (q, k, v)]
+        alone = attention.sink_attention(*one, s, window=window, first=first,
+                                         cu_seqlens=torch.tensor(c, dtype=torch.int32, device=dev))
+        alone_g = torch.autograd.grad(alone, one, do[b:b + 1])
+        live = [x.clone() for x in (q[b:b + 1], k[b:b + 1], v[b:b + 1], do[b:b + 1])]
+        for t in live[:3]:
+            t.transpose(1, 2)[dead[b:b + 1]] = 0
+        live[3][dead[b:b + 1]] = 0
+        ref = oa.attention(*live[:3], s, window=window, first=first, cu_seqlens=c, dout=live[3], bounds=True)
+        for o, g in ((out[b:b + 1], [x[b:b + 1] for x in grads]), (alone, alone_g)):
+            _close(o, ref["out"], ref["out_tol"], "out")
+            for name, x in zip(("dq", "dk", "dv"), g):
+                _close(x, ref[name], ref[name + "_tol"], name)
