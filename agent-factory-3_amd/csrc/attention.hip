@@ -282,14 +282,16 @@ __device__ __forceinline__ Keys a_keys(const SaParams& p, int pos0, int pos1, in
 // scores into its lane; the running maximum moves only when it grows by more
 // than 8 (log2 units: probabilities stay below 256), so most tiles need no
 // rescaling of the output.  Probabilities are rounded to bf16 for the product
-// with V, their sum is not: the output is 1.3 times one bf16 rounding off.
+// with V, their sum is not: the output is 1.3 times one bf16 rounding off.  Scores
+// are fp32: a probability is off by its score's rounding (2^-24 of it), and scores
+// past 2^29 overflow in the exponential.
 //
 // Bound by the vector unit, not the matrix unit: an exponential issues over 16
 // cycles, so 32 keys of 32 rows cost 256 cycles of them next to 256 of the two
 // products; the counters give 87% of the cycles to the vector unit and 48% to
 // the matrix unit.  8192 packed rows of 2144 keys on average, 64 heads over 8,
-// D 64: 342 us (840 TFLOP/s); a window of 128: 54 us; 2 x 4096 rows: 319 us (862
-// TFLOP/s).  Where a wave's rows are few the tiles are read at memory speed: one
+// D 64: 340 to 357 us by the card (845 to 805 TFLOP/s); a window of 128: 54 us; 2 x
+// 4096 rows: 315 to 337 us.  Where a wave's rows are few the tiles are read at memory speed: one
 // token over 131072 keys 43 us (6.2 TB/s), 32 tokens over 4099: 26.7 us (5.1).
 // A window's block runs three to four tiles, so its start (first copies, q rows)
 // is a third of it.  Stages as constants of six unrolled turns gain 3% on the
@@ -602,14 +604,17 @@ __global__ __launch_bounds__(256) void sa_join_kernel(SaParams p) {
 // give the true one at the end: sum dz = delta - delta0 sum p, sum p = 1 - p_sink,
 // and dq = scale (sum dz k - (delta - delta0) sum p k).  dk, dv and the sinks take
 // the true delta: dq 1.44, dk 1.41 times one rounding (of dz, and the result's),
-// dsinks none.  The bf16 remainder of out kept by the forward costs more (its
-// writing alone 15 us of 70 with a window of 128) and corrects less (dq 1.53).
+// dsinks none.  (Means over 400 heads: single calls of eight heads and two tokens
+// scatter between 1.1 and 1.9, since there one rounded dz scales a whole row.)  The
+// bf16 remainder of out kept by the forward costs more (its writing alone 15 us of
+// 70 with a window of 128) and corrects less (dq 1.53).
 //
 // Four products per step on the matrix unit; the second accumulator takes the
-// registers of a third block per CU.  8192 packed rows, 64 heads over 8, D 64:
-// 548 us (of 2144 keys on average; 4 products: 1050 TFLOP/s), matrix unit busy 56%,
-// vector unit 54%; 102 us with a window of 128, where half is a block's start: q, dout and out rows
-// and the first tiles, 5 us for each of the two blocks a CU holds.
+// registers of a third block per CU.  8192 packed rows, 64 heads over 8, D 64: 544
+// to 577 us by the card (of 2144 keys on average; 4 products: 1060 to 1000 TFLOP/s),
+// matrix unit busy 56%, vector unit 54%; 103 us with a window of 128, where half is
+// a block's start: q, dout and out rows and the first tiles, 5 us for each of the
+// two blocks a CU holds.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p) {
@@ -709,7 +714,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void sa_dq_kernel(SaParams p)
     if (i < own0 || i >= own1) return;
     // Written in the order in which it has to issue (the barriers hold it): reads ahead
     // of their use, the first half's exponentials beside the second's scores, its
-    // products beside the second's exponentials (without: 572 us, with 548).
+    // products beside the second's exponentials (without: 572 us, with 548, on one card).
     af3_bf16x8 ka[KS], va[KS], kb[KS], vb[KS], tr[DB], ts[DB];
     af3_f32x16 s0[1] = {a_zero()}, s1[1] = {a_zero()}, d0[1], d1[1];
     const bool whole = i >= free0 && i < free1;
@@ -871,10 +876,10 @@ __device__ __forceinline__ void a_dsink(const SaParams& p, int h, float* sh) {
 // own first half, held in that order, so that the matrix unit works beside them.
 //
 // Two passes over the scores (this and dq's) instead of one with atomic sums of
-// dq: five products become seven, but every sum has a fixed order and no fp32
-// copy of dq is written and read.  8192 packed rows, 64 heads over 8, D 64: 681 us
-// (of 2144 keys on average; 4 products: 845 TFLOP/s), matrix unit busy 50%, the
-// rest LDS reads and the exponentials that do not fit beside products; 82 us with
+// dq: five products become seven (eight with dq's p k), but every sum has a fixed
+// order and no fp32 copy of dq is written and read.  8192 packed rows, 64 heads over
+// 8, D 64: 668 to 707 us by the card (of 2144 keys on average; 4 products: 860 to 815
+// TFLOP/s), matrix unit busy 50%, the rest LDS reads and the exponentials that do not fit beside products; 82 us with
 // a window of 128, where a block's start and its partly visible steps count.
 // ---------------------------------------------------------------------------
 // first token after t0, whose sequence starts at s0, of a later sequence (starts does

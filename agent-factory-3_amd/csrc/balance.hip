@@ -8,20 +8,23 @@
 //   loss = E sum_e (c_e / n) (sum_t p_te / n)            (0 when n = 0)
 //   d logits_te = g E / n  p_te (c_e / n - sum_x p_tx c_x / n)
 //
-// HBM-bound: the logits are read once per direction and the gradient written
-// once; p is made again in the backward (two shuffled reductions over values
-// already in registers) instead of being stored.  A row's E logits lie in
-// LPR = E / 8 lanes (a power of two, at least 4), 8 consecutive experts each (one 16-byte
-// load), so a wave takes 64 / LPR rows at a time, the top K are K maxima over
+// The logits are read once per direction and the gradient written once; p is made
+// again in the backward (two shuffled reductions over values already in registers)
+// instead of being stored.  A row's E logits lie in LPR = E / 8 lanes (a power of
+// two, 4 to 64), 8 consecutive experts each (one 16-byte load; 16 past 512 experts),
+// so a wave takes 64 / LPR rows at a time, the top K are K maxima over
 // (order-preserving logit bits, inverted id) keys, and a lane's column sums and
-// counts stay in its registers over all its rows.  Column sums are fp32 over at
-// most a few hundred rows per lane, then joined in a fixed order.
+// counts stay in its registers over all its rows.  Column sums are fp32: a lane adds
+// T / (4096 (64 / LPR)) rows once there are 512 blocks (128000 tokens of 128 experts:
+// 8; ten million of 1024: 2441, whose additions are off by at most 2^-24 of the sum
+// each, at random about 3e-6 in all), then lanes, waves and blocks are joined in a fixed order.
 //
-// 128000 tokens of 128 experts, ids given: sums 12.1 us (35 MB: 2.9 TB/s), join
-// 4.9, gradient 19.2 (66 MB: 3.4 TB/s); 16384 tokens, top 4: 9.5, 4.1 and 7.3.  A
-// row's exponentials, its reductions and, for the top K, K rounds of maxima are
-// most of the first kernel; the gradient is near what reads and writes mixed reach
-// at this size.  A call of 77 tokens is one launch of 5.2 us and one of 3.0.
+// 128000 tokens of 128 experts, ids given: sums 12.5 us (35 MB: 2.8 TB/s), join 4.6,
+// gradient 20.2 (66 MB: 3.3 TB/s; a copy of as much takes 9.9); 16384 tokens, top 4:
+// 9.7, 3.8 and 7.6.  The vector unit is busy 78% of the sums' cycles and 60% of the
+// gradient's (67% and 27% at 16384 tokens): a row's exponentials and reductions, and
+// for the top K its K rounds of maxima; the rest is waiting for loads a pass ahead.
+// A call of 77 tokens is one launch of 5.2 us and one of 2.8.
 #include "af3_common.h"
 
 namespace {
