@@ -240,8 +240,8 @@ def sink_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sinks: tor
     fp32 and in a fixed order.  Scores are fp32: a probability is off by its score's
     rounding (2^-24 of it), and scores past 2^29 overflow.  What stands outside a
     row's ``kv_range``, or in a packed row's tokens of no sequence, has no influence;
-    a NaN or infinity inside can reach rows of the same tile (128 rows, 64 keys) that do not see it, as 0 times NaN does in
-    any masked product.
+    a NaN or infinity inside can reach rows of the same tile (128 rows, 64 keys) that
+    do not see it, as 0 times NaN does in any masked product.
 
     Args:
         q: [B, Hq, Sq, D] bf16, D 64 or 128; any strides (head vectors contiguous
@@ -326,9 +326,9 @@ def attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mas
                    use_vmap=False, **kwargs):
     """What transformers hands every layer as its mask (causal order and window are
     the attention's own): None; [B, 2] int32 key ranges of a batch padded on either
-    side; or [B, S, 1] int32, where transformers found packed sequences (position ids
+    side; or [B, S, 1] int64, where transformers found packed sequences (position ids
     that start again, which most of its models look for where neither padding nor a
-    cache is given): the start of each token's own.  Other mask functions are refused.
+    cache is given): each token's place in its own.  Other mask functions are refused.
     Reads the padding mask once per call (a host synchronisation): twice a forward for a
     model with sliding and full layers."""
     if use_vmap:
@@ -343,7 +343,7 @@ def attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mas
         at = torch.arange(kv_length, device=seq.device).expand(batch_size, kv_length)
         new = torch.ones_like(at, dtype=torch.bool)
         new[:, 1:] = seq[:, 1:] != seq[:, :-1]
-        return torch.where(new, at, 0).cummax(1).values.to(torch.int32)[..., None]
+        return (at - torch.where(new, at, 0).cummax(1).values)[..., None]
     if attention_mask is None:
         return None
     m = attention_mask[:, kv_offset:kv_offset + kv_length].to(torch.int32)
@@ -375,30 +375,27 @@ def attention_forward(module, query, key, value, attention_mask, scaling=None, d
     if not (getattr(module, "is_causal", True) if causal is None else causal):
         raise NotImplementedError("af3_sink: only causal attention is supported")
     B, S, Sk = query.shape[0], query.shape[2], key.shape[2]
-    starts = None
+    cu, pos = kwargs.get("cu_seq_lens_q"), kwargs.get("position_ids")
     if attention_mask is not None:
         if S == Sk and attention_mask.shape == (B, S, 1):
-            starts, attention_mask = attention_mask[..., 0], None
+            pos, attention_mask = attention_mask, None
         elif attention_mask.shape != (B, 2):
             raise ValueError("af3_sink: the mask must be the one that its own mask function makes (or None), got "
                              f"{tuple(attention_mask.shape)}")
     if s_aux is not None and s_aux.dtype not in (torch.bfloat16, torch.float32):
         s_aux = s_aux.float()
     args = dict(scale=scaling, window=sliding_window or 0, kv_range=attention_mask)
-    cu, pos = kwargs.get("cu_seq_lens_q"), kwargs.get("position_ids")
     if cu is not None:
         cu_k = kwargs.get("cu_seq_lens_k")
         if cu_k is not None and cu_k is not cu and cu_k.shape != cu.shape:
             raise ValueError("af3_sink: cu_seq_lens_q and cu_seq_lens_k differ")
         return sink_attention(query, key, value, s_aux, cu_seqlens=cu, **args), None
-    if starts is None and pos is not None and S == Sk > 1 and pos.numel() == B * S:
+    if pos is not None and S == Sk > 1 and pos.numel() == B * S:
         starts = sequence_starts_of_rows(pos.to(query.device, torch.int64).reshape(B, S), attention_mask)
-    if starts is not None:
         scale = query.shape[-1] ** -0.5 if scaling is None else scaling
         _check(query, key, value, s_aux, scale, args["window"], 0)
         with _device_of(query):
-            return _run(query, key, value, s_aux, scale, min(args["window"], MAX_LEN), 0, None,
-                        starts.to(query.device).contiguous(), None), None
+            return _run(query, key, value, s_aux, scale, min(args["window"], MAX_LEN), 0, None, starts, None), None
     return sink_attention(query, key, value, s_aux, **args), None
 
 

@@ -291,8 +291,8 @@ __device__ __forceinline__ Keys a_keys(const SaParams& p, int pos0, int pos1, in
 // products; the counters give 87% of the cycles to the vector unit and 48% to
 // the matrix unit.  8192 packed rows of 2144 keys on average, 64 heads over 8,
 // D 64: 340 to 357 us by the card (845 to 805 TFLOP/s); a window of 128: 54 us; 2 x
-// 4096 rows: 315 to 337 us.  Where a wave's rows are few the tiles are read at memory speed: one
-// token over 131072 keys 43 us (6.2 TB/s), 32 tokens over 4099: 26.7 us (5.1).
+// 4096 rows: 315 to 337 us.  Where a wave's rows are few the tiles are read at
+// memory speed: one token over 131072 keys 43 us (6.2 TB/s), 32 tokens over 4099: 26.7 us (5.1).
 // A window's block runs three to four tiles, so its start (first copies, q rows)
 // is a third of it.  Stages as constants of six unrolled turns gain 3% on the
 // long rows and lose 10% on the window (code fetched once per block), so the
@@ -879,8 +879,9 @@ __device__ __forceinline__ void a_dsink(const SaParams& p, int h, float* sh) {
 // dq: five products become seven (eight with dq's p k), but every sum has a fixed
 // order and no fp32 copy of dq is written and read.  8192 packed rows, 64 heads over
 // 8, D 64: 668 to 707 us by the card (of 2144 keys on average; 4 products: 860 to 815
-// TFLOP/s), matrix unit busy 50%, the rest LDS reads and the exponentials that do not fit beside products; 82 us with
-// a window of 128, where a block's start and its partly visible steps count.
+// TFLOP/s), matrix unit busy 50%, the rest LDS reads and the exponentials that do not
+// fit beside products; 82 us with a window of 128, where a block's start and its
+// partly visible steps count.
 // ---------------------------------------------------------------------------
 // first token after t0, whose sequence starts at s0, of a later sequence (starts does
 // not decrease), or n > t0: 64 probes a round, the answer stays in (lo, hi]
@@ -1287,7 +1288,7 @@ __global__ __launch_bounds__(1024) void sa_starts_pos_kernel(const int64_t* __re
     lo = min(max(range[2 * row], 0), T);
     hi = min(max(range[2 * row + 1], lo), T);
   }
-  auto starts_at = [&](int t) { return t < T && (t == 0 || pos[t] != pos[t - 1] + 1); };
+  auto starts_at = [&](int t) { return t < T && (t == 0 || (uint64_t)pos[t] - (uint64_t)pos[t - 1] != 1); };
   bool on[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) on[i] = starts_at(c0 + i * 1024 + (int)threadIdx.x);

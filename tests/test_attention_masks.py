@@ -20,6 +20,13 @@ POS = [[0, 1, 2, 0, 1, 2], [0, 1, 0, 1, 2, 3]]
 STARTS = [[0, 0, 0, 3, 3, 3], [0, 0, 2, 2, 2, 2]]
 
 
+def _starts(pos, kv_range=None):
+    at = torch.arange(pos.shape[1])
+    new = torch.ones_like(pos, dtype=torch.bool)
+    new[:, 1:] = pos[:, 1:] != pos[:, :-1] + 1
+    return torch.where(new, at, 0).cummax(1).values.to(torch.int32)
+
+
 def _stand_in(monkeypatch):
     """What the kernels would be called with."""
     import contextlib
@@ -51,14 +58,15 @@ def test_layers_read_a_batch_of_packed_rows_from_its_position_ids(monkeypatch):
 @pytest.mark.parametrize("window", [0, 8])
 def test_the_packing_that_transformers_finds(pos, starts, window, monkeypatch):
     """Models that give their mask functions position ids (one row of them may stand for all): the packing
-    is in the mask function, and every layer gets the starts made of it."""
+    is in the mask function, and every layer gets the places in their sequences that were made of it."""
     from transformers.masking_utils import create_causal_mask, create_sliding_window_causal_mask
     make = create_sliding_window_causal_mask if window else create_causal_mask
     cfg = _model(layers=2).config
     mask = make(config=cfg, inputs_embeds=torch.zeros(2, 6, 64), attention_mask=None, past_key_values=None,
                 position_ids=torch.tensor(pos))
-    assert mask.shape == (2, 6, 1) and mask.dtype == torch.int32 and mask[..., 0].tolist() == starts
+    assert mask.shape == (2, 6, 1) and (torch.arange(6) - mask[..., 0]).tolist() == starts
     seen = _stand_in(monkeypatch)
+    monkeypatch.setattr(attention, "sequence_starts_of_rows", _starts)
     q = torch.zeros(2, 2, 6, 64)
     out, _ = attention.attention_forward(None, q, q, q, mask, scaling=0.125, sliding_window=window, is_causal=True)
     assert out.shape == (2, 6, 2, 64) and seen[0][1] == window and seen[0][2].tolist() == starts

@@ -493,7 +493,7 @@ def test_a_batch_of_packed_rows(dev, G, D, window, first):
     grads = torch.autograd.grad(out, leaves, do)
     if not first:
         import types
-        for mask, ids in ((None, pos), (starts[..., None], None)):   # the layers' call, by either
+        for mask, ids in ((None, pos), (pos[..., None], None)):   # the layers' call, by either
             one, _ = attention.attention_forward(types.SimpleNamespace(is_causal=True), q, k, v, mask, position_ids=ids,
                                                  sliding_window=window, s_aux=s)
             assert torch.equal(one, out)
