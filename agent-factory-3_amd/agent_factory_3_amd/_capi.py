@@ -87,6 +87,14 @@ _SIGNATURES = {
     "af3_balance_loss_workspace_bytes": (_sz, [_i64, _i32]),
     "af3_balance_loss_fwd": (_i32, [_p, _i64, _p, _p, _i64, _i32, _i32, _p, _p, _p, _p, _sz, _p]),
     "af3_balance_loss_bwd": (_i32, [_p, _i64, _p, _i64, _i32, _p, _p, _p, _p]),
+    "af3_residual_norm_fwd": (_i32, [_p, _i32, _i64, _p, _i32, _i64, _p, _i32, _p, _i32, _p, _i32, _i32, _i64, _f32, _f32,
+                                     _i64, _i32, _p, _p, _p, _p, _p]),
+    "af3_residual_norm_bwd_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i32, _i32, _i32]),
+    "af3_residual_norm_bwd": (_i32, [_p, _i64, _p, _i64, _p, _i32, _i64, _p, _i32, _i64, _p, _p, _p, _i32, _p, _i32, _p,
+                                     _i32, _i32, _i64, _f32, _i32, _i64, _i32, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "af3_grad_norm_partials": (_sz, [_p, _i32]),
+    "af3_grad_norm": (_i32, [_p, _p, _p, _i32, _i32, _p, _i64, _p, _p, _p]),
+    "af3_grad_scale": (_i32, [_p, _p, _p, _i32, _i32, _p, _i64, _f32, _p, _p]),
 }
 
 _lib = None

@@ -1,0 +1,230 @@
+"""Root-mean-square norms with the residual stream on the MI355X.
+
+``residual_norm`` adds a block's output to the residual stream and normalises the
+sum for the next block, in one pass over the data (gpt-oss's layers do it in
+several: transformers' GptOssDecoderLayer adds, GptOssRMSNorm converts, squares,
+scales and converts back); the block's output may have a norm of its own, a gate
+and a scale.  ``rms_norm`` is the norm alone.  Both are differentiable in every
+tensor.  The HIP kernels are behind ``af3_residual_norm_fwd`` / ``_bwd``; there is
+no CPU fallback.
+"""
+from __future__ import annotations
+
+import functools
+import math
+
+import torch
+
+from . import _capi
+from .routing import _device_of, _no_forward_mode
+
+MIN_HIDDEN, MAX_HIDDEN = 8, 16384
+_TYPES = (torch.bfloat16, torch.float32)
+
+
+def _rows(t: torch.Tensor):
+    """[..., H] as [rows, H] with contiguous rows, and the rows' stride."""
+    t = t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _f32(t) -> int:
+    return int(t is not None and t.dtype == torch.float32)
+
+
+@functools.lru_cache(maxsize=64)
+def _bwd_workspace(rows, H, full, gate_cols, gate_rows, w, post, gate) -> int:
+    return int(_capi.load().af3_residual_norm_bwd_workspace_bytes(rows, H, full, gate_cols, gate_rows, w, post, gate))
+
+
+def _forward(x, residual, weight, post, gate, gate_rows, scale, eps, stats):
+    """(r, h, 1 / rms of r, 1 / rms of x); r None without a residual, h None without a weight."""
+    H = x.shape[-1]
+    dev = x.device
+    x2, ldx = _rows(x)
+    n = x2.shape[0]
+    r = h = rstd = rstd_x = None
+    res, ldr = (None, 0) if residual is None else _rows(residual)
+    if residual is not None:
+        r = torch.empty(residual.shape, dtype=residual.dtype, device=dev)
+    if weight is not None:
+        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        rstd = torch.empty(n, dtype=torch.float32, device=dev) if stats else None
+    if post is not None and stats:
+        rstd_x = torch.empty(n, dtype=torch.float32, device=dev)
+    _capi.call("af3_residual_norm_fwd", x2.data_ptr(), _f32(x), ldx, _capi.ptr(res), _f32(residual), ldr,
+               _capi.ptr(weight), _f32(weight), _capi.ptr(post), _f32(post), _capi.ptr(gate), _f32(gate),
+               0 if gate is None else gate.shape[1], gate_rows, scale, eps, n, H, _capi.ptr(r), _capi.ptr(h),
+               _capi.ptr(rstd), _capi.ptr(rstd_x), _capi.stream_of(dev))
+    return r, h, rstd, rstd_x
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, post, gate, gate_rows, scale, eps):
+        r, h, rstd, rstd_x = _forward(x, residual, weight, post, gate, gate_rows, scale, eps, True)
+        keep_x = residual is None or post is not None or (gate is not None and gate.requires_grad)
+        ctx.save_for_backward(x if keep_x else None, r if weight is not None else None, weight, post, gate, rstd, rstd_x)
+        ctx.args = (x.shape, x.dtype, None if residual is None else residual.dtype, gate_rows, scale)
+        ctx.set_materialize_grads(False)
+        if residual is None:
+            return h
+        return (r, h) if weight is not None else r
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        _no_forward_mode("residual_norm backward", *grads)
+        x, r, weight, post, gate, rstd, rstd_x = ctx.saved_tensors
+        shape, xt, rt, gate_rows, scale = ctx.args
+        need_x, need_res, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
+        dr, dh = (None, grads[0]) if rt is None else (grads + (None,))[:2]
+        if dr is None and dh is None:
+            return (None,) * 8
+        H, n = shape[-1], math.prod(shape[:-1])
+        some = dr if dr is not None else dh
+        dev = some.device
+        with _device_of(some):
+            # (saved-tensor hooks, as those that keep them on the host, may give them other strides)
+            weight, post, gate, rstd, rstd_x = (t if t is None else t.contiguous()
+                                                for t in (weight, post, gate, rstd, rstd_x))
+            dr, lddr = (None, 0) if dr is None else _rows(dr)
+            dh, lddh = (None, 0) if dh is None else _rows(dh)
+            x, ldx = (None, 0) if x is None else _rows(x)
+            r, ldr = (x, ldx) if rt is None else (None, 0) if r is None else _rows(r)
+            full = rt is not None and (post is not None or gate is not None)
+            dx = dres = dw = dpost = dgate = None
+            # without norm, gate and scale the branch has the stream's own gradient, returned for both
+            same = not full and (rt is None or (scale == 1.0 and xt == rt))
+            if need_res or (need_x and same):
+                dres = torch.empty(shape, dtype=rt or xt, device=dev)
+            if need_x and not same:
+                dx = torch.empty(shape, dtype=xt, device=dev)
+            need_w = need_w and dh is not None
+            make = torch.empty if n else torch.zeros
+            if need_w:
+                dw = make(H, dtype=weight.dtype, device=dev)
+            if need_post:
+                dpost = make(H, dtype=post.dtype, device=dev)
+            if need_gate:
+                dgate = make(gate.shape, dtype=gate.dtype, device=dev)
+            cols = 0 if gate is None else gate.shape[1]
+            ws_n = _bwd_workspace(n, H, int(full), cols, gate_rows, need_w, need_post, need_gate)
+            ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
+            if n:
+                _capi.call("af3_residual_norm_bwd", _capi.ptr(dr), lddr, _capi.ptr(dh), lddh, _capi.ptr(r),
+                           int((rt or xt) == torch.float32), ldr, _capi.ptr(x), int(xt == torch.float32), ldx,
+                           _capi.ptr(rstd), _capi.ptr(rstd_x), _capi.ptr(weight), _f32(weight), _capi.ptr(post),
+                           _f32(post), _capi.ptr(gate), _f32(gate), cols, gate_rows, scale, int(rt is not None), n, H,
+                           _capi.ptr(dx), _capi.ptr(dres), _capi.ptr(dw), _capi.ptr(dpost), _capi.ptr(dgate),
+                           _capi.ptr(ws), ws_n, _capi.stream_of(dev))
+        if same and need_x:
+            dx = dres
+        return dx, dres if need_res else None, dw, dpost, dgate, None, None, None
+
+
+def _check_tensor(who, name, t, device):
+    if not t.is_cuda:
+        raise RuntimeError(f"{who}: {name} must be a GPU tensor (the MI355X path has no CPU implementation)")
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{who}: {name} must be bfloat16 or float32 (got {t.dtype})")
+    if t.device != device:
+        raise ValueError(f"{who}: {name} is on {t.device}, x on {device}")
+
+
+def _check(who, x, weight, post, eps):
+    _check_tensor(who, "x", x, x.device)
+    H = x.shape[-1] if x.dim() else 0
+    if not MIN_HIDDEN <= H <= MAX_HIDDEN:
+        raise ValueError(f"{who}: x must be [..., H] with H from {MIN_HIDDEN} to {MAX_HIDDEN}, got {tuple(x.shape)}")
+    for name, t in (("weight", weight), ("post_weight", post)):
+        if t is not None:
+            _check_tensor(who, name, t, x.device)
+            if t.shape != (H,):
+                raise ValueError(f"{who}: {name} must be [{H}], got {tuple(t.shape)}")
+    if not (0.0 <= eps < math.inf):
+        raise ValueError(f"{who}: eps must not be negative, got {eps}")
+
+
+def _gate_rows(gate, shape):
+    """The gate as [groups, 1 or H] and the rows of x that share each of its rows."""
+    if gate.dim() > len(shape) or any(g not in (1, s) for g, s in zip(gate.shape[::-1], shape[::-1])):
+        raise ValueError(f"residual_norm: a gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+    lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
+    cols, lead = lead[-1], lead[:-1]
+    k = len(lead)   # dimensions from k on are shared
+    while k and lead[k - 1] == 1:
+        k -= 1
+    if any(g != s for g, s in zip(lead[:k], shape)):   # shared along outer dimensions only: a row for each,
+        # in fp32, so that the gradient is rounded once, after torch's sum over them
+        gate, k = gate.float().expand(*shape[:-1], cols), len(lead)
+    return gate.reshape(-1, cols).contiguous(), math.prod(shape[k:-1])
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
+    """``weight * x / sqrt(mean(x^2) + eps)`` over the last dimension, rounded once.
+
+    Args:
+        x: [..., H] bf16 or fp32, H from 8 to 16384; rows contiguous (others are copied)
+        weight: [H] bf16 or fp32
+    Returns:
+        [..., H] in x's type
+    """
+    _no_forward_mode("rms_norm", x, weight)
+    eps = float(eps)
+    _check("rms_norm", x, weight, None, eps)
+    with _device_of(x):
+        weight = weight if weight.is_contiguous() else weight.contiguous()
+        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+            return _ResidualNorm.apply(x, None, weight, None, None, 1, 1.0, eps)
+        return _forward(x, None, weight, None, None, 1, 1.0, eps, False)[1]
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, *, eps: float = 1e-5,
+                  post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0):
+    """A block's output joins the residual stream, and the next block's norm:
+
+        u = x,  or  post_weight * x / sqrt(mean(x^2) + eps)
+        r = residual + scale * gate * u
+        h = weight * r / sqrt(mean(r^2) + eps)
+
+    Statistics and products are fp32, h is made from r before its rounding, and each
+    result is rounded once; sums over rows are in a fixed order.  Where x takes the
+    stream's gradient as it is (no norm, gate or scale of its own, one type), both
+    get the same tensor, as from torch's add.
+
+    Args:
+        x: [..., H] bf16 or fp32, H from 8 to 16384
+        residual: the same shape, in x's type or fp32
+        weight: [H] bf16 or fp32; None: only r is made
+        post_weight: [H] of the block's own norm, or None
+        gate: bf16 or fp32, broadcast to x: [H], [B, 1, H], [B, S, 1], ...; or None
+    Returns:
+        (r in residual's type, h in x's type or None)
+    """
+    _no_forward_mode("residual_norm", x, residual, weight, post_weight, gate)
+    eps, scale = float(eps), float(scale)
+    _check("residual_norm", x, weight, post_weight, eps)
+    _check_tensor("residual_norm", "residual", residual, x.device)
+    if residual.shape != x.shape:
+        raise ValueError(f"residual_norm: x is {tuple(x.shape)}, the residual {tuple(residual.shape)}")
+    if x.dtype == torch.float32 and residual.dtype != torch.float32:
+        raise TypeError(f"residual_norm: a float32 x needs a float32 residual (got {residual.dtype})")
+    if not math.isfinite(scale):
+        raise ValueError(f"residual_norm: scale must be finite, got {scale}")
+    if gate is not None:
+        _check_tensor("residual_norm", "gate", gate, x.device)
+    with _device_of(x):
+        gate_rows = 1
+        if gate is not None:
+            gate, gate_rows = _gate_rows(gate, x.shape)
+            gate_rows = max(gate_rows, 1)
+        weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+        post_weight = post_weight if post_weight is None or post_weight.is_contiguous() else post_weight.contiguous()
+        ts = (x, residual, weight, post_weight, gate)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+            out = _ResidualNorm.apply(*ts, gate_rows, scale, eps)
+            return out if weight is not None else (out, None)
+        return _forward(*ts, gate_rows, scale, eps, False)[:2]

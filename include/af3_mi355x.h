@@ -490,6 +490,50 @@ int af3_seq_starts_positions(const int64_t* position_ids, int n_tokens, int32_t*
 int af3_seq_starts_rows(const int64_t* position_ids, int64_t ld, int n_rows, int n_tokens, const int32_t* kv_range,
                         int32_t* starts, void* stream);
 
+/* Root-mean-square norms with the residual stream (no counterpart in the
+ * reference, whose layers run transformers' modules).  Rows of H elements, 8 to
+ * 16384; a row's elements are contiguous, ld* are the rows' strides; no alignment
+ * beyond the elements'.  Each tensor is bf16, or fp32 where its *_f32 is set.
+ *   u = x, or post_weight x / sqrt(mean x^2 + eps);  r = residual + scale gate u
+ *   h = weight r / sqrt(mean r^2 + eps)
+ * residual NULL: r = x, not written (h has x's type; post_weight and gate NULL).
+ * weight NULL: no h.  r has residual's type (bf16 only with a bf16 x).  gate [rows /
+ * gate_rows, rounded up][gate_cols], contiguous, gate_cols 1 or H (0: none): its row i is shared by the
+ * rows i gate_rows .. .  rstd, rstd_x [rows] fp32 (of r and of x) for the
+ * backward, or NULL.
+ * Backward: dr (NULL: none) and dh (NULL: none) arrive at r and h, r as the
+ * forward wrote it (x without a residual).  dresidual = dr + the norm's gradient
+ * (without a residual this is x's gradient); dx, dweight, dpost, dgate, each NULL
+ * if not wanted, in their tensors' types; sums are fp32 in a fixed order.  x is
+ * read where there is a post_weight or gate. */
+int af3_residual_norm_fwd(const void* x, int x_f32, int64_t ldx, const void* residual, int r_f32, int64_t ldr,
+                          const void* weight, int w_f32, const void* post_weight, int post_f32, const void* gate,
+                          int gate_f32, int gate_cols, int64_t gate_rows, float scale, float eps, int64_t rows, int H,
+                          void* out_r, void* out_h, float* rstd, float* rstd_x, void* stream);
+size_t af3_residual_norm_bwd_workspace_bytes(int64_t rows, int H, int full, int gate_cols, int64_t gate_rows,
+                                             int want_w, int want_post, int want_gate);
+int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* dh, int64_t lddh, const void* r, int r_f32,
+                          int64_t ldr, const void* x, int x_f32, int64_t ldx, const float* rstd, const float* rstd_x,
+                          const void* weight, int w_f32, const void* post_weight, int post_f32, const void* gate,
+                          int gate_f32, int gate_cols, int64_t gate_rows, float scale, int has_residual, int64_t rows,
+                          int H, void* dx, void* dresidual, void* dweight, void* dpost, void* dgate, void* workspace,
+                          size_t ws_bytes, void* stream);
+
+/* The norm of n tensors taken as one vector, and their scaling by min(1, max_norm /
+ * (norm + 1e-6)).  ptrs, sizes (elements, above 0) and is_f32 (else bf16) are host
+ * arrays, read before the call returns; the tensors are contiguous on the
+ * stream's device.  norm_type 2, 1, or 0 for the largest magnitude.  af3_grad_norm
+ * writes one 64-bit partial per chunk (af3_grad_norm_partials of them), their sum
+ * (sum |g|^p, or the largest) to `sum` and the norm to `norm` (each may be NULL).
+ * af3_grad_scale takes partials, of these and of other tensors, scales where the
+ * factor is below 1 (a NaN norm gives NaN), and writes the norm (NULL: not);
+ * tensors that share memory are refused. */
+size_t af3_grad_norm_partials(const int64_t* sizes, int n);
+int af3_grad_norm(const uint64_t* ptrs, const int64_t* sizes, const uint8_t* is_f32, int n, int norm_type,
+                  double* partials, int64_t n_partials, double* sum, float* norm, void* stream);
+int af3_grad_scale(const uint64_t* ptrs, const int64_t* sizes, const uint8_t* is_f32, int n, int norm_type,
+                   const double* partials, int64_t n_partials, float max_norm, float* norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
