@@ -1,0 +1,729 @@
+// Matrix products with a bias, an activation and a residual in the epilogue, and the
+// products of their backward.  (The reference's attention projections are nn.Linear
+// calls into a library, and the residual adds passes of their own.)
+//
+//   z = x W^T + b,  y = act(z) + residual
+//   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum_rows dz,  dresidual = dy
+//
+// One kernel makes the three products, out[M][N] = sum_k P[m][k] Q[n][k], each operand
+// stored with k contiguous (x, W of the forward) or, PT / QT, with its own index
+// contiguous (W of dx; dz and x of dW), so nothing is transposed in memory.
+//
+// lin_kernel: a block of 4 waves (2 x 2) makes BM x BN of the output in 64-deep
+// k-steps.  Both operands of a k-step go global -> LDS (16-byte copies) into one of two
+// stages while the other is used; a wave's BM/2 x BN/2 part is TM x TN products
+// v_mfma_f32_32x32x16_bf16.  With 128 x 128 per wave a fragment read from LDS is used
+// four times: 64 bytes per clock and CU where the copies take another 32, under what
+// the LDS gives (147; 111 for transposing reads); with 128 x 64 (eight waves) both would
+// saturate it.  One wave per SIMD hides nothing by itself, so the loop is a fixed
+// schedule: fragments of the next 16 k are read between the products of this one, one
+// instruction per product, the k-step's last products run after the next barrier, and
+// the next stage's copies are issued in the first quarter of a step.
+// Fragments: lane (r, h) = (lane % 32, lane / 32) feeds row r, k = 16 s + 8 h + (0..7) of
+// sub-step s.  k contiguous: one 16-byte read.  Else two transposing reads of 4 k each.
+// LDS chunks of 16 bytes are XOR-swizzled so that either reads without bank conflicts.
+// Q is the matrix unit's first operand, so a lane ends up with rows of the output, 4
+// consecutive columns at a time; the epilogue turns them through LDS (32 rows of a wave
+// at a time, fp32) into 16-byte accesses and rounds once.
+//
+// Few tiles and a long k (dW): blocks share a tile's k-steps and write fp32 partials,
+// which lin_join_kernel adds in order and gives the epilogue.
+// Up to 32 rows: lin_skinny_kernel streams W once through registers.
+#include "af3_common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef const __attribute__((address_space(3))) af3_bf16x8 lds_frag;
+
+enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
+
+struct LinEpi {
+  const void* bias;
+  int bias_f32;
+  int act;
+  const uint16_t* res;
+  int64_t ldr;
+  uint16_t* y;  // [M][N]
+  uint16_t* z;  // [M][N] before the activation, or null
+};
+
+struct LinArgs {
+  const uint16_t* p;
+  int64_t ldp;
+  const uint16_t* q;
+  int64_t ldq;
+  int M, N, K;
+  int tiles_m, tiles_n, group_m;
+  int splits, steps_per_split;
+  float* part;  // [splits][M][N]
+  LinEpi e;
+};
+
+__device__ __forceinline__ float lin_act(float z, int act) {
+  if (act == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
+  if (act == kActSilu) return z / (1.f + __expf(-z));
+  if (act == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if (act == kActGeluTanh) return 0.5f * z * (1.f + tanhf(0.79788456f * (z + 0.044715f * z * z * z)));
+  return z;
+}
+__device__ __forceinline__ float lin_slope(float z, int act) {
+  if (act == kActRelu) return z > 0.f ? 1.f : 0.f;
+  if (act == kActSilu) {
+    const float s = 1.f / (1.f + __expf(-z));
+    return s * (1.f + z * (1.f - s));
+  }
+  if (act == kActGelu) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+  if (act == kActGeluTanh) {
+    const float t = tanhf(0.79788456f * (z + 0.044715f * z * z * z));
+    return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * z * z);
+  }
+  return 1.f;
+}
+
+// 8 columns from `col` of row m: sums -> output (columns past N are left out)
+__device__ __forceinline__ void lin_finish(const LinEpi& e, int64_t m, int col, int N, float (&v)[8]) {
+  const int64_t at = m * N + col;
+  if (col + 8 <= N) {
+    if (e.bias) {
+      if (e.bias_f32) {
+        float b[8];
+        __builtin_memcpy(b, (const float*)e.bias + col, 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += b[i];
+      } else {
+        uint32_t b[4];
+        __builtin_memcpy(b, (const uint16_t*)e.bias + col, 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] += af3_bf16_to_f32(b[i]);
+          v[2 * i + 1] += af3_bf16_to_f32(b[i] >> 16);
+        }
+      }
+    }
+    if (e.act) {
+      if (e.z) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = af3_pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        __builtin_memcpy(e.z + at, w, 16);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = lin_act(v[i], e.act);
+    }
+    if (e.res) {
+      uint32_t r[4];
+      __builtin_memcpy(r, e.res + m * e.ldr + col, 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] += af3_bf16_to_f32(r[i]);
+        v[2 * i + 1] += af3_bf16_to_f32(r[i] >> 16);
+      }
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = af3_pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    __builtin_memcpy(e.y + at, w, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < N) {
+        float f = v[i];
+        if (e.bias)
+          f += e.bias_f32 ? ((const float*)e.bias)[col + i] : af3_bf16_to_f32(((const uint16_t*)e.bias)[col + i]);
+        if (e.act) {
+          if (e.z) e.z[at + i] = (uint16_t)af3_f32_to_bf16(f);
+          f = lin_act(f, e.act);
+        }
+        if (e.res) f += af3_bf16_to_f32(e.res[m * e.ldr + col + i]);
+        e.y[at + i] = (uint16_t)af3_f32_to_bf16(f);
+      }
+  }
+}
+
+__device__ __forceinline__ void lin_dma16(const void* sbase, uint32_t voff, uint32_t lds_byte_addr) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_byte_addr) : "memory");
+}
+
+template <bool V>
+struct Flag {
+  static constexpr bool value = V;
+};
+
+// One operand of a tile: R of its rows (or columns, T) by 64 k in LDS.
+template <int R, bool T>
+struct LinTile {
+  static constexpr int kRowB = T ? R * 2 : 128;       // bytes per LDS row: 64 k of a row, or a k of all rows
+  static constexpr int kCh = kRowB / 16;              // 16-byte chunks per LDS row
+  static constexpr int kBytes = R * 128;
+  static constexpr int kCopies = kBytes / 1024 / 4;   // 1 KB copies per wave and k-step
+  static_assert(kCopies * 4096 == kBytes, "whole copies per wave");
+  // XOR of a chunk's index.  A 16-byte read takes 16 rows' equal chunks at a time, a
+  // transposing read 4 rows' 4 chunks; over 64 banks (16 chunks) both fall into
+  // distinct ones.
+  static __device__ __forceinline__ int swz(int row) {
+    if constexpr (!T) return (row >> 1) & 7;
+    else if constexpr (kCh % 16 == 0) return (row & 3) << 2;
+    else return (row & 2) << 1;  // (rows 8 chunks apart, modulo 16)
+  }
+  // element (LDS row, chunk) that lane `lane` of copy c of the block's 4 kCopies brings
+  static __device__ __forceinline__ void place(int c, int lane, int& row, int& chunk) {
+    const int id = c * 64 + lane;
+    row = id / kCh;
+    chunk = (id % kCh) ^ swz(row);
+  }
+};
+
+// BM x BN tile, see above.  MASKED outputs past M, N are not stored; loads there repeat the last row.
+template <int BM, int BN, bool PT, bool QT>
+__global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void lin_kernel(const LinArgs a) {
+  using TP = LinTile<BM, PT>;
+  using TQ = LinTile<BN, QT>;
+  constexpr int TM = BM / 64, TN = BN / 64;
+  constexpr int STAGE = TP::kBytes + TQ::kBytes;
+  constexpr int NC = TP::kCopies + TQ::kCopies;
+  constexpr int NS = TM * TN;      // products per sub-step
+  constexpr int NF = TM + TN;      // fragments per sub-step
+  constexpr int EPI = 32 * (BN / 2 * 4 + 16);  // bytes per wave of the epilogue's turn
+  static_assert(4 * EPI <= 2 * STAGE, "epilogue fits the ring");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, lh = lane >> 5;
+
+  // work item: blocks go round robin over 8 XCDs; each XCD takes a run of the tiles, in
+  // groups of group_m tile rows so that the ones in flight share operands in its L2
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int total = tiles * a.splits;
+  int item = blockIdx.x;
+  {
+    const int xcd = item & 7, at = item >> 3;
+    const int per = total >> 3, rest = total & 7;
+    item = xcd * per + min(xcd, rest) + at;
+  }
+  const int split = item / tiles;
+  const int tile = item - split * tiles;
+  const int gsz = a.group_m * a.tiles_n;
+  const int grp = tile / gsz, in = tile - grp * gsz;
+  const int gm = min(a.group_m, a.tiles_m - grp * a.group_m);
+  const int m0 = (grp * a.group_m + in % gm) * BM, n0 = in / gm * BN;
+  const int wm0 = (wave >> 1) * (BM / 2), wn0 = (wave & 1) * (BN / 2);
+
+  const int nk_all = (a.K + 63) / 64;
+  const int k_first = split * a.steps_per_split;
+  const int nk = min(a.steps_per_split, nk_all - k_first);
+  const bool tail = k_first + nk == nk_all && (a.K & 63);  // the last k-step is not whole
+
+  // this lane's source of each copy: byte offsets from the k-step's base
+  const uint16_t* pbase = PT ? a.p + (int64_t)k_first * 64 * a.ldp + m0 : a.p + (int64_t)m0 * a.ldp + k_first * 64;
+  const uint16_t* qbase = QT ? a.q + (int64_t)k_first * 64 * a.ldq + n0 : a.q + (int64_t)n0 * a.ldq + k_first * 64;
+  const int64_t pstep = PT ? 64 * a.ldp : 64, qstep = QT ? 64 * a.ldq : 64;
+  uint32_t off[NC];
+#pragma unroll
+  for (int j = 0; j < TP::kCopies; ++j) {
+    int row, ch;
+    TP::place(wave * TP::kCopies + j, lane, row, ch);
+    off[j] = PT ? (uint32_t)(row * a.ldp * 2 + min(ch, (a.M - m0 + 7) / 8 - 1) * 16)
+                : (uint32_t)(min(row, a.M - m0 - 1) * a.ldp * 2 + ch * 16);
+  }
+#pragma unroll
+  for (int j = 0; j < TQ::kCopies; ++j) {
+    int row, ch;
+    TQ::place(wave * TQ::kCopies + j, lane, row, ch);
+    off[TP::kCopies + j] = QT ? (uint32_t)(row * a.ldq * 2 + min(ch, (a.N - n0 + 7) / 8 - 1) * 16)
+                              : (uint32_t)(min(row, a.N - n0 - 1) * a.ldq * 2 + ch * 16);
+  }
+  const uint32_t lds0 =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+  auto lds_at = [&](int j, int stage) {
+    return lds0 + (uint32_t)(stage * STAGE + (j < TP::kCopies ? (wave * TP::kCopies + j) * 1024
+                                                              : TP::kBytes + (wave * TQ::kCopies + j - TP::kCopies) * 1024));
+  };
+  const uint16_t *pk = pbase, *qk = qbase;  // of the next k-step to copy
+  auto copy = [&](int j, int stage) { lin_dma16(j < TP::kCopies ? pk : qk, off[j], lds_at(j, stage)); };
+  // the last k-step where K is not a multiple of 64: chunks past K are zeros
+  auto copy_tail = [&](int stage) {
+    const int left = a.K & 63;
+#pragma unroll 1
+    for (int j = 0; j < NC; ++j) {
+      int row, ch;
+      const bool isp = j < TP::kCopies;
+      if (isp) TP::place(wave * TP::kCopies + j, lane, row, ch);
+      else TQ::place(wave * TQ::kCopies + j - TP::kCopies, lane, row, ch);
+      const bool trans = isp ? PT : QT;
+      const int64_t ld = isp ? a.ldp : a.ldq;
+      const int edge = isp ? a.M - m0 : a.N - n0;
+      const bool live = trans ? row < left : ch * 8 < left;
+      if (trans) ch = min(ch, (edge + 7) / 8 - 1);
+      else row = min(row, edge - 1);
+      af3_u32x4 v = {0, 0, 0, 0};
+      if (live) v = *(const af3_u32x4*)((isp ? pk : qk) + row * ld + ch * 8);
+      *(__attribute__((address_space(3))) af3_u32x4*)(uintptr_t)(lds_at(j, stage) + lane * 16) = v;
+    }
+  };
+
+  // this lane's fragment addresses in stage 0
+  constexpr int PA = PT ? TM : 4, QA = QT ? TN : 4;
+  uint32_t pa[PA], qa[QA];
+  {
+    const int tr_r = 8 * lh + ((lane & 15) >> 2);             // k of the first transposing read
+    const int tr_c = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);  // its column
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      pa[i] = lds0 + (PT ? tr_r * TP::kRowB + ((((wm0 + 32 * i + tr_c) >> 3) ^ TP::swz(tr_r)) << 4) + ((tr_c & 7) << 1)
+                         : (wm0 + lr) * 128 + (((2 * i + lh) ^ TP::swz(lr)) << 4));
+#pragma unroll
+    for (int i = 0; i < QA; ++i)
+      qa[i] = lds0 + TP::kBytes +
+              (QT ? tr_r * TQ::kRowB + ((((wn0 + 32 * i + tr_c) >> 3) ^ TQ::swz(tr_r)) << 4) + ((tr_c & 7) << 1)
+                  : (wn0 + lr) * 128 + (((2 * i + lh) ^ TQ::swz(lr)) << 4));
+  }
+  auto frag = [](bool trans, uint32_t addr, int row_bytes) {  // (8 k of one row)
+    if (trans) {
+      const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)addr);
+      const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)(addr + 4 * row_bytes));
+      return af3_bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    }
+    return *(lds_frag*)(uintptr_t)addr;
+  };
+  auto frag_p = [&](int s, int tm, uint32_t stage) {
+    return PT ? frag(true, pa[tm % PA] + stage + s * 16 * TP::kRowB, TP::kRowB)
+              : frag(false, pa[s % PA] + stage + tm * 32 * 128, 0);
+  };
+  auto frag_q = [&](int s, int tn, uint32_t stage) {
+    return QT ? frag(true, qa[tn % QA] + stage + s * 16 * TQ::kRowB, TQ::kRowB)
+              : frag(false, qa[s % QA] + stage + tn * 32 * 128, 0);
+  };
+
+  af3_f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  af3_bf16x8 fp[2][TM], fq[2][TN];
+
+#pragma unroll
+  for (int i = 0; i < TM; ++i) fp[1][i] = af3_bf16x8{};
+#pragma unroll
+  for (int i = 0; i < TN; ++i) fq[1][i] = af3_bf16x8{};
+
+  // products of fragments c, between them the reads of sub-step s into c ^ 1 and, with
+  // COPY, the next stage's copies
+  auto phase = [&](auto copy_, int c, int s, uint32_t stage, int to) {
+    constexpr bool COPY = decltype(copy_)::value;
+#pragma unroll
+    for (int i = 0; i < (NS > NF ? NS : NF); ++i) {
+      if (i < NS)
+        acc[i / TN][i % TN] =
+            __builtin_amdgcn_mfma_f32_32x32x16_bf16(fq[c][i % TN], fp[c][i / TN], acc[i / TN][i % TN], 0, 0, 0);
+      if (s >= 0 && i < NF) {
+        if (i < TN) fq[c ^ 1][i] = frag_q(s, i, stage);
+        else fp[c ^ 1][i - TN] = frag_p(s, i - TN, stage);
+      }
+      if constexpr (COPY) {
+        constexpr int PER = (NC + NS - 1) / NS;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (i * PER + j < NC) copy(i * PER + j, to);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto step = [&](auto copy_, int cur) {
+    const uint32_t stage = (uint32_t)(cur * STAGE);
+    phase(copy_, 1, 0, stage, cur ^ 1);  // (the last step's last products; of zeros in the first)
+    phase(Flag<false>{}, 0, 1, stage, 0);
+    phase(Flag<false>{}, 1, 2, stage, 0);
+    phase(Flag<false>{}, 0, 3, stage, 0);
+  };
+  // a k-step's copies have landed, and every wave has read the other stage
+#define LIN_NEXT() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+
+  if (nk > 0) {
+    const int whole = nk - (tail ? 1 : 0);
+    if (whole == 0) {
+      copy_tail(0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) copy(j, 0);
+    }
+    int kt = 0;
+    for (; kt < whole - 1; ++kt) {
+      LIN_NEXT();
+      pk += pstep, qk += qstep;
+      step(Flag<true>{}, kt & 1);
+    }
+    for (; kt < nk; ++kt) {  // the last whole step, and the one that is not
+      LIN_NEXT();
+      pk += pstep, qk += qstep;
+      if (kt + 1 < nk) copy_tail((kt & 1) ^ 1);
+      step(Flag<false>{}, kt & 1);
+    }
+    phase(Flag<false>{}, 1, -1, 0, 0);
+  }
+
+  // epilogue: lane (r, h) holds row r of a 32 x 32 part, columns 8 j + 4 h + (0..3)
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  constexpr int W = BN / 2;             // columns of a wave
+  constexpr int ROWB = W * 4 + 16;      // bytes of a staged row
+  constexpr int LPR = W / 8;            // lanes per row when read back
+  const uint32_t es = lds0 + wave * EPI;
+#pragma unroll 1
+  for (int tm = 0; tm < TM; ++tm) {  // (acc[0] is the tile's rows tm; one copy of the code)
+#pragma unroll
+    for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(__attribute__((address_space(3))) f32x4*)(uintptr_t)(es + lr * ROWB + (tn * 32 + 8 * j + 4 * lh) * 4) =
+            f32x4{acc[0][tn][4 * j], acc[0][tn][4 * j + 1], acc[0][tn][4 * j + 2], acc[0][tn][4 * j + 3]};
+#pragma unroll
+    for (int i = 0; i + 1 < TM; ++i)
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn) acc[i][tn] = acc[i + 1][tn];
+    // (a wave's own LDS writes and reads are in order; the compiler keeps them so)
+#pragma unroll 1
+    for (int id = lane; id < 32 * LPR; id += 64) {
+      const int row = id / LPR, c8 = id % LPR * 8;
+      const int64_t m = m0 + wm0 + tm * 32 + row;
+      const int col = n0 + wn0 + c8;
+      const uint32_t at = es + row * ROWB + c8 * 4;
+      const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)at;
+      const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)(at + 16);
+      if (m >= a.M || col >= a.N) continue;
+      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      if (a.part) {
+        float* const out = a.part + ((int64_t)split * a.M + m) * a.N + col;
+        if (col + 8 <= a.N) {
+          __builtin_memcpy(out, v, 32);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < a.N) out[i] = v[i];
+        }
+      } else {
+        lin_finish(a.e, m, col, a.N, v);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before the next 32 rows overwrite)
+  }
+}
+
+// partials of the splits, added in order, then the epilogue: 8 columns of a row per thread
+__global__ __launch_bounds__(256) void lin_join_kernel(const float* part, int splits, int64_t M, int N, const LinEpi e) {
+  const int ncol = (N + 7) / 8;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t m = id / ncol;
+  const int col = (int)(id - m * ncol) * 8;
+  if (m >= M) return;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int s = 0; s < splits; ++s) {
+    const float* const p = part + ((int64_t)s * M + m) * N + col;
+    if (col + 8 <= N) {
+      float f[8];
+      __builtin_memcpy(f, p, 32);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += f[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < N) v[i] += p[i];
+    }
+  }
+  lin_finish(e, m, col, N, v);
+}
+
+// Up to 16 NT rows of x: a block makes 16 columns (rows of W).  Its 16 waves share k in
+// units of 64, a wave's lane (r, g) taking k = 16 g + (0..15) of row r of W and of x (two
+// products of 32 k; both operands in the same order), so W is read once, in whole
+// 128-byte lines, with all of a wave's loads in flight; the waves' sums meet in LDS.
+// Addresses need no alignment; elements past K are zeros.
+constexpr int kSkinnyWaves = 16;
+
+// 16 elements at p of which the first n are there
+__device__ __forceinline__ void lin_get16(const uint16_t* p, int n, af3_u32x4 (&v)[2]) {
+  if (n >= 16) {
+    __builtin_memcpy(v, p, 32);
+  } else {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = 2 * i < n ? p[2 * i] : 0, hi = 2 * i + 1 < n ? p[2 * i + 1] : 0;
+      w[i] = lo | hi << 16;
+    }
+    __builtin_memcpy(v, w, 32);
+  }
+}
+
+template <int NT>
+__global__ __launch_bounds__(kSkinnyWaves * 64) void lin_skinny_kernel(const LinArgs a) {
+  __shared__ float lds[kSkinnyWaves][NT * 16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const uint16_t* const w = a.q + (int64_t)min(n0 + r, a.N - 1) * a.ldq;
+  const uint16_t* x[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) x[t] = a.p + (int64_t)min(t * 16 + r, a.M - 1) * a.ldp;
+  f32x4 acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int units = (a.K + 63) / 64;
+  for (int u = wave; u < units; u += kSkinnyWaves) {
+    const int k = u * 64 + g * 16;
+    af3_u32x4 wv[2], xv[NT][2];
+    lin_get16(w + k, a.K - k, wv);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) lin_get16(x[t] + k, a.K - k, xv[t]);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(af3_bf16x8, wv[i]),
+                                                         __builtin_bit_cast(af3_bf16x8, xv[t][i]), acc[t], 0, 0, 0);
+  }
+  // lane (c, g): row c of x, columns 4 g + (0..3)
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[wave][t * 16 + r][4 * g + i] = acc[t][i];
+  __syncthreads();
+  if (threadIdx.x >= NT * 256) return;
+  const int m = threadIdx.x >> 4, c = threadIdx.x & 15, col = n0 + c;
+  float f = 0.f;
+#pragma unroll
+  for (int v = 0; v < kSkinnyWaves; ++v) f += lds[v][m][c];
+  if (m >= a.M || col >= a.N) return;
+  const LinEpi& e = a.e;
+  const int64_t at = (int64_t)m * a.N + col;
+  if (e.bias) f += e.bias_f32 ? ((const float*)e.bias)[col] : af3_bf16_to_f32(((const uint16_t*)e.bias)[col]);
+  if (e.act) {
+    if (e.z) e.z[at] = (uint16_t)af3_f32_to_bf16(f);
+    f = lin_act(f, e.act);
+  }
+  if (e.res) f += af3_bf16_to_f32(e.res[(int64_t)m * e.ldr + col]);
+  e.y[at] = (uint16_t)af3_f32_to_bf16(f);
+}
+
+// dz = dy act'(z) in bf16 with rows of ldz elements (zeros past N), and the columns' sums
+// (of dz before rounding): a block takes 32 lanes x 8 columns by its share of the rows.
+constexpr int kDzRows = 8;  // rows a block takes at a time
+
+struct DzArgs {
+  const uint16_t* dy;
+  int64_t ldy;
+  const uint16_t* z;  // [M][N], or null
+  int act;
+  int64_t M;
+  int N;
+  uint16_t* dz;       // or null
+  int64_t ldz;
+  float* part;        // [gridDim.y][N], or null
+};
+
+__global__ __launch_bounds__(256) void lin_dz_kernel(const DzArgs a) {
+  __shared__ float lds[kDzRows][257];
+  const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int col = (blockIdx.x * 32 + c) * 8;
+  float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const int width = (int)min((int64_t)((a.N + 7) / 8 * 8), a.ldz);
+  for (int64_t m = (int64_t)blockIdx.y * kDzRows + w; m < a.M; m += (int64_t)gridDim.y * kDzRows) {
+    if (col >= a.N) break;
+    uint16_t d[8], zz[8];
+    const bool whole = col + 8 <= a.N;
+    if (whole) {
+      __builtin_memcpy(d, a.dy + m * a.ldy + col, 16);
+      if (a.act) __builtin_memcpy(zz, a.z + m * a.N + col, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        d[i] = col + i < a.N ? a.dy[m * a.ldy + col + i] : 0;
+        zz[i] = a.act && col + i < a.N ? a.z[m * a.N + col + i] : 0;
+      }
+    }
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] = af3_bf16_to_f32(d[i]);
+      if (a.act) f[i] = (whole || col + i < a.N) ? f[i] * lin_slope(af3_bf16_to_f32(zz[i]), a.act) : 0.f;
+      s[i] += f[i];
+    }
+    if (a.dz) {
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = af3_pack_bf16x2(f[2 * i], f[2 * i + 1]);
+      uint16_t* const p = a.dz + m * a.ldz + col;
+      if (col + 8 <= width) {
+        __builtin_memcpy(p, o, 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < width) p[i] = (uint16_t)(o[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lds[w][c * 8 + i] = s[i];
+  __syncthreads();
+  const int at = blockIdx.x * 256 + threadIdx.x;
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < kDzRows; ++i) t += lds[i][threadIdx.x];
+  if (at < a.N) a.part[(int64_t)blockIdx.y * a.N + at] = t;
+}
+
+__global__ __launch_bounds__(256) void lin_colsum_kernel(const float* part, int n, int N, void* out, int f32) {
+  __shared__ float lds[4][64];
+  const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int col = blockIdx.x * 64 + c;
+  float s = 0.f;
+  if (col < N)
+    for (int i = w; i < n; i += 4) s += part[(int64_t)i * N + col];
+  lds[w][c] = s;
+  __syncthreads();
+  if (w || col >= N) return;
+  s = ((s + lds[1][c]) + lds[2][c]) + lds[3][c];
+  if (f32)
+    ((float*)out)[col] = s;
+  else
+    ((uint16_t*)out)[col] = (uint16_t)af3_f32_to_bf16(s);
+}
+
+// tile shape and split of a product: what takes the fewest rounds of the CUs, in units of
+// one 256 x 256 tile's k-step
+struct LinPlan {
+  int bm, bn, splits, steps;
+};
+
+LinPlan lin_plan(int64_t M, int64_t N, int64_t K) {
+  static const struct {
+    int bm, bn, per_cu;
+    double cost;
+  } shapes[] = {{256, 256, 1, 1.0}, {256, 192, 1, 0.80}, {128, 128, 2, 0.62}};
+  const int64_t nk = af3_cdiv(K, 64);
+  LinPlan best = {0, 0, 1, (int)(nk > 0 ? nk : 1)};
+  double best_t = 1e300;
+  for (const auto& s : shapes) {
+    const int64_t tiles = af3_cdiv(M, s.bm) * af3_cdiv(N, s.bn);
+    for (int sp = 1; sp <= 16; sp *= 2) {
+      const int64_t steps = af3_cdiv(nk > 0 ? nk : 1, sp);
+      if (sp > 1 && (steps < 8 || tiles >= 512)) break;
+      const int64_t used = af3_cdiv(nk > 0 ? nk : 1, steps);
+      // a round: its k-steps, then about six of them for the start and the epilogue; joining
+      // reads and writes the partials (a 256 x 256 tile's k-step takes as long as 4 MB of HBM)
+      const double t = (double)af3_cdiv(tiles * used, 256 * s.per_cu) * ((double)steps + 6) * s.cost +
+                       (used > 1 ? (double)(used * 2 + 1) * M * N * 4 / 5e6 + 6 : 0);
+      if (t < best_t) best_t = t, best = {s.bm, s.bn, (int)used, (int)steps};
+    }
+  }
+  return best;
+}
+
+template <int BM, int BN>
+void lin_launch(const LinArgs& a, bool pt, bool qt, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.splits));
+  if (!pt && !qt)
+    hipLaunchKernelGGL((lin_kernel<BM, BN, false, false>), grid, dim3(256), 0, st, a);
+  else if (!pt)
+    hipLaunchKernelGGL((lin_kernel<BM, BN, false, true>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((lin_kernel<BM, BN, true, true>), grid, dim3(256), 0, st, a);
+}
+
+constexpr int kSkinnyRows = 32;
+bool lin_skinny(int64_t M, bool pt, bool qt) { return M <= kSkinnyRows && !pt && !qt; }
+
+}  // namespace
+
+extern "C" size_t af3_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int p_trans, int q_trans) {
+  if (M <= 0 || N <= 0 || K <= 0 || lin_skinny(M, p_trans, q_trans)) return 0;
+  const LinPlan p = lin_plan(M, N, K);
+  return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
+}
+
+extern "C" int af3_linear(const uint16_t* p, int64_t ldp, int p_trans, const uint16_t* q, int64_t ldq, int q_trans,
+                          int64_t M, int64_t N, int64_t K, const void* bias, int bias_f32, int act,
+                          const uint16_t* residual, int64_t ldr, uint16_t* y, uint16_t* z, void* workspace,
+                          size_t ws_bytes, void* stream_) {
+  AF3_REQUIRE(M >= 0 && N >= 0 && K >= 0 && M < (int64_t)1 << 30 && N < (int64_t)1 << 30 && K < (int64_t)1 << 30,
+              "linear: bad sizes");
+  AF3_REQUIRE(act >= kActNone && act <= kActGeluTanh, "linear: activation %d", act);
+  AF3_REQUIRE(!p_trans || q_trans, "linear: p_trans needs q_trans");
+  if (M == 0 || N == 0) return 0;
+  AF3_REQUIRE(K > 0, "linear: an empty sum");
+  AF3_REQUIRE(p && q && y, "linear: null pointer");
+  AF3_REQUIRE(M * N < (int64_t)1 << 40, "linear: output too large");
+  hipStream_t st = (hipStream_t)stream_;
+  LinArgs a = {};
+  a.p = p, a.ldp = ldp, a.q = q, a.ldq = ldq, a.M = (int)M, a.N = (int)N, a.K = (int)K;
+  a.e.bias = bias, a.e.bias_f32 = bias_f32, a.e.act = act, a.e.res = residual, a.e.ldr = ldr, a.e.y = y, a.e.z = z;
+  if (lin_skinny(M, p_trans, q_trans)) {
+    const dim3 grid((unsigned)af3_cdiv(N, 16)), block(kSkinnyWaves * 64);
+    if (M <= 16)
+      hipLaunchKernelGGL((lin_skinny_kernel<1>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((lin_skinny_kernel<2>), grid, block, 0, st, a);
+    return af3::check_launch("linear");
+  }
+  AF3_REQUIRE(((uintptr_t)p & 15) == 0 && ((uintptr_t)q & 15) == 0 && ldp % 8 == 0 && ldq % 8 == 0,
+              "linear: rows must be 16-byte aligned");
+  AF3_REQUIRE(ldp >= af3_cdiv(p_trans ? M : K, 8) * 8 && ldq >= af3_cdiv(q_trans ? N : K, 8) * 8,
+              "linear: rows must reach the next multiple of 8 elements");
+  AF3_REQUIRE(ldp < (int64_t)1 << 22 && ldq < (int64_t)1 << 22, "linear: rows too far apart");
+  const LinPlan pl = lin_plan(M, N, K);
+  a.tiles_m = (int)af3_cdiv(M, pl.bm), a.tiles_n = (int)af3_cdiv(N, pl.bn), a.group_m = 4;
+  AF3_REQUIRE((int64_t)a.tiles_m * a.tiles_n * pl.splits < (int64_t)1 << 30, "linear: output too large");
+  a.splits = pl.splits, a.steps_per_split = pl.steps;
+  if (pl.splits > 1) {
+    AF3_REQUIRE(workspace && ws_bytes >= (size_t)pl.splits * M * N * 4, "linear: workspace too small");
+    a.part = (float*)workspace;
+  }
+  if (pl.bm == 256 && pl.bn == 256)
+    lin_launch<256, 256>(a, p_trans, q_trans, st);
+  else if (pl.bm == 256)
+    lin_launch<256, 192>(a, p_trans, q_trans, st);
+  else
+    lin_launch<128, 128>(a, p_trans, q_trans, st);
+  if (pl.splits > 1) {
+    const int64_t n = M * af3_cdiv(N, 8);
+    hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)af3_cdiv(n, 256)), dim3(256), 0, st, a.part, pl.splits, M, (int)N,
+                       a.e);
+  }
+  return af3::check_launch("linear");
+}
+
+namespace {
+int lin_dz_blocks(int64_t M, int64_t N) {
+  const int64_t cols = af3_cdiv(N, 256), rows = af3_cdiv(M, kDzRows);
+  const int64_t want = af3_cdiv(1024, cols);  // four blocks per CU
+  const int64_t b = want < rows ? want : rows;
+  return (int)(b < 1 ? 1 : b);
+}
+}  // namespace
+
+extern "C" size_t af3_linear_dz_workspace_bytes(int64_t M, int64_t N) {
+  return M > 0 && N > 0 ? (size_t)lin_dz_blocks(M, N) * N * 4 : 0;
+}
+
+extern "C" int af3_linear_dz(const uint16_t* dy, int64_t ldy, const uint16_t* z, int act, int64_t M, int64_t N,
+                             uint16_t* dz, int64_t ldz, void* dbias, int bias_f32, void* workspace, size_t ws_bytes,
+                             void* stream_) {
+  AF3_REQUIRE(M >= 0 && N >= 0 && N < (int64_t)1 << 30 && M < (int64_t)1 << 40, "linear_dz: bad sizes");
+  AF3_REQUIRE(act >= kActNone && act <= kActGeluTanh, "linear_dz: activation %d", act);
+  if (M == 0 || N == 0) return 0;
+  AF3_REQUIRE(dy && (!act || z) && (dz || dbias), "linear_dz: null pointer");
+  AF3_REQUIRE(!dz || ldz >= N, "linear_dz: bad leading dimension");
+  const int blocks = lin_dz_blocks(M, N);
+  AF3_REQUIRE(!dbias || (workspace && ws_bytes >= (size_t)blocks * N * 4), "linear_dz: workspace too small");
+  DzArgs a = {dy, ldy, z, act, M, (int)N, dz, dz ? ldz : N, dbias ? (float*)workspace : nullptr};
+  hipStream_t st = (hipStream_t)stream_;
+  hipLaunchKernelGGL(lin_dz_kernel, dim3((unsigned)af3_cdiv(N, 256), (unsigned)blocks), dim3(256), 0, st, a);
+  if (dbias)
+    hipLaunchKernelGGL(lin_colsum_kernel, dim3((unsigned)af3_cdiv(N, 64)), dim3(256), 0, st, a.part, blocks, (int)N,
+                       dbias, bias_f32);
+  return af3::check_launch("linear_dz");
+}

@@ -519,6 +519,27 @@ int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* dh, int64_t 
                           int H, void* dx, void* dresidual, void* dweight, void* dpost, void* dgate, void* workspace,
                           size_t ws_bytes, void* stream);
 
+/* Matrix products with an epilogue (the reference's projections are library calls).
+ *   s[m][n] = sum over k < K of p[m][k] q[n][k] + bias[n],  y = act(s) + residual
+ * in fp32, rounded to bf16 once; y [M][N], z [M][N] (NULL: not) receives s where there
+ * is an activation: act 0 none, 1 relu, 2 silu, 3 gelu (error function), 4 gelu by tanh.
+ * p is stored [M][ldp], or with p_trans [K][ldp]; q [N][ldq], or with q_trans
+ * [K][ldq] (p_trans needs q_trans).  Up to 32 rows without transposition any address
+ * serves; else rows lie at 16-byte aligned addresses (ld a multiple of 8 below 2^22)
+ * and reach the next multiple of 8 elements, which are zeros where k is the
+ * contiguous index (any finite or other value where it is not).  bias bf16, or fp32
+ * with bias_f32 (NULL: none); residual [M][ldr] (NULL: none).  The workspace holds
+ * the partial sums of products whose k is split over blocks (0: none needed).
+ * af3_linear_dz: dz [M][ldz] = dy act'(z) (zeros from N to the next multiple of 8
+ * within ldz; NULL: not written) and dbias [N] = its column sums (NULL: not). */
+size_t af3_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int p_trans, int q_trans);
+int af3_linear(const uint16_t* p, int64_t ldp, int p_trans, const uint16_t* q, int64_t ldq, int q_trans, int64_t M,
+               int64_t N, int64_t K, const void* bias, int bias_f32, int act, const uint16_t* residual, int64_t ldr,
+               uint16_t* y, uint16_t* z, void* workspace, size_t ws_bytes, void* stream);
+size_t af3_linear_dz_workspace_bytes(int64_t M, int64_t N);
+int af3_linear_dz(const uint16_t* dy, int64_t ldy, const uint16_t* z, int act, int64_t M, int64_t N, uint16_t* dz,
+                  int64_t ldz, void* dbias, int bias_f32, void* workspace, size_t ws_bytes, void* stream);
+
 /* The norm of n tensors taken as one vector, and their scaling by min(1, max_norm /
  * (norm + 1e-6)).  ptrs, sizes (elements, above 0) and is_f32 (else bf16) are host
  * arrays, read before the call returns; the tensors are contiguous on the
