@@ -10,24 +10,34 @@
 // contiguous (W of dx; dz and x of dW), so nothing is transposed in memory.
 //
 // lin_kernel: a block of 4 waves (2 x 2) makes BM x BN of the output in 64-deep
-// k-steps.  Both operands of a k-step go global -> LDS (16-byte copies) into one of two
-// stages while the other is used; a wave's BM/2 x BN/2 part is TM x TN products
+// k-steps.  Both operands of a k-step go global -> LDS (16-byte copies) into one of ST
+// stages while another is used; a wave's BM/2 x BN/2 part is TM x TN products
 // v_mfma_f32_32x32x16_bf16.  With 128 x 128 per wave a fragment read from LDS is used
 // four times: 64 bytes per clock and CU where the copies take another 32, under what
 // the LDS gives (147; 111 for transposing reads); with 128 x 64 (eight waves) both would
 // saturate it.  One wave per SIMD hides nothing by itself, so the loop is a fixed
 // schedule: fragments of the next 16 k are read between the products of this one, one
 // instruction per product, the k-step's last products run after the next barrier, and
-// the next stage's copies are issued in the first quarter of a step.
+// a later stage's copies are issued in the first half of a step (all of them in the first
+// quarter, or spread over the whole, 3% slower).
 // Fragments: lane (r, h) = (lane % 32, lane / 32) feeds row r, k = 16 s + 8 h + (0..7) of
 // sub-step s.  k contiguous: one 16-byte read.  Else two transposing reads of 4 k each.
 // LDS chunks of 16 bytes are XOR-swizzled so that either reads without bank conflicts.
 // Q is the matrix unit's first operand, so a lane ends up with rows of the output, 4
 // consecutive columns at a time; the epilogue turns them through LDS (32 rows of a wave
-// at a time, fp32) into 16-byte accesses and rounds once.
+// at a time, fp32) into 16-byte accesses and rounds once.  Blocks stay for several tiles:
+// the next one's first copies are issued before the last k-step of this, and this one's
+// stores drain under the next's first.
 //
-// Few tiles and a long k (dW): blocks share a tile's k-steps and write fp32 partials,
-// which lin_join_kernel adds in order and gives the epilogue.
+// Measured (library product of the same operands in brackets), us: 8192 x 4096 from 2880
+// 155 (134), 8192 x 2880 from 4096 with W as stored 159 (190), 16384 x 2880 from 4096 313
+// (271), 16384 x 4096 from 2880 with W as stored 300 (299), 2880 x 4096 from 16384 rows
+// 331 (431); 1021 x 2880 from 2880 22.6 (24.5), 8192 x 512 from 2880 26 (27).  The large
+// ones run 1.17 to 1.29 PFLOP/s at 1.75 GHz: 73% of the CUs' busy cycles issue products, and
+// taking out the copies, or the fragment reads, gains 4 and 14%; the card's power bounds them.
+//
+// Few tiles and a long k (dW of narrow layers): blocks share a tile's k-steps and write
+// fp32 partials, which lin_join_kernel adds in order and gives the epilogue.
 // Up to 32 rows: lin_skinny_kernel streams W once through registers.
 #include "af3_common.h"
 
@@ -83,27 +93,32 @@ __device__ __forceinline__ float lin_slope(float z, int act) {
   return 1.f;
 }
 
+// the bias of 8 columns from `col` (col + 8 <= N)
+__device__ __forceinline__ void lin_bias(const LinEpi& e, int col, float (&v)[8]) {
+  if (!e.bias) return;
+  if (e.bias_f32) {
+    float b[8];
+    __builtin_memcpy(b, (const float*)e.bias + col, 32);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += b[i];
+  } else {
+    uint32_t b[4];
+    __builtin_memcpy(b, (const uint16_t*)e.bias + col, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] += af3_bf16_to_f32(b[i]);
+      v[2 * i + 1] += af3_bf16_to_f32(b[i] >> 16);
+    }
+  }
+}
+
 // 8 columns from `col` of row m: sums -> output (columns past N are left out)
+template <bool ACT>
 __device__ __forceinline__ void lin_finish(const LinEpi& e, int64_t m, int col, int N, float (&v)[8]) {
   const int64_t at = m * N + col;
   if (col + 8 <= N) {
-    if (e.bias) {
-      if (e.bias_f32) {
-        float b[8];
-        __builtin_memcpy(b, (const float*)e.bias + col, 32);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += b[i];
-      } else {
-        uint32_t b[4];
-        __builtin_memcpy(b, (const uint16_t*)e.bias + col, 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] += af3_bf16_to_f32(b[i]);
-          v[2 * i + 1] += af3_bf16_to_f32(b[i] >> 16);
-        }
-      }
-    }
-    if (e.act) {
+    lin_bias(e, col, v);
+    if (ACT) {
       if (e.z) {
         uint32_t w[4];
 #pragma unroll
@@ -133,7 +148,7 @@ __device__ __forceinline__ void lin_finish(const LinEpi& e, int64_t m, int col, 
         float f = v[i];
         if (e.bias)
           f += e.bias_f32 ? ((const float*)e.bias)[col + i] : af3_bf16_to_f32(((const uint16_t*)e.bias)[col + i]);
-        if (e.act) {
+        if (ACT) {
           if (e.z) e.z[at + i] = (uint16_t)af3_f32_to_bf16(f);
           f = lin_act(f, e.act);
         }
@@ -147,6 +162,17 @@ __device__ __forceinline__ void lin_dma16(const void* sbase, uint32_t voff, uint
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_byte_addr) : "memory");
 }
 
+// an address that is the same in all lanes, in scalar registers
+__device__ __forceinline__ const uint16_t* lin_uniform(const uint16_t* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  return (const uint16_t*)(uintptr_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
+                                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32);
+}
+
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
 template <bool V>
 struct Flag {
   static constexpr bool value = V;
@@ -176,9 +202,26 @@ struct LinTile {
   }
 };
 
+// a wave's copies of a k-step of which the first `left` k are there: zeros past them
+template <class TT, bool T>
+__device__ __forceinline__ void lin_copy_tail(int wave, int lane, int left, int edge, const uint16_t* src, int64_t ld,
+                                              uint32_t lds_byte_addr) {
+#pragma unroll 1
+  for (int j = 0; j < TT::kCopies; ++j) {
+    int row, ch;
+    TT::place(wave * TT::kCopies + j, lane, row, ch);
+    const bool live = T ? row < left : ch * 8 < left;
+    if (T) ch = min(ch, (edge + 7) / 8 - 1);
+    else row = min(row, edge - 1);
+    af3_u32x4 v = {0, 0, 0, 0};
+    if (live) v = *(const af3_u32x4*)(src + row * ld + ch * 8);
+    *(__attribute__((address_space(3))) af3_u32x4*)(uintptr_t)(lds_byte_addr + j * 1024 + lane * 16) = v;
+  }
+}
+
 // BM x BN tile, see above.  MASKED outputs past M, N are not stored; loads there repeat the last row.
-template <int BM, int BN, bool PT, bool QT>
-__global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void lin_kernel(const LinArgs a) {
+template <int BM, int BN, int ST, bool PT, bool QT>
+__global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void lin_kernel(const LinArgs a) {
   using TP = LinTile<BM, PT>;
   using TQ = LinTile<BN, QT>;
   constexpr int TM = BM / 64, TN = BN / 64;
@@ -186,82 +229,73 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void lin_kernel(
   constexpr int NC = TP::kCopies + TQ::kCopies;
   constexpr int NS = TM * TN;      // products per sub-step
   constexpr int NF = TM + TN;      // fragments per sub-step
-  constexpr int EPI = 32 * (BN / 2 * 4 + 16);  // bytes per wave of the epilogue's turn
-  static_assert(4 * EPI <= 2 * STAGE, "epilogue fits the ring");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+  constexpr int EPI = 32 * (BN / 2 * 4);  // bytes per wave of the epilogue's turn
+  static_assert(4 * EPI <= STAGE, "the epilogue fits a stage");
+  constexpr int STORES = 32 * (BN / 2) / 8 / 64 * TM;  // of a wave in a plain epilogue
+  static_assert(NC * (ST - 2) + STORES < 64, "vmcnt counts to 63");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[ST * STAGE];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, lh = lane >> 5;
 
-  // work item: blocks go round robin over 8 XCDs; each XCD takes a run of the tiles, in
-  // groups of group_m tile rows so that the ones in flight share operands in its L2
+  // work items: blocks go round robin over 8 XCDs; each XCD takes a run of the tiles, in
+  // groups of group_m tile rows so that the ones in flight share operands in its L2, and
+  // its blocks walk that run side by side
   const int tiles = a.tiles_m * a.tiles_n;
   const int total = tiles * a.splits;
-  int item = blockIdx.x;
-  {
-    const int xcd = item & 7, at = item >> 3;
-    const int per = total >> 3, rest = total & 7;
-    item = xcd * per + min(xcd, rest) + at;
-  }
-  const int split = item / tiles;
-  const int tile = item - split * tiles;
-  const int gsz = a.group_m * a.tiles_n;
-  const int grp = tile / gsz, in = tile - grp * gsz;
-  const int gm = min(a.group_m, a.tiles_m - grp * a.group_m);
-  const int m0 = (grp * a.group_m + in % gm) * BM, n0 = in / gm * BN;
+  const int xcd = blockIdx.x & 7, stride = ((int)gridDim.x - xcd + 7) >> 3;
+  const int items_end = (xcd + 1) * (total >> 3) + min(xcd + 1, total & 7);
+  int item = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
+  if (item >= items_end) return;
   const int wm0 = (wave >> 1) * (BM / 2), wn0 = (wave & 1) * (BN / 2);
-
   const int nk_all = (a.K + 63) / 64;
-  const int k_first = split * a.steps_per_split;
-  const int nk = min(a.steps_per_split, nk_all - k_first);
-  const bool tail = k_first + nk == nk_all && (a.K & 63);  // the last k-step is not whole
 
-  // this lane's source of each copy: byte offsets from the k-step's base
-  const uint16_t* pbase = PT ? a.p + (int64_t)k_first * 64 * a.ldp + m0 : a.p + (int64_t)m0 * a.ldp + k_first * 64;
-  const uint16_t* qbase = QT ? a.q + (int64_t)k_first * 64 * a.ldq + n0 : a.q + (int64_t)n0 * a.ldq + k_first * 64;
+  // the item whose copies are issued next
+  int split, m0, n0, nk;
+  bool tail;                 // its last k-step is not whole
+  const uint16_t *pk, *qk;   // of the next k-step to copy
+  uint32_t off[NC];          // this lane's source of each copy: byte offsets from there
   const int64_t pstep = PT ? 64 * a.ldp : 64, qstep = QT ? 64 * a.ldq : 64;
-  uint32_t off[NC];
+  auto setup = [&]() {
+    // (divisions run on the vector unit: their results go back to scalar registers)
+    split = __builtin_amdgcn_readfirstlane(item / tiles);
+    const int tile = item - split * tiles;
+    const int gsz = a.group_m * a.tiles_n;
+    const int grp = __builtin_amdgcn_readfirstlane(tile / gsz), in = tile - grp * gsz;
+    const int gm = min(a.group_m, a.tiles_m - grp * a.group_m);
+    const int tn = __builtin_amdgcn_readfirstlane(in / gm);
+    m0 = (grp * a.group_m + in - tn * gm) * BM, n0 = tn * BN;
+    const int k_first = split * a.steps_per_split;
+    nk = __builtin_amdgcn_readfirstlane(min(a.steps_per_split, nk_all - k_first));
+    tail = k_first + nk == nk_all && (a.K & 63);
+    pk = lin_uniform(PT ? a.p + (int64_t)k_first * 64 * a.ldp + m0 : a.p + (int64_t)m0 * a.ldp + k_first * 64);
+    qk = lin_uniform(QT ? a.q + (int64_t)k_first * 64 * a.ldq + n0 : a.q + (int64_t)n0 * a.ldq + k_first * 64);
 #pragma unroll
-  for (int j = 0; j < TP::kCopies; ++j) {
-    int row, ch;
-    TP::place(wave * TP::kCopies + j, lane, row, ch);
-    off[j] = PT ? (uint32_t)(row * a.ldp * 2 + min(ch, (a.M - m0 + 7) / 8 - 1) * 16)
-                : (uint32_t)(min(row, a.M - m0 - 1) * a.ldp * 2 + ch * 16);
-  }
+    for (int j = 0; j < TP::kCopies; ++j) {
+      int row, ch;
+      TP::place(wave * TP::kCopies + j, lane, row, ch);
+      off[j] = PT ? (uint32_t)(row * a.ldp * 2 + min(ch, (a.M - m0 + 7) / 8 - 1) * 16)
+                  : (uint32_t)(min(row, a.M - m0 - 1) * a.ldp * 2 + ch * 16);
+    }
 #pragma unroll
-  for (int j = 0; j < TQ::kCopies; ++j) {
-    int row, ch;
-    TQ::place(wave * TQ::kCopies + j, lane, row, ch);
-    off[TP::kCopies + j] = QT ? (uint32_t)(row * a.ldq * 2 + min(ch, (a.N - n0 + 7) / 8 - 1) * 16)
-                              : (uint32_t)(min(row, a.N - n0 - 1) * a.ldq * 2 + ch * 16);
-  }
+    for (int j = 0; j < TQ::kCopies; ++j) {
+      int row, ch;
+      TQ::place(wave * TQ::kCopies + j, lane, row, ch);
+      off[TP::kCopies + j] = QT ? (uint32_t)(row * a.ldq * 2 + min(ch, (a.N - n0 + 7) / 8 - 1) * 16)
+                                : (uint32_t)(min(row, a.N - n0 - 1) * a.ldq * 2 + ch * 16);
+    }
+  };
   const uint32_t lds0 =
       __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
   auto lds_at = [&](int j, int stage) {
     return lds0 + (uint32_t)(stage * STAGE + (j < TP::kCopies ? (wave * TP::kCopies + j) * 1024
                                                               : TP::kBytes + (wave * TQ::kCopies + j - TP::kCopies) * 1024));
   };
-  const uint16_t *pk = pbase, *qk = qbase;  // of the next k-step to copy
   auto copy = [&](int j, int stage) { lin_dma16(j < TP::kCopies ? pk : qk, off[j], lds_at(j, stage)); };
   // the last k-step where K is not a multiple of 64: chunks past K are zeros
   auto copy_tail = [&](int stage) {
-    const int left = a.K & 63;
-#pragma unroll 1
-    for (int j = 0; j < NC; ++j) {
-      int row, ch;
-      const bool isp = j < TP::kCopies;
-      if (isp) TP::place(wave * TP::kCopies + j, lane, row, ch);
-      else TQ::place(wave * TQ::kCopies + j - TP::kCopies, lane, row, ch);
-      const bool trans = isp ? PT : QT;
-      const int64_t ld = isp ? a.ldp : a.ldq;
-      const int edge = isp ? a.M - m0 : a.N - n0;
-      const bool live = trans ? row < left : ch * 8 < left;
-      if (trans) ch = min(ch, (edge + 7) / 8 - 1);
-      else row = min(row, edge - 1);
-      af3_u32x4 v = {0, 0, 0, 0};
-      if (live) v = *(const af3_u32x4*)((isp ? pk : qk) + row * ld + ch * 8);
-      *(__attribute__((address_space(3))) af3_u32x4*)(uintptr_t)(lds_at(j, stage) + lane * 16) = v;
-    }
+    lin_copy_tail<TP, PT>(wave, lane, a.K & 63, a.M - m0, pk, a.ldp, lds_at(0, stage));
+    lin_copy_tail<TQ, QT>(wave, lane, a.K & 63, a.N - n0, qk, a.ldq, lds_at(TP::kCopies, stage));
   };
 
   // this lane's fragment addresses in stage 0
@@ -298,23 +332,13 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void lin_kernel(
   };
 
   af3_f32x16 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   af3_bf16x8 fp[2][TM], fq[2][TN];
-
-#pragma unroll
-  for (int i = 0; i < TM; ++i) fp[1][i] = af3_bf16x8{};
-#pragma unroll
-  for (int i = 0; i < TN; ++i) fq[1][i] = af3_bf16x8{};
 
   // products of fragments c, between them the reads of sub-step s into c ^ 1 and, with
   // COPY, the next stage's copies
-  auto phase = [&](auto copy_, int c, int s, uint32_t stage, int to) {
-    constexpr bool COPY = decltype(copy_)::value;
+  auto phase = [&](auto copy_, auto c_, auto s_, uint32_t stage, int to) {
+    constexpr int c = decltype(c_)::value, s = decltype(s_)::value;
+    constexpr bool COPY = decltype(copy_)::value && s >= 0 && s < 2;
 #pragma unroll
     for (int i = 0; i < (NS > NF ? NS : NF); ++i) {
       if (i < NS)
@@ -325,90 +349,183 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void lin_kernel(
         else fp[c ^ 1][i - TN] = frag_p(s, i - TN, stage);
       }
       if constexpr (COPY) {
-        constexpr int PER = (NC + NS - 1) / NS;
+        constexpr int NP = 2;
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (i * PER + j < NC) copy(i * PER + j, to);
+        for (int j = 0; j < NC; ++j)
+          if (j * (NP * NS) / NC == s * NS + i) copy(j, to);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  auto ahead = [](int stage, int n) { return stage + n >= ST ? stage + n - ST : stage + n; };
   auto step = [&](auto copy_, int cur) {
     const uint32_t stage = (uint32_t)(cur * STAGE);
-    phase(copy_, 1, 0, stage, cur ^ 1);  // (the last step's last products; of zeros in the first)
-    phase(Flag<false>{}, 0, 1, stage, 0);
-    phase(Flag<false>{}, 1, 2, stage, 0);
-    phase(Flag<false>{}, 0, 3, stage, 0);
+    const int to = ahead(cur, ST - 1);
+    phase(copy_, Int<1>{}, Int<0>{}, stage, to);  // (the last step's last products; of zeros in the first)
+    phase(copy_, Int<0>{}, Int<1>{}, stage, to);
+    phase(copy_, Int<1>{}, Int<2>{}, stage, to);
+    phase(copy_, Int<0>{}, Int<3>{}, stage, to);
   };
-  // a k-step's copies have landed, and every wave has read the other stage
-#define LIN_NEXT() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+  // a k-step's copies have landed (all but the n youngest accesses), and every wave has
+  // read the stage before it
+#define LIN_WAIT(n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(n) : "memory")
 
-  if (nk > 0) {
+  // an item's first k-steps, up to ST - 1 of them; pk and qk are left at the next one
+  auto first_copies = [&](int stage) {
     const int whole = nk - (tail ? 1 : 0);
     if (whole == 0) {
-      copy_tail(0);
-    } else {
+      copy_tail(stage);
+      return;
+    }
 #pragma unroll
-      for (int j = 0; j < NC; ++j) copy(j, 0);
-    }
-    int kt = 0;
-    for (; kt < whole - 1; ++kt) {
-      LIN_NEXT();
-      pk += pstep, qk += qstep;
-      step(Flag<true>{}, kt & 1);
-    }
-    for (; kt < nk; ++kt) {  // the last whole step, and the one that is not
-      LIN_NEXT();
-      pk += pstep, qk += qstep;
-      if (kt + 1 < nk) copy_tail((kt & 1) ^ 1);
-      step(Flag<false>{}, kt & 1);
-    }
-    phase(Flag<false>{}, 1, -1, 0, 0);
-  }
+    for (int s = 0; s < ST - 1; ++s)
+      if (s < whole) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) copy(j, ahead(stage, s));
+        pk += pstep, qk += qstep;
+      }
+  };
 
-  // epilogue: lane (r, h) holds row r of a 32 x 32 part, columns 8 j + 4 h + (0..3)
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  constexpr int W = BN / 2;             // columns of a wave
-  constexpr int ROWB = W * 4 + 16;      // bytes of a staged row
-  constexpr int LPR = W / 8;            // lanes per row when read back
-  const uint32_t es = lds0 + wave * EPI;
+  setup();
+  int cur = 0;   // stage of the next k-step
+  first_copies(cur);
+  bool stores = false;  // this wave's accesses since its first copies are STORES stores or more
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fp[1][i] = af3_bf16x8{};
+#pragma unroll
+    for (int i = 0; i < TN; ++i) fq[1][i] = af3_bf16x8{};
+
+    // (the last item's stores may still be under way: they are younger than the copies)
+    const int whole = nk - (tail ? 1 : 0);
+    if (ST > 2 && whole < ST - 1) LIN_WAIT(0);
+    else if (stores) LIN_WAIT(NC * (ST - 2) + STORES);
+    else LIN_WAIT(NC * (ST - 2));
+    int left = whole - (ST - 1);  // k-steps that bring a whole one
+    if (left > 0) {
+      for (;;) {
+        step(Flag<true>{}, cur);
+        pk += pstep, qk += qstep;
+        cur = ahead(cur, 1);
+        LIN_WAIT(NC * (ST - 2));
+        if (--left == 0) break;
+      }
+    }
+    if (ST > 2 || (tail && nk > 1)) {
+      for (left = min(ST - 1, whole) + (tail ? 1 : 0) - 1; left > 0; --left) {
+        if (tail && left == 1) copy_tail(ahead(cur, 1));
+        step(Flag<false>{}, cur);
+        cur = ahead(cur, 1);
+        LIN_WAIT(0);
+      }
+    }
+    // the last k-step, and the next item's first copies
+    const int em0 = m0 + wm0, en0 = n0 + wn0, es_split = split;
+    const bool plain = !a.part && !a.e.act && m0 + BM <= a.M && n0 + BN <= a.N;
+    item += stride;
+    const bool more = item < items_end;
+    if (more) {
+      setup();
+      first_copies(ahead(cur, 1));
+    }
+    step(Flag<false>{}, cur);
+    phase(Flag<false>{}, Int<1>{}, Int<-1>{}, 0, 0);
+
+    // epilogue, in the last k-step's stage: lane (r, h) holds row r of a 32 x 32 part,
+    // columns 8 j + 4 h + (0..3)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    constexpr int W = BN / 2;        // columns of a wave
+    constexpr int ROWB = W * 4;      // bytes of a staged row; 16-byte chunks XORed with the row's low bits
+    constexpr int LPR = W / 8;       // lanes per row when read back
+    constexpr int IT = 32 * LPR / 64, U = IT % 4 == 0 ? 4 : 3;
+    const uint32_t es = lds0 + (uint32_t)(cur * STAGE + wave * EPI);
+    auto staged = [&](int row, int chunk) { return es + (uint32_t)(row * ROWB + ((chunk ^ (row & 7)) << 4)); };
 #pragma unroll 1
   for (int tm = 0; tm < TM; ++tm) {  // (acc[0] is the tile's rows tm; one copy of the code)
 #pragma unroll
     for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *(__attribute__((address_space(3))) f32x4*)(uintptr_t)(es + lr * ROWB + (tn * 32 + 8 * j + 4 * lh) * 4) =
+        *(__attribute__((address_space(3))) f32x4*)(uintptr_t)staged(lr, tn * 8 + 2 * j + lh) =
             f32x4{acc[0][tn][4 * j], acc[0][tn][4 * j + 1], acc[0][tn][4 * j + 2], acc[0][tn][4 * j + 3]};
 #pragma unroll
     for (int i = 0; i + 1 < TM; ++i)
 #pragma unroll
       for (int tn = 0; tn < TN; ++tn) acc[i][tn] = acc[i + 1][tn];
     // (a wave's own LDS writes and reads are in order; the compiler keeps them so)
-#pragma unroll 1
-    for (int id = lane; id < 32 * LPR; id += 64) {
+    auto out = [&](auto act_, int id) {
       const int row = id / LPR, c8 = id % LPR * 8;
-      const int64_t m = m0 + wm0 + tm * 32 + row;
-      const int col = n0 + wn0 + c8;
-      const uint32_t at = es + row * ROWB + c8 * 4;
-      const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)at;
-      const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)(at + 16);
-      if (m >= a.M || col >= a.N) continue;
+      const int64_t m = em0 + tm * 32 + row;
+      const int col = en0 + c8;
+      const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
+      const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
+      if (m >= a.M || col >= a.N) return;
       float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       if (a.part) {
-        float* const out = a.part + ((int64_t)split * a.M + m) * a.N + col;
+        float* const o = a.part + ((int64_t)es_split * a.M + m) * a.N + col;
         if (col + 8 <= a.N) {
-          __builtin_memcpy(out, v, 32);
+          __builtin_memcpy(o, v, 32);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (col + i < a.N) out[i] = v[i];
+            if (col + i < a.N) o[i] = v[i];
         }
       } else {
-        lin_finish(a.e, m, col, a.N, v);
+        lin_finish<decltype(act_)::value>(a.e, m, col, a.N, v);
       }
+    };
+    // (a whole tile without activation or partials, the common one, has its accesses side by side)
+    if (plain) {
+#pragma unroll 1
+      for (int g = 0; g < IT; g += U) {
+        float v[U][8];
+        uint32_t r[U][4];
+        int64_t m[U];
+        int col[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int id = (g + u) * 64 + lane;
+          const int row = id / LPR, c8 = id % LPR * 8;
+          m[u] = em0 + tm * 32 + row, col[u] = en0 + c8;
+          if (a.e.res) __builtin_memcpy(r[u], a.e.res + m[u] * a.e.ldr + col[u], 16);
+          const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
+          const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[u][i] = x[i], v[u][4 + i] = y[i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          lin_bias(a.e, col[u], v[u]);
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (a.e.res) {
+              v[u][2 * i] += af3_bf16_to_f32(r[u][i]);
+              v[u][2 * i + 1] += af3_bf16_to_f32(r[u][i] >> 16);
+            }
+            w[i] = af3_pack_bf16x2(v[u][2 * i], v[u][2 * i + 1]);
+          }
+          __builtin_memcpy(a.e.y + m[u] * a.N + col[u], w, 16);
+        }
+      }
+    } else if (a.e.act && !a.part) {
+#pragma unroll 1
+      for (int i = 0; i < IT; ++i) out(Flag<true>{}, i * 64 + lane);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < IT; ++i) out(Flag<false>{}, i * 64 + lane);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before the next 32 rows overwrite)
+  }
+    if (!more) break;
+    stores = plain;
+    cur = ahead(cur, 1);
   }
 }
 
@@ -433,7 +550,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* part, int sp
         if (col + i < N) v[i] += p[i];
     }
   }
-  lin_finish(e, m, col, N, v);
+  if (e.act)
+    lin_finish<true>(e, m, col, N, v);
+  else
+    lin_finish<false>(e, m, col, N, v);
 }
 
 // Up to 16 NT rows of x: a block makes 16 columns (rows of W).  Its 16 waves share k in
@@ -593,45 +713,57 @@ __global__ __launch_bounds__(256) void lin_colsum_kernel(const float* part, int 
     ((uint16_t*)out)[col] = (uint16_t)af3_f32_to_bf16(s);
 }
 
-// tile shape and split of a product: what takes the fewest rounds of the CUs, in units of
-// one 256 x 256 tile's k-step
+// Tile shape, ring depth and split of a product: what should take the least time, in us:
+// k-steps of the tile's measured time, what its start and end leave uncovered, and for a
+// split sum the joining launch and its read of the partials.  The card's power bounds full
+// rounds (the clock falls to 1.75 GHz), so a round of fewer tiles takes their share of a
+// full round's time, down to what one tile alone takes at the full clock.  Per k-step in a
+// full round, alone, and per tile: 256 x 256 1.70, 1.20 and 7; 256 x 192 1.27, 0.90 and 6;
+// 128 x 128 two to a CU (two stages each) 0.97, 0.70 and 2.7; one to a CU 0.50, 0.43 and
+// 2.7 (four stages: three k-steps under way, where two stages leave 0.73, a copy's latency).
+// 2880 x 4096 from 16384 rows: 192 tiles of 256 x 256 315 us, split in four 375.
 struct LinPlan {
-  int bm, bn, splits, steps;
+  int bm, bn, stages, splits, steps;
 };
 
 LinPlan lin_plan(int64_t M, int64_t N, int64_t K) {
   static const struct {
-    int bm, bn, per_cu;
-    double cost;
-  } shapes[] = {{256, 256, 1, 1.0}, {256, 192, 1, 0.80}, {128, 128, 2, 0.62}};
+    int bm, bn, stages, slots;  // slots: tiles that run at a time
+    double step, alone, ends;
+  } shapes[] = {{256, 256, 2, 256, 1.70, 1.20, 7.0},
+                {256, 192, 2, 256, 1.27, 0.90, 6.0},
+                {128, 128, 2, 512, 0.97, 0.70, 2.7},
+                {128, 128, 4, 256, 0.50, 0.43, 2.7}};
   const int64_t nk = af3_cdiv(K, 64);
-  LinPlan best = {0, 0, 1, (int)(nk > 0 ? nk : 1)};
+  LinPlan best = {};
   double best_t = 1e300;
   for (const auto& s : shapes) {
     const int64_t tiles = af3_cdiv(M, s.bm) * af3_cdiv(N, s.bn);
-    for (int sp = 1; sp <= 16; sp *= 2) {
-      const int64_t steps = af3_cdiv(nk > 0 ? nk : 1, sp);
-      if (sp > 1 && (steps < 8 || tiles >= 512)) break;
-      const int64_t used = af3_cdiv(nk > 0 ? nk : 1, steps);
-      // a round: its k-steps, then about six of them for the start and the epilogue; joining
-      // reads and writes the partials (a 256 x 256 tile's k-step takes as long as 4 MB of HBM)
-      const double t = (double)af3_cdiv(tiles * used, 256 * s.per_cu) * ((double)steps + 6) * s.cost +
-                       (used > 1 ? (double)(used * 2 + 1) * M * N * 4 / 5e6 + 6 : 0);
-      if (t < best_t) best_t = t, best = {s.bm, s.bn, (int)used, (int)steps};
+    for (int sp = 1; sp <= 16; ++sp) {
+      const int64_t steps = af3_cdiv(nk, sp);
+      if (sp > 1 && (steps < 8 || tiles >= 2 * s.slots)) break;
+      const int64_t used = af3_cdiv(nk, steps), items = tiles * used;
+      const int64_t rounds = items / s.slots, rest = items % s.slots;
+      const double part = s.step * (double)rest / s.slots;
+      const double t = (double)steps * ((double)rounds * s.step + (rest ? (part > s.alone ? part : s.alone) : 0.0)) +
+                       (double)af3_cdiv(items, s.slots) * s.ends +
+                       (used > 1 ? (double)used * 4 * M * N / 5e6 + 6.0 : 0.0);
+      if (t < best_t) best_t = t, best = {s.bm, s.bn, s.stages, (int)used, (int)steps};
     }
   }
   return best;
 }
 
-template <int BM, int BN>
+template <int BM, int BN, int ST>
 void lin_launch(const LinArgs& a, bool pt, bool qt, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.splits));
+  const int64_t items = (int64_t)a.tiles_m * a.tiles_n * a.splits, slots = BM * BN * ST <= 128 * 128 * 2 ? 512 : 256;
+  const dim3 grid((unsigned)(items < slots ? items : slots));
   if (!pt && !qt)
-    hipLaunchKernelGGL((lin_kernel<BM, BN, false, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, false, false>), grid, dim3(256), 0, st, a);
   else if (!pt)
-    hipLaunchKernelGGL((lin_kernel<BM, BN, false, true>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, false, true>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((lin_kernel<BM, BN, true, true>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, true, true>), grid, dim3(256), 0, st, a);
 }
 
 constexpr int kSkinnyRows = 32;
@@ -683,11 +815,13 @@ extern "C" int af3_linear(const uint16_t* p, int64_t ldp, int p_trans, const uin
     a.part = (float*)workspace;
   }
   if (pl.bm == 256 && pl.bn == 256)
-    lin_launch<256, 256>(a, p_trans, q_trans, st);
+    lin_launch<256, 256, 2>(a, p_trans, q_trans, st);
   else if (pl.bm == 256)
-    lin_launch<256, 192>(a, p_trans, q_trans, st);
+    lin_launch<256, 192, 2>(a, p_trans, q_trans, st);
+  else if (pl.stages == 4)
+    lin_launch<128, 128, 4>(a, p_trans, q_trans, st);
   else
-    lin_launch<128, 128>(a, p_trans, q_trans, st);
+    lin_launch<128, 128, 2>(a, p_trans, q_trans, st);
   if (pl.splits > 1) {
     const int64_t n = M * af3_cdiv(N, 8);
     hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)af3_cdiv(n, 256)), dim3(256), 0, st, a.part, pl.splits, M, (int)N,
