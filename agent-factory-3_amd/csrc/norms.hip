@@ -79,8 +79,8 @@ __device__ __forceinline__ void n_unpack(const uint32_t (&w)[4], float (&f)[8]) 
 
 // chunk at element e of a row of H >= 8 elements; elements past the row are 0.  A chunk
 // that the row ends in is read as the row's last 8 elements and shifted down.
-__device__ __forceinline__ void n_get(const uint16_t* row, int e, int H, float (&f)[8]) {
-  uint32_t w[4] = {0, 0, 0, 0};
+__device__ __forceinline__ void n_words(const uint16_t* row, int e, int H, uint32_t (&w)[4]) {
+  w[0] = w[1] = w[2] = w[3] = 0;
   if (e < H) {
     __builtin_memcpy(w, row + min(e, H - 8), 16);
     if (e + 8 > H) {
@@ -91,6 +91,10 @@ __device__ __forceinline__ void n_get(const uint16_t* row, int e, int H, float (
       w[0] = (uint32_t)lo, w[1] = (uint32_t)(lo >> 32), w[2] = (uint32_t)hi, w[3] = (uint32_t)(hi >> 32);
     }
   }
+}
+__device__ __forceinline__ void n_get(const uint16_t* row, int e, int H, float (&f)[8]) {
+  uint32_t w[4];
+  n_words(row, e, H, w);
   n_unpack(w, f);
 }
 __device__ __forceinline__ void n_get(const float* row, int e, int H, float (&f)[8]) {
@@ -114,6 +118,23 @@ __device__ __forceinline__ void n_get(const void* row, int f32, int64_t off, int
   else
     n_get((const uint16_t*)row + off, e, H, f);
 }
+
+// a chunk as loaded: bf16 pairs stay packed until they are used
+template <class T>
+struct NRaw {
+  float f[8];
+  __device__ __forceinline__ void load(const T* row, int e, int H) { n_get(row, e, H, f); }
+  __device__ __forceinline__ void value(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f[i];
+  }
+};
+template <>
+struct NRaw<uint16_t> {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const uint16_t* row, int e, int H) { n_words(row, e, H, w); }
+  __device__ __forceinline__ void value(float (&v)[8]) const { n_unpack(w, v); }
+};
 
 template <class W>
 __device__ __forceinline__ void n_put_tail(W* p, W (&w)[8], int n) {  // the first n < 8 words
@@ -154,18 +175,29 @@ __device__ __forceinline__ void n_set(float* row, int e, int H, const float (&f)
   }
 }
 
-// sum over the NW waves of a row, every lane gets it
+template <int CTRL>
+__device__ __forceinline__ float n_dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+
+// sum over the NW waves of a row, every lane gets it.  turn: alternates between a
+// kernel's sums, so that one barrier serves each.
 template <int NW>
-__device__ __forceinline__ float n_sum(float s, float* lds, int wave) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) s += __shfl_xor(s, o);
+__device__ __forceinline__ float n_sum(float s, float (*lds)[NW > 1 ? NW : 1], int wave, int& turn) {
+  s += n_dpp<0xB1>(s);   // lanes 1, 2, 4, 8 apart by row operations, 16 and 32 by shuffles
+  s += n_dpp<0x4E>(s);
+  s += n_dpp<0x141>(s);
+  s += n_dpp<0x140>(s);
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
   if constexpr (NW > 1) {
-    __syncthreads();  // (the last sum's readers are done)
-    if ((threadIdx.x & 63) == 0) lds[wave] = s;
-    __syncthreads();
-    s = lds[0];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) lds[turn][wave] = s;
+    // (a barrier for LDS alone: __syncthreads would also wait for the next row's loads)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    s = lds[turn][0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) s += lds[w];
+    for (int w = 1; w < NW; ++w) s += lds[turn][w];
   }
   return s;
 }
@@ -180,7 +212,8 @@ __device__ __forceinline__ float n_gate1(const NormArgs& a, int64_t grow) {
 template <class XT, class RT, int NW, int CPL, bool RES, bool FULL>
 __global__ __launch_bounds__(NW == 8 ? 512 : 256) void norm_fwd_kernel(const NormArgs a) {
   constexpr int WPB = NW == 1 ? 4 : NW;
-  __shared__ float lds[NW];
+  __shared__ float lds[2][NW];
+  int turn = 0;
   const int wave = threadIdx.x >> 6;
   const int64_t row = NW == 1 ? (int64_t)blockIdx.x * WPB + wave : (int64_t)blockIdx.x;
   if (NW == 1 && row >= a.rows) return;
@@ -201,7 +234,7 @@ __global__ __launch_bounds__(NW == 8 ? 512 : 256) void norm_fwd_kernel(const Nor
         for (int c = 0; c < CPL; ++c)
 #pragma unroll
           for (int i = 0; i < 8; ++i) ss += v[c][i] * v[c][i];
-        const float sx = n_rstd(n_sum<NW>(ss, lds, wave), H, a.eps);
+        const float sx = n_rstd(n_sum<NW>(ss, lds, wave, turn), H, a.eps);
         if (a.rstd_x && t == 0) a.rstd_x[row] = sx;
 #pragma unroll
         for (int c = 0; c < CPL; ++c) {
@@ -212,7 +245,7 @@ __global__ __launch_bounds__(NW == 8 ? 512 : 256) void norm_fwd_kernel(const Nor
         }
       }
       if (a.gate_cols) {
-        const int64_t grow = row / a.gate_rows;
+        const int64_t grow = (uint32_t)row / (uint32_t)a.gate_rows;
         const float g1 = a.gate_cols == 1 ? n_gate1(a, grow) : 0.f;
 #pragma unroll
         for (int c = 0; c < CPL; ++c) {
@@ -237,7 +270,7 @@ __global__ __launch_bounds__(NW == 8 ? 512 : 256) void norm_fwd_kernel(const Nor
   for (int c = 0; c < CPL; ++c)
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss += v[c][i] * v[c][i];
-  const float s = n_rstd(n_sum<NW>(ss, lds, wave), H, a.eps);
+  const float s = n_rstd(n_sum<NW>(ss, lds, wave, turn), H, a.eps);
   if (a.rstd && t == 0) a.rstd[row] = s;
   XT* const out_h = (XT*)a.out_h + row * H;
 #pragma unroll
@@ -256,12 +289,7 @@ template <int NW, int WPB, int CPL>
 __device__ __forceinline__ void n_join(const float (&acc)[CPL][8], float* lds, int wave, int t, int H, float* out) {
   if constexpr (NW > 1) {
 #pragma unroll
-    for (int c = 0; c < CPL; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = (c * 64 * NW + t) * 8 + i;
-        if (e < H) out[e] = acc[c][i];
-      }
+    for (int c = 0; c < CPL; ++c) n_set(out, (c * 64 * NW + t) * 8, H, acc[c]);
   } else {
     for (int w = 0; w < WPB; ++w) {
       __syncthreads();
@@ -288,7 +316,9 @@ template <class XT, class RT, int NW, int CPL, bool RES, bool FULL, bool ACC>
 __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const NormArgs a) {
   constexpr int WPB = NW == 1 ? 8 : NW;
   constexpr int AC = ACC ? CPL : 1;
-  __shared__ float lds[(ACC && NW == 1) ? CPL * 512 : 8];
+  __shared__ float sums[2][NW];
+  __shared__ float lds[(ACC && NW == 1) ? CPL * 512 : 1];
+  int turn = 0;
   const int wave = threadIdx.x >> 6;
   const int t = NW == 1 ? (threadIdx.x & 63) : threadIdx.x;
   const int H = a.H;
@@ -308,32 +338,86 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
         if constexpr (FULL) ap[c][i] = ag[c][i] = 0.f;
       }
   }
+  // a row's loads, made while the row before it is worked on
+  NRaw<RT> r_dr[CPL], r_r[CPL];
+  NRaw<XT> r_dh[CPL], r_x[FULL ? CPL : 1];
+  float r_gate[FULL ? CPL : 1][8];
+  float r_s = 0.f, r_sx = 1.f, r_g1 = 1.f;
+  const bool has_dr = RES && a.dr, has_dh = !RES || a.dh;
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      const int e = (c * 64 * NW + t) * 8;
+      if (has_dr) r_dr[c].load((const RT*)a.dr + row * a.lddr, e, H);
+      if (has_dh) r_dh[c].load((const XT*)a.dh + row * a.lddh, e, H);
+      if (has_dh) r_r[c].load((const RT*)a.res + row * a.ldr, e, H);
+      if constexpr (FULL) r_x[c].load((const XT*)a.x + row * a.ldx, e, H);
+    }
+    if (has_dh) r_s = a.s_r[row];
+    if constexpr (FULL) {
+      if (a.post) r_sx = a.s_x[row];
+      if (a.gate_cols) {
+        const uint32_t grow = (uint32_t)row / (uint32_t)a.gate_rows;
+        if (a.gate_cols == 1) {
+          r_g1 = n_gate1(a, grow);
+        } else {
+#pragma unroll
+          for (int c = 0; c < CPL; ++c)
+            n_get(a.gate, a.gate_f32, (int64_t)grow * H, (c * 64 * NW + t) * 8, H, r_gate[c]);
+        }
+      }
+    }
+  };
+  // (where the registers of two rows would not fit, a row's loads are its own, the weights' too)
+  constexpr bool AHEAD = CPL * (FULL ? 2 : 1) <= 2;
+  float w_h[AHEAD ? CPL : 1][8], w_post[FULL && AHEAD ? CPL : 1][8];
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      const int e = (c * 64 * NW + t) * 8;
+      if (has_dh) n_get(a.weight, a.w_f32, 0, e, H, w_h[c]);
+      if constexpr (FULL) {
+        if (a.post) n_get(a.post, a.post_f32, 0, e, H, w_post[c]);
+      }
+    }
+  }
+  if (AHEAD && first < last) fetch(first);
   for (int64_t row = first; row < last; row += step) {
+    if (!AHEAD) fetch(row);
     float g[CPL][8];  // the gradient of r
-    if (RES && a.dr) {
-      const RT* const dr = (const RT*)a.dr + row * a.lddr;
+    float d[CPL][8], v[CPL][8], x[FULL ? CPL : 1][8], gate[FULL ? CPL : 1][8];
+    const float s_r = r_s, s_x = r_sx, g1 = r_g1;
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) n_get(dr, (c * 64 * NW + t) * 8, H, g[c]);
-    } else {
-#pragma unroll
-      for (int c = 0; c < CPL; ++c)
+    for (int c = 0; c < CPL; ++c) {
+      if (has_dr) {
+        r_dr[c].value(g[c]);
+      } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[c][i] = 0.f;
-    }
-    if (!RES || a.dh) {
-      const XT* const dh = (const XT*)a.dh + row * a.lddh;
-      const RT* const r = (const RT*)a.res + row * a.ldr;
-      const float s = a.s_r[row];
-      float d[CPL][8], v[CPL][8], dot = 0.f;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        n_get(dh, (c * 64 * NW + t) * 8, H, d[c]);
-        n_get(r, (c * 64 * NW + t) * 8, H, v[c]);
       }
+      if (has_dh) {
+        r_dh[c].value(d[c]);
+        r_r[c].value(v[c]);
+      }
+      if constexpr (FULL) {
+        r_x[c].value(x[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gate[c][i] = r_gate[c][i];
+      }
+    }
+    if (AHEAD && row + step < last) fetch(row + step);
+    if (has_dh) {
+      const float s = s_r;
+      float dot = 0.f;
 #pragma unroll
       for (int c = 0; c < CPL; ++c) {
         float w[8];
-        n_get(a.weight, a.w_f32, 0, (c * 64 * NW + t) * 8, H, w);
+        if constexpr (AHEAD) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = w_h[c][i];
+        } else {
+          n_get(a.weight, a.w_f32, 0, (c * 64 * NW + t) * 8, H, w);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if constexpr (ACC) aw[c][i] += d[c][i] * (v[c][i] * s);
@@ -341,7 +425,7 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
           dot += d[c][i] * v[c][i];
         }
       }
-      const float m = n_sum<NW>(dot, lds, wave) / (float)H * s * s;
+      const float m = n_sum<NW>(dot, sums, wave, turn) / (float)H * s * s;
 #pragma unroll
       for (int c = 0; c < CPL; ++c)
 #pragma unroll
@@ -354,23 +438,22 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
     }
     if constexpr (!RES) continue;
     if constexpr (FULL) {
-      const XT* const xr = (const XT*)a.x + row * a.ldx;
-      const int64_t grow = a.gate_cols ? row / a.gate_rows : 0;
-      const float g1 = a.gate_cols == 1 ? n_gate1(a, grow) : 1.f;
-      const float s = a.post ? a.s_x[row] : 1.f;
-      float x[CPL][8], dot = 0.f, gdot = 0.f;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) n_get(xr, (c * 64 * NW + t) * 8, H, x[c]);
+      const float s = s_x;
+      float dot = 0.f, gdot = 0.f;
 #pragma unroll
       for (int c = 0; c < CPL; ++c) {
         const int e = (c * 64 * NW + t) * 8;
-        float w[8], gt[8], gg[8];
-        if (a.post) n_get(a.post, a.post_f32, 0, e, H, w);
-        if (a.gate_cols > 1) n_get(a.gate, a.gate_f32, grow * H, e, H, gt);
+        float w[8], gg[8];
+        if constexpr (AHEAD) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = w_post[c][i];
+        } else {
+          if (a.post) n_get(a.post, a.post_f32, 0, e, H, w);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float wi = a.post ? w[i] : 1.f;
-          const float gi = a.gate_cols > 1 ? gt[i] : g1;
+          const float gi = a.gate_cols > 1 ? gate[c][i] : g1;
           const float gu = a.scale * g[c][i] * (x[c][i] * s * wi);  // the gate's gradient
           gdot += gu;
           gg[i] = gu;
@@ -388,11 +471,11 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
         }
       }
       if (a.gate_dots) {
-        const float sum = n_sum<NW>(gdot, lds, wave);
+        const float sum = n_sum<NW>(gdot, sums, wave, turn);
         if (t == 0) a.gate_dots[row] = sum;
       }
       if (a.post) {
-        const float m = n_sum<NW>(dot, lds, wave) / (float)H * s * s;
+        const float m = n_sum<NW>(dot, sums, wave, turn) / (float)H * s * s;
 #pragma unroll
         for (int c = 0; c < CPL; ++c)
 #pragma unroll
@@ -429,7 +512,7 @@ struct JoinArgs {
   int blocks_per_group;
   int H;
 };
-constexpr int kJoinCols = 64, kJoinRows = 16;
+constexpr int kJoinCols = 16, kJoinRows = 64;  // 2880 columns: 180 blocks (45 of 64 columns took 11 us, these 5)
 
 __global__ __launch_bounds__(kJoinCols* kJoinRows) void norm_join_kernel(const JoinArgs a) {
   __shared__ float lds[kJoinRows][kJoinCols];
@@ -440,16 +523,21 @@ __global__ __launch_bounds__(kJoinCols* kJoinRows) void norm_join_kernel(const J
   const int64_t group = which == 2 ? what - 2 : 0;
   const int64_t begin = which == 2 ? group * a.blocks_per_group : 0;
   const int64_t end = which == 2 ? begin + a.blocks_per_group : a.blocks;
-  const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = threadIdx.x % kJoinCols, w = threadIdx.x / kJoinCols;
   const int64_t col = (int64_t)(blockIdx.x % ncb) * kJoinCols + c;
   float s = 0.f;
   if (col < a.H)
+#pragma unroll 4
     for (int64_t b = begin + w; b < end; b += kJoinRows) s += part[b * a.H + col];
   lds[w][c] = s;
   __syncthreads();
-  if (w || col >= a.H) return;
 #pragma unroll
-  for (int i = 1; i < kJoinRows; ++i) s += lds[i][c];
+  for (int n = kJoinRows / 2; n > 1; n /= 2) {  // (pairs, the last two below)
+    if (w < n) lds[w][c] = s = s + lds[w + n][c];
+    __syncthreads();
+  }
+  if (w || col >= a.H) return;
+  s += lds[1][c];
   const int64_t at = group * a.H + col;
   if (a.f32[which])
     ((float*)a.out[which])[at] = s;
@@ -460,12 +548,13 @@ __global__ __launch_bounds__(kJoinCols* kJoinRows) void norm_join_kernel(const J
 // a one-value gate's gradient: group g sums dots[g * per .. ) (one block each)
 __global__ __launch_bounds__(256) void norm_gate_dots_kernel(const float* dots, int64_t rows, int64_t per, void* out,
                                                              int f32) {
-  __shared__ float lds[4];
+  __shared__ float lds[2][4];
+  int turn = 0;
   const int64_t g = blockIdx.x;
   const int64_t end = min(g * per + per, rows);
   float s = 0.f;
   for (int64_t i = g * per + threadIdx.x; i < end; i += 256) s += dots[i];
-  s = n_sum<4>(s, lds, threadIdx.x >> 6);
+  s = n_sum<4>(s, lds, threadIdx.x >> 6, turn);
   if (threadIdx.x == 0) {
     if (f32)
       ((float*)out)[g] = s;
@@ -518,7 +607,11 @@ void norm_bwd_launch(const NormArgs& a, unsigned blocks, hipStream_t st) {
   if constexpr (!FULL) if (norm_wide(a.rows, a.H, FULL, 2)) {
     AF3_NB(1, 2);
   }
-  if (chunks <= 64 * 8) AF3_NB(4, 2);
+  if constexpr (FULL) {
+    if (chunks <= 64 * 8) AF3_NB(8, 1);
+  } else {
+    if (chunks <= 64 * 8) AF3_NB(4, 2);
+  }
   if (chunks <= 64 * 16) AF3_NB(8, 2);
   AF3_NB(8, 4);
 #undef AF3_NB
@@ -555,7 +648,7 @@ int norm_check(const char* who, int64_t rows, int H, int gate_cols, int64_t gate
   AF3_REQUIRE(H >= kNormMinH && H <= kNormMaxH, "%s: %d channels (%d to %d)", who, H, kNormMinH, kNormMaxH);
   AF3_REQUIRE(rows < (int64_t)1 << 31, "%s: too many rows", who);
   AF3_REQUIRE(eps >= 0.f, "%s: eps must not be negative", who);
-  AF3_REQUIRE(gate_cols == 0 || ((gate_cols == 1 || gate_cols == H) && gate_rows > 0),
+  AF3_REQUIRE(gate_cols == 0 || ((gate_cols == 1 || gate_cols == H) && gate_rows > 0 && gate_rows < (int64_t)1 << 32),
               "%s: a gate has 1 or H columns, and rows that share each of its rows", who);
   return 0;
 }
