@@ -72,90 +72,110 @@ struct LinArgs {
   LinEpi e;
 };
 
-__device__ __forceinline__ float lin_act(float z, int act) {
-  if (act == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
-  if (act == kActSilu) return z / (1.f + __expf(-z));
-  if (act == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678f));
-  if (act == kActGeluTanh) return 0.5f * z * (1.f + tanhf(0.79788456f * (z + 0.044715f * z * z * z)));
-  return z;
+// 0.5 (1 + erf(z / sqrt 2)) by Abramowitz and Stegun's 7.1.26 (erf within 1.5e-7, where
+// fp32's own 1 + erf is within 1.2e-7), as 0.5 erfc for negative z; e receives e^(-z^2 / 2)
+__device__ __forceinline__ float lin_phi(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678f;
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+  e = __expf(-x * x);
+  const float half_erfc =
+      0.5f * e * (t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))));
+  return z < 0.f ? half_erfc : 1.f - half_erfc;
+}
+// the argument of gelu's tanh as t = 1 / (1 + e^(-2 u)): (1 + tanh u) / 2
+__device__ __forceinline__ float lin_half_tanh(float z) {
+  const float u = 0.79788456f * (z + 0.044715f * z * z * z);
+  return __builtin_amdgcn_rcpf(1.f + __expf(-2.f * u));
+}
+template <int N>
+__device__ __forceinline__ void lin_act(float (&z)[N], int act) {
+  float e;
+  if (act == kActRelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? z[i] : (z[i] != z[i] ? z[i] : 0.f);
+  } else if (act == kActSilu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] * __builtin_amdgcn_rcpf(1.f + __expf(-z[i]));
+  } else if (act == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] * lin_phi(z[i], e);
+  } else if (act == kActGeluTanh) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] * lin_half_tanh(z[i]);
+  }
 }
 __device__ __forceinline__ float lin_slope(float z, int act) {
   if (act == kActRelu) return z > 0.f ? 1.f : 0.f;
   if (act == kActSilu) {
-    const float s = 1.f / (1.f + __expf(-z));
+    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
     return s * (1.f + z * (1.f - s));
   }
-  if (act == kActGelu) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+  if (act == kActGelu) {
+    float e;
+    const float phi = lin_phi(z, e);
+    return phi + z * 0.39894228f * e;
+  }
   if (act == kActGeluTanh) {
-    const float t = tanhf(0.79788456f * (z + 0.044715f * z * z * z));
-    return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * z * z);
+    z = fminf(fmaxf(z, -30.f), 30.f);  // (0 and 1 there; its square must not overflow)
+    const float s = lin_half_tanh(z);
+    return s + z * 2.f * s * (1.f - s) * 0.79788456f * (1.f + 0.134145f * z * z);
   }
   return 1.f;
 }
 
-// the bias of 8 columns from `col` (col + 8 <= N)
-__device__ __forceinline__ void lin_bias(const LinEpi& e, int col, float (&v)[8]) {
-  if (!e.bias) return;
-  if (e.bias_f32) {
-    float b[8];
-    __builtin_memcpy(b, (const float*)e.bias + col, 32);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += b[i];
-  } else {
-    uint32_t b[4];
-    __builtin_memcpy(b, (const uint16_t*)e.bias + col, 16);
+// 8 elements of a row from p of which the first n are there, as fp32 (n >= 8: one access)
+__device__ __forceinline__ void lin_get8(const uint16_t* p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    uint32_t w[4];
+    __builtin_memcpy(w, p, 16);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] += af3_bf16_to_f32(b[i]);
-      v[2 * i + 1] += af3_bf16_to_f32(b[i] >> 16);
+      v[2 * i] = af3_bf16_to_f32(w[i]);
+      v[2 * i + 1] = af3_bf16_to_f32(w[i] >> 16);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? af3_bf16_to_f32(p[i]) : 0.f;
   }
 }
-
-// 8 columns from `col` of row m: sums -> output (columns past N are left out)
-template <bool ACT>
-__device__ __forceinline__ void lin_finish(const LinEpi& e, int64_t m, int col, int N, float (&v)[8]) {
-  const int64_t at = m * N + col;
-  if (col + 8 <= N) {
-    lin_bias(e, col, v);
-    if (ACT) {
-      if (e.z) {
-        uint32_t w[4];
+__device__ __forceinline__ void lin_put8(uint16_t* p, int n, const float (&v)[8]) {
+  uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = af3_pack_bf16x2(v[2 * i], v[2 * i + 1]);
-        __builtin_memcpy(e.z + at, w, 16);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = lin_act(v[i], e.act);
-    }
-    if (e.res) {
-      uint32_t r[4];
-      __builtin_memcpy(r, e.res + m * e.ldr + col, 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] += af3_bf16_to_f32(r[i]);
-        v[2 * i + 1] += af3_bf16_to_f32(r[i] >> 16);
-      }
-    }
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = af3_pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    __builtin_memcpy(e.y + at, w, 16);
+  for (int i = 0; i < 4; ++i) w[i] = af3_pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  if (n >= 8) {
+    __builtin_memcpy(p, w, 16);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (col + i < N) {
-        float f = v[i];
-        if (e.bias)
-          f += e.bias_f32 ? ((const float*)e.bias)[col + i] : af3_bf16_to_f32(((const uint16_t*)e.bias)[col + i]);
-        if (ACT) {
-          if (e.z) e.z[at + i] = (uint16_t)af3_f32_to_bf16(f);
-          f = lin_act(f, e.act);
-        }
-        if (e.res) f += af3_bf16_to_f32(e.res[m * e.ldr + col + i]);
-        e.y[at + i] = (uint16_t)af3_f32_to_bf16(f);
-      }
+      if (i < n) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
   }
+}
+// the bias of 8 columns from `col`
+__device__ __forceinline__ void lin_bias(const LinEpi& e, int col, int N, float (&b)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = 0.f;
+  if (!e.bias || col >= N) return;
+  if (!e.bias_f32) {
+    lin_get8((const uint16_t*)e.bias + col, N - col, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < N) b[i] = ((const float*)e.bias)[col + i];
+  }
+}
+// sums v (bias added) and residual r of 8 columns from `col` of row m -> output
+template <bool ACT>
+__device__ __forceinline__ void lin_finish(const LinEpi& e, int64_t m, int col, int N, float (&v)[8], const float (&r)[8]) {
+  const int64_t at = m * N + col;
+  if (ACT) {
+    if (e.z) lin_put8(e.z + at, N - col, v);
+    lin_act(v, e.act);
+  }
+  if (e.res) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += r[i];
+  }
+  lin_put8(e.y + at, N - col, v);
 }
 
 __device__ __forceinline__ void lin_dma16(const void* sbase, uint32_t voff, uint32_t lds_byte_addr) {
@@ -231,7 +251,7 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
   constexpr int NF = TM + TN;      // fragments per sub-step
   constexpr int EPI = 32 * (BN / 2 * 4);  // bytes per wave of the epilogue's turn
   static_assert(4 * EPI <= STAGE, "the epilogue fits a stage");
-  constexpr int STORES = 32 * (BN / 2) / 8 / 64 * TM;  // of a wave in a plain epilogue
+  constexpr int STORES = (32 + 64 / (BN / 16) - 1) / (64 / (BN / 16)) * TM;  // of a wave for a whole tile, at least
   static_assert(NC * (ST - 2) + STORES < 64, "vmcnt counts to 63");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[ST * STAGE];
   const int lane = threadIdx.x & 63;
@@ -427,7 +447,7 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
     }
     // the last k-step, and the next item's first copies
     const int em0 = m0 + wm0, en0 = n0 + wn0, es_split = split;
-    const bool plain = !a.part && !a.e.act && m0 + BM <= a.M && n0 + BN <= a.N;
+    const bool whole_tile = m0 + BM <= a.M && n0 + BN <= a.N;
     item += stride;
     const bool more = item < items_end;
     if (more) {
@@ -443,9 +463,13 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
     constexpr int W = BN / 2;        // columns of a wave
     constexpr int ROWB = W * 4;      // bytes of a staged row; 16-byte chunks XORed with the row's low bits
     constexpr int LPR = W / 8;       // lanes per row when read back
-    constexpr int IT = 32 * LPR / 64, U = IT % 4 == 0 ? 4 : 3;
+    constexpr int RPI = 64 / LPR;    // rows a wave reads at a time: a lane keeps its 8 columns
+    constexpr int IT = (32 + RPI - 1) / RPI;
     const uint32_t es = lds0 + (uint32_t)(cur * STAGE + wave * EPI);
     auto staged = [&](int row, int chunk) { return es + (uint32_t)(row * ROWB + ((chunk ^ (row & 7)) << 4)); };
+    const int c8 = lane % LPR * 8, col = en0 + c8;
+    float bias[8];
+    lin_bias(a.e, lane < RPI * LPR ? col : a.N, a.N, bias);
 #pragma unroll 1
   for (int tm = 0; tm < TM; ++tm) {  // (acc[0] is the tile's rows tm; one copy of the code)
 #pragma unroll
@@ -459,15 +483,43 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
 #pragma unroll
       for (int tn = 0; tn < TN; ++tn) acc[i][tn] = acc[i + 1][tn];
     // (a wave's own LDS writes and reads are in order; the compiler keeps them so)
-    auto out = [&](auto act_, int id) {
-      const int row = id / LPR, c8 = id % LPR * 8;
-      const int64_t m = em0 + tm * 32 + row;
-      const int col = en0 + c8;
-      const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
-      const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
-      if (m >= a.M || col >= a.N) return;
-      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      if (a.part) {
+    // U rows' accesses side by side; EDGE: rows and columns past the output are left out
+    auto out = [&](auto edge_, auto act_, auto u_) __attribute__((always_inline)) {
+      constexpr bool EDGE = decltype(edge_)::value, ACT = decltype(act_)::value;
+      constexpr int U = decltype(u_)::value;
+#pragma unroll 1
+      for (int g = 0; g < IT; g += U) {
+        float v[U][8], r[U][8];
+        bool live[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int row = (g + u) * RPI + lane / LPR;
+          const int64_t m = em0 + tm * 32 + row;
+          live[u] = g + u < IT && row < 32 && lane < RPI * LPR && (!EDGE || (m < a.M && col < a.N));
+          if (live[u]) {
+            if (a.e.res) lin_get8(a.e.res + m * a.e.ldr + col, EDGE ? a.N - col : 8, r[u]);
+            const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
+            const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[u][i] = x[i] + bias[i], v[u][4 + i] = y[i] + bias[4 + i];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t m = em0 + tm * 32 + (g + u) * RPI + lane / LPR;
+          if (live[u]) lin_finish<ACT>(a.e, m, col, a.N, v[u], r[u]);
+        }
+      }
+    };
+    if (a.part) {
+#pragma unroll 2
+      for (int g = 0; g < IT; ++g) {
+        const int row = g * RPI + lane / LPR;
+        const int64_t m = em0 + tm * 32 + row;
+        if (row >= 32 || lane >= RPI * LPR || m >= a.M || col >= a.N) continue;
+        const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
+        const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
+        float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
         float* const o = a.part + ((int64_t)es_split * a.M + m) * a.N + col;
         if (col + 8 <= a.N) {
           __builtin_memcpy(o, v, 32);
@@ -476,55 +528,18 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
           for (int i = 0; i < 8; ++i)
             if (col + i < a.N) o[i] = v[i];
         }
-      } else {
-        lin_finish<decltype(act_)::value>(a.e, m, col, a.N, v);
       }
-    };
-    // (a whole tile without activation or partials, the common one, has its accesses side by side)
-    if (plain) {
-#pragma unroll 1
-      for (int g = 0; g < IT; g += U) {
-        float v[U][8];
-        uint32_t r[U][4];
-        int64_t m[U];
-        int col[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int id = (g + u) * 64 + lane;
-          const int row = id / LPR, c8 = id % LPR * 8;
-          m[u] = em0 + tm * 32 + row, col[u] = en0 + c8;
-          if (a.e.res) __builtin_memcpy(r[u], a.e.res + m[u] * a.e.ldr + col[u], 16);
-          const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
-          const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[u][i] = x[i], v[u][4 + i] = y[i];
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          lin_bias(a.e, col[u], v[u]);
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (a.e.res) {
-              v[u][2 * i] += af3_bf16_to_f32(r[u][i]);
-              v[u][2 * i + 1] += af3_bf16_to_f32(r[u][i] >> 16);
-            }
-            w[i] = af3_pack_bf16x2(v[u][2 * i], v[u][2 * i + 1]);
-          }
-          __builtin_memcpy(a.e.y + m[u] * a.N + col[u], w, 16);
-        }
-      }
-    } else if (a.e.act && !a.part) {
-#pragma unroll 1
-      for (int i = 0; i < IT; ++i) out(Flag<true>{}, i * 64 + lane);
+    } else if (whole_tile) {
+      if (a.e.act) out(Flag<false>{}, Flag<true>{}, Int<2>{});
+      else out(Flag<false>{}, Flag<false>{}, Int<4>{});
     } else {
-#pragma unroll 1
-      for (int i = 0; i < IT; ++i) out(Flag<false>{}, i * 64 + lane);
+      if (a.e.act) out(Flag<true>{}, Flag<true>{}, Int<2>{});
+      else out(Flag<true>{}, Flag<false>{}, Int<2>{});
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before the next 32 rows overwrite)
   }
     if (!more) break;
-    stores = plain;
+    stores = !a.part && whole_tile;
     cur = ahead(cur, 1);
   }
 }
@@ -536,7 +551,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* part, int sp
   const int64_t m = id / ncol;
   const int col = (int)(id - m * ncol) * 8;
   if (m >= M) return;
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float v[8], r[8];
+  lin_bias(e, col, N, v);
+  if (e.res) lin_get8(e.res + m * e.ldr + col, N - col, r);
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const float* const p = part + ((int64_t)s * M + m) * N + col;
     if (col + 8 <= N) {
@@ -551,59 +569,81 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* part, int sp
     }
   }
   if (e.act)
-    lin_finish<true>(e, m, col, N, v);
+    lin_finish<true>(e, m, col, N, v, r);
   else
-    lin_finish<false>(e, m, col, N, v);
+    lin_finish<false>(e, m, col, N, v, r);
 }
 
 // Up to 16 NT rows of x: a block makes 16 columns (rows of W).  Its 16 waves share k in
-// units of 64, a wave's lane (r, g) taking k = 16 g + (0..15) of row r of W and of x (two
-// products of 32 k; both operands in the same order), so W is read once, in whole
-// 128-byte lines, with all of a wave's loads in flight; the waves' sums meet in LDS.
+// units of 64, a wave's lane (r, g) taking k = 8 g + (0..7) and 32 more of row r of W and of
+// x (two products of 32 k), so W is read once, 64 contiguous bytes of 16 rows at a time,
+// with all of a wave's loads in flight; the waves' sums meet in LDS.
 // Addresses need no alignment; elements past K are zeros.
 constexpr int kSkinnyWaves = 16;
 
-// 16 elements at p of which the first n are there
-__device__ __forceinline__ void lin_get16(const uint16_t* p, int n, af3_u32x4 (&v)[2]) {
-  if (n >= 16) {
-    __builtin_memcpy(v, p, 32);
+// 8 elements at p of which the first n are there, zeros after them
+__device__ __forceinline__ void lin_words(const uint16_t* p, int n, af3_u32x4& v) {
+  if (n >= 8) {
+    __builtin_memcpy(&v, p, 16);
   } else {
-    uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const uint32_t lo = 2 * i < n ? p[2 * i] : 0, hi = 2 * i + 1 < n ? p[2 * i + 1] : 0;
-      w[i] = lo | hi << 16;
+      v[i] = lo | hi << 16;
     }
-    __builtin_memcpy(v, w, 32);
   }
 }
 
 template <int NT>
 __global__ __launch_bounds__(kSkinnyWaves * 64) void lin_skinny_kernel(const LinArgs a) {
   __shared__ float lds[kSkinnyWaves][NT * 16][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
-  const uint16_t* const w = a.q + (int64_t)min(n0 + r, a.N - 1) * a.ldq;
+  const uint16_t* const w = a.q + (int64_t)min(n0 + r, a.N - 1) * a.ldq + g * 8;
   const uint16_t* x[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) x[t] = a.p + (int64_t)min(t * 16 + r, a.M - 1) * a.ldp;
+  for (int t = 0; t < NT; ++t) x[t] = a.p + (int64_t)min(t * 16 + r, a.M - 1) * a.ldp + g * 8;
   f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int units = (a.K + 63) / 64;
-  for (int u = wave; u < units; u += kSkinnyWaves) {
-    const int k = u * 64 + g * 16;
-    af3_u32x4 wv[2], xv[NT][2];
-    lin_get16(w + k, a.K - k, wv);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) lin_get16(x[t] + k, a.K - k, xv[t]);
+  auto mul = [&](const af3_u32x4 (&wv)[2], const af3_u32x4 (&xv)[NT][2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(af3_bf16x8, wv[i]),
                                                          __builtin_bit_cast(af3_bf16x8, xv[t][i]), acc[t], 0, 0, 0);
+  };
+  // U units' loads side by side (one after the other's latency costs 32 rows of 4096 14 us instead of 8)
+  constexpr int U = NT == 1 ? 4 : 2;
+  const int whole = a.K / 64;
+  int u = wave;
+  for (; u + (U - 1) * kSkinnyWaves < whole; u += U * kSkinnyWaves) {
+    af3_u32x4 wv[U][2], xv[U][NT][2];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = (u + i * kSkinnyWaves) * 64;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        __builtin_memcpy(&wv[i][h], w + k + 32 * h, 16);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) __builtin_memcpy(&xv[i][t][h], x[t] + k + 32 * h, 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) mul(wv[i], xv[i]);
+  }
+  for (; u * 64 < a.K; u += kSkinnyWaves) {  // fewer, and the one that K ends in
+    af3_u32x4 wv[2], xv[NT][2];
+    const int k = u * 64, n = a.K - k - g * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      lin_words(w + k + 32 * h, n - 32 * h, wv[h]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) lin_words(x[t] + k + 32 * h, n - 32 * h, xv[t][h]);
+    }
+    mul(wv, xv);
   }
   // lane (c, g): row c of x, columns 4 g + (0..3)
 #pragma unroll
@@ -622,7 +662,9 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void lin_skinny_kernel(const Lin
   if (e.bias) f += e.bias_f32 ? ((const float*)e.bias)[col] : af3_bf16_to_f32(((const uint16_t*)e.bias)[col]);
   if (e.act) {
     if (e.z) e.z[at] = (uint16_t)af3_f32_to_bf16(f);
-    f = lin_act(f, e.act);
+    float one[1] = {f};
+    lin_act(one, e.act);
+    f = one[0];
   }
   if (e.res) f += af3_bf16_to_f32(e.res[(int64_t)m * e.ldr + col]);
   e.y[at] = (uint16_t)af3_f32_to_bf16(f);
@@ -696,17 +738,26 @@ __global__ __launch_bounds__(256) void lin_dz_kernel(const DzArgs a) {
   if (at < a.N) a.part[(int64_t)blockIdx.y * a.N + at] = t;
 }
 
-__global__ __launch_bounds__(256) void lin_colsum_kernel(const float* part, int n, int N, void* out, int f32) {
-  __shared__ float lds[4][64];
-  const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int col = blockIdx.x * 64 + c;
+// partials' columns -> the bias's gradient: 16 columns a block, 64 lanes of rows joined in pairs
+constexpr int kSumCols = 16, kSumRows = 64;
+
+__global__ __launch_bounds__(kSumCols* kSumRows) void lin_colsum_kernel(const float* part, int n, int N, void* out, int f32) {
+  __shared__ float lds[kSumRows][kSumCols];
+  const int c = threadIdx.x % kSumCols, w = threadIdx.x / kSumCols;
+  const int col = blockIdx.x * kSumCols + c;
   float s = 0.f;
-  if (col < N)
-    for (int i = w; i < n; i += 4) s += part[(int64_t)i * N + col];
+  if (col < N) {
+#pragma unroll 4
+    for (int i = w; i < n; i += kSumRows) s += part[(int64_t)i * N + col];
+  }
   lds[w][c] = s;
   __syncthreads();
+#pragma unroll
+  for (int h = kSumRows / 2; h > 0; h /= 2) {
+    if (w < h) lds[w][c] = s = s + lds[w + h][c];
+    __syncthreads();
+  }
   if (w || col >= N) return;
-  s = ((s + lds[1][c]) + lds[2][c]) + lds[3][c];
   if (f32)
     ((float*)out)[col] = s;
   else
@@ -857,7 +908,7 @@ extern "C" int af3_linear_dz(const uint16_t* dy, int64_t ldy, const uint16_t* z,
   hipStream_t st = (hipStream_t)stream_;
   hipLaunchKernelGGL(lin_dz_kernel, dim3((unsigned)af3_cdiv(N, 256), (unsigned)blocks), dim3(256), 0, st, a);
   if (dbias)
-    hipLaunchKernelGGL(lin_colsum_kernel, dim3((unsigned)af3_cdiv(N, 64)), dim3(256), 0, st, a.part, blocks, (int)N,
+    hipLaunchKernelGGL(lin_colsum_kernel, dim3((unsigned)af3_cdiv(N, kSumCols)), dim3(kSumCols * kSumRows), 0, st, a.part, blocks, (int)N,
                        dbias, bias_f32);
   return af3::check_launch("linear_dz");
 }
