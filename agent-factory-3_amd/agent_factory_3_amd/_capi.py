@@ -135,7 +135,7 @@ def exported_symbols() -> list[str]:
 
 def call(name: str, *args) -> None:
     """Call an entry point; raise RuntimeError on a non-zero status."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.af3_last_error().decode(errors="replace")

@@ -9,14 +9,16 @@ them) are counted once over their mesh.  The HIP kernels are behind
 """
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
+from operator import attrgetter
 
 import torch
 
 from . import _capi
 from .routing import _device_of
 
+_DTYPE, _LAYOUT = attrgetter("dtype"), attrgetter("layout")
 _NORMS = {2.0: 2, 1.0: 1, math.inf: 0}
 
 
@@ -33,18 +35,15 @@ class _Tensors:
 
     def __init__(self, tensors):
         self.copies = []
-        dense = []
-        for t in tensors:
-            if not t.is_contiguous():
-                t = self._run(t)
-            dense.append(t)
-        n = len(dense)
-        self.n = n
-        self.kept = dense
-        self.device = dense[0].device
-        self.ptrs = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in dense])
-        self.sizes = (ctypes.c_int64 * n)(*[t.numel() for t in dense])
-        self.f32 = (ctypes.c_uint8 * n)(*[t.dtype is torch.float32 for t in dense])
+        if not all(map(torch.Tensor.is_contiguous, tensors)):
+            tensors = [t if t.is_contiguous() else self._run(t) for t in tensors]
+        self.n = len(tensors)
+        self.kept = tensors
+        self.device = tensors[0].device
+        # (host arrays: the calls read them before they return)
+        self._arrays = (array("Q", map(torch.Tensor.data_ptr, tensors)), array("q", map(torch.Tensor.numel, tensors)),
+                        array("B", [d is torch.float32 for d in map(_DTYPE, tensors)]))
+        self.ptrs, self.sizes, self.f32 = (a.buffer_info()[0] for a in self._arrays)
 
     def _run(self, t):
         order = sorted(range(t.dim()), key=t.stride, reverse=True)
@@ -87,6 +86,10 @@ def _local(t):
 
 def _gather(tensors):
     """Tensors by (device, process groups), in order of first appearance; doubles and empty ones left out."""
+    if (set(map(type, tensors)) == {torch.Tensor} and len(set(map(torch.Tensor.get_device, tensors))) == 1
+            and len(set(map(id, tensors))) == len(tensors) and all(map(torch.Tensor.numel, tensors))
+            and set(map(_LAYOUT, tensors)) == {torch.strided}):
+        return {(tensors[0].device, ()): tensors}   # the common case, without a step per tensor
     buckets, seen = {}, set()
     for t in tensors:
         if id(t) in seen:
@@ -109,9 +112,9 @@ def _check(buckets):
     for (device, _), ts in buckets.items():
         if device.type != "cuda":
             raise RuntimeError("grad_norm: gradients must be GPU tensors (the MI355X path has no CPU implementation)")
-        for t in ts:
-            if t.dtype is not torch.float32 and t.dtype is not torch.bfloat16:
-                raise TypeError(f"grad_norm: gradients must be bfloat16 or float32 (got {t.dtype})")
+        for dtype in set(map(_DTYPE, ts)):
+            if dtype is not torch.float32 and dtype is not torch.bfloat16:
+                raise TypeError(f"grad_norm: gradients must be bfloat16 or float32 (got {dtype})")
 
 
 def _bucket_sum(tensors, code):
@@ -165,7 +168,7 @@ def _norm_of(partials, code):
 def _grads(parameters):
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    return [g for g in [p.grad for p in parameters] if g is not None]
+    return [g for p in parameters if (g := p.grad) is not None]
 
 
 @torch.no_grad()

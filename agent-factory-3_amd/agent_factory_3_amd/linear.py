@@ -23,7 +23,8 @@ _MAX_STRIDE = 1 << 22
 
 def _rows(t: torch.Tensor):
     """[..., C] as [rows, C] with contiguous rows."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -100,13 +101,12 @@ class _Linear(torch.autograd.Function):
         T = math.prod(x_shape[:-1])
         dx = dw = db = None
         if need_x or need_w or need_b:
-            dev = dy.device
             with _device_of(dy):
-                new = torch.empty if T else torch.zeros
+                new, dev = (torch.empty if T else torch.zeros), dy.device
                 if need_x:
                     dx = new(x_shape, dtype=torch.bfloat16, device=dev)
                 if need_w:
-                    dw = new(N, K, dtype=torch.bfloat16, device=dev)
+                    dw = new((N, K), dtype=torch.bfloat16, device=dev)
                 if need_b:
                     db = new(N, dtype=bias_type, device=dev)
                 if T:
@@ -158,17 +158,17 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     Returns:
         [..., N] bf16
     """
-    ts = (x, weight, bias, residual)
-    _no_forward_mode("linear", *ts)
+    _no_forward_mode("linear", x, weight, bias, residual)
+    device = x.device
     for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is None:
+        if t is None or (t.dtype is torch.bfloat16 and t.is_cuda and (t is x or t.device == device)):
             continue
         if not t.is_cuda:
             raise RuntimeError(f"linear: {name} must be a GPU tensor (the MI355X path has no CPU implementation)")
         if t.dtype != torch.bfloat16 and not (name == "bias" and t.dtype == torch.float32):
             raise TypeError(f"linear: {name} must be bfloat16{' or float32' if name == 'bias' else ''} (got {t.dtype})")
-        if t.device != x.device:
-            raise ValueError(f"linear: {name} is on {t.device}, x on {x.device}")
+        if t.device != device:
+            raise ValueError(f"linear: {name} is on {t.device}, x on {device}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
     N, K = weight.shape
@@ -185,6 +185,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     act = ACTIVATIONS[activation]
     with _device_of(x):
         bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                        or (bias is not None and bias.requires_grad)
+                                        or (residual is not None and residual.requires_grad)):
             return _Linear.apply(x, weight, bias, residual, act)
         return _forward(x, weight, bias, act, residual, False)[0]

@@ -23,11 +23,20 @@ _TYPES = (torch.bfloat16, torch.float32)
 
 
 def _rows(t: torch.Tensor):
-    """[..., H] as [rows, H] with contiguous rows, and the rows' stride."""
+    """[..., H] as a tensor of contiguous rows evenly apart, and the rows' stride."""
+    if t.is_contiguous():   # (as it is: only its address is used)
+        return t, t.shape[-1]
     t = t.reshape(-1, t.shape[-1])
     if t.stride(1) != 1:
         t = t.contiguous()
     return t, t.stride(0)
+
+
+def _like(t: torch.Tensor, shape, dtype):
+    """A new contiguous tensor of that shape and type (of t's, where t has them: the shorter call)."""
+    if t.dtype == dtype and t.shape == shape and t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(shape, dtype=dtype, device=t.device)
 
 
 def _f32(t) -> int:
@@ -42,22 +51,22 @@ def _bwd_workspace(rows, H, full, gate_cols, gate_rows, w, post, gate) -> int:
 def _forward(x, residual, weight, post, gate, gate_rows, scale, eps, stats):
     """(r, h, 1 / rms of r, 1 / rms of x); r None without a residual, h None without a weight."""
     H = x.shape[-1]
+    n = x.numel() // H
     dev = x.device
     x2, ldx = _rows(x)
-    n = x2.shape[0]
     r = h = rstd = rstd_x = None
     res, ldr = (None, 0) if residual is None else _rows(residual)
     if residual is not None:
-        r = torch.empty(residual.shape, dtype=residual.dtype, device=dev)
+        r = _like(residual, residual.shape, residual.dtype)
     if weight is not None:
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        h = _like(x, x.shape, x.dtype)
         rstd = torch.empty(n, dtype=torch.float32, device=dev) if stats else None
     if post is not None and stats:
         rstd_x = torch.empty(n, dtype=torch.float32, device=dev)
-    _capi.call("af3_residual_norm_fwd", x2.data_ptr(), _f32(x), ldx, _capi.ptr(res), _f32(residual), ldr,
-               _capi.ptr(weight), _f32(weight), _capi.ptr(post), _f32(post), _capi.ptr(gate), _f32(gate),
-               0 if gate is None else gate.shape[1], gate_rows, scale, eps, n, H, _capi.ptr(r), _capi.ptr(h),
-               _capi.ptr(rstd), _capi.ptr(rstd_x), _capi.stream_of(dev))
+    ptr = _capi.ptr
+    _capi.call("af3_residual_norm_fwd", x2.data_ptr(), _f32(x), ldx, ptr(res), _f32(residual), ldr, ptr(weight),
+               _f32(weight), ptr(post), _f32(post), ptr(gate), _f32(gate), 0 if gate is None else gate.shape[1],
+               gate_rows, scale, eps, n, H, ptr(r), ptr(h), ptr(rstd), ptr(rstd_x), _capi.stream_of(dev))
     return r, h, rstd, rstd_x
 
 
@@ -67,7 +76,11 @@ class _ResidualNorm(torch.autograd.Function):
         r, h, rstd, rstd_x = _forward(x, residual, weight, post, gate, gate_rows, scale, eps, True)
         keep_x = residual is None or post is not None or (gate is not None and gate.requires_grad)
         ctx.save_for_backward(x if keep_x else None, r if weight is not None else None, weight, post, gate, rstd, rstd_x)
-        ctx.args = (x.shape, x.dtype, None if residual is None else residual.dtype, gate_rows, scale)
+        full = residual is not None and (post is not None or gate is not None)
+        rt = None if residual is None else residual.dtype
+        # without norm, gate and scale the branch has the stream's own gradient, returned for both
+        same = not full and (rt is None or (scale == 1.0 and x.dtype == rt))
+        ctx.args = (x.shape, x.numel() // x.shape[-1], x.dtype, rt, gate_rows, scale, full, same)
         ctx.set_materialize_grads(False)
         if residual is None:
             return h
@@ -77,49 +90,64 @@ class _ResidualNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         _no_forward_mode("residual_norm backward", *grads)
-        x, r, weight, post, gate, rstd, rstd_x = ctx.saved_tensors
-        shape, xt, rt, gate_rows, scale = ctx.args
-        need_x, need_res, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
-        dr, dh = (None, grads[0]) if rt is None else (grads + (None,))[:2]
+        if ctx.args[3] is None:
+            dr, dh = None, grads[0]
+        else:
+            dr, dh = grads if len(grads) == 2 else (grads[0], None)
         if dr is None and dh is None:
             return (None,) * 8
-        H, n = shape[-1], math.prod(shape[:-1])
+        with _device_of(dr if dr is not None else dh):
+            return _ResidualNorm._gradients(ctx, dr, dh)
+
+    @staticmethod
+    def _gradients(ctx, dr, dh):
+        x, r, weight, post, gate, rstd, rstd_x = ctx.saved_tensors
+        shape, n, xt, rt, gate_rows, scale, full, same = ctx.args
+        need_x, need_res, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
+        H = shape[-1]
         some = dr if dr is not None else dh
-        dev = some.device
-        with _device_of(some):
-            # (saved-tensor hooks, as those that keep them on the host, may give them other strides)
-            weight, post, gate, rstd, rstd_x = (t if t is None else t.contiguous()
-                                                for t in (weight, post, gate, rstd, rstd_x))
-            dr, lddr = (None, 0) if dr is None else _rows(dr)
-            dh, lddh = (None, 0) if dh is None else _rows(dh)
-            x, ldx = (None, 0) if x is None else _rows(x)
-            r, ldr = (x, ldx) if rt is None else (None, 0) if r is None else _rows(r)
-            full = rt is not None and (post is not None or gate is not None)
-            dx = dres = dw = dpost = dgate = None
-            # without norm, gate and scale the branch has the stream's own gradient, returned for both
-            same = not full and (rt is None or (scale == 1.0 and xt == rt))
-            if need_res or (need_x and same):
-                dres = torch.empty(shape, dtype=rt or xt, device=dev)
-            if need_x and not same:
-                dx = torch.empty(shape, dtype=xt, device=dev)
-            need_w = need_w and dh is not None
-            make = torch.empty if n else torch.zeros
+        lddr = lddh = ldx = ldr = cols = ws_n = 0
+        # (saved-tensor hooks, as those that keep them on the host, may give them other strides)
+        if dr is not None:
+            dr, lddr = _rows(dr)
+        if dh is not None:
+            dh, lddh = _rows(dh)
+            weight, rstd = weight.contiguous(), rstd.contiguous()
+        if x is not None:
+            x, ldx = _rows(x)
+        if rt is None:
+            r, ldr = x, ldx
+        elif r is not None:
+            r, ldr = _rows(r)
+        if post is not None:
+            post, rstd_x = post.contiguous(), rstd_x.contiguous()
+        if gate is not None:
+            gate, cols = gate.contiguous(), gate.shape[1]
+        dx = dres = dw = dpost = dgate = ws = None
+        if need_res or (need_x and same):
+            dres = _like(some, shape, rt or xt)
+        if need_x and not same:
+            dx = _like(some, shape, xt)
+        need_w = need_w and dh is not None
+        if n:
             if need_w:
-                dw = make(H, dtype=weight.dtype, device=dev)
+                dw = torch.empty_like(weight)
             if need_post:
-                dpost = make(H, dtype=post.dtype, device=dev)
+                dpost = torch.empty_like(post)
             if need_gate:
-                dgate = make(gate.shape, dtype=gate.dtype, device=dev)
-            cols = 0 if gate is None else gate.shape[1]
-            ws_n = _bwd_workspace(n, H, int(full), cols, gate_rows, need_w, need_post, need_gate)
-            ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
-            if n:
-                _capi.call("af3_residual_norm_bwd", _capi.ptr(dr), lddr, _capi.ptr(dh), lddh, _capi.ptr(r),
-                           int((rt or xt) == torch.float32), ldr, _capi.ptr(x), int(xt == torch.float32), ldx,
-                           _capi.ptr(rstd), _capi.ptr(rstd_x), _capi.ptr(weight), _f32(weight), _capi.ptr(post),
-                           _f32(post), _capi.ptr(gate), _f32(gate), cols, gate_rows, scale, int(rt is not None), n, H,
-                           _capi.ptr(dx), _capi.ptr(dres), _capi.ptr(dw), _capi.ptr(dpost), _capi.ptr(dgate),
-                           _capi.ptr(ws), ws_n, _capi.stream_of(dev))
+                dgate = torch.empty_like(gate)
+            if need_w or need_post or need_gate:
+                ws_n = _bwd_workspace(n, H, int(full), cols, gate_rows, need_w, need_post, need_gate)
+                ws = torch.empty(ws_n, dtype=torch.uint8, device=some.device) if ws_n else None
+            ptr = _capi.ptr
+            _capi.call("af3_residual_norm_bwd", ptr(dr), lddr, ptr(dh), lddh, ptr(r), int((rt or xt) == torch.float32),
+                       ldr, ptr(x), int(xt == torch.float32), ldx, ptr(rstd), ptr(rstd_x), ptr(weight), _f32(weight),
+                       ptr(post), _f32(post), ptr(gate), _f32(gate), cols, gate_rows, scale, int(rt is not None), n, H,
+                       ptr(dx), ptr(dres), ptr(dw), ptr(dpost), ptr(dgate), ptr(ws), ws_n, _capi.stream_of(some.device))
+        else:
+            dw = torch.zeros_like(weight) if need_w else None
+            dpost = torch.zeros_like(post) if need_post else None
+            dgate = torch.zeros_like(gate) if need_gate else None
         if same and need_x:
             dx = dres
         return dx, dres if need_res else None, dw, dpost, dgate, None, None, None

@@ -359,10 +359,13 @@ def _no_forward_mode(who: str, *tensors):
             raise NotImplementedError(f"{who}: forward-mode derivatives are not supported")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _device_of(t: torch.Tensor):
     """Context with the tensor's GPU as the current one (nothing done when it already is)."""
     if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(t.device)
 
 
