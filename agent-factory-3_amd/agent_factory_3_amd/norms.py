@@ -74,13 +74,16 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, post, gate, gate_rows, scale, eps):
         r, h, rstd, rstd_x = _forward(x, residual, weight, post, gate, gate_rows, scale, eps, True)
-        keep_x = residual is None or post is not None or (gate is not None and gate.requires_grad)
-        ctx.save_for_backward(x if keep_x else None, r if weight is not None else None, weight, post, gate, rstd, rstd_x)
+        # r for the backward: as stored, or, for a weight's gradient beside a bf16 stream, made again from x and residual
+        again = residual is not None and ctx.needs_input_grad[2] and residual.dtype == torch.bfloat16
+        keep_x = residual is None or again or post is not None or gate is not None
+        ctx.save_for_backward(x if keep_x else None, None if weight is None else residual if again else r, weight, post,
+                              gate, rstd, rstd_x)
         full = residual is not None and (post is not None or gate is not None)
         rt = None if residual is None else residual.dtype
         # without norm, gate and scale the branch has the stream's own gradient, returned for both
         same = not full and (rt is None or (scale == 1.0 and x.dtype == rt))
-        ctx.args = (x.shape, x.numel() // x.shape[-1], x.dtype, rt, gate_rows, scale, full, same)
+        ctx.args = (x.shape, x.numel() // x.shape[-1], x.dtype, rt, gate_rows, scale, full, same, again)
         ctx.set_materialize_grads(False)
         if residual is None:
             return h
@@ -102,7 +105,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, dr, dh):
         x, r, weight, post, gate, rstd, rstd_x = ctx.saved_tensors
-        shape, n, xt, rt, gate_rows, scale, full, same = ctx.args
+        shape, n, xt, rt, gate_rows, scale, full, same, again = ctx.args
         need_x, need_res, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
         H = shape[-1]
         some = dr if dr is not None else dh
@@ -128,7 +131,7 @@ class _ResidualNorm(torch.autograd.Function):
             dres = _like(some, shape, rt or xt)
         if need_x and not same:
             dx = _like(some, shape, xt)
-        need_w = need_w and dh is not None
+        need_w, again = (need_w or again) and dh is not None, again and dh is not None
         if n:
             if need_w:
                 dw = torch.empty_like(weight)
@@ -141,7 +144,7 @@ class _ResidualNorm(torch.autograd.Function):
                 ws = torch.empty(ws_n, dtype=torch.uint8, device=some.device) if ws_n else None
             ptr = _capi.ptr
             _capi.call("af3_residual_norm_bwd", ptr(dr), lddr, ptr(dh), lddh, ptr(r), int((rt or xt) == torch.float32),
-                       ldr, ptr(x), int(xt == torch.float32), ldx, ptr(rstd), ptr(rstd_x), ptr(weight), _f32(weight),
+                       int(again), ldr, ptr(x), int(xt == torch.float32), ldx, ptr(rstd), ptr(rstd_x), ptr(weight), _f32(weight),
                        ptr(post), _f32(post), ptr(gate), _f32(gate), cols, gate_rows, scale, int(rt is not None), n, H,
                        ptr(dx), ptr(dres), ptr(dw), ptr(dpost), ptr(dgate), ptr(ws), ws_n, _capi.stream_of(some.device))
         else:

@@ -12,7 +12,10 @@
 //   dweight = sum_rows dh r s_r,  dpost_weight = sum_rows du x s_x
 //
 // Everything between the tensors' types is fp32; h comes from r before its rounding
-// (one rounding per output), the backward reads r as it was stored.
+// (one rounding per output).  The backward reads r as it was stored, except where the
+// weight's gradient is wanted and r is bf16: its sum over rows would be 1.45 bf16 roundings
+// off instead of 1, so r is made again from x and the residual (REC: one more tensor
+// read, 5 for 4, where neither norm nor gate needs x anyway).
 //
 // A row stays in registers from its loads to its stores, so each direction reads and
 // writes every tensor once: HBM bounds both.  NW waves share a row, a lane holding CPL
@@ -311,8 +314,8 @@ __device__ __forceinline__ void n_join(const float (&acc)[CPL][8], float* lds, i
   }
 }
 
-// ACC: some column sum is wanted
-template <class XT, class RT, int NW, int CPL, bool RES, bool FULL, bool ACC>
+// ACC: some column sum is wanted; REC: a.res is the residual, and r is made of it and x
+template <class XT, class RT, int NW, int CPL, bool RES, bool FULL, bool ACC, bool REC>
 __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const NormArgs a) {
   constexpr int WPB = NW == 1 ? 8 : NW;
   constexpr int AC = ACC ? CPL : 1;
@@ -340,7 +343,8 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
   }
   // a row's loads, made while the row before it is worked on
   NRaw<RT> r_dr[CPL], r_r[CPL];
-  NRaw<XT> r_dh[CPL], r_x[FULL ? CPL : 1];
+  constexpr bool X = FULL || REC;
+  NRaw<XT> r_dh[CPL], r_x[X ? CPL : 1];
   float r_gate[FULL ? CPL : 1][8];
   float r_s = 0.f, r_sx = 1.f, r_g1 = 1.f;
   const bool has_dr = RES && a.dr, has_dh = !RES || a.dh;
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
       if (has_dr) r_dr[c].load((const RT*)a.dr + row * a.lddr, e, H);
       if (has_dh) r_dh[c].load((const XT*)a.dh + row * a.lddh, e, H);
       if (has_dh) r_r[c].load((const RT*)a.res + row * a.ldr, e, H);
-      if constexpr (FULL) r_x[c].load((const XT*)a.x + row * a.ldx, e, H);
+      if constexpr (X) r_x[c].load((const XT*)a.x + row * a.ldx, e, H);
     }
     if (has_dh) r_s = a.s_r[row];
     if constexpr (FULL) {
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
   for (int64_t row = first; row < last; row += step) {
     if (!AHEAD) fetch(row);
     float g[CPL][8];  // the gradient of r
-    float d[CPL][8], v[CPL][8], x[FULL ? CPL : 1][8], gate[FULL ? CPL : 1][8];
+    float d[CPL][8], v[CPL][8], x[X ? CPL : 1][8], gate[FULL ? CPL : 1][8];
     const float s_r = r_s, s_x = r_sx, g1 = r_g1;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
@@ -399,10 +403,33 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
         r_dh[c].value(d[c]);
         r_r[c].value(v[c]);
       }
+      if constexpr (X) r_x[c].value(x[c]);
       if constexpr (FULL) {
-        r_x[c].value(x[c]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) gate[c][i] = r_gate[c][i];
+      }
+    }
+    if constexpr (REC) {
+      if (has_dh) {
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) {
+          float w[8];
+          if constexpr (FULL && AHEAD) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = w_post[c][i];
+          } else if constexpr (FULL) {
+            if (a.post) n_get(a.post, a.post_f32, 0, (c * 64 * NW + t) * 8, H, w);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float u = x[c][i];
+            if constexpr (FULL) {
+              if (a.post) u *= s_x * w[i];
+              if (a.gate_cols) u *= a.gate_cols > 1 ? gate[c][i] : g1;
+            }
+            v[c][i] += a.scale * u;
+          }
+        }
       }
     }
     if (AHEAD && row + step < last) fetch(row + step);
@@ -595,13 +622,13 @@ void norm_fwd_launch(const NormArgs& a, hipStream_t st) {
 #undef AF3_NF
 }
 
-template <class XT, class RT, bool RES, bool FULL, bool ACC>
+template <class XT, class RT, bool RES, bool FULL, bool ACC, bool REC>
 void norm_bwd_launch(const NormArgs& a, unsigned blocks, hipStream_t st) {
   const int chunks = (int)af3_cdiv(a.H, 8);
 #define AF3_NB(NW, CPL)                                                                                           \
   do {                                                                                                            \
     const dim3 block(NW == 4 ? 256 : 512);                                                                         \
-    hipLaunchKernelGGL((norm_bwd_kernel<XT, RT, NW, CPL, RES, FULL, ACC>), dim3(blocks), block, 0, st, a);         \
+    hipLaunchKernelGGL((norm_bwd_kernel<XT, RT, NW, CPL, RES, FULL, ACC, REC>), dim3(blocks), block, 0, st, a);         \
     return;                                                                                                       \
   } while (0)
   if constexpr (!FULL) if (norm_wide(a.rows, a.H, FULL, 2)) {
@@ -710,14 +737,14 @@ namespace {
 template <class XT, class RT, bool RES, bool FULL>
 void norm_bwd_pick(const NormArgs& a, unsigned blocks, bool acc, hipStream_t st) {
   if (acc)
-    norm_bwd_launch<XT, RT, RES, FULL, true>(a, blocks, st);
+    norm_bwd_launch<XT, RT, RES, FULL, true, false>(a, blocks, st);
   else
-    norm_bwd_launch<XT, RT, RES, FULL, false>(a, blocks, st);
+    norm_bwd_launch<XT, RT, RES, FULL, false, false>(a, blocks, st);
 }
 }  // namespace
 
 extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* dh, int64_t lddh, const void* r, int r_f32,
-                                     int64_t ldr, const void* x, int x_f32, int64_t ldx, const float* rstd,
+                                     int r_again, int64_t ldr, const void* x, int x_f32, int64_t ldx, const float* rstd,
                                      const float* rstd_x, const void* weight, int w_f32, const void* post_weight,
                                      int post_f32, const void* gate, int gate_f32, int gate_cols, int64_t gate_rows,
                                      float scale, int has_residual, int64_t rows, int H, void* dx, void* dresidual,
@@ -735,6 +762,8 @@ extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* d
   const bool full = has_residual && (post_weight || gate_cols);
   AF3_REQUIRE(!dh || (r && rstd && weight), "residual_norm_bwd: dh needs r, rstd and weight");
   AF3_REQUIRE(dr || dh, "residual_norm_bwd: no gradient arrives");
+  AF3_REQUIRE(!r_again || (has_residual && !r_f32 && !x_f32 && x && dh && dweight),
+              "residual_norm_bwd: r_again goes with a bf16 residual, x, dh and dweight");
   AF3_REQUIRE(!full || (x && (!post_weight || rstd_x) && (!gate_cols || gate)), "residual_norm_bwd: null pointer");
   const NormPlan p = norm_plan(rows, H, gate_cols, gate_rows, full, dweight != nullptr, dpost != nullptr, dgate != nullptr);
   AF3_REQUIRE(p.blocks < (int64_t)1 << 31 && (p.groups + 2) * af3_cdiv(H, kJoinCols) < (int64_t)1 << 31, "residual_norm_bwd: too many gate rows");
@@ -770,6 +799,11 @@ extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* d
       norm_bwd_pick<uint16_t, float, true, true>(a, blocks, acc, st);
     else
       norm_bwd_pick<uint16_t, float, true, false>(a, blocks, acc, st);
+  } else if (r_again) {
+    if (full)
+      norm_bwd_launch<uint16_t, uint16_t, true, true, true, true>(a, blocks, st);
+    else
+      norm_bwd_launch<uint16_t, uint16_t, true, false, true, true>(a, blocks, st);
   } else {
     if (full)
       norm_bwd_pick<uint16_t, uint16_t, true, true>(a, blocks, acc, st);

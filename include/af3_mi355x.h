@@ -502,10 +502,11 @@ int af3_seq_starts_rows(const int64_t* position_ids, int64_t ld, int n_rows, int
  * rows i gate_rows .. .  rstd, rstd_x [rows] fp32 (of r and of x) for the
  * backward, or NULL.
  * Backward: dr (NULL: none) and dh (NULL: none) arrive at r and h, r as the
- * forward wrote it (x without a residual).  dresidual = dr + the norm's gradient
+ * forward wrote it (x without a residual); with r_again the residual itself, bf16: r
+ * is made again from it and x, for a dweight of one rounding.  dresidual = dr + the norm's gradient
  * (without a residual this is x's gradient); dx, dweight, dpost, dgate, each NULL
  * if not wanted, in their tensors' types; sums are fp32 in a fixed order.  x is
- * read where there is a post_weight or gate. */
+ * read where there is a post_weight or gate, and with r_again. */
 int af3_residual_norm_fwd(const void* x, int x_f32, int64_t ldx, const void* residual, int r_f32, int64_t ldr,
                           const void* weight, int w_f32, const void* post_weight, int post_f32, const void* gate,
                           int gate_f32, int gate_cols, int64_t gate_rows, float scale, float eps, int64_t rows, int H,
@@ -513,7 +514,7 @@ int af3_residual_norm_fwd(const void* x, int x_f32, int64_t ldx, const void* res
 size_t af3_residual_norm_bwd_workspace_bytes(int64_t rows, int H, int full, int gate_cols, int64_t gate_rows,
                                              int want_w, int want_post, int want_gate);
 int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* dh, int64_t lddh, const void* r, int r_f32,
-                          int64_t ldr, const void* x, int x_f32, int64_t ldx, const float* rstd, const float* rstd_x,
+                          int r_again, int64_t ldr, const void* x, int x_f32, int64_t ldx, const float* rstd, const float* rstd_x,
                           const void* weight, int w_f32, const void* post_weight, int post_f32, const void* gate,
                           int gate_f32, int gate_cols, int64_t gate_rows, float scale, int has_residual, int64_t rows,
                           int H, void* dx, void* dresidual, void* dweight, void* dpost, void* dgate, void* workspace,

@@ -55,7 +55,8 @@ def residual_norm(x, residual=None, weight=None, *, eps=1e-5, post=None, gate=No
         e_m = (dw.abs() * d_r).mean(-1, keepdim=True) + 2.0 ** -18 * am
         e_g = e_g + s ** 3 * (r.abs() * e_m + d_r * m.abs()) + (3 * e_s + 2.0 ** -20) * (s * dw.abs() + s ** 3 * r.abs() * am)
         o["dweight"] = (dh * r * s).sum(0)
-        o["dweight_tol"] = ((dh * s).abs() * d_r + (e_s + 2.0 ** -14) * (dh * r * s).abs()).sum(0)
+        # (over a bf16 stream r is made again for it)
+        o["dweight_tol"] = ((dh * s).abs() * (e_r if u_r > 2.0 ** -20 else d_r) + (e_s + 2.0 ** -14) * (dh * r * s).abs()).sum(0)
     if res is None:
         o["dx"], o["dx_tol"] = G, u_x * G.abs() + e_g
     else:
