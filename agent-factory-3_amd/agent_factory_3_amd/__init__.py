@@ -8,11 +8,12 @@ hand-written HIP kernels behind the C ABI of ``libaf3_mi355x.so``.
 Public modules mirror the reference's file names:
 ``kernels``, ``quantization``, ``quantizer_config``, ``routing_replay``,
 ``fsdp2_fix``; ``routing`` holds the routing objects the reference imports
-from ``triton_kernels``.
+from ``triton_kernels``.  Beside them: ``attention``, ``norms``, ``linear`` and
+``grad_clip`` (``fused_layers`` puts the norms and projections into a model).
 """
 from . import _capi  # noqa: F401
 
-__all__ = ["Mxfp4Bf16DequantConfig", "enable_routing_replay"]
+__all__ = ["Mxfp4Bf16DequantConfig", "enable_fused_layers", "enable_routing_replay"]
 
 
 def __getattr__(name):
@@ -23,4 +24,7 @@ def __getattr__(name):
     if name == "enable_routing_replay":
         from .routing_replay import enable_routing_replay
         return enable_routing_replay
+    if name == "enable_fused_layers":
+        from .fused_layers import enable_fused_layers
+        return enable_fused_layers
     raise AttributeError(name)

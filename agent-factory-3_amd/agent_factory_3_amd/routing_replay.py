@@ -15,6 +15,7 @@ the recomputed forward replays the same experts.
 """
 from __future__ import annotations
 
+import contextlib
 import logging
 
 logger = logging.getLogger(__name__)
@@ -25,6 +26,30 @@ _ATTR = "_af3_replay_router_indices"
 def current_router_indices(mlp):
     """Indices the enclosing decoder layer set for this MLP (None outside replay)."""
     return getattr(mlp, _ATTR, None)
+
+
+@contextlib.contextmanager
+def layer_indices(layer, kwargs):
+    """For a forward that stands in for a decoder layer's: the layer's expert choices out of its keyword
+    arguments, exposed to its MLP while it runs (where replay is enabled and they are given; an enclosing
+    wrapper's stay)."""
+    if not getattr(type(layer), "_af3_routing_replay", False):
+        yield
+        return
+    of_model, indices = kwargs.pop("routing_indices", None), kwargs.pop("router_indices", None)
+    if indices is None and of_model is not None:
+        if of_model.dim() != 4:
+            raise ValueError(f"routing_indices must be [B, S, L, K], got {tuple(of_model.shape)}")
+        indices = of_model[:, :, layer.self_attn.layer_idx, :]
+    if indices is None:
+        yield
+        return
+    prev = getattr(layer.mlp, _ATTR, None)
+    setattr(layer.mlp, _ATTR, indices)
+    try:
+        yield
+    finally:
+        setattr(layer.mlp, _ATTR, prev)
 
 
 def enable_routing_replay(model=None):

@@ -1,0 +1,195 @@
+"""gpt-oss trained with the operators together: fused norms and projections, sink attention, MXFP4 experts with
+adapters, the balance loss, and the gradients' clipping.
+
+Inside the model every norm, add-and-norm and projection call is held to the float64 oracle on the tensors that it
+saw, forward and backward; the model's output to the same model without them.
+"""
+import pytest
+import torch
+
+from agent_factory_3_amd import fused_layers, grad_clip, linear as lin, norms, routing, routing_replay
+from agent_factory_3_amd import quantization as Q
+from oracle import linear as ol
+from oracle import norms as on
+from tests.test_gpu_attention_model import E, H, K, _ids, _model, _rel, _replay
+
+pytestmark = pytest.mark.gpu
+
+
+class _Spy:
+    """Records the operators' calls in a model, with the gradients that arrive."""
+
+    def __init__(self, monkeypatch):
+        self.calls = []
+
+        def record(kind, orig):
+            def call(*args, **kw):
+                out = orig(*args, **kw)
+                c = dict(kind=kind, args=args, kw=kw, out=out, g={})
+                for i, t in enumerate(out if isinstance(out, tuple) else (out,)):
+                    if t.requires_grad:
+                        t.register_hook(lambda g, i=i, c=c: c["g"].__setitem__(i, g.detach().clone()))
+                self.calls.append(c)
+                return out
+            return call
+        monkeypatch.setattr(norms, "rms_norm", record("rms", norms.rms_norm))
+        monkeypatch.setattr(norms, "residual_norm", record("residual", norms.residual_norm))
+        monkeypatch.setattr(fused_layers, "linear", record("linear", lin.linear))
+
+    def check(self):
+        """Values of every call, and the gradients of the call made again alone with what arrived."""
+        cpu = lambda t: None if t is None else t.detach().cpu()  # noqa: E731
+        for i, c in enumerate(self.calls):
+            a = c["args"]
+            up = [c["g"].get(j) for j in range(2)]
+            leaf = [t.detach().requires_grad_() if isinstance(t, torch.Tensor) else t for t in a]
+            flat = lambda t: None if t is None else cpu(t).reshape(-1, t.shape[-1])  # noqa: E731
+            if c["kind"] == "linear":
+                ref = ol.linear(flat(a[0]), cpu(a[1]), cpu(a[2]), dy=flat(up[0]))
+                got, names = {"y": c["out"]}, ("dx", "dweight", "dbias")
+                again = ORIG["linear"](*leaf)
+            elif c["kind"] == "rms":
+                ref = on.residual_norm(flat(a[0]), None, cpu(a[1]), eps=a[2], dh=flat(up[0]))
+                got, names = {"h": c["out"]}, ("dx", "dweight")
+                again = ORIG["rms"](*leaf)
+            else:
+                ref = on.residual_norm(flat(a[0]), flat(a[1]), cpu(a[2]), eps=c["kw"]["eps"], dr=flat(up[0]), dh=flat(up[1]))
+                got, names = {"r": c["out"][0], "h": c["out"][1]}, ("dx", "dresidual", "dweight")
+                again = ORIG["residual"](*leaf, **c["kw"])
+            outs = [(o, u) for o, u in zip(again if isinstance(again, tuple) else (again,), up) if u is not None]
+            ts = [t for t in leaf if isinstance(t, torch.Tensor)]
+            if outs:
+                got.update(zip(names, torch.autograd.grad([o for o, _ in outs], ts, [u for _, u in outs])))
+            for n, t in got.items():
+                err = (t.detach().cpu().double().reshape(ref[n].shape) - ref[n]).abs()
+                assert (err <= ref[n + "_tol"]).all(), (i, c["kind"], n, float((err / ref[n + "_tol"]).max()))
+
+
+ORIG = {"linear": lin.linear, "rms": norms.rms_norm, "residual": norms.residual_norm}
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_model_matches_oracle_and_the_unfused_model(dev, padded, monkeypatch):
+    routing_replay.enable_routing_replay()
+    ids, ri = _ids(2, 50).to(dev), _replay(2, 50).to(dev)
+    mask = torch.ones(2, 50, dtype=torch.long, device=dev)
+    if padded:
+        mask[1, 37:] = 0
+    w = torch.randn(2, 50, H, generator=torch.Generator().manual_seed(3)).to(dev) * mask[..., None]
+    plain = _model(dev, "af3_sink")
+    with torch.no_grad():
+        want = plain(input_ids=ids, attention_mask=mask, routing_indices=ri, use_cache=False).last_hidden_state
+    model = _model(dev, "af3_sink")
+    assert fused_layers.enable_fused_layers(model) == 2
+    spy = _Spy(monkeypatch)
+    out = model(input_ids=ids, attention_mask=mask, routing_indices=ri, use_cache=False).last_hidden_state
+    (out.float() * w).sum().backward()
+    kinds = [c["kind"] for c in spy.calls]
+    assert kinds == ["rms"] + ["linear"] * 4 + ["residual"] + ["rms"] + ["linear"] * 4 + ["residual"] + ["rms"]
+    spy.check()
+    assert all(p.grad is not None and p.grad.isfinite().all() for n, p in model.named_parameters()
+               if p.requires_grad and "embed" not in n and "router" not in n)
+    # per layer about ten roundings to bf16 (2^-9 rms each) meet on the stream, in each of the two evaluations:
+    # 2^-9 sqrt(2 * 10 * 2) = 1.3e-2; allowed: three times that
+    assert _rel(out.detach() * mask[..., None], want * mask[..., None]) < 4e-2
+
+
+def test_generation_with_a_cache(dev):
+    """Single tokens (the weight-streaming products) after a prompt match the whole row."""
+    routing_replay.enable_routing_replay()
+    model = _model(dev, "af3_sink")
+    fused_layers.enable_fused_layers(model)
+    ids, ri = _ids(1, 48).to(dev), _replay(1, 48).to(dev)
+    with torch.no_grad():
+        whole = model(input_ids=ids, routing_indices=ri, use_cache=False).last_hidden_state
+        out = model(input_ids=ids[:, :40], routing_indices=ri[:, :40], use_cache=True)
+        got = []
+        for t in range(40, 48):
+            out = model(input_ids=ids[:, t:t + 1], routing_indices=ri[:, t:t + 1], past_key_values=out.past_key_values,
+                        use_cache=True)
+            got.append(out.last_hidden_state)
+    # the same products in another order of sums: roundings alike but for a few
+    assert _rel(torch.cat(got, 1), whole[:, 40:]) < 2e-2
+
+
+def test_training_step_of_everything(dev):
+    """Expert adapters, routers and norms trained with a balance loss under activation checkpointing, gradients
+    clipped: the gradients are those of the step without clipping times one factor, the same bits every time."""
+    routing_replay.enable_routing_replay()
+    model = _model(dev, "af3_sink")
+    for layer in model.layers:
+        Q.enable_expert_lora(layer.mlp.experts, r=16, lora_alpha=32)
+        for n in ("gate_up_proj_lora_B", "down_proj_lora_B"):
+            p = getattr(layer.mlp.experts, n)
+            with torch.no_grad():
+                p.copy_(torch.randn(p.shape, generator=torch.Generator().manual_seed(5)) * 0.05)
+    fused_layers.enable_fused_layers(model)
+    model.gradient_checkpointing_enable(dict(use_reentrant=False))
+    model.train()
+    ids = _ids(2, 60).to(dev)
+    mask = torch.ones(2, 60, dtype=torch.long, device=dev)
+    mask[1, 41:] = 0
+    w = torch.randn(2, 60, H, generator=torch.Generator().manual_seed(3)).to(dev) * mask[..., None]
+    params = [p for n, p in model.named_parameters() if p.requires_grad and "embed" not in n]
+
+    def step(max_norm):
+        for p in params:
+            p.grad = None
+        with routing.collect_balance(mask) as balance:
+            out = model(input_ids=ids, attention_mask=mask, use_cache=False).last_hidden_state
+        ((out.float() * w).sum() + 10.0 * balance.loss()).backward()
+        norm = grad_clip.clip_grad_norm_(params, max_norm)
+        return norm, [None if p.grad is None else p.grad.clone() for p in params]
+    norm, free = step(1e9)
+    flat = torch.cat([g.double().reshape(-1) for g in free if g is not None])
+    assert abs(float(norm) - float(flat.norm())) <= 2.0 ** -23 * float(norm)
+    again, clipped = step(1.0)
+    assert torch.equal(norm, again) and float(norm) > 1.0
+    f = 1.0 / (float(norm) + 1e-6)
+    for a, b in zip(free, clipped):
+        if a is not None:   # fp32's roundings of the factor and the product, then the type's
+            tol = a.double().abs() * f * (torch.finfo(a.dtype).eps / 2 + 2.0 ** -21) + 2.0 ** -133
+            assert ((b.double() - a.double() * f).abs() <= tol).all()
+    assert sum(g is not None for g in free) >= len(params) - 4   # (the routers get theirs from the balance loss)
+
+
+def test_projections_under_peft_style_wrappers(dev):
+    """A wrapper with a base_layer inside (as PEFT's) keeps its adapter's share around the fused product."""
+    class Wrapped(torch.nn.Module):
+        def __init__(self, base):
+            super().__init__()
+            self.base_layer = base
+            self.a = torch.nn.Parameter(torch.randn(4, base.in_features, device=dev).to(torch.bfloat16) * 0.1)
+            self.b = torch.nn.Parameter(torch.randn(base.out_features, 4, device=dev).to(torch.bfloat16) * 0.1)
+
+        def forward(self, x):
+            return self.base_layer(x) + x @ self.a.t() @ self.b.t()
+    model = _model(dev, "af3_sink")
+    torch.manual_seed(1)
+    for layer in model.layers:
+        layer.self_attn.q_proj = Wrapped(layer.self_attn.q_proj)
+    ids = _ids(1, 33).to(dev)
+    routing_replay.enable_routing_replay()
+    ri = _replay(1, 33).to(dev)
+    with torch.no_grad():
+        want = model(input_ids=ids, routing_indices=ri, use_cache=False).last_hidden_state
+    fused_layers.enable_fused_layers(model)
+    assert model.layers[0].self_attn.q_proj.base_layer.forward.__func__ is fused_layers._linear_forward
+    with torch.no_grad():
+        got = model(input_ids=ids, routing_indices=ri, use_cache=False).last_hidden_state
+    assert _rel(got, want) < 4e-2   # (as for the whole model above)
+
+
+def test_other_types_run_as_they_did(dev):
+    """A model in fp32 keeps transformers' projections (and takes the fp32 norms)."""
+    from transformers.models.gpt_oss.modeling_gpt_oss import GptOssRMSNorm
+    norm = GptOssRMSNorm(128).to(dev)
+    norm.forward = fused_layers._norm_forward.__get__(norm)
+    x = torch.randn(5, 128, device=dev)
+    assert torch.allclose(norm(x), type(norm).forward(norm, x), rtol=2e-6, atol=1e-6)
+    half = norm.half()
+    assert torch.equal(half(x.half()), type(norm).forward(half, x.half()))
+    m = torch.nn.Linear(8, 4).to(dev)
+    m.forward = fused_layers._linear_forward.__get__(m)
+    y = torch.randn(3, 8, device=dev)
+    assert torch.equal(m(y), torch.nn.functional.linear(y, m.weight, m.bias))
