@@ -38,9 +38,9 @@ def _aligned(t: torch.Tensor):
         if ld % 8 == 0 and C <= ld < _MAX_STRIDE:
             return t, ld
     width = (C + 7) // 8 * 8
-    c = torch.empty(t.shape[0], width, dtype=t.dtype, device=t.device)
-    c[:, :C].copy_(t)
-    c[:, C:].zero_()
+    c = torch.empty((t.shape[0], width), dtype=t.dtype, device=t.device)
+    _capi.call("af3_linear_dz", t.data_ptr(), ld, None, 0, t.shape[0], C, c.data_ptr(), width, None, 0, None, 0,
+               _capi.stream_of(t.device))   # (without an activation: a copy with zeros after each row)
     return c, width
 
 
@@ -115,20 +115,21 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def _products(dy, x, weight, z, act, T, N, K, dx, dw, db):
-        dev = dy.device
-        dz, ldz = dy, dy.stride(0) if T > 1 else N
+        dz, ldy = dy, dy.stride(0) if T > 1 else N
+        ldz = ldy
         use = dx is not None or dw is not None
-        make = act or (use and (N % 8 or dz.data_ptr() % 16 or ldz % 8 or not N <= ldz < _MAX_STRIDE))
-        if make and use:
+        # dz in a tensor of its own: behind an activation, or where dy's rows are not as the products read them
+        make = use and (act or N % 8 or ldy % 8 or dy.data_ptr() % 16 or not N <= ldy < _MAX_STRIDE)
+        if make:
             ldz = (N + 7) // 8 * 8
-            dz = torch.empty(T, ldz, dtype=torch.bfloat16, device=dev)
-        if (make and use) or db is not None:
+            dz = torch.empty((T, ldz), dtype=torch.bfloat16, device=dy.device)
+        if make or db is not None:
             ws_n = _dz_workspace(T, N) if db is not None else 0
-            ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
+            ws = torch.empty(ws_n, dtype=torch.uint8, device=dy.device) if ws_n else None
             z = z if z is None else z.contiguous()
-            _capi.call("af3_linear_dz", dy.data_ptr(), dy.stride(0), _capi.ptr(z), act, T, N,
-                       dz.data_ptr() if make and use else None, ldz, _capi.ptr(db),
-                       int(db is not None and db.dtype == torch.float32), _capi.ptr(ws), ws_n, _capi.stream_of(dev))
+            _capi.call("af3_linear_dz", dy.data_ptr(), ldy, _capi.ptr(z), act, T, N, dz.data_ptr() if make else None, ldz,
+                       _capi.ptr(db), int(db is not None and db.dtype == torch.float32), _capi.ptr(ws), ws_n,
+                       _capi.stream_of(dy.device))
         if dx is not None:
             w, ldw = _aligned(_rows(weight))
             _product(dz, ldz, 0, w, ldw, 1, T, K, N, dx)

@@ -93,66 +93,78 @@ class _ResidualNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         _no_forward_mode("residual_norm backward", *grads)
-        if ctx.args[3] is None:
-            dr, dh = None, grads[0]
-        else:
-            dr, dh = grads if len(grads) == 2 else (grads[0], None)
-        if dr is None and dh is None:
+        dr, dh = (None, grads[0]) if ctx.args[3] is None else grads if len(grads) == 2 else (grads[0], None)
+        some = dr if dr is not None else dh
+        if some is None:
             return (None,) * 8
-        with _device_of(dr if dr is not None else dh):
-            return _ResidualNorm._gradients(ctx, dr, dh)
+        if some.get_device() == torch.cuda.current_device():
+            return _ResidualNorm._gradients(ctx, dr, dh, some)
+        with torch.cuda.device(some.device):
+            return _ResidualNorm._gradients(ctx, dr, dh, some)
 
     @staticmethod
-    def _gradients(ctx, dr, dh):
+    def _gradients(ctx, dr, dh, some):
         x, r, weight, post, gate, rstd, rstd_x = ctx.saved_tensors
         shape, n, xt, rt, gate_rows, scale, full, same, again = ctx.args
         need_x, need_res, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
         H = shape[-1]
-        some = dr if dr is not None else dh
-        lddr = lddh = ldx = ldr = cols = ws_n = 0
+        p_dr = p_dh = p_r = p_x = p_w = p_rstd = p_post = p_rstd_x = p_gate = p_dx = p_dres = p_dw = p_ws = None
+        lddr = lddh = ldx = ldr = cols = w32 = ws_n = 0
+        dx = dres = dw = dpost = dgate = None
         # (saved-tensor hooks, as those that keep them on the host, may give them other strides)
         if dr is not None:
             dr, lddr = _rows(dr)
+            p_dr = dr.data_ptr()
         if dh is not None:
             dh, lddh = _rows(dh)
             weight, rstd = weight.contiguous(), rstd.contiguous()
+            p_dh, p_w, p_rstd, w32 = dh.data_ptr(), weight.data_ptr(), rstd.data_ptr(), _f32(weight)
+        else:
+            need_w = again = False
         if x is not None:
             x, ldx = _rows(x)
+            p_x = x.data_ptr()
         if rt is None:
-            r, ldr = x, ldx
+            p_r, ldr = p_x, ldx
         elif r is not None:
             r, ldr = _rows(r)
-        if post is not None:
-            post, rstd_x = post.contiguous(), rstd_x.contiguous()
-        if gate is not None:
-            gate, cols = gate.contiguous(), gate.shape[1]
-        dx = dres = dw = dpost = dgate = ws = None
+            p_r = r.data_ptr()
+        if full:
+            if post is not None:
+                post, rstd_x = post.contiguous(), rstd_x.contiguous()
+                p_post, p_rstd_x = post.data_ptr(), rstd_x.data_ptr()
+            if gate is not None:
+                gate, cols = gate.contiguous(), gate.shape[1]
+                p_gate = gate.data_ptr()
         if need_res or (need_x and same):
             dres = _like(some, shape, rt or xt)
-        if need_x and not same:
-            dx = _like(some, shape, xt)
-        need_w, again = (need_w or again) and dh is not None, again and dh is not None
-        if n:
-            if need_w:
-                dw = torch.empty_like(weight)
-            if need_post:
-                dpost = torch.empty_like(post)
-            if need_gate:
-                dgate = torch.empty_like(gate)
-            if need_w or need_post or need_gate:
-                ws_n = _bwd_workspace(n, H, int(full), cols, gate_rows, need_w, need_post, need_gate)
-                ws = torch.empty(ws_n, dtype=torch.uint8, device=some.device) if ws_n else None
-            ptr = _capi.ptr
-            _capi.call("af3_residual_norm_bwd", ptr(dr), lddr, ptr(dh), lddh, ptr(r), int((rt or xt) == torch.float32),
-                       int(again), ldr, ptr(x), int(xt == torch.float32), ldx, ptr(rstd), ptr(rstd_x), ptr(weight), _f32(weight),
-                       ptr(post), _f32(post), ptr(gate), _f32(gate), cols, gate_rows, scale, int(rt is not None), n, H,
-                       ptr(dx), ptr(dres), ptr(dw), ptr(dpost), ptr(dgate), ptr(ws), ws_n, _capi.stream_of(some.device))
-        else:
-            dw = torch.zeros_like(weight) if need_w else None
-            dpost = torch.zeros_like(post) if need_post else None
-            dgate = torch.zeros_like(gate) if need_gate else None
-        if same and need_x:
-            dx = dres
+            p_dres = dres.data_ptr()
+        if need_x:
+            if same:
+                dx = dres
+            else:
+                dx = _like(some, shape, xt)
+                p_dx = dx.data_ptr()
+        if not n:
+            return (dx, dres if need_res else None, *(torch.zeros_like(t) if need else None for t, need in
+                                                      ((weight, need_w), (post, need_post), (gate, need_gate))),
+                    None, None, None)
+        if need_w or again:
+            dw = torch.empty_like(weight)
+            p_dw = dw.data_ptr()
+        if need_post:
+            dpost = torch.empty_like(post)
+        if need_gate:
+            dgate = torch.empty_like(gate)
+        if p_dw is not None or need_post or need_gate:
+            ws_n = _bwd_workspace(n, H, int(full), cols, gate_rows, p_dw is not None, need_post, need_gate)
+            if ws_n:
+                ws = torch.empty(ws_n, dtype=torch.uint8, device=some.device)
+                p_ws = ws.data_ptr()
+        _capi.call("af3_residual_norm_bwd", p_dr, lddr, p_dh, lddh, p_r, int((rt or xt) == torch.float32), int(again), ldr,
+                   p_x, int(xt == torch.float32), ldx, p_rstd, p_rstd_x, p_w, w32, p_post, _f32(post), p_gate,
+                   _f32(gate), cols, gate_rows, scale, int(rt is not None), n, H, p_dx, p_dres, p_dw, _capi.ptr(dpost),
+                   _capi.ptr(dgate), p_ws, ws_n, _capi.stream_of(some.device))
         return dx, dres if need_res else None, dw, dpost, dgate, None, None, None
 
 
@@ -166,17 +178,23 @@ def _check_tensor(who, name, t, device):
 
 
 def _check(who, x, weight, post, eps):
-    _check_tensor(who, "x", x, x.device)
-    H = x.shape[-1] if x.dim() else 0
+    device, shape = x.device, x.shape
+    _check_tensor(who, "x", x, device)
+    H = shape[-1] if shape else 0
     if not MIN_HIDDEN <= H <= MAX_HIDDEN:
-        raise ValueError(f"{who}: x must be [..., H] with H from {MIN_HIDDEN} to {MAX_HIDDEN}, got {tuple(x.shape)}")
-    for name, t in (("weight", weight), ("post_weight", post)):
-        if t is not None:
-            _check_tensor(who, name, t, x.device)
-            if t.shape != (H,):
-                raise ValueError(f"{who}: {name} must be [{H}], got {tuple(t.shape)}")
+        raise ValueError(f"{who}: x must be [..., H] with H from {MIN_HIDDEN} to {MAX_HIDDEN}, got {tuple(shape)}")
+    if weight is not None:
+        _check_weight(who, "weight", weight, device, H)
+    if post is not None:
+        _check_weight(who, "post_weight", post, device, H)
     if not (0.0 <= eps < math.inf):
         raise ValueError(f"{who}: eps must not be negative, got {eps}")
+
+
+def _check_weight(who, name, t, device, H):
+    _check_tensor(who, name, t, device)
+    if t.shape != (H,):
+        raise ValueError(f"{who}: {name} must be [{H}], got {tuple(t.shape)}")
 
 
 def _gate_rows(gate, shape):
@@ -254,8 +272,10 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
             gate_rows = max(gate_rows, 1)
         weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
         post_weight = post_weight if post_weight is None or post_weight.is_contiguous() else post_weight.contiguous()
-        ts = (x, residual, weight, post_weight, gate)
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-            out = _ResidualNorm.apply(*ts, gate_rows, scale, eps)
+        if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad
+                                        or (weight is not None and weight.requires_grad)
+                                        or (post_weight is not None and post_weight.requires_grad)
+                                        or (gate is not None and gate.requires_grad)):
+            out = _ResidualNorm.apply(x, residual, weight, post_weight, gate, gate_rows, scale, eps)
             return out if weight is not None else (out, None)
-        return _forward(*ts, gate_rows, scale, eps, False)[:2]
+        return _forward(x, residual, weight, post_weight, gate, gate_rows, scale, eps, False)[:2]
