@@ -30,11 +30,13 @@
 // stores drain under the next's first.
 //
 // Measured (library product of the same operands in brackets), us: 8192 x 4096 from 2880
-// 155 (134), 8192 x 2880 from 4096 with W as stored 159 (190), 16384 x 2880 from 4096 313
-// (271), 16384 x 4096 from 2880 with W as stored 300 (299), 2880 x 4096 from 16384 rows
-// 331 (431); 1021 x 2880 from 2880 22.6 (24.5), 8192 x 512 from 2880 26 (27).  The large
-// ones run 1.17 to 1.29 PFLOP/s at 1.75 GHz: 73% of the CUs' busy cycles issue products, and
-// taking out the copies, or the fragment reads, gains 4 and 14%; the card's power bounds them.
+// 157 (140), 8192 x 2880 from 4096 with W as stored 168 (193), 16384 x 2880 from 4096 329
+// (285), with bias and residual 335 (and an add of 55), 16384 x 4096 from 2880 with W as
+// stored 309 (308), 2880 x 4096 from 16384 rows 326 (446); 1021 x 2880 from 2880 24 (26),
+// 8192 x 512 from 2880 28 (29).  The large ones run 1.17 to 1.29 PFLOP/s at 1.75 GHz: 73% of
+// the CUs' busy cycles issue products, and taking out the copies, or the fragment reads,
+// gains 4 and 14%; the card's power bounds them.  Products of 16 x 16 x 32 (3 to 5% less time
+// in 128 x 128 tiles) leave the compiler moving accumulators between register files.
 //
 // Few tiles and a long k (dW of narrow layers): blocks share a tile's k-steps and write
 // fp32 partials, which lin_join_kernel adds in order and gives the epilogue.
@@ -193,6 +195,15 @@ template <int V>
 struct Int {
   static constexpr int value = V;
 };
+// f(Int<0>) .. f(Int<N - 1>)
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void lin_unroll(F&& f) {
+  if constexpr (I < N) {
+    f(Int<I>{});
+    lin_unroll<N, I + 1>(f);
+  }
+}
+
 template <bool V>
 struct Flag {
   static constexpr bool value = V;
@@ -239,8 +250,9 @@ __device__ __forceinline__ void lin_copy_tail(int wave, int lane, int left, int 
   }
 }
 
-// BM x BN tile, see above.  MASKED outputs past M, N are not stored; loads there repeat the last row.
-template <int BM, int BN, int ST, bool PT, bool QT>
+// BM x BN tile, see above.  RES: with a residual and no activation, whole tiles load it ahead
+// (a kernel of its own: the registers that takes cost the others 5%).  MASKED outputs past M, N are not stored; loads there repeat the last row.
+template <int BM, int BN, int ST, bool PT, bool QT, bool RES>
 __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void lin_kernel(const LinArgs a) {
   using TP = LinTile<BM, PT>;
   using TQ = LinTile<BN, QT>;
@@ -454,37 +466,60 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
       setup();
       first_copies(ahead(cur, 1));
     }
+    // what the epilogue reads from memory lands meanwhile: the bias of the lane's 8 columns, and
+    // with RES the residual of a whole tile's first two bands of 32 rows
+    constexpr int W = BN / 2;        // columns of a wave
+    constexpr int LPR = W / 8;       // lanes per row when read back
+    constexpr int RPI = 64 / LPR;    // rows a wave reads at a time: a lane keeps its 8 columns
+    constexpr int IT = (32 + RPI - 1) / RPI;
+    const int c8 = lane % LPR * 8, col = en0 + c8;
+    float bias[8];
+    lin_bias(a.e, lane < RPI * LPR ? col : a.N, a.N, bias);
+    const bool plain = RES && whole_tile;
+    auto there = [&](int g) { return g * RPI + lane / LPR < 32 && lane < RPI * LPR; };
+    uint32_t res[2][RES ? IT : 1][4];
+    auto fetch_res = [&](int tm, uint32_t (&r)[RES ? IT : 1][4]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int g = 0; g < (RES ? IT : 0); ++g)
+        __builtin_memcpy(r[g], a.e.res + (int64_t)(em0 + tm * 32 + min(g * RPI + lane / LPR, 31)) * a.e.ldr + col, 16);
+    };
+    if (plain) {
+      fetch_res(0, res[0]);
+      fetch_res(1, res[1]);
+    }
     step(Flag<false>{}, cur);
     phase(Flag<false>{}, Int<1>{}, Int<-1>{}, 0, 0);
 
     // epilogue, in the last k-step's stage: lane (r, h) holds row r of a 32 x 32 part,
     // columns 8 j + 4 h + (0..3)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    constexpr int W = BN / 2;        // columns of a wave
+    // (the bias is taken here whichever path uses it: left to some, its wait would stand in the
+    // next tile's k-steps, and wait for the copies too)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(bias[i]));
     constexpr int ROWB = W * 4;      // bytes of a staged row; 16-byte chunks XORed with the row's low bits
-    constexpr int LPR = W / 8;       // lanes per row when read back
-    constexpr int RPI = 64 / LPR;    // rows a wave reads at a time: a lane keeps its 8 columns
-    constexpr int IT = (32 + RPI - 1) / RPI;
     const uint32_t es = lds0 + (uint32_t)(cur * STAGE + wave * EPI);
     auto staged = [&](int row, int chunk) { return es + (uint32_t)(row * ROWB + ((chunk ^ (row & 7)) << 4)); };
-    const int c8 = lane % LPR * 8, col = en0 + c8;
-    float bias[8];
-    lin_bias(a.e, lane < RPI * LPR ? col : a.N, a.N, bias);
-#pragma unroll 1
-  for (int tm = 0; tm < TM; ++tm) {  // (acc[0] is the tile's rows tm; one copy of the code)
+    // a wave's 32 rows of products into its part of the stage (its own LDS accesses are in
+    // order, and the compiler keeps them so)
+    auto put = [&](auto i_) __attribute__((always_inline)) {
+      constexpr int i = decltype(i_)::value;
 #pragma unroll
-    for (int tn = 0; tn < TN; ++tn)
+      for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *(__attribute__((address_space(3))) f32x4*)(uintptr_t)staged(lr, tn * 8 + 2 * j + lh) =
-            f32x4{acc[0][tn][4 * j], acc[0][tn][4 * j + 1], acc[0][tn][4 * j + 2], acc[0][tn][4 * j + 3]};
+        for (int j = 0; j < 4; ++j)
+          *(__attribute__((address_space(3))) f32x4*)(uintptr_t)staged(lr, tn * 8 + 2 * j + lh) =
+              f32x4{acc[i][tn][4 * j], acc[i][tn][4 * j + 1], acc[i][tn][4 * j + 2], acc[i][tn][4 * j + 3]};
+    };
+    auto get = [&](int row, float (&v)[8]) __attribute__((always_inline)) {
+      const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
+      const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
 #pragma unroll
-    for (int i = 0; i + 1 < TM; ++i)
-#pragma unroll
-      for (int tn = 0; tn < TN; ++tn) acc[i][tn] = acc[i + 1][tn];
-    // (a wave's own LDS writes and reads are in order; the compiler keeps them so)
-    // U rows' accesses side by side; EDGE: rows and columns past the output are left out
-    auto out = [&](auto edge_, auto act_, auto u_) __attribute__((always_inline)) {
+      for (int i = 0; i < 4; ++i) v[i] = x[i], v[4 + i] = y[i];
+    };
+    auto read = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };  // (before the next 32 rows overwrite)
+    // rows tm of the tile, U at a time; EDGE: rows and columns past the output are left out
+    auto out = [&](int tm, auto edge_, auto act_, auto u_) __attribute__((always_inline)) {
       constexpr bool EDGE = decltype(edge_)::value, ACT = decltype(act_)::value;
       constexpr int U = decltype(u_)::value;
 #pragma unroll 1
@@ -495,13 +530,12 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
         for (int u = 0; u < U; ++u) {
           const int row = (g + u) * RPI + lane / LPR;
           const int64_t m = em0 + tm * 32 + row;
-          live[u] = g + u < IT && row < 32 && lane < RPI * LPR && (!EDGE || (m < a.M && col < a.N));
+          live[u] = g + u < IT && there(g + u) && (!EDGE || (m < a.M && col < a.N));
           if (live[u]) {
             if (a.e.res) lin_get8(a.e.res + m * a.e.ldr + col, EDGE ? a.N - col : 8, r[u]);
-            const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
-            const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
+            get(row, v[u]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[u][i] = x[i] + bias[i], v[u][4 + i] = y[i] + bias[4 + i];
+            for (int i = 0; i < 8; ++i) v[u][i] += bias[i];
           }
         }
 #pragma unroll
@@ -511,33 +545,65 @@ __global__ __launch_bounds__(256, BM * BN * ST <= 128 * 128 * 2 ? 2 : 1) void li
         }
       }
     };
-    if (a.part) {
-#pragma unroll 2
-      for (int g = 0; g < IT; ++g) {
-        const int row = g * RPI + lane / LPR;
-        const int64_t m = em0 + tm * 32 + row;
-        if (row >= 32 || lane >= RPI * LPR || m >= a.M || col >= a.N) continue;
-        const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4);
-        const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)staged(row, c8 / 4 + 1);
-        float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        float* const o = a.part + ((int64_t)es_split * a.M + m) * a.N + col;
-        if (col + 8 <= a.N) {
-          __builtin_memcpy(o, v, 32);
-        } else {
+    if (whole_tile && !a.e.act && !a.part) {
+      lin_unroll<TM>([&](auto tm_) __attribute__((always_inline)) {
+        constexpr int tm = decltype(tm_)::value;
+        put(tm_);
+        if constexpr (RES) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + i < a.N) o[i] = v[i];
+          for (int g = 0; g < IT; ++g) {
+            const int row = min(g * RPI + lane / LPR, 31);  // (a lane past the rows repeats the last, and stores nothing)
+            float v[8];
+            uint32_t w[4];
+            get(row, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = af3_pack_bf16x2(v[2 * i] + bias[2 * i] + af3_bf16_to_f32(res[tm & 1][g][i]),
+                                     v[2 * i + 1] + bias[2 * i + 1] + af3_bf16_to_f32(res[tm & 1][g][i] >> 16));
+            if (there(g)) __builtin_memcpy(a.e.y + (int64_t)(em0 + tm * 32 + row) * a.N + col, w, 16);
+          }
+          if constexpr (tm + 2 < TM) fetch_res(tm + 2, res[tm & 1]);
+        } else {
+          out(tm, Flag<false>{}, Flag<false>{}, Int<4>{});
         }
-      }
-    } else if (whole_tile) {
-      if (a.e.act) out(Flag<false>{}, Flag<true>{}, Int<2>{});
-      else out(Flag<false>{}, Flag<false>{}, Int<4>{});
+        read();
+      });
     } else {
-      if (a.e.act) out(Flag<true>{}, Flag<true>{}, Int<2>{});
-      else out(Flag<true>{}, Flag<false>{}, Int<2>{});
+#pragma unroll 1
+      for (int tm = 0; tm < TM; ++tm) {  // (one copy of the code: acc[0] becomes the next rows')
+        put(Int<0>{});
+#pragma unroll
+        for (int i = 0; i + 1 < TM; ++i)
+#pragma unroll
+          for (int tn = 0; tn < TN; ++tn) acc[i][tn] = acc[i + 1][tn];
+        if (!RES && a.part) {
+#pragma unroll 2
+          for (int g = 0; g < IT; ++g) {
+            const int row = g * RPI + lane / LPR;
+            const int64_t m = em0 + tm * 32 + row;
+            if (!there(g) || m >= a.M || col >= a.N) continue;
+            float v[8];
+            get(row, v);
+            float* const o = a.part + ((int64_t)es_split * a.M + m) * a.N + col;
+            if (col + 8 <= a.N) {
+              __builtin_memcpy(o, v, 32);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (col + i < a.N) o[i] = v[i];
+            }
+          }
+        } else if (!RES && a.e.act) {
+          if (whole_tile) out(tm, Flag<false>{}, Flag<true>{}, Int<2>{});
+          else out(tm, Flag<true>{}, Flag<true>{}, Int<2>{});
+        } else {
+          out(tm, Flag<true>{}, Flag<false>{}, Int<2>{});
+        }
+        read();
+      }
+      // (vmcnt(0), for the same reason: loads of edges and residuals that some path leaves open)
+      if (!a.part) __builtin_amdgcn_s_waitcnt(0x0F70);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before the next 32 rows overwrite)
-  }
     if (!more) break;
     stores = !a.part && whole_tile;
     cur = ahead(cur, 1);
@@ -809,12 +875,14 @@ template <int BM, int BN, int ST>
 void lin_launch(const LinArgs& a, bool pt, bool qt, hipStream_t st) {
   const int64_t items = (int64_t)a.tiles_m * a.tiles_n * a.splits, slots = BM * BN * ST <= 128 * 128 * 2 ? 512 : 256;
   const dim3 grid((unsigned)(items < slots ? items : slots));
-  if (!pt && !qt)
-    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, false, false>), grid, dim3(256), 0, st, a);
+  if (!pt && !qt && a.e.res && !a.e.act && !a.part)
+    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, false, false, true>), grid, dim3(256), 0, st, a);
+  else if (!pt && !qt)
+    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, false, false, false>), grid, dim3(256), 0, st, a);
   else if (!pt)
-    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, false, true>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, false, true, false>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, true, true>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((lin_kernel<BM, BN, ST, true, true, false>), grid, dim3(256), 0, st, a);
 }
 
 constexpr int kSkinnyRows = 32;
