@@ -63,6 +63,11 @@ def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None, 
     return residual + h
 
 
+def _bind(module, forward):
+    """Make ``forward`` the module's, under a hook of accelerate's where it has one."""
+    setattr(module, "_old_forward" if hasattr(module, "_hf_hook") else "forward", types.MethodType(forward, module))
+
+
 def _patch_layer_class():
     from transformers.models.gpt_oss.modeling_gpt_oss import GptOssDecoderLayer
     if getattr(GptOssDecoderLayer, "_af3_fused_layers", False):
@@ -97,14 +102,16 @@ def enable_fused_layers(model, projections: bool = True) -> int:
     _patch_layer_class()
     for m in model.modules():
         if type(m) is GptOssRMSNorm:
-            m.forward = types.MethodType(_norm_forward, m)
+            _bind(m, _norm_forward)
     for layer in layers:
         setattr(layer, _ATTR, True)
+        if hasattr(layer, "_hf_hook"):   # (it holds the class's forward of before)
+            _bind(layer, GptOssDecoderLayer.forward)
         if projections:
             for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
                 m = getattr(layer.self_attn, name)
                 m = getattr(m, "base_layer", m)
                 if type(m) is torch.nn.Linear:
-                    m.forward = types.MethodType(_linear_forward, m)
+                    _bind(m, _linear_forward)
     logger.info("fused norms%s enabled for %d layers", " and projections" if projections else "", len(layers))
     return len(layers)

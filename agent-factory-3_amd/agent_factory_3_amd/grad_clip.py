@@ -14,6 +14,7 @@ from array import array
 from operator import attrgetter
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _capi
 from .routing import _device_of
@@ -67,6 +68,7 @@ class _Tensors:
     def scale(self, code, partials, max_norm, norm_out):
         _capi.call("af3_grad_scale", self.ptrs, self.sizes, self.f32, self.n, code, partials.data_ptr(),
                    partials.numel(), max_norm, _capi.ptr(norm_out), _capi.stream_of(self.device))
+        increment_version(self.kept)   # (a graph that saved one of them must see that it changed)
         for t, c in self.copies:
             t.copy_(c)
 

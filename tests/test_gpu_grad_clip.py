@@ -196,3 +196,15 @@ def test_refusals(dev):
     assert (g == 1).all()
     with pytest.raises(NotImplementedError):
         grad_clip.grad_norm([g.to_sparse()])
+
+
+def test_saved_gradients_are_seen_to_change(dev):
+    """A graph that holds a gradient as a saved tensor refuses its backward after the gradient was scaled."""
+    from agent_factory_3_amd import grad_clip
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    p.grad = torch.full((8,), 3.0, device=dev)
+    w = torch.ones(8, device=dev, requires_grad=True)
+    y = (w * p.grad).sum()   # (saves the gradient for w's)
+    grad_clip.clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

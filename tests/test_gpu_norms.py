@@ -266,3 +266,49 @@ def test_refusals(dev):
             norms.residual_norm(*args, **kw)
     with pytest.raises(ValueError):
         norms.rms_norm(x[0, 0], w)
+
+
+def test_one_tensor_in_several_places(dev):
+    """x as the residual too, one weight for both norms: the gradients add up."""
+    from agent_factory_3_amd import norms
+    t, d = _inputs(30, 264, BF, BF, dev)
+    x, w = (d[n].detach().requires_grad_() for n in ("x", "weight"))
+    want = on.residual_norm(t["x"], t["x"], t["weight"], dr=t["dr"], dh=t["dh"])
+    r, h = norms.residual_norm(x, x, w)
+    (g,) = torch.autograd.grad([r, h], [x], [d["dr"], d["dh"]])
+    both = want["dx"] + want["dresidual"]   # (each half rounded, and the sum)
+    tol = want["dx_tol"] + want["dresidual_tol"] + 2.0 ** -8 * both.abs()
+    assert ((g.cpu().double() - both).abs() <= tol).all()
+    want = on.residual_norm(t["x"], t["residual"], t["weight"], post=t["weight"], dr=t["dr"], dh=t["dh"])
+    r, h = norms.residual_norm(x, d["residual"], w, post_weight=w)
+    (g,) = torch.autograd.grad([r, h], [w], [d["dr"], d["dh"]])
+    both = want["dweight"] + want["dpost_weight"]
+    tol = want["dweight_tol"] + want["dpost_weight_tol"] + 2.0 ** -8 * both.abs()
+    assert ((g.cpu().double() - both).abs() <= tol).all()
+
+
+def test_gate_of_no_dimension_and_fp32_rows_at_any_element(dev):
+    from agent_factory_3_amd import norms
+    t, d = _inputs(20, 77, F32, F32, dev)
+    wide = torch.full((20, 90), float("nan"), device=dev)
+    wide[:, 5:82] = d["x"]
+    gate = torch.tensor(0.5, device=dev, requires_grad=True)
+    want = on.residual_norm(t["x"], t["residual"], t["weight"], gate=torch.full((20, 1), 0.5), dr=t["dr"], dh=t["dh"])
+    r, h = norms.residual_norm(wide[:, 5:82], d["residual"], d["weight"], gate=gate)
+    (g,) = torch.autograd.grad([r, h], [gate], [d["dr"], d["dh"]])
+    _compare({"r": r, "h": h}, {k: v for k, v in want.items() if k[0] in "rh"}, 20)
+    # (20 rows' sums, each within its bound, added in fp32 and rounded to it)
+    assert g.shape == () and abs(float(g) - float(want["dgate"].sum())) <= float(want["dgate_tol"].sum()) + 2.0 ** -20 * float(want["dgate"].abs().sum())
+
+
+def test_frozen_weight_uses_the_stored_stream(dev):
+    """Only x's and the residual's gradients (adapters trained elsewhere): within the bounds too, and
+    where the weight is trained but its gradient not asked for."""
+    from agent_factory_3_amd import norms
+    t, d = _inputs(300, 1000, BF, BF, dev)
+    want = on.residual_norm(t["x"], t["residual"], t["weight"], dr=t["dr"], dh=t["dh"])
+    for trained in (False, True):
+        leaf = {n: d[n].detach().requires_grad_(n != "weight" or trained) for n in ("x", "residual", "weight")}
+        r, h = norms.residual_norm(leaf["x"], leaf["residual"], leaf["weight"])
+        g = torch.autograd.grad([r, h], [leaf["x"], leaf["residual"]], [d["dr"], d["dh"]])
+        _compare({"dx": g[0], "dresidual": g[1]}, {k: want[k] for k in ("dx", "dx_tol", "dresidual", "dresidual_tol")}, 300)
