@@ -94,6 +94,9 @@ _SIGNATURES = {
                                      _i32, _i32, _i64, _f32, _i32, _i64, _i32, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "af3_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
     "af3_linear": (_i32, [_p, _i64, _i32, _p, _i64, _i32, _i64, _i64, _i64, _p, _i32, _i32, _p, _i64, _p, _p, _p, _sz, _p]),
+    "af3_linear_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32, _i32]),
+    "af3_linear_bwd": (_i32, [_p, _i64, _p, _i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i32, _p,
+                              _sz, _p]),
     "af3_linear_dz_workspace_bytes": (_sz, [_i64, _i64]),
     "af3_linear_dz": (_i32, [_p, _i64, _p, _i32, _i64, _i64, _p, _i64, _p, _i32, _p, _sz, _p]),
     "af3_grad_norm_partials": (_sz, [_p, _i32]),

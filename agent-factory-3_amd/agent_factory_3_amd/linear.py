@@ -14,7 +14,7 @@ import math
 import torch
 
 from . import _capi
-from .routing import _device_of, _no_forward_mode
+from .routing import _device_of, _no_forward_mode, _once
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 SKINNY_ROWS = 32     # rows of x up to which the forward streams the weight (any alignment)
@@ -45,23 +45,13 @@ def _aligned(t: torch.Tensor):
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace(M, N, K, pt, qt) -> int:
-    return int(_capi.load().af3_linear_workspace_bytes(M, N, K, pt, qt))
+def _workspace(M, N, K) -> int:
+    return int(_capi.load().af3_linear_workspace_bytes(M, N, K, 0, 0))
 
 
-@functools.lru_cache(maxsize=64)
-def _dz_workspace(M, N) -> int:
-    return int(_capi.load().af3_linear_dz_workspace_bytes(M, N))
-
-
-def _product(p, ldp, pt, q, ldq, qt, M, N, K, y, bias=None, act=0, residual=None, z=None):
-    """y [M, N] = sum_k p q over k = 0 .. K - 1 (pt, qt: stored [k][row])."""
-    ws_n = _workspace(M, N, K, pt, qt)
-    ws = torch.empty(ws_n, dtype=torch.uint8, device=y.device) if ws_n else None
-    _capi.call("af3_linear", p.data_ptr(), ldp, pt, q.data_ptr(), ldq, qt, M, N, K, _capi.ptr(bias),
-               int(bias is not None and bias.dtype == torch.float32), act, _capi.ptr(residual),
-               0 if residual is None else residual.stride(0), y.data_ptr(), _capi.ptr(z), _capi.ptr(ws), ws_n,
-               _capi.stream_of(y.device))
+@functools.lru_cache(maxsize=256)
+def _bwd_workspace(T, N, K, dx, dw, db) -> int:
+    return int(_capi.load().af3_linear_bwd_workspace_bytes(T, N, K, dx, dw, db))
 
 
 def _forward(x, weight, bias, act, residual, keep_z):
@@ -78,7 +68,13 @@ def _forward(x, weight, bias, act, residual, keep_z):
             (p, ldp), (q, ldq) = (x2, x2.stride(0)), (w, w.stride(0))
         else:
             (p, ldp), (q, ldq) = _aligned(x2), _aligned(w)
-        _product(p, ldp, 0, q, ldq, 0, T, N, K, y, bias, act, None if residual is None else _rows(residual), z)
+        res = None if residual is None else _rows(residual)
+        ws_n = _workspace(T, N, K)
+        ws = torch.empty(ws_n, dtype=torch.uint8, device=x.device) if ws_n else None
+        ptr = _capi.ptr
+        _capi.call("af3_linear", p.data_ptr(), ldp, 0, q.data_ptr(), ldq, 0, T, N, K, ptr(bias),
+                   int(bias is not None and bias.dtype == torch.float32), act, ptr(res),
+                   0 if res is None else res.stride(0), y.data_ptr(), ptr(z), ptr(ws), ws_n, _capi.stream_of(x.device))
     return y, z
 
 
@@ -92,7 +88,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         _no_forward_mode("linear backward", dy)
         x, weight, z = ctx.saved_tensors
@@ -110,32 +106,33 @@ class _Linear(torch.autograd.Function):
                 if need_b:
                     db = new(N, dtype=bias_type, device=dev)
                 if T:
-                    _Linear._products(_rows(dy), x, weight, z, act, T, N, K, dx, dw, db)
+                    _Linear._gradients(_rows(dy), x, weight, z, act, T, N, K, dx, dw, db)
         return dx, dw, db, dy if need_res else None, None
 
     @staticmethod
-    def _products(dy, x, weight, z, act, T, N, K, dx, dw, db):
-        dz, ldy = dy, dy.stride(0) if T > 1 else N
-        ldz = ldy
-        use = dx is not None or dw is not None
+    def _gradients(dy, x, weight, z, act, T, N, K, dx, dw, db):
+        dev = dy.device
+        ldy = dy.stride(0) if T > 1 else N
+        dz = ws = p_w = p_x = None
+        ldz = ldw = ldx = 0
         # dz in a tensor of its own: behind an activation, or where dy's rows are not as the products read them
-        make = use and (act or N % 8 or ldy % 8 or dy.data_ptr() % 16 or not N <= ldy < _MAX_STRIDE)
-        if make:
+        if (dx is not None or dw is not None) and (act or N % 8 or ldy % 8 or dy.data_ptr() % 16
+                                                   or not N <= ldy < _MAX_STRIDE):
             ldz = (N + 7) // 8 * 8
-            dz = torch.empty((T, ldz), dtype=torch.bfloat16, device=dy.device)
-        if make or db is not None:
-            ws_n = _dz_workspace(T, N) if db is not None else 0
-            ws = torch.empty(ws_n, dtype=torch.uint8, device=dy.device) if ws_n else None
-            z = z if z is None else z.contiguous()
-            _capi.call("af3_linear_dz", dy.data_ptr(), ldy, _capi.ptr(z), act, T, N, dz.data_ptr() if make else None, ldz,
-                       _capi.ptr(db), int(db is not None and db.dtype == torch.float32), _capi.ptr(ws), ws_n,
-                       _capi.stream_of(dy.device))
+            dz = torch.empty((T, ldz), dtype=torch.bfloat16, device=dev)
         if dx is not None:
-            w, ldw = _aligned(_rows(weight))
-            _product(dz, ldz, 0, w, ldw, 1, T, K, N, dx)
+            weight, ldw = _aligned(_rows(weight))
+            p_w = weight.data_ptr()
         if dw is not None:
             x, ldx = _aligned(_rows(x))
-            _product(dz, ldz, 1, x, ldx, 1, N, K, T, dw)
+            p_x = x.data_ptr()
+        z = z if z is None else z.contiguous()
+        ws_n = _bwd_workspace(T, N, K, dx is not None, dw is not None, db is not None)
+        if ws_n:
+            ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+        ptr = _capi.ptr
+        _capi.call("af3_linear_bwd", dy.data_ptr(), ldy, ptr(z), act, p_w, ldw, p_x, ldx, T, N, K, ptr(dz), ldz, ptr(dx),
+                   ptr(dw), ptr(db), int(db is not None and db.dtype == torch.float32), ptr(ws), ws_n, _capi.stream_of(dev))
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,

@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _capi
-from .routing import _device_of, _no_forward_mode
+from .routing import _device_of, _no_forward_mode, _once
 
 MIN_HIDDEN, MAX_HIDDEN = 8, 16384
 _TYPES = (torch.bfloat16, torch.float32)
@@ -90,7 +90,7 @@ class _ResidualNorm(torch.autograd.Function):
         return (r, h) if weight is not None else r
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, *grads):
         _no_forward_mode("residual_norm backward", *grads)
         dr, dh = (None, grads[0]) if ctx.args[3] is None else grads if len(grads) == 2 else (grads[0], None)

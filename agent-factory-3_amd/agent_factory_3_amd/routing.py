@@ -359,6 +359,17 @@ def _no_forward_mode(who: str, *tensors):
             raise NotImplementedError(f"{who}: forward-mode derivatives are not supported")
 
 
+def _once(backward):
+    """once_differentiable for a backward: where no graph of the gradients is asked for (the common case),
+    without its step into no_grad."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return wrapper
+
+
 _HERE = contextlib.nullcontext()
 
 

@@ -980,3 +980,32 @@ extern "C" int af3_linear_dz(const uint16_t* dy, int64_t ldy, const uint16_t* z,
                        dbias, bias_f32);
   return af3::check_launch("linear_dz");
 }
+
+extern "C" size_t af3_linear_bwd_workspace_bytes(int64_t T, int64_t N, int64_t K, int want_dx, int want_dw, int want_db) {
+  size_t n = 0;  // (one after the other on one stream: they share it)
+  const size_t each[3] = {want_dx ? af3_linear_workspace_bytes(T, K, N, 0, 1) : 0,
+                          want_dw ? af3_linear_workspace_bytes(N, K, T, 1, 1) : 0,
+                          want_db ? af3_linear_dz_workspace_bytes(T, N) : 0};
+  for (size_t e : each) n = e > n ? e : n;
+  return n;
+}
+
+extern "C" int af3_linear_bwd(const uint16_t* dy, int64_t ldy, const uint16_t* z, int act, const uint16_t* weight,
+                              int64_t ldw, const uint16_t* x, int64_t ldx, int64_t T, int64_t N, int64_t K, uint16_t* dz,
+                              int64_t ldz, uint16_t* dx, uint16_t* dweight, void* dbias, int bias_f32, void* workspace,
+                              size_t ws_bytes, void* stream) {
+  AF3_REQUIRE(T >= 0 && N > 0 && K > 0, "linear_bwd: bad sizes");
+  AF3_REQUIRE(dy && (!dx || weight) && (!dweight || x), "linear_bwd: null pointer");
+  AF3_REQUIRE(!act || dz || !(dx || dweight), "linear_bwd: the products behind an activation need dz");
+  int rc = 0;
+  if (dz || dbias) rc = af3_linear_dz(dy, ldy, z, act, T, N, dz, ldz, dbias, bias_f32, workspace, ws_bytes, stream);
+  if (rc) return rc;
+  const uint16_t* const g = dz ? dz : dy;
+  const int64_t ldg = dz ? ldz : ldy;
+  if (dx)
+    rc = af3_linear(g, ldg, 0, weight, ldw, 1, T, K, N, nullptr, 0, 0, nullptr, 0, dx, nullptr, workspace, ws_bytes, stream);
+  if (rc) return rc;
+  if (dweight)
+    rc = af3_linear(g, ldg, 1, x, ldx, 1, N, K, T, nullptr, 0, 0, nullptr, 0, dweight, nullptr, workspace, ws_bytes, stream);
+  return rc;
+}

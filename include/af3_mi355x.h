@@ -531,12 +531,21 @@ int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* dh, int64_t 
  * contiguous index (any finite or other value where it is not).  bias bf16, or fp32
  * with bias_f32 (NULL: none); residual [M][ldr] (NULL: none).  The workspace holds
  * the partial sums of products whose k is split over blocks (0: none needed).
+ * af3_linear_bwd: the gradients of y = act(x W^T + b), x [T][ldx], W [N][ldw], from
+ * dy [T][ldy]: dz (as below, NULL where there is no activation and dy's own rows
+ * serve the products), then dx [T][K] = dz W, dweight [N][K] = dz^T x, dbias [N], each
+ * NULL if not wanted; rows as af3_linear takes them.
  * af3_linear_dz: dz [M][ldz] = dy act'(z) (zeros from N to the next multiple of 8
  * within ldz; NULL: not written) and dbias [N] = its column sums (NULL: not). */
 size_t af3_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int p_trans, int q_trans);
 int af3_linear(const uint16_t* p, int64_t ldp, int p_trans, const uint16_t* q, int64_t ldq, int q_trans, int64_t M,
                int64_t N, int64_t K, const void* bias, int bias_f32, int act, const uint16_t* residual, int64_t ldr,
                uint16_t* y, uint16_t* z, void* workspace, size_t ws_bytes, void* stream);
+size_t af3_linear_bwd_workspace_bytes(int64_t T, int64_t N, int64_t K, int want_dx, int want_dw, int want_db);
+int af3_linear_bwd(const uint16_t* dy, int64_t ldy, const uint16_t* z, int act, const uint16_t* weight, int64_t ldw,
+                   const uint16_t* x, int64_t ldx, int64_t T, int64_t N, int64_t K, uint16_t* dz, int64_t ldz,
+                   uint16_t* dx, uint16_t* dweight, void* dbias, int bias_f32, void* workspace, size_t ws_bytes,
+                   void* stream);
 size_t af3_linear_dz_workspace_bytes(int64_t M, int64_t N);
 int af3_linear_dz(const uint16_t* dy, int64_t ldy, const uint16_t* z, int act, int64_t M, int64_t N, uint16_t* dz,
                   int64_t ldz, void* dbias, int bias_f32, void* workspace, size_t ws_bytes, void* stream);

@@ -225,3 +225,20 @@ def test_refusals(dev):
                           (TypeError, (x, w), dict(residual=torch.zeros(4, 32, device=dev))), (ValueError, (x, w[0]), {})]:
         with pytest.raises(exc):
             linear(*args, **kw)
+
+
+def test_second_derivatives_are_refused(dev):
+    """A graph of the gradients can be asked for and gives the same bits, but is not differentiated: where dy
+    has no gradient they have none either (torch's own error), else the error names the backward."""
+    from agent_factory_3_amd import norms
+    from agent_factory_3_amd.linear import linear
+    t, d = _inputs(40, 64, 64, dev)
+    x = d["x"].detach().requires_grad_()
+    dy = d["dy"].detach().requires_grad_()
+    for f in (lambda: linear(x, d["weight"], activation="silu"), lambda: norms.rms_norm(x, d["bias"])):
+        (g,) = torch.autograd.grad(f(), x, d["dy"])
+        for grad, message in ((d["dy"], "does not require grad"), (dy, "once_differentiable")):
+            (g2,) = torch.autograd.grad(f(), x, grad, create_graph=True)
+            assert torch.equal(g, g2)
+            with pytest.raises(RuntimeError, match=message):
+                g2.float().sum().backward()
