@@ -19,10 +19,17 @@
 //
 // A row stays in registers from its loads to its stores, so each direction reads and
 // writes every tensor once: HBM bounds both.  NW waves share a row, a lane holding CPL
-// chunks of 8 consecutive elements: a wave alone up to H = 4096 (its two reductions are
-// shuffles, no barrier), four waves to 16384 and wherever there are too few rows to
-// give every CU waves.  Rows may start at any element: 16-byte loads need no alignment
-// here, and a row's last H % 8 elements come out of a load of its last 8.
+// chunks of 8 consecutive elements: a wave alone up to H = 1024 (its two reductions are
+// shuffles, no barrier), four waves to 4096, eight to 16384.  Rows may start at any
+// element: 16-byte loads need no alignment here, and a row's last H % 8 elements come out
+// of a load of its last 8.
+//
+// Measured, us (TB/s of the tensors read and written): 128000 x 2880 bf16 with a residual
+// forward 513 (5.7), backward with dweight 732 (6.0; 640 without it), joining 5; 8192 x
+// 2880 29 and 47; 3 x 1021 rows with post_weight and a gate 23 and 48; 1 row 2.5.
+// A wave a row against four: 8192 x 512 forward 6.6 for 11.3, 300 rows 3.0 for 3.1, one
+// row of 1024 2.8 for 2.7; at 2880 (six chunks a lane) 8192 rows 29.0 for 29.2, but 300
+// rows 5.3 for 3.6.  Backward, 8192 x 960 24.5 for 32.8, 300 x 1024 8.4 for 8.0.
 //
 // Column sums (dweight, dpost_weight, dgate): a lane adds up its columns over all its
 // rows, the waves of a block are joined through LDS, each block writes one row of fp32
@@ -32,8 +39,12 @@
 namespace {
 
 constexpr int kNormMinH = 8, kNormMaxH = 16384;
-constexpr int kNormWideRows = 2048;   // rows from which a wave has a row of its own
-constexpr int kNormBwdBlocks = 512;   // blocks of the backward's row pass (per group of the gate)
+constexpr int kNormWaveRows = 512;  // rows from which a wave of the backward has a row of its own
+// Blocks of the backward's row pass: 256 of eight waves or 512 of four hold all the waves that
+// their registers allow, and more only add partials.  8192 x 2880 with 256, 512, 1024 blocks:
+// four waves a row 73, 57, 62 us, eight (FULL) 66, 70, 78 (FULL with four, 130).  Up to 1024
+// rows, 256 either way: 500 rows 11.2, 12.3, 13.1.
+constexpr int kNormBwdBlocks = 256;
 
 struct NormArgs {
   const void* x;
@@ -314,6 +325,142 @@ __device__ __forceinline__ void n_join(const float (&acc)[CPL][8], float* lds, i
   }
 }
 
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+// One row of a backward with FULL and CPL chunks a lane, whose tensors would not fit in the
+// registers beside the column sums: dh, r (x and the gate where r is made again) are read a
+// second time, from the L2, after the first sum; du and x stay for the second.  Two of the
+// column sums are in LDS: own[0] of post_weight, own[1] of the gate, a lane's own elements.
+// 8192 x 16384 with post_weight: 537 us (kept whole it spilled, 3140).
+template <class XT, class RT, int NW, int CPL, bool ACC, bool REC, int AC>
+__device__ __forceinline__ void n_bwd_long(const NormArgs& a, int64_t row, int wave, int t, float (*sums)[NW], int& turn,
+                                           float (&aw)[AC][8], f32x4 (*own)[ACC ? CPL : 1][2][ACC ? NW * 64 : 1]) {
+  const int H = a.H;
+  const int64_t grow = a.gate_cols ? (uint32_t)row / (uint32_t)a.gate_rows : 0;
+  const float s_x = a.post ? a.s_x[row] : 1.f, g1 = a.gate_cols == 1 ? n_gate1(a, grow) : 1.f;
+  const XT* const x_row = (const XT*)a.x + row * a.ldx;
+  // chunk c's first element, opaque: its addresses in eight tensors are not kept over the rows
+  auto at = [&](int c) __attribute__((always_inline)) {
+    int e = (c * 64 * NW + t) * 8;
+    asm volatile("" : "+v"(e));
+    return e;
+  };
+  auto post = [&](int e, float (&w)[8]) __attribute__((always_inline)) {
+    if (a.post) {
+      n_get(a.post, a.post_f32, 0, e, H, w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = 1.f;
+    }
+  };
+  auto gate = [&](int e, float (&w)[8]) __attribute__((always_inline)) {
+    if (a.gate_cols > 1) {
+      n_get(a.gate, a.gate_f32, grow * H, e, H, w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = g1;
+    }
+  };
+  // r, from the residual as read and u's factors
+  auto remake = [&](const float (&x)[8], const float (&p)[8], const float (&gt)[8], float (&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float u = x[i];
+      if (a.post) u *= s_x * p[i];
+      if (a.gate_cols) u *= gt[i];
+      v[i] += a.scale * u;
+    }
+  };
+  float s = 0.f, m = 0.f;
+  if (a.dh) {
+    s = a.s_r[row];
+    float dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      const int e = at(c);
+      float d[8], v[8], w[8];
+      n_get((const XT*)a.dh + row * a.lddh, e, H, d);
+      n_get((const RT*)a.res + row * a.ldr, e, H, v);
+      n_get(a.weight, a.w_f32, 0, e, H, w);
+      if constexpr (REC) {
+        float x[8], p[8], gt[8];
+        n_get(x_row, e, H, x);
+        post(e, p);
+        gate(e, gt);
+        remake(x, p, gt, v);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot += d[i] * w[i] * v[i];
+    }
+    m = n_sum<NW>(dot, sums, wave, turn) / (float)H * s * s;
+  }
+  float du[CPL][8];
+  NRaw<XT> x_raw[CPL];
+  float dot = 0.f, gdot = 0.f;
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int e = at(c);
+    float x[8], p[8], gt[8], g[8];
+    x_raw[c].load(x_row, e, H);
+    x_raw[c].value(x);
+    post(e, p);
+    gate(e, gt);
+    if (a.dr) {
+      n_get((const RT*)a.dr + row * a.lddr, e, H, g);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = 0.f;
+    }
+    if (a.dh) {
+      float d[8], v[8], w[8];
+      n_get((const XT*)a.dh + row * a.lddh, e, H, d);
+      n_get((const RT*)a.res + row * a.ldr, e, H, v);
+      n_get(a.weight, a.w_f32, 0, e, H, w);
+      if constexpr (REC) remake(x, p, gt, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (ACC) aw[c][i] += d[i] * (v[i] * s);
+        g[i] += s * (d[i] * w[i] - v[i] * m);
+      }
+    }
+    if (a.dres) n_set((RT*)a.dres + row * H, e, H, g);
+    float gg[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      gg[i] = a.scale * g[i] * (x[i] * s_x * p[i]);  // the gate's gradient
+      gdot += gg[i];
+      const float dgu = a.scale * gt[i] * g[i];
+      if constexpr (ACC) {
+        own[0][c][i / 4][t][i % 4] += dgu * (x[i] * s_x);
+        own[1][c][i / 4][t][i % 4] += gg[i];
+      }
+      du[c][i] = dgu * p[i];
+      dot += du[c][i] * x[i];
+    }
+    if (a.dgate) {
+      if (a.gate_f32)
+        n_set((float*)a.dgate + row * H, e, H, gg);
+      else
+        n_set((uint16_t*)a.dgate + row * H, e, H, gg);
+    }
+  }
+  if (a.gate_dots) {
+    const float sum = n_sum<NW>(gdot, sums, wave, turn);
+    if (t == 0) a.gate_dots[row] = sum;
+  }
+  const float m_x = a.post ? n_sum<NW>(dot, sums, wave, turn) / (float)H * s_x * s_x : 0.f;
+  if (a.dx) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      float x[8];
+      x_raw[c].value(x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) du[c][i] = s_x * (du[c][i] - x[i] * m_x);
+      n_set((XT*)a.dx + row * H, at(c), H, du[c]);
+    }
+  }
+}
+
 // ACC: some column sum is wanted; REC: a.res is the residual, and r is made of it and x
 template <class XT, class RT, int NW, int CPL, bool RES, bool FULL, bool ACC, bool REC>
 __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const NormArgs a) {
@@ -321,9 +468,11 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
   constexpr int AC = ACC ? CPL : 1;
   __shared__ float sums[2][NW];
   __shared__ float lds[(ACC && NW == 1) ? CPL * 512 : 1];
+  constexpr bool LONG = FULL && CPL > 2;
+  __shared__ f32x4 own[LONG && ACC ? 2 : 1][LONG && ACC ? CPL : 1][2][LONG && ACC ? NW * 64 : 1];
   int turn = 0;
   const int wave = threadIdx.x >> 6;
-  const int t = NW == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  int t = NW == 1 ? (threadIdx.x & 63) : threadIdx.x;
   const int H = a.H;
   // the block's group: the rows that share a gate row (one group of all rows without column sums of a gate)
   const int64_t per = a.part_gate ? a.gate_rows : a.rows;
@@ -341,183 +490,201 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
         if constexpr (FULL) ap[c][i] = ag[c][i] = 0.f;
       }
   }
-  // a row's loads, made while the row before it is worked on
-  NRaw<RT> r_dr[CPL], r_r[CPL];
-  constexpr bool X = FULL || REC;
-  NRaw<XT> r_dh[CPL], r_x[X ? CPL : 1];
-  float r_gate[FULL ? CPL : 1][8];
-  float r_s = 0.f, r_sx = 1.f, r_g1 = 1.f;
-  const bool has_dr = RES && a.dr, has_dh = !RES || a.dh;
-  auto fetch = [&](int64_t row) {
+  if constexpr (LONG) {
+    if constexpr (ACC) {
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      const int e = (c * 64 * NW + t) * 8;
-      if (has_dr) r_dr[c].load((const RT*)a.dr + row * a.lddr, e, H);
-      if (has_dh) r_dh[c].load((const XT*)a.dh + row * a.lddh, e, H);
-      if (has_dh) r_r[c].load((const RT*)a.res + row * a.ldr, e, H);
-      if constexpr (X) r_x[c].load((const XT*)a.x + row * a.ldx, e, H);
+      for (int j = 0; j < 4 * CPL; ++j) own[j / (2 * CPL)][j / 2 % CPL][j % 2][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (has_dh) r_s = a.s_r[row];
-    if constexpr (FULL) {
-      if (a.post) r_sx = a.s_x[row];
-      if (a.gate_cols) {
-        const uint32_t grow = (uint32_t)row / (uint32_t)a.gate_rows;
-        if (a.gate_cols == 1) {
-          r_g1 = n_gate1(a, grow);
-        } else {
-#pragma unroll
-          for (int c = 0; c < CPL; ++c)
-            n_get(a.gate, a.gate_f32, (int64_t)grow * H, (c * 64 * NW + t) * 8, H, r_gate[c]);
-        }
-      }
-    }
-  };
-  // (where the registers of two rows would not fit, a row's loads are its own, the weights' too)
-  constexpr bool AHEAD = CPL * (FULL ? 2 : 1) <= 2;
-  float w_h[AHEAD ? CPL : 1][8], w_post[FULL && AHEAD ? CPL : 1][8];
-  if constexpr (AHEAD) {
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      const int e = (c * 64 * NW + t) * 8;
-      if (has_dh) n_get(a.weight, a.w_f32, 0, e, H, w_h[c]);
-      if constexpr (FULL) {
-        if (a.post) n_get(a.post, a.post_f32, 0, e, H, w_post[c]);
-      }
-    }
-  }
-  if (AHEAD && first < last) fetch(first);
-  for (int64_t row = first; row < last; row += step) {
-    if (!AHEAD) fetch(row);
-    float g[CPL][8];  // the gradient of r
-    float d[CPL][8], v[CPL][8], x[X ? CPL : 1][8], gate[FULL ? CPL : 1][8];
-    const float s_r = r_s, s_x = r_sx, g1 = r_g1;
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      if (has_dr) {
-        r_dr[c].value(g[c]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] = 0.f;
-      }
-      if (has_dh) {
-        r_dh[c].value(d[c]);
-        r_r[c].value(v[c]);
-      }
-      if constexpr (X) r_x[c].value(x[c]);
-      if constexpr (FULL) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) gate[c][i] = r_gate[c][i];
-      }
-    }
-    if constexpr (REC) {
-      if (has_dh) {
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          float w[8];
-          if constexpr (FULL && AHEAD) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = w_post[c][i];
-          } else if constexpr (FULL) {
-            if (a.post) n_get(a.post, a.post_f32, 0, (c * 64 * NW + t) * 8, H, w);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float u = x[c][i];
-            if constexpr (FULL) {
-              if (a.post) u *= s_x * w[i];
-              if (a.gate_cols) u *= a.gate_cols > 1 ? gate[c][i] : g1;
-            }
-            v[c][i] += a.scale * u;
-          }
-        }
-      }
-    }
-    if (AHEAD && row + step < last) fetch(row + step);
-    if (has_dh) {
-      const float s = s_r;
-      float dot = 0.f;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        float w[8];
-        if constexpr (AHEAD) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = w_h[c][i];
-        } else {
-          n_get(a.weight, a.w_f32, 0, (c * 64 * NW + t) * 8, H, w);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if constexpr (ACC) aw[c][i] += d[c][i] * (v[c][i] * s);
-          d[c][i] *= w[i];
-          dot += d[c][i] * v[c][i];
-        }
-      }
-      const float m = n_sum<NW>(dot, sums, wave, turn) / (float)H * s * s;
+    for (int64_t row = first; row < last; row += step)
+      n_bwd_long<XT, RT, NW, CPL, ACC, REC>(a, row, wave, t, sums, turn, aw, own);
+    if constexpr (ACC) {
 #pragma unroll
       for (int c = 0; c < CPL; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] += s * (d[c][i] - v[c][i] * m);
+        for (int i = 0; i < 8; ++i) ap[c][i] = own[0][c][i / 4][t][i % 4], ag[c][i] = own[1][c][i / 4][t][i % 4];
     }
-    if (a.dres) {
-      RT* const dres = (RT*)a.dres + row * H;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) n_set(dres, (c * 64 * NW + t) * 8, H, g[c]);
-    }
-    if constexpr (!RES) continue;
-    if constexpr (FULL) {
-      const float s = s_x;
-      float dot = 0.f, gdot = 0.f;
+  } else {
+    // a row's loads, made while the row before it is worked on
+    NRaw<RT> r_dr[CPL], r_r[CPL];
+    constexpr bool X = FULL || REC;
+    NRaw<XT> r_dh[CPL], r_x[X ? CPL : 1];
+    float r_gate[FULL ? CPL : 1][8];
+    float r_s = 0.f, r_sx = 1.f, r_g1 = 1.f;
+    const bool has_dr = RES && a.dr, has_dh = !RES || a.dh;
+    auto fetch = [&](int64_t row) {
 #pragma unroll
       for (int c = 0; c < CPL; ++c) {
         const int e = (c * 64 * NW + t) * 8;
-        float w[8], gg[8];
-        if constexpr (AHEAD) {
+        if (has_dr) r_dr[c].load((const RT*)a.dr + row * a.lddr, e, H);
+        if (has_dh) r_dh[c].load((const XT*)a.dh + row * a.lddh, e, H);
+        if (has_dh) r_r[c].load((const RT*)a.res + row * a.ldr, e, H);
+        if constexpr (X) r_x[c].load((const XT*)a.x + row * a.ldx, e, H);
+      }
+      if (has_dh) r_s = a.s_r[row];
+      if constexpr (FULL) {
+        if (a.post) r_sx = a.s_x[row];
+        if (a.gate_cols) {
+          const uint32_t grow = (uint32_t)row / (uint32_t)a.gate_rows;
+          if (a.gate_cols == 1) {
+            r_g1 = n_gate1(a, grow);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = w_post[c][i];
+            for (int c = 0; c < CPL; ++c)
+              n_get(a.gate, a.gate_f32, (int64_t)grow * H, (c * 64 * NW + t) * 8, H, r_gate[c]);
+          }
+        }
+      }
+    };
+    // (where the registers of two rows would not fit, a row's loads are its own, the weights' too)
+    constexpr bool AHEAD = CPL * (FULL ? 2 : 1) <= 2;
+    float w_h[AHEAD ? CPL : 1][8], w_post[FULL && AHEAD ? CPL : 1][8];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) {
+        const int e = (c * 64 * NW + t) * 8;
+        if (has_dh) n_get(a.weight, a.w_f32, 0, e, H, w_h[c]);
+        if constexpr (FULL) {
+          if (a.post) n_get(a.post, a.post_f32, 0, e, H, w_post[c]);
+        }
+      }
+    }
+    if (AHEAD && first < last) fetch(first);
+    for (int64_t row = first; row < last; row += step) {
+      if (!AHEAD) {
+        asm volatile("" : "+v"(t));  // (opaque: the addresses in eight tensors are not kept over the rows)
+        fetch(row);
+      }
+      float g[CPL][8];  // the gradient of r
+      float d[CPL][8], v[CPL][8], x[X ? CPL : 1][8], gate[FULL ? CPL : 1][8];
+      const float s_r = r_s, s_x = r_sx, g1 = r_g1;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) {
+        if (has_dr) {
+          r_dr[c].value(g[c]);
         } else {
-          if (a.post) n_get(a.post, a.post_f32, 0, e, H, w);
-        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float wi = a.post ? w[i] : 1.f;
-          const float gi = a.gate_cols > 1 ? gate[c][i] : g1;
-          const float gu = a.scale * g[c][i] * (x[c][i] * s * wi);  // the gate's gradient
-          gdot += gu;
-          gg[i] = gu;
-          if constexpr (ACC) ag[c][i] += gu;
-          const float du = a.scale * gi * g[c][i];
-          if constexpr (ACC) ap[c][i] += du * (x[c][i] * s);
-          g[c][i] = du * wi;
-          dot += g[c][i] * x[c][i];
+          for (int i = 0; i < 8; ++i) g[c][i] = 0.f;
         }
-        if (a.dgate) {
-          if (a.gate_f32)
-            n_set((float*)a.dgate + row * H, e, H, gg);
-          else
-            n_set((uint16_t*)a.dgate + row * H, e, H, gg);
+        if (has_dh) {
+          r_dh[c].value(d[c]);
+          r_r[c].value(v[c]);
+        }
+        if constexpr (X) r_x[c].value(x[c]);
+        if constexpr (FULL) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) gate[c][i] = r_gate[c][i];
         }
       }
-      if (a.gate_dots) {
-        const float sum = n_sum<NW>(gdot, sums, wave, turn);
-        if (t == 0) a.gate_dots[row] = sum;
+      if constexpr (REC) {
+        if (has_dh) {
+#pragma unroll
+          for (int c = 0; c < CPL; ++c) {
+            float w[8];
+            if constexpr (FULL && AHEAD) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = w_post[c][i];
+            } else if constexpr (FULL) {
+              if (a.post) n_get(a.post, a.post_f32, 0, (c * 64 * NW + t) * 8, H, w);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float u = x[c][i];
+              if constexpr (FULL) {
+                if (a.post) u *= s_x * w[i];
+                if (a.gate_cols) u *= a.gate_cols > 1 ? gate[c][i] : g1;
+              }
+              v[c][i] += a.scale * u;
+            }
+          }
+        }
       }
-      if (a.post) {
+      if (AHEAD && row + step < last) fetch(row + step);
+      if (has_dh) {
+        const float s = s_r;
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) {
+          float w[8];
+          if constexpr (AHEAD) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = w_h[c][i];
+          } else {
+            n_get(a.weight, a.w_f32, 0, (c * 64 * NW + t) * 8, H, w);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (ACC) aw[c][i] += d[c][i] * (v[c][i] * s);
+            d[c][i] *= w[i];
+            dot += d[c][i] * v[c][i];
+          }
+        }
         const float m = n_sum<NW>(dot, sums, wave, turn) / (float)H * s * s;
 #pragma unroll
         for (int c = 0; c < CPL; ++c)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[c][i] = s * (g[c][i] - x[c][i] * m);
+          for (int i = 0; i < 8; ++i) g[c][i] += s * (d[c][i] - v[c][i] * m);
       }
-    } else {
+      if (a.dres) {
+        RT* const dres = (RT*)a.dres + row * H;
 #pragma unroll
-      for (int c = 0; c < CPL; ++c)
+        for (int c = 0; c < CPL; ++c) n_set(dres, (c * 64 * NW + t) * 8, H, g[c]);
+      }
+      if constexpr (!RES) continue;
+      if constexpr (FULL) {
+        const float s = s_x;
+        float dot = 0.f, gdot = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] *= a.scale;
-    }
-    if (a.dx) {
-      XT* const dx = (XT*)a.dx + row * H;
+        for (int c = 0; c < CPL; ++c) {
+          const int e = (c * 64 * NW + t) * 8;
+          float w[8], gg[8];
+          if constexpr (AHEAD) {
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) n_set(dx, (c * 64 * NW + t) * 8, H, g[c]);
+            for (int i = 0; i < 8; ++i) w[i] = w_post[c][i];
+          } else {
+            if (a.post) n_get(a.post, a.post_f32, 0, e, H, w);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float wi = a.post ? w[i] : 1.f;
+            const float gi = a.gate_cols > 1 ? gate[c][i] : g1;
+            const float gu = a.scale * g[c][i] * (x[c][i] * s * wi);  // the gate's gradient
+            gdot += gu;
+            gg[i] = gu;
+            if constexpr (ACC) ag[c][i] += gu;
+            const float du = a.scale * gi * g[c][i];
+            if constexpr (ACC) ap[c][i] += du * (x[c][i] * s);
+            g[c][i] = du * wi;
+            dot += g[c][i] * x[c][i];
+          }
+          if (a.dgate) {
+            if (a.gate_f32)
+              n_set((float*)a.dgate + row * H, e, H, gg);
+            else
+              n_set((uint16_t*)a.dgate + row * H, e, H, gg);
+          }
+        }
+        if (a.gate_dots) {
+          const float sum = n_sum<NW>(gdot, sums, wave, turn);
+          if (t == 0) a.gate_dots[row] = sum;
+        }
+        if (a.post) {
+          const float m = n_sum<NW>(dot, sums, wave, turn) / (float)H * s * s;
+#pragma unroll
+          for (int c = 0; c < CPL; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[c][i] = s * (g[c][i] - x[c][i] * m);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < CPL; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[c][i] *= a.scale;
+      }
+      if (a.dx) {
+        XT* const dx = (XT*)a.dx + row * H;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) n_set(dx, (c * 64 * NW + t) * 8, H, g[c]);
+      }
     }
   }
   if constexpr (ACC) {
@@ -600,8 +767,8 @@ __global__ __launch_bounds__(256) void norm_gate_rows_kernel(const float* dots, 
     ((uint16_t*)out)[i] = (uint16_t)af3_f32_to_bf16(dots[i]);
 }
 
-// a wave a row where H and the rows allow (the backward's column sums: up to 2 chunks per lane)
-bool norm_wide(int64_t rows, int H, bool full, int cpl) { return !full && H <= 64 * 8 * cpl && rows >= kNormWideRows; }
+// whether the backward gives a wave a row of its own
+bool norm_bwd_wave_row(int64_t rows, int H, bool full) { return !full && H <= 64 * 8 * 2 && rows >= kNormWaveRows; }
 
 template <class XT, class RT, bool RES, bool FULL>
 void norm_fwd_launch(const NormArgs& a, hipStream_t st) {
@@ -612,10 +779,7 @@ void norm_fwd_launch(const NormArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((norm_fwd_kernel<XT, RT, NW, CPL, RES, FULL>), grid, dim3(NW == 8 ? 512 : 256), 0, st, a);                  \
     return;                                                                                                       \
   } while (0)
-  if constexpr (!FULL) if (norm_wide(a.rows, a.H, FULL, 6)) {
-    if (chunks <= 64 * 2) AF3_NF(1, 2);
-    AF3_NF(1, 6);
-  }
+  if constexpr (!FULL) if (chunks <= 64 * 2) AF3_NF(1, 2);
   if (chunks <= 64 * 8) AF3_NF(4, 2);
   if (chunks <= 64 * 16) AF3_NF(8, 2);
   AF3_NF(8, 4);
@@ -631,9 +795,7 @@ void norm_bwd_launch(const NormArgs& a, unsigned blocks, hipStream_t st) {
     hipLaunchKernelGGL((norm_bwd_kernel<XT, RT, NW, CPL, RES, FULL, ACC, REC>), dim3(blocks), block, 0, st, a);         \
     return;                                                                                                       \
   } while (0)
-  if constexpr (!FULL) if (norm_wide(a.rows, a.H, FULL, 2)) {
-    AF3_NB(1, 2);
-  }
+  if constexpr (!FULL) if (norm_bwd_wave_row(a.rows, a.H, FULL)) AF3_NB(1, 2);
   if constexpr (FULL) {
     if (chunks <= 64 * 8) AF3_NB(8, 1);
   } else {
@@ -656,8 +818,10 @@ NormPlan norm_plan(int64_t rows, int H, int gate_cols, int64_t gate_rows, bool f
   const bool sums = want_gate && gate_cols > 1 && gate_rows > 1;  // of a gate row over its group
   p.groups = sums ? af3_cdiv(rows, gate_rows) : 1;
   const int64_t per = sums ? gate_rows : rows;
-  const int64_t units = norm_wide(rows, H, full, 2) ? af3_cdiv(per, 8) : per;  // row steps of one block
-  int64_t bpg = af3_cdiv(kNormBwdBlocks, p.groups);
+  const bool wave_row = norm_bwd_wave_row(rows, H, full);
+  const int64_t units = wave_row ? af3_cdiv(per, 8) : per;  // row steps of one block
+  const int64_t total = full || (!wave_row && rows < 4 * kNormBwdBlocks) ? kNormBwdBlocks : 2 * kNormBwdBlocks;
+  int64_t bpg = af3_cdiv(total, p.groups);
   p.blocks_per_group = (int)(bpg < units ? bpg : units);
   if (p.blocks_per_group < 1) p.blocks_per_group = 1;
   p.blocks = p.groups * p.blocks_per_group;

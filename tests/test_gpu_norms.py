@@ -312,3 +312,38 @@ def test_frozen_weight_uses_the_stored_stream(dev):
         r, h = norms.residual_norm(leaf["x"], leaf["residual"], leaf["weight"])
         g = torch.autograd.grad([r, h], [leaf["x"], leaf["residual"]], [d["dr"], d["dh"]])
         _compare({"dx": g[0], "dresidual": g[1]}, {k: want[k] for k in ("dx", "dx_tol", "dresidual", "dresidual_tol")}, 300)
+
+
+@pytest.mark.parametrize("rows,H", [(1, 64), (511, 512), (512, 1016), (513, 333), (1023, 1032), (1024, 1025), (1025, 1030)])
+@pytest.mark.parametrize("rt", [None, BF])
+def test_row_counts_where_the_launch_changes(dev, rows, H, rt):
+    t, d = _inputs(rows, H, BF, rt, dev, seed=rows)
+    want = on.residual_norm(t["x"], t["residual"], t["weight"], dr=t["dr"], dh=t["dh"])
+    _compare(_call(d), want, rows)
+
+
+@pytest.mark.parametrize("xt,rt", [(BF, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("H,post,gate", [(9001, True, "sequence"), (8200, False, "token"), (12000, True, "channel"),
+                                         (8193, True, "full"), (5003, True, "sequence")])
+def test_long_rows_several_a_block(dev, xt, rt, H, post, gate):
+    B, S = 2, 301
+    shape = {"channel": (H,), "sequence": (B, 1, H), "token": (B, S, 1), "full": (B, S, H)}[gate]
+    t, d = _inputs(B * S, H, xt, rt, dev, post=post, gate=shape, seed=H)
+    full = t["gate"].expand(B, S, shape[-1]).reshape(B * S, shape[-1])
+    for dh in (t["dh"], None):
+        want = on.residual_norm(t["x"], t["residual"], t["weight"] if dh is not None else None, post=t["post"], gate=full,
+                                scale=0.7, dr=t["dr"], dh=dh)
+        for n in ("dgate", "dgate_tol"):
+            v = want[n].view(B, S, shape[-1])
+            want[n] = v.sum_to_size(shape) if len(shape) == 3 else v.sum((0, 1))
+        got = _call({**d, "weight": d["weight"] if dh is not None else None}, scale=0.7, shape=(B, S))
+        _compare(got, want, B * S)
+        # each output of its own: the rows' gradients do not depend on which sums are wanted
+        from agent_factory_3_amd import norms
+        leaf = {n: d[n].view(B, S, H).detach().requires_grad_() for n in ("x", "residual")}
+        r, h = norms.residual_norm(leaf["x"], leaf["residual"], d["weight"] if dh is not None else None,
+                                   post_weight=d["post"], gate=d["gate"], scale=0.7)
+        g = torch.autograd.grad([o for o in (r, h) if o is not None], list(leaf.values()),
+                                [d["dr"].view(r.shape)] + ([d["dh"].view(r.shape)] if h is not None else []))
+        keys = ("dx", "dresidual", "dx_tol", "dresidual_tol")
+        _compare({"dx": g[0], "dresidual": g[1]}, {k: want[k] for k in keys}, B * S)
