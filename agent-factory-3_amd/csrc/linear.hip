@@ -644,7 +644,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* part, int sp
 // units of 64, a wave's lane (r, g) taking k = 8 g + (0..7) and 32 more of row r of W and of
 // x (two products of 32 k), so W is read once, 64 contiguous bytes of 16 rows at a time,
 // with all of a wave's loads in flight; the waves' sums meet in LDS.
-// Addresses need no alignment; elements past K are zeros.
+// Addresses need no alignment; elements past K are zeros.  One row at a stated N x K, us:
+// 512 x 2880 5.2, 4096 x 2880 6.1, 2880 x 4096 6.7 (4.0 TB/s of W); 32 rows 9.7, 10.3, 12.9,
+// where gathering x's 16-row fragments costs 3 to 6 of it.  Eight waves, two columns' tiles
+// a block, or a start rotated by block gain nothing.
 constexpr int kSkinnyWaves = 16;
 
 // 8 elements at p of which the first n are there, zeros after them
@@ -885,6 +888,8 @@ void lin_launch(const LinArgs& a, bool pt, bool qt, hipStream_t st) {
     hipLaunchKernelGGL((lin_kernel<BM, BN, ST, true, true, false>), grid, dim3(256), 0, st, a);
 }
 
+// (the tiles instead, us: 512 x 2880 1 row 10.3, 16 11.2 for 7.2, 32 11.5 for 9.7; 2880 x 4096
+// 32 rows 13.8 for 12.9, so a third row tile would lose)
 constexpr int kSkinnyRows = 32;
 bool lin_skinny(int64_t M, bool pt, bool qt) { return M <= kSkinnyRows && !pt && !qt; }
 

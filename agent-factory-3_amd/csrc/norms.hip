@@ -26,7 +26,7 @@
 //
 // Measured, us (TB/s of the tensors read and written): 128000 x 2880 bf16 with a residual
 // forward 513 (5.7), backward with dweight 732 (6.0; 640 without it), joining 5; 8192 x
-// 2880 29 and 47; 3 x 1021 rows with post_weight and a gate 23 and 48; 1 row 2.5.
+// 2880 29 and 47; 3 x 1021 rows with post_weight and a gate 21 and 40; 1 row 2.5.
 // A wave a row against four: 8192 x 512 forward 6.6 for 11.3, 300 rows 3.0 for 3.1, one
 // row of 1024 2.8 for 2.7; at 2880 (six chunks a lane) 8192 rows 29.0 for 29.2, but 300
 // rows 5.3 for 3.6.  Backward, 8192 x 960 24.5 for 32.8, 300 x 1024 8.4 for 8.0.
@@ -821,7 +821,7 @@ NormPlan norm_plan(int64_t rows, int H, int gate_cols, int64_t gate_rows, bool f
   const bool wave_row = norm_bwd_wave_row(rows, H, full);
   const int64_t units = wave_row ? af3_cdiv(per, 8) : per;  // row steps of one block
   const int64_t total = full || (!wave_row && rows < 4 * kNormBwdBlocks) ? kNormBwdBlocks : 2 * kNormBwdBlocks;
-  int64_t bpg = af3_cdiv(total, p.groups);
+  const int64_t bpg = total / p.groups;  // (not rounded up: a block too many is a second round)
   p.blocks_per_group = (int)(bpg < units ? bpg : units);
   if (p.blocks_per_group < 1) p.blocks_per_group = 1;
   p.blocks = p.groups * p.blocks_per_group;
