@@ -91,9 +91,9 @@ def enable_fused_layers(model, projections: bool = True) -> int:
     Every GptOssRMSNorm runs on ``norms.rms_norm``, the add and norm between attention
     and experts on ``norms.residual_norm`` (whose module's forward, and hooks on it, are
     then not called), and with ``projections`` q, k, v and o (the layers inside PEFT's
-    wrappers too) on ``linear.linear``: together about as fast as the library's products
-    forward and faster backward, and deterministic.  Results differ from transformers'
-    by roundings.  Again is harmless.
+    wrappers too) on ``linear.linear``: a few percent slower than the library's products
+    forward, faster backward, and deterministic.  Results differ from transformers' by
+    roundings.  Again is harmless.
     """
     from transformers.models.gpt_oss.modeling_gpt_oss import GptOssDecoderLayer, GptOssRMSNorm
     layers = [m for m in model.modules() if isinstance(m, GptOssDecoderLayer)]

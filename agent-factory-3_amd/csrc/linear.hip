@@ -741,6 +741,9 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void lin_skinny_kernel(const Lin
 
 // dz = dy act'(z) in bf16 with rows of ldz elements (zeros past N), and the columns' sums
 // (of dz before rounding): a block takes 32 lanes x 8 columns by its share of the rows.
+// HBM: 16384 x 2880 sums alone 19 us (5.0 TB/s), with gelu and dz 71 (4.0; the slope's
+// exponential and two reciprocals per element beside it).  Two, four and eight rows' loads
+// side by side: 19 and 63, 31 and 92, 42 and 129.
 constexpr int kDzRows = 8;  // rows a block takes at a time
 
 struct DzArgs {
