@@ -159,7 +159,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     _no_forward_mode("linear", x, weight, bias, residual)
     device = x.device
     for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is None or (t.dtype is torch.bfloat16 and t.is_cuda and (t is x or t.device == device)):
+        if t is None or (t.dtype is torch.bfloat16 and t.is_cuda and (t is x or t.device == device) and t.data_ptr()):
             continue
         if not t.is_cuda:
             raise RuntimeError(f"linear: {name} must be a GPU tensor (the MI355X path has no CPU implementation)")
@@ -167,6 +167,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             raise TypeError(f"linear: {name} must be bfloat16{' or float32' if name == 'bias' else ''} (got {t.dtype})")
         if t.device != device:
             raise ValueError(f"linear: {name} is on {t.device}, x on {device}")
+        if not t.data_ptr() and t.numel():
+            raise TypeError(f"linear: {name} is a {type(t).__name__} without memory of its own (of a DTensor, pass the "
+                            "local tensor)")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
     N, K = weight.shape

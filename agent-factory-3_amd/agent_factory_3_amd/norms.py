@@ -175,6 +175,8 @@ def _check_tensor(who, name, t, device):
         raise TypeError(f"{who}: {name} must be bfloat16 or float32 (got {t.dtype})")
     if t.device != device:
         raise ValueError(f"{who}: {name} is on {t.device}, x on {device}")
+    if not t.data_ptr() and t.numel():
+        raise TypeError(f"{who}: {name} is a {type(t).__name__} without memory of its own (of a DTensor, pass the local tensor)")
 
 
 def _check(who, x, weight, post, eps):

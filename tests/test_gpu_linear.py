@@ -242,3 +242,24 @@ def test_second_derivatives_are_refused(dev):
             assert torch.equal(g, g2)
             with pytest.raises(RuntimeError, match=message):
                 g2.float().sum().backward()
+
+
+def test_tensors_without_memory_of_their_own_are_refused(dev):
+    """A DTensor's address is 0: it must not pass for a tensor that is not given."""
+    from agent_factory_3_amd.linear import linear
+
+    class Held(torch.Tensor):
+        @classmethod
+        def of(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError(f"{func} of a tensor without memory")
+
+    x, w, b = (torch.ones(*s, device=dev, dtype=BF) for s in ((2, 64), (64, 64), (64,)))
+    for name in ("x", "weight", "bias", "residual"):
+        t = {"x": x, "weight": w, "bias": b, "residual": x}
+        t[name] = Held.of(t[name])
+        with pytest.raises(TypeError, match=name):
+            linear(t["x"], t["weight"], t["bias"], residual=t["residual"])
