@@ -19,7 +19,7 @@ from torch.autograd.graph import increment_version
 from . import _capi
 from .routing import _device_of
 
-_DTYPE, _LAYOUT = attrgetter("dtype"), attrgetter("layout")
+_DTYPE = attrgetter("dtype")
 _NORMS = {2.0: 2, 1.0: 1, math.inf: 0}
 
 
@@ -34,19 +34,25 @@ class _Tensors:
     """GPU tensors of one device as the kernels take them: addresses, lengths, types.
     Tensors that do not fill one run of memory are read (and scaled) through a copy."""
 
-    def __init__(self, tensors):
+    def __init__(self, tensors, sizes=None):
+        self.n = len(tensors)
+        self.device = tensors[0].device
+        dtypes = set(map(_DTYPE, tensors))
+        _check([(self.device, dtypes)])
         self.copies = []
         if not all(map(torch.Tensor.is_contiguous, tensors)):
             tensors = [t if t.is_contiguous() else self._run(t) for t in tensors]
-        self.n = len(tensors)
         self.kept = tensors
-        self.device = tensors[0].device
+        f32 = array("B", [torch.float32 in dtypes]) * self.n
+        if len(dtypes) > 1:
+            f32 = array("B", [d is torch.float32 for d in map(_DTYPE, tensors)])
         # (host arrays: the calls read them before they return)
-        self._arrays = (array("Q", map(torch.Tensor.data_ptr, tensors)), array("q", map(torch.Tensor.numel, tensors)),
-                        array("B", [d is torch.float32 for d in map(_DTYPE, tensors)]))
+        self._arrays = (array("Q", map(torch.Tensor.data_ptr, tensors)), sizes or array("q", map(torch.Tensor.numel, tensors)), f32)
         self.ptrs, self.sizes, self.f32 = (a.buffer_info()[0] for a in self._arrays)
 
     def _run(self, t):
+        if t.layout is not torch.strided:
+            raise NotImplementedError("grad_norm: sparse gradients are not supported")
         order = sorted(range(t.dim()), key=t.stride, reverse=True)
         run = t.detach().permute(order)
         if run.is_contiguous():   # the same memory in another order
@@ -86,12 +92,22 @@ def _local(t):
     return t.to_local(), tuple(groups)
 
 
-def _gather(tensors):
-    """Tensors by (device, process groups), in order of first appearance; doubles and empty ones left out."""
+def _held(tensors):
+    """Tensors by (device, process groups), in order of first appearance, as the kernels take them (None
+    where all of them are empty)."""
     if (set(map(type, tensors)) == {torch.Tensor} and len(set(map(torch.Tensor.get_device, tensors))) == 1
-            and len(set(map(id, tensors))) == len(tensors) and all(map(torch.Tensor.numel, tensors))
-            and set(map(_LAYOUT, tensors)) == {torch.strided}):
-        return {(tensors[0].device, ()): tensors}   # the common case, without a step per tensor
+            and len(set(map(id, tensors))) == len(tensors)):
+        sizes = array("q", map(torch.Tensor.numel, tensors))
+        if all(sizes):   # the common case, without a step per tensor
+            one = _Tensors(tensors, sizes)
+            return {(one.device, ()): one}
+    buckets = _gather(tensors)
+    _check([(device, set(map(_DTYPE, ts))) for (device, _), ts in buckets.items()])
+    return {key: _Tensors(ts) if ts else None for key, ts in buckets.items()}
+
+
+def _gather(tensors):
+    """Tensors by (device, process groups); doubles and empty ones left out."""
     buckets, seen = {}, set()
     for t in tensors:
         if id(t) in seen:
@@ -100,8 +116,6 @@ def _gather(tensors):
         groups = ()
         if type(t) is not torch.Tensor:
             t, groups = _local(t)
-        if t.is_sparse:
-            raise NotImplementedError("grad_norm: sparse gradients are not supported")
         bucket = buckets.get((t.device, groups))
         if bucket is None:
             bucket = buckets[t.device, groups] = []
@@ -110,11 +124,11 @@ def _gather(tensors):
     return buckets
 
 
-def _check(buckets):
-    for (device, _), ts in buckets.items():
+def _check(types):
+    for device, dtypes in types:
         if device.type != "cuda":
             raise RuntimeError("grad_norm: gradients must be GPU tensors (the MI355X path has no CPU implementation)")
-        for dtype in set(map(_DTYPE, ts)):
+        for dtype in dtypes:
             if dtype is not torch.float32 and dtype is not torch.bfloat16:
                 raise TypeError(f"grad_norm: gradients must be bfloat16 or float32 (got {dtype})")
 
@@ -142,9 +156,8 @@ def _join_ranks(total, groups, code):
     return torch.where(both[1:] > 0, math.nan, both[:1])
 
 
-def _partials(buckets, code):
+def _partials(held, code):
     """[(tensors of a device, partials on that device)], a device each; all partials together make the norm."""
-    held = {key: _Tensors(ts) if ts else None for key, ts in buckets.items()}
     if len(held) == 1 and not next(iter(held))[1]:   # one GPU, nothing sharded: the partials as they are
         (t,) = held.values()
         if t is None:
@@ -184,16 +197,15 @@ def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     code = _norm_code(norm_type)
-    buckets = _gather(tensors)
-    _check(buckets)
-    if len(buckets) == 1 and not next(iter(buckets))[1]:   # one GPU, nothing sharded
-        (ts,) = buckets.values()
-        if ts:
-            out = torch.empty((), dtype=torch.float32, device=ts[0].device)
+    held = _held(tensors)
+    if len(held) == 1 and not next(iter(held))[1]:   # one GPU, nothing sharded
+        (t,) = held.values()
+        if t is not None:
+            out = torch.empty((), dtype=torch.float32, device=t.device)
             with _device_of(out):
-                _Tensors(ts).norm(code, norm_out=out)
+                t.norm(code, norm_out=out)
             return out
-    parts = _partials(buckets, code)
+    parts = _partials(held, code)
     if not parts:
         return torch.zeros((), device=tensors[0].device if tensors else None)
     return _norm_of(parts[0][1], code)
@@ -227,9 +239,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
     if not grads:
         return torch.tensor(0.0)
-    buckets = _gather(grads)
-    _check(buckets)
-    parts = _partials(buckets, code)
+    parts = _partials(_held(grads), code)
     if not parts:
         return torch.zeros((), device=grads[0].device)
     if error_if_nonfinite:
