@@ -65,7 +65,7 @@ def _forward(x, residual, weight, post, gate, gate_rows, scale, eps, stats):
         rstd_x = torch.empty(n, dtype=torch.float32, device=dev)
     ptr = _capi.ptr
     _capi.call("af3_residual_norm_fwd", x2.data_ptr(), _f32(x), ldx, ptr(res), _f32(residual), ldr, ptr(weight),
-               _f32(weight), ptr(post), _f32(post), ptr(gate), _f32(gate), 0 if gate is None else gate.shape[1],
+               _f32(weight), ptr(post), _f32(post), ptr(gate), _f32(gate), _cols(gate),
                gate_rows, scale, eps, n, H, ptr(r), ptr(h), ptr(rstd), ptr(rstd_x), _capi.stream_of(dev))
     return r, h, rstd, rstd_x
 
@@ -134,7 +134,7 @@ class _ResidualNorm(torch.autograd.Function):
                 post, rstd_x = post.contiguous(), rstd_x.contiguous()
                 p_post, p_rstd_x = post.data_ptr(), rstd_x.data_ptr()
             if gate is not None:
-                gate, cols = gate.contiguous(), gate.shape[1]
+                gate, cols = gate.contiguous(), _cols(gate)
                 p_gate = gate.data_ptr()
         if need_res or (need_x and same):
             dres = _like(some, shape, rt or xt)
@@ -200,7 +200,7 @@ def _check_weight(who, name, t, device, H):
 
 
 def _gate_rows(gate, shape):
-    """The gate as [groups, 1 or H] and the rows of x that share each of its rows."""
+    """The gate as rows of 1 or H in a row, and the rows of x that share each of its rows."""
     if gate.dim() > len(shape) or any(g not in (1, s) for g, s in zip(gate.shape[::-1], shape[::-1])):
         raise ValueError(f"residual_norm: a gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
     lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
@@ -211,7 +211,11 @@ def _gate_rows(gate, shape):
     if any(g != s for g, s in zip(lead[:k], shape)):   # shared along outer dimensions only: a row for each,
         # in fp32, so that the gradient is rounded once, after torch's sum over them
         gate, k = gate.float().expand(*shape[:-1], cols), len(lead)
-    return gate.reshape(-1, cols).contiguous(), math.prod(shape[k:-1])
+    return gate if gate.is_contiguous() else gate.contiguous(), math.prod(shape[k:-1])
+
+
+def _cols(gate) -> int:
+    return 0 if gate is None else gate.shape[-1] if gate.dim() else 1
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
