@@ -916,7 +916,7 @@ extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* d
                                      void* stream_) {
   const int rc = norm_check("residual_norm_bwd", rows, H, gate_cols, gate_rows, 0.f);
   if (rc) return rc;
-  AF3_REQUIRE(has_residual || (dh && dresidual && !dx && !dr && !post_weight && !gate_cols),
+  AF3_REQUIRE(has_residual || (dh && (dresidual || dweight) && !dx && !dr && !post_weight && !gate_cols),
               "residual_norm_bwd: without a residual, x's gradient is dresidual, and only dh arrives");
   AF3_REQUIRE(!dpost || post_weight, "residual_norm_bwd: dpost without post_weight");
   AF3_REQUIRE(!dgate || gate_cols, "residual_norm_bwd: dgate without a gate");

@@ -504,8 +504,8 @@ int af3_seq_starts_rows(const int64_t* position_ids, int64_t ld, int n_rows, int
  * Backward: dr (NULL: none) and dh (NULL: none) arrive at r and h, r as the
  * forward wrote it (x without a residual); with r_again the residual itself, bf16: r
  * is made again from it and x, for a dweight of one rounding.  dresidual = dr + the norm's gradient
- * (without a residual this is x's gradient); dx, dweight, dpost, dgate, each NULL
- * if not wanted, in their tensors' types; sums are fp32 in a fixed order.  x is
+ * (without a residual this is x's gradient); dresidual, dx, dweight, dpost, dgate, each
+ * NULL if not wanted, in their tensors' types; sums are fp32 in a fixed order.  x is
  * read where there is a post_weight or gate, and with r_again. */
 int af3_residual_norm_fwd(const void* x, int x_f32, int64_t ldx, const void* residual, int r_f32, int64_t ldr,
                           const void* weight, int w_f32, const void* post_weight, int post_f32, const void* gate,

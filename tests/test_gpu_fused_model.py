@@ -193,3 +193,25 @@ def test_other_types_run_as_they_did(dev):
     m.forward = fused_layers._linear_forward.__get__(m)
     y = torch.randn(3, 8, device=dev)
     assert torch.equal(m(y), torch.nn.functional.linear(y, m.weight, m.bias))
+
+
+def test_only_the_norms_trained(dev):
+    """Frozen embeddings, projections and experts: the first layer's input norm has a trained weight and an x
+    without a gradient.  Every norm's weight gets the gradient that it has beside everything else trained."""
+    routing_replay.enable_routing_replay()
+    ids, ri = _ids(2, 50).to(dev), _replay(2, 50).to(dev)
+    w = torch.randn(2, 50, H, generator=torch.Generator().manual_seed(3)).to(dev)
+    model = _model(dev, "af3_sink")
+    fused_layers.enable_fused_layers(model)
+    names = [n for n, _ in model.named_parameters() if "norm" in n]
+    assert len(names) == 5
+
+    def grads():
+        out = model(input_ids=ids, routing_indices=ri, use_cache=False).last_hidden_state
+        params = dict(model.named_parameters())
+        return torch.autograd.grad((out.float() * w).sum(), [params[n] for n in names])
+    want = grads()
+    for n, p in model.named_parameters():
+        p.requires_grad_(n in names)
+    for n, a, b in zip(names, grads(), want):
+        assert b.abs().max() > 0 and torch.equal(a, b), n

@@ -370,3 +370,17 @@ def test_tensors_without_memory_of_their_own_are_refused(dev):
             norms.residual_norm(t["x"], t["residual"], t["weight"], post_weight=t["post_weight"], gate=t["gate"])
     with pytest.raises(TypeError, match="weight"):
         norms.rms_norm(x, Held.of(w))
+
+
+@pytest.mark.parametrize("rows,H", [(1, 8), (300, 2880), (600, 512), (2048, 1000), (5, 9001)])
+@pytest.mark.parametrize("xt,wt", [(BF, BF), (F32, F32), (BF, F32)])
+def test_rms_norm_with_one_of_its_tensors_trained(dev, rows, H, xt, wt):
+    """A trained weight behind a frozen x, and the other way round."""
+    from agent_factory_3_amd import norms
+    t, d = _inputs(rows, H, xt, None, dev, wt=wt, seed=H)
+    want = on.residual_norm(t["x"], None, t["weight"], dh=t["dh"])
+    for name in ("weight", "x"):
+        leaf = {n: d[n].detach().requires_grad_(n == name) for n in ("x", "weight")}
+        h = norms.rms_norm(leaf["x"], leaf["weight"])
+        (g,) = torch.autograd.grad(h, leaf[name], d["dh"])
+        _compare({"h": h, "d" + name: g}, {k: v for k, v in want.items() if k.removesuffix("_tol") in ("h", "d" + name)}, rows)
