@@ -87,7 +87,7 @@ def _local(t):
     for dim, p in enumerate(t.placements):
         if p.is_partial():
             raise NotImplementedError("grad_norm: a gradient that is still to be reduced (a Partial DTensor)")
-        if p.is_shard():
+        if not p.is_replicate():   # (is_shard leaves out the strided shards of FSDP2 over tensor parallelism)
             groups.append(t.device_mesh.get_group(dim))
     return t.to_local(), tuple(groups)
 
