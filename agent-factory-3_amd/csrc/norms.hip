@@ -448,16 +448,19 @@ __device__ __forceinline__ void n_bwd_long(const NormArgs& a, int64_t row, int w
     const float sum = n_sum<NW>(gdot, sums, wave, turn);
     if (t == 0) a.gate_dots[row] = sum;
   }
-  const float m_x = a.post ? n_sum<NW>(dot, sums, wave, turn) / (float)H * s_x * s_x : 0.f;
-  if (a.dx) {
+  if (a.post) {  // (du alone without a norm of x: an infinite x must not meet a 0)
+    const float m_x = n_sum<NW>(dot, sums, wave, turn) / (float)H * s_x * s_x;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
       float x[8];
       x_raw[c].value(x);
 #pragma unroll
       for (int i = 0; i < 8; ++i) du[c][i] = s_x * (du[c][i] - x[i] * m_x);
-      n_set((XT*)a.dx + row * H, at(c), H, du[c]);
     }
+  }
+  if (a.dx) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) n_set((XT*)a.dx + row * H, at(c), H, du[c]);
   }
 }
 

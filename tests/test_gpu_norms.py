@@ -384,3 +384,26 @@ def test_rms_norm_with_one_of_its_tensors_trained(dev, rows, H, xt, wt):
         h = norms.rms_norm(leaf["x"], leaf["weight"])
         (g,) = torch.autograd.grad(h, leaf[name], d["dh"])
         _compare({"h": h, "d" + name: g}, {k: v for k, v in want.items() if k.removesuffix("_tol") in ("h", "d" + name)}, rows)
+
+
+@pytest.mark.parametrize("H", [64, 2880, 8192, 9000, 16384])
+@pytest.mark.parametrize("xt,rt", [(BF, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("gate", ["channel", "token", "full"])
+def test_a_gated_branch_that_is_not_finite(dev, H, xt, rt, gate):
+    """dx = scale gate dr whatever x holds, where only r's gradient arrives and x has no norm of its own; the
+    gate's gradient is not finite where x is not."""
+    from agent_factory_3_amd import norms
+    rows = 9
+    shape = {"channel": (H,), "token": (rows, 1), "full": (rows, H)}[gate]
+    t, d = _inputs(rows, H, xt, rt, dev, gate=shape, seed=H)
+    want = on.residual_norm(t["x"], t["residual"], None, gate=t["gate"], scale=0.5, dr=t["dr"])
+    x = d["x"].clone()
+    x[2, 5], x[4, H - 1], x[7, 0] = float("inf"), float("-inf"), float("nan")
+    for used in (False, True):   # no weight; a weight whose output no loss reads
+        leaf = {n: v.detach().requires_grad_() for n, v in (("x", x), ("residual", d["residual"]), ("gate", d["gate"]))}
+        r, h = norms.residual_norm(leaf["x"], leaf["residual"], d["weight"] if used else None, gate=leaf["gate"], scale=0.5)
+        dx, dres, dg = torch.autograd.grad(r, list(leaf.values()), d["dr"])
+        _compare({"dx": dx, "dresidual": dres}, {k: v for k, v in want.items() if k.split("_")[0] in ("dx", "dresidual")}, rows)
+        bad = ~x.isfinite()
+        bad = bad.any(0) if gate == "channel" else bad.any(1, keepdim=True) if gate == "token" else bad
+        assert torch.equal(dg.isfinite(), ~bad)
