@@ -45,6 +45,7 @@ constexpr int kNormWaveRows = 512;  // rows from which a wave of the backward ha
 // four waves a row 73, 57, 62 us, eight (FULL) 66, 70, 78 (FULL with four, 130).  Up to 1024
 // rows, 256 either way: 500 rows 11.2, 12.3, 13.1.
 constexpr int kNormBwdBlocks = 256;
+constexpr int64_t kNormGrid = 1 << 22;  // blocks per launch of the forward: a launch holds less than 2^32 threads
 
 struct NormArgs {
   const void* x;
@@ -61,6 +62,7 @@ struct NormArgs {
   int64_t rows;
   int H;
   // forward
+  int64_t row0;       // the launch's first row
   void* out_r;
   void* out_h;
   float* rstd;
@@ -229,7 +231,7 @@ __global__ __launch_bounds__(NW == 8 ? 512 : 256) void norm_fwd_kernel(const Nor
   __shared__ float lds[2][NW];
   int turn = 0;
   const int wave = threadIdx.x >> 6;
-  const int64_t row = NW == 1 ? (int64_t)blockIdx.x * WPB + wave : (int64_t)blockIdx.x;
+  const int64_t row = a.row0 + (NW == 1 ? (int64_t)blockIdx.x * WPB + wave : (int64_t)blockIdx.x);
   if (NW == 1 && row >= a.rows) return;
   const int t = NW == 1 ? (threadIdx.x & 63) : threadIdx.x;
   const int H = a.H;
@@ -742,21 +744,22 @@ __global__ __launch_bounds__(kJoinCols* kJoinRows) void norm_join_kernel(const J
     ((uint16_t*)a.out[which])[at] = (uint16_t)af3_f32_to_bf16(s);
 }
 
-// a one-value gate's gradient: group g sums dots[g * per .. ) (one block each)
-__global__ __launch_bounds__(256) void norm_gate_dots_kernel(const float* dots, int64_t rows, int64_t per, void* out,
-                                                             int f32) {
+// a one-value gate's gradient: group g sums dots[g * per .. ) (a block at a time)
+__global__ __launch_bounds__(256) void norm_gate_dots_kernel(const float* dots, int64_t rows, int64_t per,
+                                                             int64_t groups, void* out, int f32) {
   __shared__ float lds[2][4];
   int turn = 0;
-  const int64_t g = blockIdx.x;
-  const int64_t end = min(g * per + per, rows);
-  float s = 0.f;
-  for (int64_t i = g * per + threadIdx.x; i < end; i += 256) s += dots[i];
-  s = n_sum<4>(s, lds, threadIdx.x >> 6, turn);
-  if (threadIdx.x == 0) {
-    if (f32)
-      ((float*)out)[g] = s;
-    else
-      ((uint16_t*)out)[g] = (uint16_t)af3_f32_to_bf16(s);
+  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
+    const int64_t end = min(g * per + per, rows);
+    float s = 0.f;
+    for (int64_t i = g * per + threadIdx.x; i < end; i += 256) s += dots[i];
+    s = n_sum<4>(s, lds, threadIdx.x >> 6, turn);
+    if (threadIdx.x == 0) {
+      if (f32)
+        ((float*)out)[g] = s;
+      else
+        ((uint16_t*)out)[g] = (uint16_t)af3_f32_to_bf16(s);
+    }
   }
 }
 
@@ -774,12 +777,16 @@ __global__ __launch_bounds__(256) void norm_gate_rows_kernel(const float* dots, 
 bool norm_bwd_wave_row(int64_t rows, int H, bool full) { return !full && H <= 64 * 8 * 2 && rows >= kNormWaveRows; }
 
 template <class XT, class RT, bool RES, bool FULL>
-void norm_fwd_launch(const NormArgs& a, hipStream_t st) {
+void norm_fwd_launch(NormArgs a, hipStream_t st) {
   const int chunks = (int)af3_cdiv(a.H, 8);
 #define AF3_NF(NW, CPL)                                                                                           \
   do {                                                                                                            \
-    const dim3 grid((unsigned)(NW == 1 ? af3_cdiv(a.rows, 4) : a.rows));                                           \
-    hipLaunchKernelGGL((norm_fwd_kernel<XT, RT, NW, CPL, RES, FULL>), grid, dim3(NW == 8 ? 512 : 256), 0, st, a);                  \
+    constexpr int RPB = NW == 1 ? 4 : 1;                                                                          \
+    for (a.row0 = 0; a.row0 < a.rows; a.row0 += kNormGrid * RPB) {                                                \
+      const int64_t left = af3_cdiv(a.rows - a.row0, RPB);                                                        \
+      const dim3 grid((unsigned)(left < kNormGrid ? left : kNormGrid));                                           \
+      hipLaunchKernelGGL((norm_fwd_kernel<XT, RT, NW, CPL, RES, FULL>), grid, dim3(NW == 8 ? 512 : 256), 0, st, a); \
+    }                                                                                                             \
     return;                                                                                                       \
   } while (0)
   if constexpr (!FULL) if (chunks <= 64 * 2) AF3_NF(1, 2);
@@ -993,9 +1000,11 @@ extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* d
     if (gate_rows == 1)
       hipLaunchKernelGGL(norm_gate_rows_kernel, dim3((unsigned)af3_cdiv(rows, 256)), dim3(256), 0, st, a.gate_dots,
                          rows, dgate, gate_f32);
-    else
-      hipLaunchKernelGGL(norm_gate_dots_kernel, dim3((unsigned)af3_cdiv(rows, gate_rows)), dim3(256), 0, st,
-                         a.gate_dots, rows, gate_rows, dgate, gate_f32);
+    else {
+      const int64_t groups = af3_cdiv(rows, gate_rows);
+      hipLaunchKernelGGL(norm_gate_dots_kernel, dim3((unsigned)(groups < kNormGrid ? groups : kNormGrid)), dim3(256), 0, st,
+                         a.gate_dots, rows, gate_rows, groups, dgate, gate_f32);
+    }
   }
   return af3::check_launch("residual_norm_bwd: sums");
 }

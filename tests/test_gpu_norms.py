@@ -407,3 +407,17 @@ def test_a_gated_branch_that_is_not_finite(dev, H, xt, rt, gate):
         bad = ~x.isfinite()
         bad = bad.any(0) if gate == "channel" else bad.any(1, keepdim=True) if gate == "token" else bad
         assert torch.equal(dg.isfinite(), ~bad)
+
+
+def test_more_rows_and_gates_than_a_launch_holds(dev):
+    """Past 2^24 rows of four waves each, and 2^24 gate values shared by two rows (a launch holds less than 2^32
+    threads).  Small whole numbers: every sum is exact."""
+    from agent_factory_3_amd import norms
+    G, H = (1 << 24) + 77, 8
+    g = torch.Generator(dev).manual_seed(0)
+    draw = lambda *s: torch.randint(-2, 3, s, generator=g, device=dev, dtype=torch.int8).to(BF)  # noqa: E731
+    x, res, gate = draw(G, 2, H), draw(G, 2, H), draw(G, 1, 1).requires_grad_()
+    r, _ = norms.residual_norm(x, res, gate=gate)
+    assert torch.equal(r, res + gate.detach() * x)   # (at most 6)
+    (dg,) = torch.autograd.grad(r, gate, res)
+    assert torch.equal(dg, (res * x).sum((1, 2), dtype=F32)[:, None, None].to(BF))   # (at most 64)
