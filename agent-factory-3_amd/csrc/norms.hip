@@ -82,6 +82,8 @@ struct NormArgs {
   float* gate_dots;  // [rows] fp32: a one-value gate's row sums
   void* dgate;       // a gate of x's own shape: its gradient, no sums
   int blocks_per_group;
+  int64_t groups;    // OWN: of rows that share a gate row, and the gate's gradient
+  void* dgate_sum;
 };
 
 // 8 elements at any address that is a multiple of the element's size, as fp32
@@ -466,8 +468,10 @@ __device__ __forceinline__ void n_bwd_long(const NormArgs& a, int64_t row, int w
   }
 }
 
-// ACC: some column sum is wanted; REC: a.res is the residual, and r is made of it and x
-template <class XT, class RT, int NW, int CPL, bool RES, bool FULL, bool ACC, bool REC>
+// ACC: some column sum is wanted; REC: a.res is the residual, and r is made of it and x; OWN: a
+// block has whole groups of the gate, one after the other, and writes their sums itself (a kernel of
+// its own: the test after each row costs the others 3 to 5%)
+template <class XT, class RT, int NW, int CPL, bool RES, bool FULL, bool ACC, bool REC, bool OWN>
 __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const NormArgs a) {
   constexpr int WPB = NW == 1 ? 8 : NW;
   constexpr int AC = ACC ? CPL : 1;
@@ -482,9 +486,29 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
   // the block's group: the rows that share a gate row (one group of all rows without column sums of a gate)
   const int64_t per = a.part_gate ? a.gate_rows : a.rows;
   const int64_t group = blockIdx.x / a.blocks_per_group;
-  const int64_t first = group * per + (int64_t)(blockIdx.x % a.blocks_per_group) * (NW == 1 ? WPB : 1) + (NW == 1 ? wave : 0);
-  const int64_t last = min(group * per + per, a.rows);
-  const int64_t step = (int64_t)a.blocks_per_group * (NW == 1 ? WPB : 1);
+  int64_t first = group * per + (int64_t)(blockIdx.x % a.blocks_per_group) * (NW == 1 ? WPB : 1) + (NW == 1 ? wave : 0);
+  int64_t last = min(group * per + per, a.rows);
+  int64_t step = (int64_t)a.blocks_per_group * (NW == 1 ? WPB : 1);
+  int64_t group_end = 0;  // of the group that the block is in
+  if constexpr (OWN) {
+    first = (int64_t)blockIdx.x * a.groups / gridDim.x * a.gate_rows;
+    last = min(((int64_t)blockIdx.x + 1) * a.groups / gridDim.x * a.gate_rows, a.rows);
+    step = 1;
+    group_end = first + a.gate_rows;
+  }
+  // whether a group's rows end with `row`, whose gradients are in the block's sums
+  auto ends = [&](int64_t row) {
+    if (row + 1 != group_end && row + 1 != last) return false;
+    group_end += a.gate_rows;
+    return true;
+  };
+  auto put_group = [&](int64_t row, int c, const float (&sum)[8]) {
+    const int64_t at = (int64_t)((uint32_t)row / (uint32_t)a.gate_rows) * H;
+    if (a.gate_f32)
+      n_set((float*)a.dgate_sum + at, (c * 64 * NW + t) * 8, H, sum);
+    else
+      n_set((uint16_t*)a.dgate_sum + at, (c * 64 * NW + t) * 8, H, sum);
+  };
   float aw[AC][8], ap[FULL ? AC : 1][8], ag[FULL ? AC : 1][8];
   if constexpr (ACC) {
 #pragma unroll
@@ -500,8 +524,21 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
 #pragma unroll
       for (int j = 0; j < 4 * CPL; ++j) own[j / (2 * CPL)][j / 2 % CPL][j % 2][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int64_t row = first; row < last; row += step)
+    for (int64_t row = first; row < last; row += step) {
       n_bwd_long<XT, RT, NW, CPL, ACC, REC>(a, row, wave, t, sums, turn, aw, own);
+      if constexpr (OWN) {
+        if (ends(row)) {
+#pragma unroll 1
+          for (int c = 0; c < CPL; ++c) {
+            float g[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[i] = own[1][c][i / 4][t][i % 4];
+            own[1][c][0][t] = own[1][c][1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            put_group(row, c, g);
+          }
+        }
+      }
+    }
     if constexpr (ACC) {
 #pragma unroll
       for (int c = 0; c < CPL; ++c)
@@ -690,6 +727,16 @@ __global__ __launch_bounds__(NW == 4 ? 256 : 512) void norm_bwd_kernel(const Nor
 #pragma unroll
         for (int c = 0; c < CPL; ++c) n_set(dx, (c * 64 * NW + t) * 8, H, g[c]);
       }
+      if constexpr (OWN) {
+        if (ends(row)) {
+#pragma unroll
+          for (int c = 0; c < CPL; ++c) {
+            put_group(row, c, ag[c]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ag[c][i] = 0.f;
+          }
+        }
+      }
     }
   }
   if constexpr (ACC) {
@@ -802,7 +849,13 @@ void norm_bwd_launch(const NormArgs& a, unsigned blocks, hipStream_t st) {
 #define AF3_NB(NW, CPL)                                                                                           \
   do {                                                                                                            \
     const dim3 block(NW == 4 ? 256 : 512);                                                                         \
-    hipLaunchKernelGGL((norm_bwd_kernel<XT, RT, NW, CPL, RES, FULL, ACC, REC>), dim3(blocks), block, 0, st, a);         \
+    if constexpr (FULL && ACC) {                                                                                  \
+      if (a.dgate_sum) {                                                                                          \
+        hipLaunchKernelGGL((norm_bwd_kernel<XT, RT, NW, CPL, RES, FULL, ACC, REC, true>), dim3(blocks), block, 0, st, a); \
+        return;                                                                                                   \
+      }                                                                                                           \
+    }                                                                                                             \
+    hipLaunchKernelGGL((norm_bwd_kernel<XT, RT, NW, CPL, RES, FULL, ACC, REC, false>), dim3(blocks), block, 0, st, a); \
     return;                                                                                                       \
   } while (0)
   if constexpr (!FULL) if (norm_bwd_wave_row(a.rows, a.H, FULL)) AF3_NB(1, 2);
@@ -821,20 +874,25 @@ struct NormPlan {
   int64_t groups, blocks;
   int blocks_per_group;
   int64_t off_w, off_post, off_gate, off_dots, bytes;
+  bool own_groups;  // blocks have whole groups of a gate
 };
 
 NormPlan norm_plan(int64_t rows, int H, int gate_cols, int64_t gate_rows, bool full, int want_w, int want_post, int want_gate) {
   NormPlan p;
-  const bool sums = want_gate && gate_cols > 1 && gate_rows > 1;  // of a gate row over its group
+  bool sums = want_gate && gate_cols > 1 && gate_rows > 1;  // of a gate row over its group
   p.groups = sums ? af3_cdiv(rows, gate_rows) : 1;
-  const int64_t per = sums ? gate_rows : rows;
   const bool wave_row = norm_bwd_wave_row(rows, H, full);
-  const int64_t units = wave_row ? af3_cdiv(per, 8) : per;  // row steps of one block
   const int64_t total = full || (!wave_row && rows < 4 * kNormBwdBlocks) ? kNormBwdBlocks : 2 * kNormBwdBlocks;
-  const int64_t bpg = total / p.groups;  // (not rounded up: a block too many is a second round)
+  // More groups than blocks: a block takes whole ones and writes their sums, so partials stay a row per block.
+  // A block and a row of partials for each group instead, us: 8000 x 2 x 2880 bf16 4370 for 181, 300 x 10 with a
+  // post norm and an fp32 stream 204 for 61, 257 x 100 608 for 500.
+  p.own_groups = p.groups > total;
+  if (p.own_groups) sums = false;
+  const int64_t per = sums ? gate_rows : rows;
+  const int64_t units = wave_row ? af3_cdiv(per, 8) : per;  // row steps of one block
+  const int64_t bpg = p.own_groups ? total : total / p.groups;  // (not rounded up: a block too many is a second round)
   p.blocks_per_group = (int)(bpg < units ? bpg : units);
-  if (p.blocks_per_group < 1) p.blocks_per_group = 1;
-  p.blocks = p.groups * p.blocks_per_group;
+  p.blocks = p.own_groups ? total : p.groups * p.blocks_per_group;
   const int64_t part = p.blocks * H * 4;
   p.off_w = 0;
   p.off_post = p.off_w + (want_w ? part : 0);
@@ -940,11 +998,10 @@ extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* d
               "residual_norm_bwd: r_again goes with a bf16 residual, x, dh and dweight");
   AF3_REQUIRE(!full || (x && (!post_weight || rstd_x) && (!gate_cols || gate)), "residual_norm_bwd: null pointer");
   const NormPlan p = norm_plan(rows, H, gate_cols, gate_rows, full, dweight != nullptr, dpost != nullptr, dgate != nullptr);
-  AF3_REQUIRE(p.blocks < (int64_t)1 << 31 && (p.groups + 2) * af3_cdiv(H, kJoinCols) < (int64_t)1 << 31, "residual_norm_bwd: too many gate rows");
   AF3_REQUIRE((size_t)p.bytes <= ws_bytes && (p.bytes == 0 || workspace), "residual_norm_bwd: workspace too small");
   hipStream_t st = (hipStream_t)stream_;
   uint8_t* const ws = (uint8_t*)workspace;
-  const bool gate_sums = dgate && gate_cols > 1 && gate_rows > 1;
+  const bool gate_sums = dgate && gate_cols > 1 && gate_rows > 1 && !p.own_groups;
   NormArgs a = {};
   a.x = x, a.ldx = ldx, a.res = r, a.ldr = ldr, a.weight = weight, a.w_f32 = w_f32;
   a.post = post_weight, a.post_f32 = post_f32, a.gate = gate, a.gate_f32 = gate_f32, a.gate_cols = gate_cols;
@@ -956,7 +1013,8 @@ extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* d
   a.dgate = dgate && gate_cols > 1 && gate_rows == 1 ? dgate : nullptr;
   a.gate_dots = dgate && gate_cols == 1 ? (float*)(ws + p.off_dots) : nullptr;
   a.blocks_per_group = p.blocks_per_group;
-  const bool acc = a.part_w || a.part_post || a.part_gate;
+  if (p.own_groups) a.groups = p.groups, a.dgate_sum = dgate;
+  const bool join = a.part_w || a.part_post || a.part_gate, acc = join || a.dgate_sum;
   const unsigned blocks = (unsigned)p.blocks;
   if (!has_residual) {
     if (x_f32)
@@ -986,7 +1044,7 @@ extern "C" int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* d
   }
   int e = af3::check_launch("residual_norm_bwd");
   if (e) return e;
-  if (acc) {
+  if (join) {
     JoinArgs j = {};
     j.part[0] = a.part_w, j.part[1] = a.part_post, j.part[2] = a.part_gate;
     j.out[0] = dweight, j.out[1] = dpost, j.out[2] = dgate;

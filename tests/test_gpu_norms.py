@@ -421,3 +421,61 @@ def test_more_rows_and_gates_than_a_launch_holds(dev):
     assert torch.equal(r, res + gate.detach() * x)   # (at most 6)
     (dg,) = torch.autograd.grad(r, gate, res)
     assert torch.equal(dg, (res * x).sum((1, 2), dtype=F32)[:, None, None].to(BF))   # (at most 64)
+
+
+@pytest.mark.parametrize("G,S,H,post,rt", [(257, 3, 264, True, BF), (3001, 3, 264, False, F32), (5000, 2, 77, True, BF),
+                                           (700, 2, 5003, True, F32), (600, 2, 5003, False, BF), (300, 3, 9001, True, BF),
+                                           (513, 2, 8200, False, F32)])
+def test_gate_of_many_short_groups(dev, G, S, H, post, rt):
+    """More groups than the backward has blocks: a gate [G, 1, H] shared by two or three rows."""
+    t, d = _inputs(G * S, H, BF, rt, dev, post=post, gate=(G, 1, H), seed=H)
+    full = t["gate"].expand(G, S, H).reshape(G * S, H)
+    want = on.residual_norm(t["x"], t["residual"], t["weight"], post=t["post"], gate=full, dr=t["dr"], dh=t["dh"])
+    want["dgate"], want["dgate_tol"] = (want[n].view(G, S, H).sum(1, keepdim=True) for n in ("dgate", "dgate_tol"))
+    _compare(_call(d, shape=(G, S)), want, G * S)
+    # the gate's gradient alone, which no other sum is made beside
+    from agent_factory_3_amd import norms
+    gate = d["gate"].detach().requires_grad_()
+    r, h = norms.residual_norm(d["x"].view(G, S, H), d["residual"].view(G, S, H), d["weight"], post_weight=d["post"], gate=gate)
+    (g,) = torch.autograd.grad([r, h], gate, [d["dr"].view(r.shape), d["dh"].view(r.shape)])
+    _compare({"dgate": g}, {k: want[k] for k in ("dgate", "dgate_tol")}, G * S)
+
+
+def test_gate_of_heads_and_a_last_group_that_is_not_whole(dev):
+    """[B, S, heads, D] with a gate [B, S, 1, D]; the C entry with 1001 rows in groups of two."""
+    from agent_factory_3_amd import _capi
+    B, S, N, D = 2, 301, 4, 64
+    t, d = _inputs(B * S * N, D, BF, BF, dev, gate=(B, S, 1, D), seed=1)
+    full = t["gate"].expand(B, S, N, D).reshape(-1, D)
+    want = on.residual_norm(t["x"], t["residual"], t["weight"], gate=full, dr=t["dr"], dh=t["dh"])
+    want["dgate"], want["dgate_tol"] = (want[n].view(B, S, N, D).sum(2, keepdim=True) for n in ("dgate", "dgate_tol"))
+    _compare(_call(d, shape=(B, S, N)), want, B * S * N)
+    for G, per in ((501, 2), (101, 10)):
+        rows, H = G * per - 1, 72
+        t, d = _inputs(rows, H, F32, F32, dev, gate=(G, H), seed=2)
+        full = t["gate"].repeat_interleave(per, 0)[:rows]
+        want = on.residual_norm(t["x"], t["residual"], None, gate=full, dr=t["dr"])
+        for n in ("dgate", "dgate_tol"):
+            want[n] = torch.cat([want[n], want[n].new_zeros(1, H)]).view(G, per, H).sum(1)
+        want = {k: v for k, v in want.items() if k[0] == "d"}
+        n = int(_capi.load().af3_residual_norm_bwd_workspace_bytes(rows, H, 1, H, per, 0, 0, 1))
+        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=dev)
+        dx, dres, dg = torch.empty_like(d["x"]), torch.empty_like(d["x"]), torch.full((G + 1, H), 7.0, device=dev)
+        p = lambda v: v.data_ptr()  # noqa: E731
+        _capi.call("af3_residual_norm_bwd", p(d["dr"]), H, None, 0, None, 1, 0, 0, p(d["x"]), 1, H, None, None, None, 0, None, 0,
+                   p(d["gate"]), 1, H, per, 1.0, 1, rows, H, p(dx), p(dres), None, None, p(dg), p(ws), n,
+                   torch.cuda.current_stream().cuda_stream)
+        _compare({"dx": dx, "dresidual": dres, "dgate": dg[:G]}, want, rows)
+        assert (dg[G] == 7).all()
+
+
+def test_gate_of_more_groups_than_the_joining_launch_held(dev):
+    """24000 groups of two rows of 2880.  Small whole numbers: every sum is exact."""
+    from agent_factory_3_amd import norms
+    G, S, H = 24000, 2, 2880
+    g = torch.Generator(dev).manual_seed(0)
+    draw = lambda *s: torch.randint(-2, 3, s, generator=g, device=dev, dtype=torch.int8).to(BF)  # noqa: E731
+    x, res, gate = draw(G, S, H), draw(G, S, H), draw(G, 1, H).requires_grad_()
+    r, _ = norms.residual_norm(x, res, gate=gate)
+    (dg,) = torch.autograd.grad(r, gate, res)
+    assert torch.equal(dg, (res * x).sum(1, keepdim=True))

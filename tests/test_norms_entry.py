@@ -29,3 +29,13 @@ def test_backward_without_a_residual_takes_either_gradient():
         _bwd(dh=None, dresidual=P)
     with pytest.raises(RuntimeError, match="without a residual"):
         _bwd(dresidual=P, dx=P)
+
+
+def test_workspace_does_not_grow_with_a_gates_groups():
+    """A row of partials per block and sum, however many groups a gate has."""
+    if not _capi.lib_path().exists():
+        pytest.skip("library not built")
+    size = _capi.load().af3_residual_norm_bwd_workspace_bytes
+    H = 2880
+    for groups in (1, 2, 100, 256, 257, 8000, 1 << 20):
+        assert size(2 * groups, H, 1, H, 2, 1, 1, 1) <= 3 * 256 * H * 4, groups
