@@ -37,8 +37,9 @@ def linear(x, weight, bias=None, activation=None, residual=None, dy=None):
     if bias is not None:
         z, e_z = z + bias, e_z + 2.0 ** -24 * (z.abs() + bias.abs())
     y, slope, curve = act(z, activation)
-    # fp32 activations: exponentials, error function and tanh within 2^-20 of values up to |z| + 1
-    e_y = e_z if activation is None else 1.2 * e_z + 2.0 ** -20 * (y.abs() + (z.abs() < 20) * 1e-1 * z.abs())
+    # fp32 activations: an exponential of up to 88 after five roundings, 5 * 88 * 2^-24 < 2^-15 of the value, and as
+    # much for the rest; 0 where the exponential leaves fp32 (values below |z| e^-87 < 2^-118)
+    e_y = e_z if activation is None else 1.2 * e_z + 2.0 ** -14 * y.abs() + 2.0 ** -118
     if residual is not None:
         y, e_y = y + residual, e_y + 2.0 ** -24 * (y.abs() + residual.abs())
     o = {"y": y, "y_tol": BF * y.abs() + e_y}

@@ -263,3 +263,33 @@ def test_tensors_without_memory_of_their_own_are_refused(dev):
         t[name] = Held.of(t[name])
         with pytest.raises(TypeError, match=name):
             linear(t["x"], t["weight"], t["bias"], residual=t["residual"])
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("T", [3, 40])
+def test_activations_keep_their_digits_in_the_tail(dev, activation, T):
+    """Arguments from -13 to 13 (the bias, exact, beside a product of 0): values within one rounding of their own
+    size, however small; slopes within 2^-14 of their terms'."""
+    from agent_factory_3_amd.linear import linear
+    z = torch.linspace(-13, 13, 1041).to(BF).float()
+    w, x = torch.zeros(z.numel(), 8, dtype=BF, device=dev), torch.ones(T, 8, dtype=BF, device=dev)
+    b = z.to(dev).requires_grad_()
+    y = linear(x, w, b, activation=activation)
+    dy = torch.zeros_like(y)
+    dy[T - 1] = 1
+    (db,) = torch.autograd.grad(y, b, dy)
+    zd = z.double()
+    want, slope, _ = ol.act(zd, activation)
+    if activation == "gelu":        # (1 + erf loses the tail's digits in 64 bits too, from -7 on)
+        phi = 0.5 * torch.erfc(-zd / 2 ** 0.5)
+        want, slope = zd * phi, phi + zd * torch.exp(-zd * zd / 2) / (2 * torch.pi) ** 0.5
+    elif activation == "gelu_tanh":
+        u = (2 / torch.pi) ** 0.5 * (zd + 0.044715 * zd ** 3)
+        s = torch.sigmoid(2 * u)
+        want = zd * s
+        slope = s + zd * 2 * s * torch.sigmoid(-2 * u) * (2 / torch.pi) ** 0.5 * (1 + 0.134145 * zd * zd)
+    # fp32's errors as in the oracle; bf16 and fp32 below 2^-118 are left alone (their exponentials vanish)
+    err = (y.detach()[T - 1].cpu().double() - want).abs()
+    assert (err <= (2.0 ** -8 + 2.0 ** -14) * want.abs() + 2.0 ** -118).all(), float(z[(err / want.abs()).nan_to_num().argmax()])
+    terms = (want / zd).nan_to_num(nan=0.5).abs() + (slope - (want / zd).nan_to_num(nan=0.5)).abs()
+    assert ((db.cpu().double() - slope).abs() <= 2.0 ** -14 * terms + 2.0 ** -118).all()
