@@ -19,6 +19,7 @@ _p = C.c_void_p
 _i32 = C.c_int
 _i64 = C.c_int64
 _f32 = C.c_float
+_f64 = C.c_double
 _sz = C.c_size_t
 
 # name -> (restype, argtypes)
@@ -101,7 +102,7 @@ _SIGNATURES = {
     "af3_linear_dz": (_i32, [_p, _i64, _p, _i32, _i64, _i64, _p, _i64, _p, _i32, _p, _sz, _p]),
     "af3_grad_norm_partials": (_sz, [_p, _i32]),
     "af3_grad_norm": (_i32, [_p, _p, _p, _i32, _i32, _p, _i64, _p, _p, _p]),
-    "af3_grad_scale": (_i32, [_p, _p, _p, _i32, _i32, _p, _i64, _f32, _p, _p]),
+    "af3_grad_scale": (_i32, [_p, _p, _p, _i32, _i32, _p, _i64, _f64, _p, _p]),
 }
 
 _lib = None

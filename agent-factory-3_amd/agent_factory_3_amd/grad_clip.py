@@ -220,7 +220,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
 
     Within the limit the gradients are read once and not written.  The norm is summed in
     64 bits in a fixed order and returned in fp32 (torch takes a norm per tensor in the
-    tensor's type, and a norm of those).  Nothing synchronises the host unless
+    tensor's type, and a norm of those); the factor is formed from the 64-bit norm and
+    rounded to fp32 once.  Nothing synchronises the host unless
     ``error_if_nonfinite``.
 
     Args:

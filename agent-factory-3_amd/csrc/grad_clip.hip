@@ -136,8 +136,8 @@ __device__ __forceinline__ double clip_total(const double* partials, int n, doub
 }
 
 template <int P>
-__device__ __forceinline__ float clip_norm_of(double s) {
-  return P == 2 ? (float)sqrt(s) : (float)s;
+__device__ __forceinline__ double clip_norm_of(double s) {
+  return P == 2 ? sqrt(s) : s;
 }
 
 template <int P>
@@ -146,19 +146,22 @@ __global__ __launch_bounds__(256) void clip_sum_kernel(const double* partials, i
   const double s = clip_total<P>(partials, n, lds);
   if (threadIdx.x == 0) {
     if (sum) *sum = s;
-    if (norm) *norm = clip_norm_of<P>(s);
+    if (norm) *norm = (float)clip_norm_of<P>(s);
   }
 }
 
 template <int P>
 __global__ __launch_bounds__(256) void clip_scale_kernel(const ClipTab tab, int n_tab, int64_t chunk,
-                                                         const double* partials, int n_partials, float max_norm,
+                                                         const double* partials, int n_partials, double max_norm,
                                                          float* norm_out) {
   __shared__ double lds[4];
-  const float norm = clip_norm_of<P>(clip_total<P>(partials, n_partials, lds));
-  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
-  float f = max_norm / (norm + 1e-6f);
-  if (f >= 1.0f) return;  // (a NaN norm goes on, and makes every gradient NaN)
+  const double norm = clip_norm_of<P>(clip_total<P>(partials, n_partials, lds));
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  // the factor is every gradient's, so it is rounded once, from 64 bits.  (A norm that is infinite in fp32, as
+  // it is returned, scales by 0.)
+  const double factor = max_norm / (isinf((float)norm) ? (double)INFINITY : norm + 1e-6);
+  if (factor >= 1.0) return;  // (a NaN norm goes on, and makes every gradient NaN)
+  const float f = (float)factor;
   const ClipPos c = clip_find(tab, n_tab, chunk, blockIdx.x);
   if (c.f32) {
     float* const p = (float*)c.p;
@@ -291,7 +294,7 @@ extern "C" int af3_grad_norm(const uint64_t* ptrs, const int64_t* sizes, const u
 }
 
 extern "C" int af3_grad_scale(const uint64_t* ptrs, const int64_t* sizes, const uint8_t* is_f32, int n, int norm_type,
-                              const double* partials, int64_t n_partials, float max_norm, float* norm, void* stream_) {
+                              const double* partials, int64_t n_partials, double max_norm, float* norm, void* stream_) {
   int64_t total, chunks;
   const int rc = clip_check("grad_scale", ptrs, sizes, is_f32, n, norm_type, &total, &chunks);
   if (rc) return rc;

@@ -557,13 +557,13 @@ int af3_linear_dz(const uint16_t* dy, int64_t ldy, const uint16_t* z, int act, i
  * writes one 64-bit partial per chunk (af3_grad_norm_partials of them), their sum
  * (sum |g|^p, or the largest) to `sum` and the norm to `norm` (each may be NULL).
  * af3_grad_scale takes partials, of these and of other tensors, scales where the
- * factor is below 1 (a NaN norm gives NaN), and writes the norm (NULL: not);
+ * factor, formed in 64 bits and rounded to fp32 once, is below 1 (a NaN norm gives NaN), and writes the norm (NULL: not);
  * tensors that share memory are refused. */
 size_t af3_grad_norm_partials(const int64_t* sizes, int n);
 int af3_grad_norm(const uint64_t* ptrs, const int64_t* sizes, const uint8_t* is_f32, int n, int norm_type,
                   double* partials, int64_t n_partials, double* sum, float* norm, void* stream);
 int af3_grad_scale(const uint64_t* ptrs, const int64_t* sizes, const uint8_t* is_f32, int n, int norm_type,
-                   const double* partials, int64_t n_partials, float max_norm, float* norm, void* stream);
+                   const double* partials, int64_t n_partials, double max_norm, float* norm, void* stream);
 
 #ifdef __cplusplus
 }

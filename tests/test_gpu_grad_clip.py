@@ -208,3 +208,26 @@ def test_saved_gradients_are_seen_to_change(dev):
     grad_clip.clip_grad_norm_([p], 1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("p", [2, 1, math.inf])
+def test_the_factor_is_rounded_once(dev, p):
+    """Factor and product: two roundings of fp32, 2^-24 each (and the type's own), from the norm in 64 bits and a
+    limit that fp32 does not hold."""
+    from agent_factory_3_amd import grad_clip
+    for seed in range(12):
+        ts = _tensors((30000, 77), (F32, BF) if seed % 3 == 2 else (F32,), dev, seed=seed)
+        before = [t.cpu().double() for t in ts]
+        f = 0.1 / (_norm(ts, p) + 1e-6)
+        grad_clip.clip_grad_norm_(_params(ts), 0.1, p)
+        for t, b in zip(ts, before):
+            half = torch.finfo(t.dtype).eps / 2
+            tol = half + (2.0 ** -24 + 2.0 ** -47 if t.dtype is F32 else 2.0 ** -22)
+            assert ((t.cpu().double() - b * f).abs() <= (b * f).abs() * tol + 2.0 ** -133).all(), seed
+
+
+def test_a_norm_that_fp32_does_not_hold(dev):
+    """It is returned as infinite, and scales by 0."""
+    from agent_factory_3_amd import grad_clip
+    g = torch.full((1000,), 3e38, device=dev)
+    assert grad_clip.clip_grad_norm_(_params([g]), 1.0).isinf() and (g == 0).all()
