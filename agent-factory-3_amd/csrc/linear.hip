@@ -122,7 +122,7 @@ __device__ __forceinline__ float lin_slope(float z, int act) {
     return phi + z * 0.39894228f * e;
   }
   if (act == kActGeluTanh) {
-    z = fminf(fmaxf(z, -30.f), 30.f);  // (0 and 1 there; its square must not overflow)
+    z = z > 30.f ? 30.f : z < -30.f ? -30.f : z;  // (0 and 1 there; its square must not overflow.  A NaN stays)
     const float s = lin_half_tanh(z);
     return s + z * 2.f * s * (1.f - s) * 0.79788456f * (1.f + 0.134145f * z * z);
   }

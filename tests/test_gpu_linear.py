@@ -293,3 +293,17 @@ def test_activations_keep_their_digits_in_the_tail(dev, activation, T):
     assert (err <= (2.0 ** -8 + 2.0 ** -14) * want.abs() + 2.0 ** -118).all(), float(z[(err / want.abs()).nan_to_num().argmax()])
     terms = (want / zd).nan_to_num(nan=0.5).abs() + (slope - (want / zd).nan_to_num(nan=0.5)).abs()
     assert ((db.cpu().double() - slope).abs() <= 2.0 ** -14 * terms + 2.0 ** -118).all()
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("T", [3, 40])
+def test_slope_of_nan_is_nan(dev, activation, T):
+    """A NaN row of x: its gradient is NaN too, and no other row's."""
+    from agent_factory_3_amd.linear import linear
+    t, d = _inputs(T, 64, 24, dev, residual=False)
+    x = d["x"].clone()
+    x[1, 7] = float("nan")
+    x.requires_grad_()
+    (dx,) = torch.autograd.grad(linear(x, d["weight"], d["bias"], activation=activation), x, d["dy"])
+    ok = torch.arange(T, device=dev) != 1
+    assert dx[1].isnan().all() and dx[ok].isfinite().all()
