@@ -94,6 +94,7 @@ _SIGNATURES = {
     "af3_residual_norm_bwd": (_i32, [_p, _i64, _p, _i64, _p, _i32, _i32, _i64, _p, _i32, _i64, _p, _p, _p, _i32, _p, _i32, _p,
                                      _i32, _i32, _i64, _f32, _i32, _i64, _i32, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "af3_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "af3_linear_tile": (_i32, [_i64, _i64, _i64, _i32, _i32, _p]),
     "af3_linear": (_i32, [_p, _i64, _i32, _p, _i64, _i32, _i64, _i64, _i64, _p, _i32, _i32, _p, _i64, _p, _p, _p, _sz, _p]),
     "af3_linear_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32, _i32]),
     "af3_linear_bwd": (_i32, [_p, _i64, _p, _i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i32, _p,

@@ -908,6 +908,14 @@ extern "C" size_t af3_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, in
   return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
 }
 
+extern "C" int af3_linear_tile(int64_t M, int64_t N, int64_t K, int p_trans, int q_trans, int* tile) {
+  AF3_REQUIRE(tile && M > 0 && N > 0 && K > 0 && M < (int64_t)1 << 30 && N < (int64_t)1 << 30 && K < (int64_t)1 << 30,
+              "linear_tile: bad sizes");
+  const LinPlan p = lin_skinny(M, p_trans, q_trans) ? LinPlan{} : lin_plan(M, N, K);
+  tile[0] = p.bm, tile[1] = p.bn, tile[2] = p.stages, tile[3] = p.splits;
+  return 0;
+}
+
 extern "C" int af3_linear(const uint16_t* p, int64_t ldp, int p_trans, const uint16_t* q, int64_t ldq, int q_trans,
                           int64_t M, int64_t N, int64_t K, const void* bias, int bias_f32, int act,
                           const uint16_t* residual, int64_t ldr, uint16_t* y, uint16_t* z, void* workspace,

@@ -536,7 +536,11 @@ int af3_residual_norm_bwd(const void* dr, int64_t lddr, const void* dh, int64_t 
  * serve the products), then dx [T][K] = dz W, dweight [N][K] = dz^T x, dbias [N], each
  * NULL if not wanted; rows as af3_linear takes them.
  * af3_linear_dz: dz [M][ldz] = dy act'(z) (zeros from N to the next multiple of 8
- * within ldz; NULL: not written) and dbias [N] = its column sums (NULL: not). */
+ * within ldz; NULL: not written) and dbias [N] = its column sums (NULL: not).
+ * af3_linear_tile: tile[4] = rows and columns of the tiles that af3_linear makes such
+ * a product in, the ring's stages, and the blocks that share a tile's k (zeros: the
+ * kernel for few rows). */
+int af3_linear_tile(int64_t M, int64_t N, int64_t K, int p_trans, int q_trans, int* tile);
 size_t af3_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int p_trans, int q_trans);
 int af3_linear(const uint16_t* p, int64_t ldp, int p_trans, const uint16_t* q, int64_t ldq, int q_trans, int64_t M,
                int64_t N, int64_t K, const void* bias, int bias_f32, int act, const uint16_t* residual, int64_t ldr,
