@@ -231,3 +231,40 @@ def test_a_norm_that_fp32_does_not_hold(dev):
     from agent_factory_3_amd import grad_clip
     g = torch.full((1000,), 3e38, device=dev)
     assert grad_clip.clip_grad_norm_(_params([g]), 1.0).isinf() and (g == 0).all()
+
+
+def test_sharded_and_whole_gradients_together(dev):
+    """DTensor gradients in several groups beside plain ones: a sum per group on the GPU, joined, one factor.  (A
+    process group whose reductions leave what is there: this rank's elements are all that counts.)"""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Replicate, Shard
+    from torch.testing._internal.distributed.fake_pg import FakeStore
+
+    from agent_factory_3_amd import grad_clip
+    dist.init_process_group("fake", store=FakeStore(), rank=0, world_size=4)
+    try:
+        mesh = init_device_mesh("cuda", (2, 2), mesh_dim_names=("dp", "tp"))
+        sizes = (70000, 9, 0, 30001, 8192, 64 * 50)
+        for p in (2, 1, math.inf):
+            for max_norm in (0.1, 1e9):
+                local = _tensors(sizes, (BF, F32), dev, seed=int(max_norm))
+                before = [t.cpu().double() for t in local]
+                local[5] = local[5].view(50, 64).t()   # another memory order
+                places = ([Shard(0), Replicate()], None, [Shard(0), Shard(0)], [Shard(0), Shard(0)], [Replicate(), Replicate()],
+                          [Replicate(), Shard(1)])
+                grads = [t if q is None else DTensor.from_local(t, mesh, q, run_check=False) for t, q in zip(local, places)]
+                want = _norm(before, p)
+                assert abs(float(grad_clip.grad_norm(grads, p)) - want) <= 2.0 ** -23 * want
+                norm = grad_clip.clip_grad_norm_(_params(grads), max_norm, p)
+                assert norm.device == local[0].device and abs(float(norm) - want) <= 2.0 ** -23 * want
+                f = min(1.0, max_norm / (want + 1e-6))
+                before[5] = before[5].view(50, 64).t()
+                for t, b in zip(local, before):
+                    half = torch.finfo(t.dtype).eps / 2 if f < 1 else 0.0
+                    assert ((t.cpu().double() - b * f).abs() <= (b * f).abs() * (half + 2.0 ** -22) + 2.0 ** -133).all()
+        # ranks that hold nothing of a group still take part, and get the norm
+        empty = [DTensor.from_local(torch.zeros(0, 3, device=dev), mesh, [Shard(0), Shard(0)], run_check=False)]
+        assert float(grad_clip.clip_grad_norm_(_params(empty), 1.0)) == 0
+    finally:
+        dist.destroy_process_group()
