@@ -47,6 +47,10 @@ def _linear_forward(self, input):
     return linear(input, self.weight, self.bias)
 
 
+# (a bound method is pickled by its name: a model saved whole loads with its classes' own forwards)
+_norm_forward.__name__ = _linear_forward.__name__ = "forward"
+
+
 def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None, past_key_values=None, use_cache=False,
                    position_embeddings=None, **kwargs):
     """GptOssDecoderLayer.forward with the add and the norm between attention and experts as one."""
@@ -93,7 +97,8 @@ def enable_fused_layers(model, projections: bool = True) -> int:
     then not called), and with ``projections`` q, k, v and o (the layers inside PEFT's
     wrappers too) on ``linear.linear``: a few percent slower than the library's products
     forward, faster backward, and deterministic.  Results differ from transformers' by
-    roundings.  Again is harmless.
+    roundings.  Again is harmless; a copy of the model is fused too, one saved and loaded whole
+    needs the call again.
     """
     from transformers.models.gpt_oss.modeling_gpt_oss import GptOssDecoderLayer, GptOssRMSNorm
     layers = [m for m in model.modules() if isinstance(m, GptOssDecoderLayer)]
