@@ -44,6 +44,8 @@ def _linear_forward(self, input):
     ts = [t for t in (input, self.weight, self.bias) if t is not None]
     if not all(t.is_cuda and t.dtype == torch.bfloat16 and t.device == input.device and _plain(t) for t in ts):
         return type(self).forward(self, input)
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != torch.bfloat16:   # (its product's type)
+        return type(self).forward(self, input)
     return linear(input, self.weight, self.bias)
 
 

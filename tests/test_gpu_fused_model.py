@@ -215,3 +215,22 @@ def test_only_the_norms_trained(dev):
         p.requires_grad_(n in names)
     for n, a, b in zip(names, grads(), want):
         assert b.abs().max() > 0 and torch.equal(a, b), n
+
+
+def test_autocast_to_another_type_runs_as_it_did(dev):
+    """Under autocast nn.Linear's output has autocast's type: only bf16's is the fused product's."""
+    m = torch.nn.Linear(64, 40).to(dev, torch.bfloat16)
+    x = torch.randn(3, 64, device=dev).to(torch.bfloat16)
+    with torch.no_grad():
+        want = {}
+        for t in (torch.float16, torch.float32, torch.bfloat16):
+            with torch.autocast("cuda", dtype=t):
+                want[t] = m(x)
+        m.forward = fused_layers._linear_forward.__get__(m)
+        for t, w in want.items():
+            with torch.autocast("cuda", dtype=t):
+                got = m(x)
+            assert got.dtype == w.dtype
+            assert t == torch.bfloat16 or torch.equal(got, w)
+        with torch.autocast("cuda", dtype=torch.float16, enabled=False):
+            assert m(x).dtype == torch.bfloat16
