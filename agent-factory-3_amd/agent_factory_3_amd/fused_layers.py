@@ -31,6 +31,7 @@ def _norm_takes(norm, x) -> bool:
     w = getattr(norm, "weight", None)
     return (x.is_cuda and x.dtype in norms._TYPES and w is not None and w.dtype in norms._TYPES and w.device == x.device
             and hasattr(norm, "variance_epsilon") and _plain(w)
+            and w.shape == x.shape[-1:]   # (else a placeholder: the weight comes with the module's call)
             and norms.MIN_HIDDEN <= x.shape[-1] <= norms.MAX_HIDDEN)
 
 
