@@ -33,10 +33,10 @@
 // 157 (140), 8192 x 2880 from 4096 with W as stored 168 (193), 16384 x 2880 from 4096 329
 // (285), with bias and residual 335 (and an add of 55), 16384 x 4096 from 2880 with W as
 // stored 309 (308), 2880 x 4096 from 16384 rows 326 (446); 1021 x 2880 from 2880 24 (26),
-// 8192 x 512 from 2880 28 (29).  The large ones run 1.17 to 1.29 PFLOP/s at 1.75 GHz: 73% of
-// the CUs' busy cycles issue products, and taking out the copies, or the fragment reads,
-// gains 4 and 14%; the card's power bounds them.  Products of 16 x 16 x 32 (3 to 5% less time
-// in 128 x 128 tiles) leave the compiler moving accumulators between register files.
+// 8192 x 512 from 2880 28 (29).  The large ones run 1.17 to 1.29 PFLOP/s: 73% of the CUs' busy
+// cycles issue products, at a clock of 1.75 GHz (2.4 without load), so the card's power bounds
+// them.  Products of 16 x 16 x 32 (3 to 5% less time in 128 x 128 tiles) leave the compiler
+// moving accumulators between register files.
 //
 // Few tiles and a long k (dW of narrow layers): blocks share a tile's k-steps and write
 // fp32 partials, which lin_join_kernel adds in order and gives the epilogue.
@@ -646,8 +646,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* part, int sp
 
 // Up to 16 NT rows of x: a block makes 16 columns (rows of W).  Its 16 waves share k in
 // units of 64, a wave's lane (r, g) taking k = 8 g + (0..7) and 32 more of row r of W and of
-// x (two products of 32 k), so W is read once, 64 contiguous bytes of 16 rows at a time,
-// with all of a wave's loads in flight; the waves' sums meet in LDS.
+// x (two products of 32 k), so W is read once, 64 contiguous bytes of 16 rows at a time; the
+// waves' sums meet in LDS.  A wave has the loads of U units in flight together where K brings it
+// as many (U 4, or 2 for 17 to 32 rows: all waves from K = 1024 U on, none below 64 (16 U - 15),
+// 3136 and 1088); units past a multiple of U go one after the other.
 // Addresses need no alignment; elements past K are zeros.  One row at a stated N x K, us:
 // 512 x 2880 5.2, 4096 x 2880 6.1, 2880 x 4096 6.7 (4.0 TB/s of W); 32 rows 9.7, 10.3, 12.9,
 // where gathering x's 16-row fragments costs 3 to 6 of it.  Eight waves, two columns' tiles

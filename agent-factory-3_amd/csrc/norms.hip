@@ -19,31 +19,37 @@
 //
 // A row stays in registers from its loads to its stores, so each direction reads and
 // writes every tensor once: HBM bounds both.  NW waves share a row, a lane holding CPL
-// chunks of 8 consecutive elements: a wave alone up to H = 1024 (its two reductions are
-// shuffles, no barrier), four waves to 4096, eight to 16384.  Rows may start at any
-// element: 16-byte loads need no alignment here, and a row's last H % 8 elements come out
-// of a load of its last 8.
+// chunks of 8 consecutive elements:
+//   without a post norm or gate: a wave alone up to H = 1024 (its reductions are shuffles,
+//     no barrier; the backward from 512 rows on), else four waves to 4096, eight to 16384;
+//   with one (FULL): the forward four waves to 4096, the backward eight, eight above.
+// Rows may start at any element: 16-byte loads need no alignment here, and a row's last
+// H % 8 elements come out of a load of its last 8.
 //
 // Measured, us (TB/s of the tensors read and written): 128000 x 2880 bf16 with a residual
-// forward 513 (5.7), backward with dweight 732 (6.0; 640 without it), joining 5; 8192 x
-// 2880 29 and 47; 3 x 1021 rows with post_weight and a gate 21 and 40; 1 row 2.5.
+// forward 494 to 513 (5.7 to 6.0), backward with dweight 732 to 760 (5.8 to 6.0; 640 without it),
+// joining 5; 8192 x 2880 29 and 47; 3 x 1021 rows with post_weight and a gate 22 and 40; 1 row 2.5.
 // A wave a row against four: 8192 x 512 forward 6.6 for 11.3, 300 rows 3.0 for 3.1, one
 // row of 1024 2.8 for 2.7; at 2880 (six chunks a lane) 8192 rows 29.0 for 29.2, but 300
-// rows 5.3 for 3.6.  Backward, 8192 x 960 24.5 for 32.8, 300 x 1024 8.4 for 8.0.
+// rows 5.3 for 3.6.  Backward, 8192 x 960 24.5 for 32.8, 300 x 1024 8.4 for 8.0.  FULL has no
+// wave a row: its forward would take, with launch, 12.1 for 22.2 (8192 x 512), 16.3 for 24.1
+// (8192 x 1024), 59 for 181 (128000 x 64), 6.8 for 6.3 (300 x 1024).
 //
 // Column sums (dweight, dpost_weight, dgate): a lane adds up its columns over all its
 // rows, the waves of a block are joined through LDS, each block writes one row of fp32
-// partials, and a second launch adds the blocks' rows: fixed order, no atomics.
+// partials, and a second launch adds the blocks' rows: fixed order, no atomics.  A gate's
+// sums are over each group of rows that share it: some blocks per group, or, where there
+// are more groups than blocks, groups that a block finishes by itself (OWN).
 #include "af3_common.h"
 
 namespace {
 
 constexpr int kNormMinH = 8, kNormMaxH = 16384;
 constexpr int kNormWaveRows = 512;  // rows from which a wave of the backward has a row of its own
-// Blocks of the backward's row pass: 256 of eight waves or 512 of four hold all the waves that
-// their registers allow, and more only add partials.  8192 x 2880 with 256, 512, 1024 blocks:
-// four waves a row 73, 57, 62 us, eight (FULL) 66, 70, 78 (FULL with four, 130).  Up to 1024
-// rows, 256 either way: 500 rows 11.2, 12.3, 13.1.
+// Blocks of the backward's row pass: 256 with a post norm or gate (eight waves a row) and for
+// up to 1024 rows of several waves, else twice as many (of four waves, or of eight with a row
+// each): more only add partials.  8192 x 2880 with 256, 512, 1024 blocks: four waves a row 73,
+// 57, 62 us, eight (FULL) 66, 70, 78 (FULL with four, 130); 500 rows 11.2, 12.3, 13.1.
 constexpr int kNormBwdBlocks = 256;
 constexpr int64_t kNormGrid = 1 << 22;  // blocks per launch of the forward: a launch holds less than 2^32 threads
 
